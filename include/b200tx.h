@@ -54,7 +54,9 @@ const char* b2_last_error(void);
 
 /* Reads (and with clear != 0 resets) the current device's pipeline status word:
  * 0 = no kernel gave up waiting since the last clear; otherwise (kernel << 16) | (site << 8) |
- * reason, kernel 2 = linear, 3 = attention. Synchronous: it waits for the device. */
+ * reason, kernel 2 = linear, 3 = attention, 5 = rotary, 6 = cache append, 7 = cache attention;
+ * reason 1 = a wait ran out, 3 = a position, length or page number read from device memory lay
+ * outside its table (what it names was skipped). Synchronous: it waits for the device. */
 int b2_device_status(uint32_t* out_status, int clear);
 
 /* Enqueues a copy of the current device's status word (the value b2_device_status reads, not
@@ -242,6 +244,84 @@ int b2_layernorm_gather_fwd(const float* x, const void* gamma, const void* beta,
  * b2_device_status() instead of hanging. world == 1 is a no-op.
  */
 int b2_peer_barrier(void* const* pads, int world, int rank, int channel, void* stream);
+
+/*
+ * Rotary positions, in place or into `out`: of each head's first rotary_dim elements the pairs
+ * (x[i], x[i + rotary_dim / 2]), or with interleaved != 0 (x[2i], x[2i + 1]), become
+ *   (x1 c - x2 s, x2 c + x1 s),  (c, s) = table[positions[token]][i]   (inverse != 0: s -> -s, the
+ * transpose, which takes the gradient of the output to that of the input); the others are copied.
+ * No counterpart in the reference (its stack has no positions).
+ *   x, out     [tokens, ld] bf16, heads side by side; out may be x. Strides multiples of 8
+ *   positions  [tokens] int32; a negative one marks a row without a token, which is not written
+ *   table      [max_positions, rotary_dim / 2, 2] fp32 (cos, sin)
+ * head_dim: a multiple of 16 up to 256; rotary_dim: a multiple of 16 up to head_dim.
+ */
+int b2_rotary_fwd(const void* x, int64_t ld_x, int64_t tokens, int64_t heads, int64_t head_dim, int64_t rotary_dim,
+                  int interleaved, int inverse, const int32_t* positions, const float* table, int64_t max_positions,
+                  void* out, int64_t ld_out, void* stream);
+
+/* Element type of a cache's pages. */
+#define B2_CACHE_BF16 0
+#define B2_CACHE_E4M3 1 /* e4m3 codes, one power-of-two fp32 scale per page and head */
+
+/*
+ * A paged key/value cache: a page holds page_size (16, 32, 64, 128 or 256) consecutive tokens of one sequence for
+ * every key head, element (page, head, slot, dim) of K at k + page * page_stride + head * head_stride +
+ * slot * head_dim + dim (in elements; likewise V). Sequences own pages through a page table,
+ * [batch, table_pages] int32: token j of sequence b is in slot j % page_size of page
+ * page_table[b][j / page_size]. In 8 bits the value of a code is e4m3(code) * scale[page][head]. The scales are
+ * powers of two between 2^-40 and 2^40; b2_cache_append_fwd writes them. The reference has no cache.
+ */
+typedef struct b2_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale; /* [pages, kv_heads]; NULL for bf16 */
+  float* v_scale;
+  int64_t pages, kv_heads, page_size, head_dim, page_stride, head_stride;
+  int dtype;
+} b2_kv_cache;
+
+/*
+ * Stores the keys and values of new tokens in a cache and, with rotary_dim > 0, rotates K (before it
+ * is stored) and Q by the tokens' positions. Sequence b's new_len[b] new tokens are rows
+ * new_start[b] ... of qkv and stand at positions past_len[b] ...; max_new is at least every new_len.
+ * 8-bit pages: the scale 2^e has the least e with max|x| <= 448 * 2^e over the new values of the page and head,
+ * or the page's scale before where that is larger and the page holds earlier tokens of the sequence;
+ * where it grows the earlier tokens' codes are rounded again. Codes are rounded to nearest even from
+ * fp32, values that are not finite become NaN.
+ *   qkv    [tokens, ld_qkv] bf16, heads of Q at columns q_col ..., of K at k_col ..., of V at v_col ...
+ *   table  as in b2_rotary_fwd
+ *   q_out  [tokens, ld_q_out] bf16: rotated Q (rotary_dim > 0 only; may be qkv's own columns)
+ *   k_out  [tokens, ld_k_out] bf16: K as it was before rounding to the cache's type, or NULL
+ */
+int b2_cache_append_fwd(const b2_kv_cache* cache, const void* qkv, int64_t ld_qkv, int64_t q_col, int64_t k_col,
+                        int64_t v_col, int64_t tokens, int64_t num_heads, int64_t batch, const int32_t* new_start,
+                        const int32_t* new_len, const int32_t* past_len, const int32_t* page_table,
+                        int64_t table_pages, int64_t max_new, const float* table, int64_t max_positions,
+                        int64_t rotary_dim, int interleaved, void* q_out, int64_t ld_q_out, void* k_out,
+                        int64_t ld_k_out, void* stream);
+
+/* Bytes of b2_cache_attention_fwd's workspace. sm_count 0 asks the current device. */
+int b2_cache_attention_workspace(int64_t batch, int64_t q_len, int64_t num_heads, int64_t kv_heads, int64_t head_dim,
+                                 int sm_count, int64_t* bytes);
+
+/*
+ * Attention of each sequence's q_len newest tokens over its cached keys and values: row b * q_len + t stands
+ * at p = kv_len[b] - q_len + t and sees the keys j <= p with window == 0, p - j < window or j < sinks;
+ * out = softmax(scale * q k^T) v, zero where nothing is visible. What lies in pages and slots that no row
+ * sees is not used, whatever it is. Of the tokens that some of the q_len rows see and others do not,
+ * a value that is not finite reaches them all.
+ *   q, out     [batch * q_len, ld] bf16, num_heads heads side by side, a multiple of the cache's kv_heads:
+ *              query head i reads key head i / (num_heads / kv_heads). head_dim 32, 64 or 128
+ *   kv_len     [batch] int32, the tokens in the cache, the q_len newest included
+ *   workspace  at least b2_cache_attention_workspace bytes, zeroed by the caller once; the kernel leaves its
+ *              counters zero. One made for the largest batch, q_len and num_heads serves smaller calls too;
+ *              calls that may run at the same time need one each
+ */
+int b2_cache_attention_fwd(const b2_kv_cache* cache, const void* q, int64_t ld_q, int64_t batch, int64_t q_len,
+                           int64_t num_heads, const int32_t* page_table, int64_t table_pages, const int32_t* kv_len,
+                           int64_t window, int64_t sinks, float scale, void* out, int64_t ld_out, void* workspace,
+                           int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -8,11 +8,13 @@ names, forward signature and mask semantics; computation in hand-written tcgen05
 from .cases import BASELINE_CONFIGS, TransformerConfig, Workload, config_from
 from .correctness import AccuracyResult, GateResult, baseline_gate, compare_outputs
 from .models import UserOptimizedTransformer, copy_model_weights
+from .serving import KVCache, rotary, rotary_table
 
 __all__ = [
     "AccuracyResult",
     "BASELINE_CONFIGS",
     "GateResult",
+    "KVCache",
     "TransformerConfig",
     "UserOptimizedTransformer",
     "Workload",
@@ -20,4 +22,6 @@ __all__ = [
     "compare_outputs",
     "config_from",
     "copy_model_weights",
+    "rotary",
+    "rotary_table",
 ]

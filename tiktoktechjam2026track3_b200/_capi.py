@@ -28,9 +28,24 @@ EPI_RESIDUAL_ZERO = 3
 EPI_STORE_F32 = 4
 TILE_PAIR = 0x10000
 
+REASON_BAD_INDEX = 3  # of the status word: a position, length or page number lay outside its table
+CACHE_BF16 = 0
+CACHE_E4M3 = 1
+
 # Every symbol include/b200tx.h declares, with its ctypes signature.
 _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
+
+
+class KVCacheDesc(ctypes.Structure):
+    """b2_kv_cache: where a paged cache's keys, values and scales lie."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", _i64), ("kv_heads", _i64),
+                ("page_size", _i64), ("head_dim", _i64), ("page_stride", _i64), ("head_stride", _i64),
+                ("dtype", ctypes.c_int)]
+
+
+_cache_p = ctypes.POINTER(KVCacheDesc)
 SIGNATURES = {
     "b2_abi_version": (ctypes.c_int, []),
     "b2_last_error": (ctypes.c_char_p, []),
@@ -82,6 +97,22 @@ SIGNATURES = {
     ),
     "b2_layernorm_gather_fwd": (
         ctypes.c_int, [_vp, _vp, _vp, ctypes.c_float, ctypes.POINTER(_vp), ctypes.c_int, _vp, _i64, _i64, _vp],
+    ),
+    "b2_rotary_fwd": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, _vp, _vp, _i64, _vp, _i64, _vp],
+    ),
+    "b2_cache_append_fwd": (
+        ctypes.c_int,
+        [_cache_p, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64,
+         ctypes.c_int, _vp, _i64, _vp, _i64, _vp],
+    ),
+    "b2_cache_attention_workspace": (
+        ctypes.c_int, [_i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.POINTER(_i64)],
+    ),
+    "b2_cache_attention_fwd": (
+        ctypes.c_int,
+        [_cache_p, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, ctypes.c_float, _vp, _i64, _vp, _i64, _vp],
     ),
 }
 
@@ -201,9 +232,11 @@ class StatusWatch:
         if value:
             self.status = value
             kernel, site, reason = value >> 16, (value >> 8) & 0xFF, value & 0xFF
-            names = {1: "layernorm", 2: "linear", 3: "attention", 4: "peer barrier"}
+            names = {1: "layernorm", 2: "linear", 3: "attention", 4: "peer barrier", 5: "rotary", 6: "cache append",
+                     7: "cache attention"}
+            what = "met an index outside its table" if reason == REASON_BAD_INDEX else "gave up waiting"
             raise RuntimeError(
-                f"a {names.get(kernel, kernel)} kernel gave up waiting (status {value:#x}: site {site}, reason "
+                f"a {names.get(kernel, kernel)} kernel {what} (status {value:#x}: site {site}, reason "
                 f"{reason}); outputs computed since then are not valid. Clear the status with "
                 "_capi.device_status(clear=True) after handling it")
         return 0
@@ -489,3 +522,96 @@ def linear_bcast(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
         _stream_ptr(a.device),
     )
     _check(status, "b2_linear_bcast_fwd")
+
+
+def _rows(t: torch.Tensor, name: str, dtype: torch.dtype = torch.bfloat16) -> int:
+    """Row stride of a 2-D tensor whose rows are contiguous (a column slice of packed rows is one)."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (this package has no CPU path)")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 2 or t.stride(1) != 1:
+        raise ValueError(f"{name} must be 2-D with contiguous rows")
+    # A single row's stride may be anything; the kernels take it as a row length.
+    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, head_dim: int, out: torch.Tensor,
+           interleaved: bool = False, inverse: bool = False) -> None:
+    """out = the rows of x with every head turned by its row's position (see b2_rotary_fwd)."""
+    ld_x, ld_out = _rows(x, "x"), _rows(out, "out")
+    _require(positions, torch.int32, "positions")
+    _require(table, torch.float32, "table")
+    tokens, width = x.shape
+    if width % head_dim or out.shape != x.shape:
+        raise ValueError(f"x and out must both be [tokens, heads * {head_dim}]")
+    if positions.numel() != tokens or table.dim() != 3 or table.shape[2] != 2:
+        raise ValueError("positions must have one entry per row and table be [positions, rotary_dim / 2, 2]")
+    status = load_library().b2_rotary_fwd(
+        x.data_ptr(), ld_x, tokens, width // head_dim, head_dim, 2 * table.shape[1], 1 if interleaved else 0,
+        1 if inverse else 0, positions.data_ptr(), table.data_ptr(), table.shape[0], out.data_ptr(), ld_out,
+        _stream_ptr(x.device))
+    _check(status, "b2_rotary_fwd")
+
+
+def cache_append(cache: KVCacheDesc, qkv: torch.Tensor, num_heads: int, q_col: int, k_col: int, v_col: int,
+                 new_start: torch.Tensor, new_len: torch.Tensor, past_len: torch.Tensor, page_table: torch.Tensor,
+                 max_new: int, table: Optional[torch.Tensor] = None, interleaved: bool = False,
+                 q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None) -> None:
+    """Stores (and with `table` rotates) the new tokens of packed rows qkv (see b2_cache_append_fwd)."""
+    ld = _rows(qkv, "qkv")
+    batch = new_len.numel()
+    for t, name in ((new_start, "new_start"), (new_len, "new_len"), (past_len, "past_len"), (page_table, "page_table")):
+        _require(t, torch.int32, name)
+    if new_start.numel() != batch or past_len.numel() != batch or page_table.dim() != 2 or page_table.shape[0] != batch:
+        raise ValueError("new_start, new_len, past_len and page_table must have one entry (row) per sequence")
+    tokens, positions, rotary_dim = qkv.shape[0], 0, 0
+    if table is not None:
+        _require(table, torch.float32, "table")
+        if table.dim() != 3 or table.shape[2] != 2:
+            raise ValueError("table must be [positions, rotary_dim / 2, 2]")
+        if q_out is None:
+            raise ValueError("a rotation needs q_out")
+        positions, rotary_dim = table.shape[0], 2 * table.shape[1]
+    ld_q = ld_k = 0
+    if q_out is not None:
+        ld_q = _rows(q_out, "q_out")
+        if table is None or q_out.shape[0] != tokens or q_out.shape[1] != num_heads * cache.head_dim:
+            raise ValueError("q_out needs a table and the shape [tokens, num_heads * head_dim]")
+    if k_out is not None:
+        ld_k = _rows(k_out, "k_out")
+        if k_out.shape[0] != tokens or k_out.shape[1] != cache.kv_heads * cache.head_dim:
+            raise ValueError("k_out must be [tokens, kv_heads * head_dim]")
+    status = load_library().b2_cache_append_fwd(
+        cache, qkv.data_ptr(), ld, q_col, k_col, v_col, tokens, num_heads, batch, new_start.data_ptr(),
+        new_len.data_ptr(), past_len.data_ptr(), page_table.data_ptr(), page_table.shape[1], max_new, _ptr(table),
+        positions, rotary_dim, 1 if interleaved else 0, _ptr(q_out), ld_q, _ptr(k_out), ld_k, _stream_ptr(qkv.device))
+    _check(status, "b2_cache_append_fwd")
+
+
+def cache_attention_workspace(batch: int, q_len: int, num_heads: int, kv_heads: int, head_dim: int,
+                              sm_count: int = 0) -> int:
+    """Bytes of cache_attention's workspace (see b2_cache_attention_workspace)."""
+    out = _i64(0)
+    _check(load_library().b2_cache_attention_workspace(batch, q_len, num_heads, kv_heads, head_dim, sm_count,
+                                                       ctypes.byref(out)), "b2_cache_attention_workspace")
+    return int(out.value)
+
+
+def cache_attention(cache: KVCacheDesc, q: torch.Tensor, q_len: int, page_table: torch.Tensor, kv_len: torch.Tensor,
+                    window: int, sinks: int, scale: float, out: torch.Tensor, workspace: torch.Tensor) -> None:
+    """out = attention of the q_len newest tokens of each sequence over the cache (see b2_cache_attention_fwd)."""
+    ld_q, ld_out = _rows(q, "q"), _rows(out, "out")
+    _require(page_table, torch.int32, "page_table")
+    _require(kv_len, torch.int32, "kv_len")
+    rows, width = q.shape
+    batch = kv_len.numel()
+    if page_table.dim() != 2 or page_table.shape[0] != batch or rows != batch * q_len:
+        raise ValueError("q needs q_len rows, page_table a row and kv_len an entry per sequence")
+    if width % cache.head_dim or out.shape != q.shape:
+        raise ValueError("q and out must both be [batch * q_len, heads * head_dim]")
+    status = load_library().b2_cache_attention_fwd(
+        cache, q.data_ptr(), ld_q, batch, q_len, width // cache.head_dim, page_table.data_ptr(), page_table.shape[1],
+        kv_len.data_ptr(), window, sinks, scale, out.data_ptr(), ld_out, workspace.data_ptr(),
+        workspace.numel() * workspace.element_size(), _stream_ptr(q.device))
+    _check(status, "b2_cache_attention_fwd")

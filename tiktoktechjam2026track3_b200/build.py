@@ -32,7 +32,8 @@ def nvcc_path() -> str:
 
 
 def sources() -> list[Path]:
-    return sorted(CSRC_DIR.glob("*.cu")) + sorted(CSRC_DIR.glob("*.cuh"))
+    header = PKG_DIR.parent / "include" / "b200tx.h"
+    return sorted(CSRC_DIR.glob("*.cu")) + sorted(CSRC_DIR.glob("*.cuh")) + ([header] if header.exists() else [])
 
 
 def is_stale() -> bool:

@@ -16,6 +16,7 @@
 #include <mutex>
 #include <string>
 
+#include "../../include/b200tx.h"
 #include "b2_common.cuh"
 #include "layernorm.cuh"
 #include "gemm.cuh"
@@ -25,6 +26,9 @@
 #include "attention_simt.cuh"
 #include "peer.cuh"
 #include "mask.cuh"
+#include "rotary.cuh"
+#include "cache_append.cuh"
+#include "cache_attention.cuh"
 
 #define B2_API extern "C" __attribute__((visibility("default")))
 
@@ -416,4 +420,202 @@ B2_API int b2_linear_bcast_fwd(const void* a, const void* w, const void* bias, i
                                   static_cast<const __nv_bfloat16*>(bias), m, n, k, kEpiBiasPeers, peers[rank], ldo,
                                   nullptr, tile_n, static_cast<cudaStream_t>(stream), peers, world, rank, 0, col_begin),
                       "b2_linear_bcast_fwd");
+}
+
+B2_API int b2_rotary_fwd(const void* x, int64_t ld_x, int64_t tokens, int64_t heads, int64_t head_dim,
+                         int64_t rotary_dim, int interleaved, int inverse, const int32_t* positions,
+                         const float* table, int64_t max_positions, void* out, int64_t ld_out, void* stream) {
+  if (tokens < 0 || heads <= 0 || max_positions <= 0)
+    return fail(1, "b2_rotary_fwd: invalid shape tokens=%lld heads=%lld max_positions=%lld", (long long)tokens,
+                (long long)heads, (long long)max_positions);
+  if (head_dim % 16 != 0 || head_dim < 16 || head_dim > 256)
+    return fail(2, "b2_rotary_fwd: head_dim=%lld must be a multiple of 16 up to 256", (long long)head_dim);
+  if (rotary_dim % 16 != 0 || rotary_dim < 16 || rotary_dim > head_dim)
+    return fail(2, "b2_rotary_fwd: rotary_dim=%lld must be a multiple of 16 up to head_dim", (long long)rotary_dim);
+  if (heads > 65536 || tokens > 0x7fffffffLL) return fail(2, "b2_rotary_fwd: problem too large");
+  if (ld_x < heads * head_dim || ld_out < heads * head_dim || ld_x % 8 != 0 || ld_out % 8 != 0)
+    return fail(2, "b2_rotary_fwd: row strides must be multiples of 8 and at least heads * head_dim");
+  if (tokens == 0) return 0;
+  if (x == nullptr || positions == nullptr || table == nullptr || out == nullptr)
+    return fail(1, "b2_rotary_fwd: null pointer argument");
+  if (!aligned16(x) || !aligned16(out) || !aligned16(table))
+    return fail(2, "b2_rotary_fwd: pointers must be 16-byte aligned");
+  RotaryParams p{};
+  p.x = static_cast<const __nv_bfloat16*>(x);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.ld_x = ld_x;
+  p.ld_out = ld_out;
+  p.positions = positions;
+  p.table = reinterpret_cast<const float2*>(table);
+  p.max_positions = max_positions;
+  p.tokens = static_cast<int>(tokens);
+  p.heads = static_cast<int>(heads);
+  p.head_dim = static_cast<int>(head_dim);
+  p.rotary_dim = static_cast<int>(rotary_dim);
+  p.inverse = inverse != 0;
+  return check_launch(launch_rotary(p, interleaved, static_cast<cudaStream_t>(stream)), "b2_rotary_fwd");
+}
+
+// The pages of a cache as the kernels take them, or a status.
+static int cache_pages(const b2_kv_cache* c, const char* what, CachePages* out, bool* fp8) {
+  if (c == nullptr || c->k == nullptr || c->v == nullptr) return fail(1, "%s: null pointer argument", what);
+  if (c->dtype != B2_CACHE_E4M3 && c->dtype != B2_CACHE_BF16) return fail(1, "%s: unknown cache dtype %d", what, c->dtype);
+  *fp8 = c->dtype == B2_CACHE_E4M3;
+  if (*fp8 && (c->k_scale == nullptr || c->v_scale == nullptr))
+    return fail(1, "%s: an e4m3 cache needs k_scale and v_scale", what);
+  if (c->pages <= 0 || c->kv_heads <= 0) return fail(1, "%s: invalid cache shape", what);
+  int shift = 0;
+  while (shift < 8 && (int64_t{1} << shift) < c->page_size) ++shift;
+  if (c->page_size < 16 || (int64_t{1} << shift) != c->page_size)
+    return fail(2, "%s: page_size=%lld must be 16, 32, 64, 128 or 256", what, (long long)c->page_size);
+  if (c->head_dim % 16 != 0 || c->head_dim < 16 || c->head_dim > 256)
+    return fail(2, "%s: head_dim=%lld must be a multiple of 16 up to 256", what, (long long)c->head_dim);
+  if (c->kv_heads > 16384 || c->pages > 0x7fffffffLL) return fail(2, "%s: cache too large", what);
+  const int64_t head = c->page_size * c->head_dim;
+  if (c->head_stride < head || c->page_stride < c->head_stride * (c->kv_heads - 1) + head)
+    return fail(1, "%s: page_stride or head_stride too small", what);
+  if (c->head_stride % 16 != 0 || c->page_stride % 16 != 0 || !aligned16(c->k) || !aligned16(c->v))
+    return fail(2, "%s: cache pointers must be 16-byte aligned, strides multiples of 16 elements", what);
+  out->k = static_cast<uint8_t*>(c->k);
+  out->v = static_cast<uint8_t*>(c->v);
+  out->k_scale = c->k_scale;
+  out->v_scale = c->v_scale;
+  out->pages = c->pages;
+  out->page_stride = c->page_stride;
+  out->head_stride = c->head_stride;
+  out->kv_heads = static_cast<int>(c->kv_heads);
+  out->head_dim = static_cast<int>(c->head_dim);
+  out->page_shift = shift;
+  return 0;
+}
+
+B2_API int b2_cache_append_fwd(const b2_kv_cache* cache, const void* qkv, int64_t ld_qkv, int64_t q_col,
+                               int64_t k_col, int64_t v_col, int64_t tokens, int64_t num_heads, int64_t batch,
+                               const int32_t* new_start, const int32_t* new_len, const int32_t* past_len,
+                               const int32_t* page_table, int64_t table_pages, int64_t max_new, const float* table,
+                               int64_t max_positions, int64_t rotary_dim, int interleaved, void* q_out,
+                               int64_t ld_q_out, void* k_out, int64_t ld_k_out, void* stream) {
+  AppendParams p{};
+  bool fp8 = false;
+  if (const int rc = cache_pages(cache, "b2_cache_append_fwd", &p.c, &fp8)) return rc;
+  const int64_t hd = cache->head_dim, hk = cache->kv_heads;
+  if (tokens < 0 || batch < 0 || max_new < 0 || num_heads <= 0 || table_pages <= 0)
+    return fail(1, "b2_cache_append_fwd: invalid shape");
+  if (num_heads % hk != 0)
+    return fail(1, "b2_cache_append_fwd: num_heads=%lld must be a multiple of the cache's kv_heads=%lld",
+                (long long)num_heads, (long long)hk);
+  if (rotary_dim < 0 || rotary_dim > hd || rotary_dim % 16 != 0)
+    return fail(2, "b2_cache_append_fwd: rotary_dim=%lld must be 0 or a multiple of 16 up to head_dim", (long long)rotary_dim);
+  if (q_col < 0 || k_col < 0 || v_col < 0 || q_col % 8 != 0 || k_col % 8 != 0 || v_col % 8 != 0 || ld_qkv % 8 != 0)
+    return fail(2, "b2_cache_append_fwd: q/k/v columns and ld_qkv must be non-negative multiples of 8");
+  if (k_col + hk * hd > ld_qkv || v_col + hk * hd > ld_qkv || (rotary_dim > 0 && q_col + num_heads * hd > ld_qkv))
+    return fail(1, "b2_cache_append_fwd: q/k/v columns exceed ld_qkv");
+  if (rotary_dim > 0 && max_positions <= 0) return fail(1, "b2_cache_append_fwd: max_positions must be positive");
+  if (batch > 65535 || tokens > 0x7fffffffLL || max_new > 0x7fffffffLL || num_heads > 65536 ||
+      table_pages > (0x7fffffffLL >> p.c.page_shift) || ld_qkv > 0x7fffffffLL)
+    return fail(2, "b2_cache_append_fwd: problem too large");
+  if (rotary_dim > 0 && (ld_q_out < num_heads * hd || ld_q_out % 8 != 0))
+    return fail(2, "b2_cache_append_fwd: ld_q_out must be a multiple of 8 and at least num_heads * head_dim");
+  if (k_out != nullptr && (ld_k_out < hk * hd || ld_k_out % 8 != 0))
+    return fail(2, "b2_cache_append_fwd: ld_k_out must be a multiple of 8 and at least kv_heads * head_dim");
+  if (tokens == 0 || batch == 0 || max_new == 0) return 0;
+  if (qkv == nullptr || new_start == nullptr || new_len == nullptr || past_len == nullptr || page_table == nullptr ||
+      (rotary_dim > 0 && (table == nullptr || q_out == nullptr)))
+    return fail(1, "b2_cache_append_fwd: null pointer argument");
+  if (!aligned16(qkv) || !aligned16(table) || !aligned16(q_out) || !aligned16(k_out))
+    return fail(2, "b2_cache_append_fwd: pointers must be 16-byte aligned");
+  if (!is_sm100(nullptr)) return fail(2, "b2_cache_append_fwd: needs an sm_100 (B200) device");
+  p.qkv = static_cast<const __nv_bfloat16*>(qkv);
+  p.ld = ld_qkv;
+  p.tokens = tokens;
+  p.q_col = static_cast<int>(q_col);
+  p.k_col = static_cast<int>(k_col);
+  p.v_col = static_cast<int>(v_col);
+  p.batch = static_cast<int>(batch);
+  p.group = static_cast<int>(num_heads / hk);
+  p.max_new = max_new;
+  p.new_start = new_start;
+  p.new_len = new_len;
+  p.past_len = past_len;
+  p.page_table = page_table;
+  p.ld_table = table_pages;
+  p.table_pages = static_cast<int>(table_pages);
+  p.rotary_dim = static_cast<int>(rotary_dim);
+  p.table = reinterpret_cast<const float2*>(table);
+  p.max_positions = max_positions;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.ld_q_out = ld_q_out;
+  p.ld_k_out = ld_k_out;
+  return check_launch(launch_cache_append(p, max_new, fp8, interleaved, static_cast<cudaStream_t>(stream)),
+                      "b2_cache_append_fwd");
+}
+
+B2_API int b2_cache_attention_workspace(int64_t batch, int64_t q_len, int64_t num_heads, int64_t kv_heads,
+                                        int64_t head_dim, int sm_count, int64_t* bytes) {
+  if (bytes == nullptr) return fail(1, "b2_cache_attention_workspace: null pointer argument");
+  if (batch < 0 || q_len <= 0 || num_heads <= 0 || kv_heads <= 0 || num_heads % kv_heads != 0)
+    return fail(1, "b2_cache_attention_workspace: invalid shape");
+  int sms = sm_count;
+  if (sms <= 0) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return fail(2, "b2_cache_attention_workspace: no CUDA device and no sm_count");
+    sms = device_sm_count(dev);
+  }
+  *bytes = cache_attention_workspace_bytes(batch, kv_heads, head_dim, q_len * (num_heads / kv_heads), sms);
+  return 0;
+}
+
+B2_API int b2_cache_attention_fwd(const b2_kv_cache* cache, const void* q, int64_t ld_q, int64_t batch, int64_t q_len,
+                                  int64_t num_heads, const int32_t* page_table, int64_t table_pages,
+                                  const int32_t* kv_len, int64_t window, int64_t sinks, float scale, void* out,
+                                  int64_t ld_out, void* workspace, int64_t workspace_bytes, void* stream) {
+  CacheAttnParams p{};
+  bool fp8 = false;
+  if (const int rc = cache_pages(cache, "b2_cache_attention_fwd", &p.c, &fp8)) return rc;
+  const int64_t hd = cache->head_dim, hk = cache->kv_heads;
+  if (hd != 32 && hd != 64 && hd != 128)
+    return fail(2, "b2_cache_attention_fwd: head_dim=%lld not supported (32, 64, 128)", (long long)hd);
+  if (batch < 0 || q_len <= 0 || num_heads <= 0 || table_pages <= 0) return fail(1, "b2_cache_attention_fwd: invalid shape");
+  if (num_heads % hk != 0)
+    return fail(1, "b2_cache_attention_fwd: num_heads=%lld must be a multiple of the cache's kv_heads=%lld",
+                (long long)num_heads, (long long)hk);
+  if (window < 0 || sinks < 0 || (window == 0 && sinks != 0))
+    return fail(1, "b2_cache_attention_fwd: window and sinks must not be negative, and sinks need a window");
+  if (!(scale > 0.f)) return fail(1, "b2_cache_attention_fwd: scale must be positive");
+  if (ld_q < num_heads * hd || ld_out < num_heads * hd || ld_q % 8 != 0 || ld_out % 8 != 0)
+    return fail(2, "b2_cache_attention_fwd: row strides must be multiples of 8 and at least num_heads * head_dim");
+  const int64_t units = (table_pages << p.c.page_shift) / (16 * kCacheWarps) + 1;
+  const int64_t rows = q_len * (num_heads / hk);
+  // Token positions stay below 2^30, so that sums of a position and a window do not leave 32 bits.
+  if (batch > 16384 || q_len > 1024 || num_heads > 65536 || table_pages > ((int64_t{1} << 30) >> p.c.page_shift) ||
+      batch * hk > 0x7fffffffLL / units)
+    return fail(2, "b2_cache_attention_fwd: problem too large");
+  if (batch == 0) return 0;
+  if (q == nullptr || page_table == nullptr || kv_len == nullptr || out == nullptr || workspace == nullptr)
+    return fail(1, "b2_cache_attention_fwd: null pointer argument");
+  if (!aligned16(q) || !aligned16(out) || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(2, "b2_cache_attention_fwd: pointers must be 16-byte aligned, the workspace 256-byte aligned");
+  if (!is_sm100(nullptr)) return fail(2, "b2_cache_attention_fwd: needs an sm_100 (B200) device");
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int sms = device_sm_count(dev);
+  if (workspace_bytes < cache_attention_workspace_bytes(batch, hk, hd, rows, sms))
+    return fail(1, "b2_cache_attention_fwd: the workspace is smaller than b2_cache_attention_workspace says");
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.ld_q = ld_q;
+  p.ld_out = ld_out;
+  p.page_table = page_table;
+  p.ld_table = table_pages;
+  p.table_pages = static_cast<int>(table_pages);
+  p.kv_len = kv_len;
+  p.batch = static_cast<int>(batch);
+  p.q_len = static_cast<int>(q_len);
+  p.group = static_cast<int>(num_heads / hk);
+  p.window = static_cast<int>(window < (int64_t{1} << 30) ? window : 0);  // beyond every position: none
+  p.sinks = static_cast<int>(sinks < (int64_t{1} << 30) ? sinks : (int64_t{1} << 30));
+  p.scale_log2 = scale * 1.4426950408889634f;
+  return check_launch(launch_cache_attention(p, workspace, workspace_bytes, fp8, sms, static_cast<cudaStream_t>(stream)),
+                      "b2_cache_attention_fwd");
 }

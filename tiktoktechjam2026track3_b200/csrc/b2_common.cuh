@@ -25,10 +25,14 @@ enum : uint32_t {
   kKernelGemm = 2,
   kKernelAttention = 3,
   kKernelPeerBarrier = 4,
+  kKernelRotary = 5,
+  kKernelCacheAppend = 6,
+  kKernelCacheAttention = 7,
 };
 enum : uint32_t {
   kReasonTimeout = 1,
   kReasonAbortSeen = 2,
+  kReasonBadIndex = 3,  // a position, length or page read from device memory lies outside its table
 };
 
 // Defined once: the library is a single translation unit (b200tx.cu includes every kernel).
