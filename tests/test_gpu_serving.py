@@ -407,3 +407,92 @@ def test_cache_slices_of_one_buffer():
     v = _gather(small, "v", seqs.table[0], n)
     exact = qkv.double().view(n, 3, hk, d)[:, 2].transpose(0, 1)
     _close(v, exact, 2**-4 * exact.abs() + 2**-9)
+
+
+# ---------------------------------------------------------------------------------- prompt attention with a window
+WINDOWS = [
+    # batch, seq, heads, kv_heads, head_dim, window, sinks
+    (1, 1, 1, 1, 64, 0, 0),
+    (2, 77, 4, 4, 64, 32, 4),
+    (1, 300, 4, 1, 128, 100, 20),
+    (2, 129, 3, 3, 32, 1, 0),
+    (1, 517, 6, 2, 64, 130, 1),       # a group of three: no packing
+    (1, 400, 12, 2, 128, 64, 0),      # a group of six: two heads to a tile
+    (1, 1000, 16, 1, 64, 256, 130),   # sixteen heads to a tile; sinks over more than a tile
+    (1, 260, 32, 1, 32, 40, 16),      # thirty-two heads: two tiles of sixteen
+    (3, 640, 2, 2, 128, 128, 0),
+    (1, 1100, 8, 4, 64, 0, 0),
+    (2, 700, 2, 1, 128, 699, 3),
+    (1, 900, 1, 1, 128, 300, 600),    # sinks beyond the window
+]
+
+
+def _check_window(q, k, v, out, batch, seq, heads, kv_heads, d, window, sinks, lengths, scale):
+    q, k, v = (x.cpu().double().view(batch, seq, -1, d) for x in (q, k, v))
+    got = out.cpu().view(batch, seq, heads, d)
+    for b in range(batch):
+        n = lengths[b]
+        assert not bool(got[b, n:].any())
+        seen = oracle.visible_keys(torch.arange(n), n, window, sinks)
+        for h in range(heads):
+            ref, absum, size = oracle.attend(q[b, :n, h], k[b, :n, h * kv_heads // heads], v[b, :n, h * kv_heads // heads],
+                                             seen, scale)
+            _close(got[b, :n, h], ref, 2**-8 * ref.abs() + (2**-8 + 2**-12 + 2 * d * 2**-23 * size) * absum)
+
+
+@pytest.mark.parametrize("batch,seq,heads,kv_heads,d,window,sinks", WINDOWS)
+@pytest.mark.parametrize("ragged", [False, True])
+def test_window_attention(batch, seq, heads, kv_heads, d, window, sinks, ragged):
+    g = _gen(seq + heads)
+    width = (heads + 2 * kv_heads) * d
+    packed = torch.randn(batch * seq, width + 8, generator=g).bfloat16()
+    lengths = [seq] * batch
+    if ragged:
+        lengths = [max(0, seq - 1 - 61 * b) for b in range(batch)]
+        for b, n in enumerate(lengths):
+            packed[b * seq + n:(b + 1) * seq] = math.nan  # what padding rows hold
+    packed = packed.cuda()
+    q, k, v = packed[:, :heads * d], packed[:, heads * d:(heads + kv_heads) * d], packed[:, (heads + kv_heads) * d:width]
+    out = torch.full((batch * seq, heads * d + 16), 3.0, dtype=BF16, device="cuda")[:, 8:8 + heads * d]
+    serving.window_attention(q, k, v, batch, seq, d, window=window, sinks=sinks,
+                             kv_len=_i32(lengths) if ragged else None, out=out)
+    _check_window(q, k, v, out, batch, seq, heads, kv_heads, d, window, sinks, lengths, d**-0.5)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_window_attention_scores_far_apart(d):
+    """The running maximum moves by far more than the rescale threshold, up and down along the list."""
+    n = 700
+    g = _gen(d)
+    q, k, v = (torch.randn(n, 2 * d, generator=g) for _ in range(3))
+    k *= torch.linspace(0.1, 40.0, n)[:, None] * torch.where(torch.arange(n) % 300 < 150, 1.0, 0.01)[:, None]
+    q, k, v = (x.bfloat16().cuda() for x in (q, k, v))
+    for window, sinks in ((0, 0), (200, 5)):
+        out = serving.window_attention(q, k, v, 1, n, d, window=window, sinks=sinks)
+        _check_window(q, k, v, out, 1, n, 2, 2, d, window, sinks, [n], d**-0.5)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_window_attention_without_a_window_is_causal_attention(d):
+    batch, seq, heads = 2, 333, 2
+    qkv = torch.randn(batch * seq, 3 * heads * d, generator=_gen(d)).bfloat16().cuda()
+    ctx = torch.empty(batch * seq, heads * d, dtype=BF16, device="cuda")
+    _capi.attention(qkv, batch, seq, heads, d, 0, heads * d, 2 * heads * d, None, True, d**-0.5, ctx)
+    parts = qkv.split(heads * d, 1)
+    for window in (0, seq, 1 << 40):
+        out = serving.window_attention(*parts, batch, seq, d, window=window)
+        assert float((out.float() - ctx.float()).abs().max()) <= 2**-6 * float(ctx.float().abs().max())
+
+
+def test_window_attention_long_sequence_tail():
+    """Far positions (the head-major order, list places of a long band): the last rows of 20000 against 64 bits."""
+    n, d, window, sinks = 20000, 64, 3000, 7
+    qkv = torch.randn(n, 6 * d, generator=_gen(2)).bfloat16().cuda()
+    q, k, v = qkv[:, :4 * d], qkv[:, 4 * d:5 * d], qkv[:, 5 * d:]
+    out = serving.window_attention(q, k, v, 1, n, d, window=window, sinks=sinks)
+    rows = torch.tensor([0, 31, 3000, 3007, 9999, 19968, 19999])
+    seen = oracle.visible_keys(rows, n, window, sinks)
+    for h in range(4):
+        ref, absum, size = oracle.attend(q.cpu().double().view(n, 4, d)[rows, h], k.cpu().double(), v.cpu().double(), seen,
+                                         d**-0.5)
+        _close(out.view(n, 4, d)[rows.cuda(), h], ref, 2**-8 * ref.abs() + (2**-8 + 2**-12 + 2 * d * 2**-23 * size) * absum)

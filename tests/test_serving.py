@@ -131,6 +131,23 @@ def test_cache_attention_rejects_bad_arguments(lib):
         _capi.cache_attention_workspace(3, 1, 5, 2, 64, sm_count=148)
 
 
+def test_window_attention_rejects_bad_arguments(lib):
+    def call(q=P, ld_q=256, k=P, ld_k=128, v=P, ld_v=128, batch=2, seq=100, heads=4, kv_heads=2, head_dim=64, kv_len=None,
+             window=10, sinks=2, scale=0.125, out=P, ld_out=256):
+        return lib.b2_window_attention_fwd(q, ld_q, k, ld_k, v, ld_v, batch, seq, heads, kv_heads, head_dim, kv_len, window,
+                                           sinks, scale, out, ld_out, None)
+
+    for name in ("q", "k", "v", "out"):
+        assert call(**{name: None}) == 1, name
+        assert call(**{name: ctypes.c_void_p(8)}) == 2, name
+    assert call(heads=3) == 1 and call(kv_heads=0) == 1 and call(batch=-1) == 1 and call(scale=-1.0) == 1
+    assert call(window=-1) == 1 and call(sinks=-1) == 1 and call(window=0) == 1  # sinks without a window
+    assert call(head_dim=48) == 2 and call(head_dim=256, ld_q=1024, ld_k=512, ld_v=512, ld_out=1024) == 2
+    assert call(ld_q=248) == 1 and call(ld_k=120) == 1 and call(ld_out=257) == 2
+    assert call(seq=1 << 40) == 2 and call(batch=70000) == 2
+    assert call(batch=0) == 0 and call(seq=0) == 0
+
+
 def test_wrappers_refuse_cpu_tensors():
     x = torch.zeros(4, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="CUDA"):

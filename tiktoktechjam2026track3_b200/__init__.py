@@ -8,7 +8,7 @@ names, forward signature and mask semantics; computation in hand-written tcgen05
 from .cases import BASELINE_CONFIGS, TransformerConfig, Workload, config_from
 from .correctness import AccuracyResult, GateResult, baseline_gate, compare_outputs
 from .models import UserOptimizedTransformer, copy_model_weights
-from .serving import KVCache, rotary, rotary_table
+from .serving import KVCache, rotary, rotary_table, window_attention
 
 __all__ = [
     "AccuracyResult",
@@ -24,4 +24,5 @@ __all__ = [
     "copy_model_weights",
     "rotary",
     "rotary_table",
+    "window_attention",
 ]

@@ -107,6 +107,10 @@ SIGNATURES = {
         [_cache_p, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64,
          ctypes.c_int, _vp, _i64, _vp, _i64, _vp],
     ),
+    "b2_window_attention_fwd": (
+        ctypes.c_int,
+        [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, ctypes.c_float, _vp, _i64, _vp],
+    ),
     "b2_cache_attention_workspace": (
         ctypes.c_int, [_i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.POINTER(_i64)],
     ),
@@ -615,3 +619,22 @@ def cache_attention(cache: KVCacheDesc, q: torch.Tensor, q_len: int, page_table:
         kv_len.data_ptr(), window, sinks, scale, out.data_ptr(), ld_out, workspace.data_ptr(),
         workspace.numel() * workspace.element_size(), _stream_ptr(q.device))
     _check(status, "b2_cache_attention_fwd")
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: int, seq_len: int, head_dim: int,
+                     window: int, sinks: int, kv_len: Optional[torch.Tensor], scale: float, out: torch.Tensor) -> None:
+    """out = causal attention with a sliding window and sinks (see b2_window_attention_fwd)."""
+    ld_q, ld_k, ld_v, ld_out = _rows(q, "q"), _rows(k, "k"), _rows(v, "v"), _rows(out, "out")
+    if q.shape[0] != batch * seq_len or k.shape[0] != q.shape[0] or v.shape != k.shape or out.shape != q.shape:
+        raise ValueError("q, k, v and out must have batch * seq_len rows, k and v alike, out like q")
+    if q.shape[1] % head_dim or k.shape[1] % head_dim:
+        raise ValueError(f"q and k must be whole heads of {head_dim}")
+    if kv_len is not None:
+        _require(kv_len, torch.int32, "kv_len")
+        if kv_len.numel() != batch:
+            raise ValueError("kv_len must have one entry per sequence")
+    status = load_library().b2_window_attention_fwd(
+        q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(), ld_v, batch, seq_len, q.shape[1] // head_dim,
+        k.shape[1] // head_dim, head_dim, _ptr(kv_len), window, sinks, scale, out.data_ptr(), ld_out,
+        _stream_ptr(q.device))
+    _check(status, "b2_window_attention_fwd")

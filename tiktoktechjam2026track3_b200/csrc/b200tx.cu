@@ -29,6 +29,7 @@
 #include "rotary.cuh"
 #include "cache_append.cuh"
 #include "cache_attention.cuh"
+#include "attention_window.cuh"
 
 #define B2_API extern "C" __attribute__((visibility("default")))
 
@@ -72,6 +73,23 @@ cudaError_t make_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner
   cuuint32_t box[2] = {box_inner, box_outer};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+cudaError_t make_tmap_bf16_4d(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
+                              const uint32_t (&box)[4]) {
+  auto enc = tensor_map_encoder();
+  if (enc == nullptr) return cudaErrorNotSupported;
+  cuuint64_t d[4], s[3];
+  cuuint32_t x[4], one[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) {
+    d[i] = dims[i];
+    x[i] = box[i];
+    if (i < 3) s[i] = strides[i];
+  }
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, s, x, one,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
@@ -618,4 +636,51 @@ B2_API int b2_cache_attention_fwd(const b2_kv_cache* cache, const void* q, int64
   p.scale_log2 = scale * 1.4426950408889634f;
   return check_launch(launch_cache_attention(p, workspace, workspace_bytes, fp8, sms, static_cast<cudaStream_t>(stream)),
                       "b2_cache_attention_fwd");
+}
+
+B2_API int b2_window_attention_fwd(const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* v,
+                                   int64_t ld_v, int64_t batch, int64_t seq_len, int64_t num_heads, int64_t kv_heads,
+                                   int64_t head_dim, const int32_t* kv_len, int64_t window, int64_t sinks, float scale,
+                                   void* out, int64_t ld_out, void* stream) {
+  if (batch < 0 || seq_len < 0 || num_heads <= 0 || kv_heads <= 0) return fail(1, "b2_window_attention_fwd: invalid shape");
+  if (num_heads % kv_heads != 0)
+    return fail(1, "b2_window_attention_fwd: num_heads=%lld must be a multiple of kv_heads=%lld", (long long)num_heads,
+                (long long)kv_heads);
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128)
+    return fail(2, "b2_window_attention_fwd: head_dim=%lld not supported (32, 64, 128)", (long long)head_dim);
+  if (window < 0 || sinks < 0 || (window == 0 && sinks != 0))
+    return fail(1, "b2_window_attention_fwd: window and sinks must not be negative, and sinks need a window");
+  if (!(scale > 0.f)) return fail(1, "b2_window_attention_fwd: scale must be positive");
+  const int64_t kv_width = kv_heads * head_dim;
+  if (ld_q < num_heads * head_dim || ld_out < num_heads * head_dim || ld_k < kv_width || ld_v < kv_width)
+    return fail(1, "b2_window_attention_fwd: row strides must be at least heads * head_dim");
+  if (ld_q % 8 != 0 || ld_k % 8 != 0 || ld_v % 8 != 0 || ld_out % 8 != 0)
+    return fail(2, "b2_window_attention_fwd: row strides must be multiples of 8");
+  // List places (sinks + window + tokens) stay below 2^31; the tensor maps' strides below 2^40 bytes.
+  if (seq_len > (int64_t{1} << 28) || batch > 65535 || num_heads > 65535 || batch * num_heads > 0x7fffffffLL ||
+      ((seq_len > 0) && (ld_q | ld_k | ld_v) > ((int64_t{1} << 38) / seq_len)) ||
+      (batch * num_heads > 65535 && seq_len >= (int64_t{1} << 18)))
+    return fail(2, "b2_window_attention_fwd: problem too large");
+  if (batch == 0 || seq_len == 0) return 0;
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr)
+    return fail(1, "b2_window_attention_fwd: null pointer argument");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+    return fail(2, "b2_window_attention_fwd: pointers must be 16-byte aligned");
+  if (!is_sm100(nullptr)) return fail(2, "b2_window_attention_fwd: needs an sm_100 (B200) device");
+  WindowParams p{};
+  p.ctx = static_cast<__nv_bfloat16*>(out);
+  p.ld_ctx = ld_out;
+  p.kv_len = kv_len;
+  p.B = static_cast<int>(batch);
+  p.S = static_cast<int>(seq_len);
+  p.heads = static_cast<int>(num_heads);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.window = window < seq_len ? static_cast<int>(window) : 0;  // a window of the whole sequence hides nothing
+  p.sinks = p.window > 0 ? static_cast<int>(sinks < seq_len ? sinks : seq_len) : 0;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  return check_launch(launch_window_attention(static_cast<const __nv_bfloat16*>(q), ld_q,
+                                              static_cast<const __nv_bfloat16*>(k), ld_k,
+                                              static_cast<const __nv_bfloat16*>(v), ld_v, head_dim, p,
+                                              static_cast<cudaStream_t>(stream)),
+                      "b2_window_attention_fwd");
 }

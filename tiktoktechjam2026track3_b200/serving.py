@@ -85,6 +85,22 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, head_d
     return out
 
 
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: int, seq_len: int, head_dim: int, *,
+                     window: int = 0, sinks: int = 0, kv_len: Optional[torch.Tensor] = None,
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of prompts: query i sees key j <= i iff window == 0, i - j < window or j < sinks.
+
+    q [batch * seq_len, heads * head_dim], k and v [batch * seq_len, kv_heads * head_dim] (bf16, any row strides: they
+    may be column ranges of one packed projection). Query head i reads key head i // (heads / kv_heads).
+    Rows past kv_len (int32 [batch]) are zeros. scale is head_dim^-0.5 unless given.
+    """
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _capi.window_attention(q, k, v, batch, seq_len, head_dim, window, sinks, kv_len,
+                           head_dim**-0.5 if scale is None else scale, out)
+    return out
+
+
 class KVCache:
     """Pages of keys and values, [pages, kv_heads, page_size, head_dim] each, and the operators on them.
 
