@@ -155,7 +155,14 @@ def _check(status: int, what: str) -> None:
         raise RuntimeError(f"{what} failed with status {status}: {message}")
 
 
+# The current stream's handle without making a torch.cuda.Stream object for it (0.15 us against 2.3 us of host time a
+# call, a quarter of a small kernel's launch); the object's way where this build of torch lacks the query.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream_ptr(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -528,34 +535,60 @@ def linear_bcast(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
     _check(status, "b2_linear_bcast_fwd")
 
 
-def _rows(t: torch.Tensor, name: str, dtype: torch.dtype = torch.bfloat16) -> int:
-    """Row stride of a 2-D tensor whose rows are contiguous (a column slice of packed rows is one)."""
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor (this package has no CPU path)")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != 2 or t.stride(1) != 1:
+def _rows(t: torch.Tensor, name: str) -> int:
+    """Row stride of a bf16 CUDA matrix whose rows are contiguous (a column slice of packed rows is one)."""
+    stride = t.stride()
+    if len(stride) != 2 or stride[1] != 1 or t.dtype is not torch.bfloat16 or not t.is_cuda:
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (this package has no CPU path)")
+        if t.dtype != torch.bfloat16:
+            raise ValueError(f"{name} must be {torch.bfloat16}, got {t.dtype}")
         raise ValueError(f"{name} must be 2-D with contiguous rows")
-    # A single row's stride may be anything; the kernels take it as a row length.
-    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+    # A single row's stride may be anything: its length takes the place.
+    return stride[0] if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
+
+
+def _table(t: torch.Tensor) -> Tuple[int, int]:
+    """(positions, rotary_dim) of a rotary table [positions, rotary_dim / 2, 2]."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != 2:
+        raise ValueError("table must be [positions, rotary_dim / 2, 2]")
+    _require(t, torch.float32, "table")
+    return shape[0], 2 * shape[1]
+
+
+def _indices(t: torch.Tensor, n: int, name: str) -> int:
+    """Pointer of n contiguous int32 entries on the GPU."""
+    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous():
+        _require(t, torch.int32, name)
+    if t.numel() != n:
+        raise ValueError(f"{name} must have {n} entries, got {t.numel()}")
+    return t.data_ptr()
+
+
+def _page_table(t: torch.Tensor, batch: int) -> Tuple[int, int]:
+    """(pointer, pages per sequence) of an int32 page table."""
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != batch:
+        raise ValueError(f"page_table must be [{batch}, pages], got {tuple(shape)}")
+    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous():
+        _require(t, torch.int32, "page_table")
+    return t.data_ptr(), shape[1]
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, head_dim: int, out: torch.Tensor,
            interleaved: bool = False, inverse: bool = False) -> None:
     """out = the rows of x with every head turned by its row's position (see b2_rotary_fwd)."""
     ld_x, ld_out = _rows(x, "x"), _rows(out, "out")
-    _require(positions, torch.int32, "positions")
-    _require(table, torch.float32, "table")
     tokens, width = x.shape
     if width % head_dim or out.shape != x.shape:
         raise ValueError(f"x and out must both be [tokens, heads * {head_dim}]")
-    if positions.numel() != tokens or table.dim() != 3 or table.shape[2] != 2:
-        raise ValueError("positions must have one entry per row and table be [positions, rotary_dim / 2, 2]")
+    most, rotary_dim = _table(table)
     status = load_library().b2_rotary_fwd(
-        x.data_ptr(), ld_x, tokens, width // head_dim, head_dim, 2 * table.shape[1], 1 if interleaved else 0,
-        1 if inverse else 0, positions.data_ptr(), table.data_ptr(), table.shape[0], out.data_ptr(), ld_out,
-        _stream_ptr(x.device))
-    _check(status, "b2_rotary_fwd")
+        x.data_ptr(), ld_x, tokens, width // head_dim, head_dim, rotary_dim, interleaved, inverse,
+        _indices(positions, tokens, "positions"), table.data_ptr(), most, out.data_ptr(), ld_out, _stream_ptr(x.device))
+    if status:
+        _check(status, "b2_rotary_fwd")
 
 
 def cache_append(cache: KVCacheDesc, qkv: torch.Tensor, num_heads: int, q_col: int, k_col: int, v_col: int,
@@ -564,33 +597,27 @@ def cache_append(cache: KVCacheDesc, qkv: torch.Tensor, num_heads: int, q_col: i
                  q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None) -> None:
     """Stores (and with `table` rotates) the new tokens of packed rows qkv (see b2_cache_append_fwd)."""
     ld = _rows(qkv, "qkv")
-    batch = new_len.numel()
-    for t, name in ((new_start, "new_start"), (new_len, "new_len"), (past_len, "past_len"), (page_table, "page_table")):
-        _require(t, torch.int32, name)
-    if new_start.numel() != batch or past_len.numel() != batch or page_table.dim() != 2 or page_table.shape[0] != batch:
-        raise ValueError("new_start, new_len, past_len and page_table must have one entry (row) per sequence")
-    tokens, positions, rotary_dim = qkv.shape[0], 0, 0
+    batch, tokens = new_len.numel(), qkv.shape[0]
+    pages, table_pages = _page_table(page_table, batch)
+    positions = rotary_dim = ld_q = ld_k = 0
     if table is not None:
-        _require(table, torch.float32, "table")
-        if table.dim() != 3 or table.shape[2] != 2:
-            raise ValueError("table must be [positions, rotary_dim / 2, 2]")
+        positions, rotary_dim = _table(table)
         if q_out is None:
             raise ValueError("a rotation needs q_out")
-        positions, rotary_dim = table.shape[0], 2 * table.shape[1]
-    ld_q = ld_k = 0
     if q_out is not None:
         ld_q = _rows(q_out, "q_out")
-        if table is None or q_out.shape[0] != tokens or q_out.shape[1] != num_heads * cache.head_dim:
+        if table is None or q_out.shape != (tokens, num_heads * cache.head_dim):
             raise ValueError("q_out needs a table and the shape [tokens, num_heads * head_dim]")
     if k_out is not None:
         ld_k = _rows(k_out, "k_out")
-        if k_out.shape[0] != tokens or k_out.shape[1] != cache.kv_heads * cache.head_dim:
+        if k_out.shape != (tokens, cache.kv_heads * cache.head_dim):
             raise ValueError("k_out must be [tokens, kv_heads * head_dim]")
     status = load_library().b2_cache_append_fwd(
-        cache, qkv.data_ptr(), ld, q_col, k_col, v_col, tokens, num_heads, batch, new_start.data_ptr(),
-        new_len.data_ptr(), past_len.data_ptr(), page_table.data_ptr(), page_table.shape[1], max_new, _ptr(table),
-        positions, rotary_dim, 1 if interleaved else 0, _ptr(q_out), ld_q, _ptr(k_out), ld_k, _stream_ptr(qkv.device))
-    _check(status, "b2_cache_append_fwd")
+        cache, qkv.data_ptr(), ld, q_col, k_col, v_col, tokens, num_heads, batch, _indices(new_start, batch, "new_start"),
+        _indices(new_len, batch, "new_len"), _indices(past_len, batch, "past_len"), pages, table_pages, max_new,
+        _ptr(table), positions, rotary_dim, interleaved, _ptr(q_out), ld_q, _ptr(k_out), ld_k, _stream_ptr(qkv.device))
+    if status:
+        _check(status, "b2_cache_append_fwd")
 
 
 def cache_attention_workspace(batch: int, q_len: int, num_heads: int, kv_heads: int, head_dim: int,
@@ -606,35 +633,33 @@ def cache_attention(cache: KVCacheDesc, q: torch.Tensor, q_len: int, page_table:
                     window: int, sinks: int, scale: float, out: torch.Tensor, workspace: torch.Tensor) -> None:
     """out = attention of the q_len newest tokens of each sequence over the cache (see b2_cache_attention_fwd)."""
     ld_q, ld_out = _rows(q, "q"), _rows(out, "out")
-    _require(page_table, torch.int32, "page_table")
-    _require(kv_len, torch.int32, "kv_len")
     rows, width = q.shape
     batch = kv_len.numel()
-    if page_table.dim() != 2 or page_table.shape[0] != batch or rows != batch * q_len:
-        raise ValueError("q needs q_len rows, page_table a row and kv_len an entry per sequence")
+    pages, table_pages = _page_table(page_table, batch)
+    if rows != batch * q_len:
+        raise ValueError("q needs q_len rows and kv_len an entry per sequence")
     if width % cache.head_dim or out.shape != q.shape:
         raise ValueError("q and out must both be [batch * q_len, heads * head_dim]")
     status = load_library().b2_cache_attention_fwd(
-        cache, q.data_ptr(), ld_q, batch, q_len, width // cache.head_dim, page_table.data_ptr(), page_table.shape[1],
-        kv_len.data_ptr(), window, sinks, scale, out.data_ptr(), ld_out, workspace.data_ptr(),
-        workspace.numel() * workspace.element_size(), _stream_ptr(q.device))
-    _check(status, "b2_cache_attention_fwd")
+        cache, q.data_ptr(), ld_q, batch, q_len, width // cache.head_dim, pages, table_pages,
+        _indices(kv_len, batch, "kv_len"), window, sinks, scale, out.data_ptr(), ld_out, workspace.data_ptr(),
+        workspace.numel(), _stream_ptr(q.device))
+    if status:
+        _check(status, "b2_cache_attention_fwd")
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: int, seq_len: int, head_dim: int,
                      window: int, sinks: int, kv_len: Optional[torch.Tensor], scale: float, out: torch.Tensor) -> None:
     """out = causal attention with a sliding window and sinks (see b2_window_attention_fwd)."""
     ld_q, ld_k, ld_v, ld_out = _rows(q, "q"), _rows(k, "k"), _rows(v, "v"), _rows(out, "out")
-    if q.shape[0] != batch * seq_len or k.shape[0] != q.shape[0] or v.shape != k.shape or out.shape != q.shape:
+    (rows, width), (k_rows, k_width) = q.shape, k.shape
+    if rows != batch * seq_len or k_rows != rows or v.shape != k.shape or out.shape != q.shape:
         raise ValueError("q, k, v and out must have batch * seq_len rows, k and v alike, out like q")
-    if q.shape[1] % head_dim or k.shape[1] % head_dim:
+    if width % head_dim or k_width % head_dim:
         raise ValueError(f"q and k must be whole heads of {head_dim}")
-    if kv_len is not None:
-        _require(kv_len, torch.int32, "kv_len")
-        if kv_len.numel() != batch:
-            raise ValueError("kv_len must have one entry per sequence")
     status = load_library().b2_window_attention_fwd(
-        q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(), ld_v, batch, seq_len, q.shape[1] // head_dim,
-        k.shape[1] // head_dim, head_dim, _ptr(kv_len), window, sinks, scale, out.data_ptr(), ld_out,
-        _stream_ptr(q.device))
-    _check(status, "b2_window_attention_fwd")
+        q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(), ld_v, batch, seq_len, width // head_dim,
+        k_width // head_dim, head_dim, None if kv_len is None else _indices(kv_len, batch, "kv_len"), window, sinks, scale,
+        out.data_ptr(), ld_out, _stream_ptr(q.device))
+    if status:
+        _check(status, "b2_window_attention_fwd")

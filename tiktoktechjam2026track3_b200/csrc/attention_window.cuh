@@ -19,6 +19,7 @@
 //   - Values behind the band's last key are cleared in shared memory: a weight of zero does not remove a NaN there.
 #pragma once
 #include <mutex>
+#include <type_traits>
 
 #include "b2_common.cuh"
 #include "attention.cuh"
@@ -97,19 +98,44 @@ struct RowKeys {
   int a, c, d;
 };
 
-__device__ __forceinline__ RowKeys window_row(const WindowParams& p, const KeyList& l, int i) {
+__device__ __forceinline__ RowKeys window_row(const WindowParams& p, int lo, int sink_rows, int i) {
   RowKeys r;
   r.a = p.sinks;
-  r.c = (p.window > 0 ? max(i - p.window + 1 - l.lo, 0) : 0) + l.sink_rows;
-  r.d = i - l.lo + l.sink_rows;
+  r.c = (p.window > 0 ? max(i - p.window + 1 - lo, 0) : 0) + sink_rows;
+  r.d = i - lo + sink_rows;
   return r;
 }
 
-// Whether tile t hides a key from some row of the query tile.
-__device__ __forceinline__ bool window_masked(const WindowParams& p, const KeyList& l, int t) {
-  const int v0 = 128 * t;
-  const RowKeys first = window_row(p, l, l.i0), last = window_row(p, l, l.i1 - 1);
-  return v0 + 127 > first.d || (v0 < last.c && v0 + 128 > p.sinks);
+// What the softmax threads need to know of the list, kept in shared memory: their registers are all in use on the tiles
+// that hide nothing.
+struct WindowTiles {
+  int i0, lo, sink_rows, rows, count;
+  int open_a, open_c, open_d;  // tiles below open_d that lie from open_c on or below open_a hide no key from any row
+  __device__ __forceinline__ bool open(int t) const { return t < open_d && (t >= open_c || t < open_a); }
+  __device__ __forceinline__ RowKeys row(const WindowParams& p, int i) const { return window_row(p, lo, sink_rows, i); }
+};
+
+__device__ __forceinline__ WindowTiles window_tiles(const WindowParams& p, const KeyList& l) {
+  WindowTiles t;
+  t.i0 = l.i0;
+  t.count = l.tiles;
+  t.lo = l.lo;
+  t.sink_rows = l.sink_rows;
+  t.rows = l.rows;
+  t.open_a = p.sinks >> 7;
+  t.open_c = (window_row(p, l.lo, l.sink_rows, l.i1 - 1).c + 127) >> 7;
+  t.open_d = (window_row(p, l.lo, l.sink_rows, l.i0).d + 1) >> 7;
+  return t;
+}
+
+// Bit k: whether a row sees place v0 + k.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t window_bits(const RowKeys& r, int v0) {
+  return low_bits(r.d + 1 - v0) & (~low_bits(r.c - v0) | low_bits(r.a - v0));
+}
+__device__ __forceinline__ void window_hide(float* v, uint32_t bits) {
+#pragma unroll
+  for (int k = 0; k < 32; ++k) v[k] = (bits >> k) & 1u ? v[k] : -INFINITY;
 }
 
 // Zeros for the rows of a query tile that lie behind the sequence's end.
@@ -174,6 +200,7 @@ __global__ void __launch_bounds__(192, 2)
   uint64_t* drain = s_free + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  WindowTiles* s_tiles = reinterpret_cast<WindowTiles*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -211,6 +238,7 @@ __global__ void __launch_bounds__(192, 2)
   }
   const int n = keys.tiles;
   const int last_rows = keys.rows - 128 * (n - 1);  // of the last tile
+  if (threadIdx.x == 0) *s_tiles = window_tiles(p, keys);
   if (warp == 1) {
     tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
@@ -339,15 +367,12 @@ __global__ void __launch_bounds__(192, 2)
     }
   } else {
     // ---------------- softmax: one row per thread ----------------
-    const int quad = warp & 3;
-    const int r = quad * 32 + lane;
-    const int token = keys.i0 + (r >> p.group_shift);
-    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t t_s = t_lane;
     const uint32_t t_p = t_lane + 128;
     const uint32_t t_o = t_lane + 192;
     const float c = p.scale_log2;
-    const RowKeys row = window_row(p, keys, token);
     constexpr float kRescaleThreshold = 8.0f;
 
     float m_ref = -INFINITY;  // reference maximum, -inf until the row has seen a key
@@ -355,49 +380,93 @@ __global__ void __launch_bounds__(192, 2)
     bool alive = true;
 
 #pragma unroll 1
-    for (int j = 0; j < n; ++j) {
+    for (int j = 0; j < s_tiles->count; ++j) {
       float alpha = 1.f;
       softmax_wait(s_full, j & 1, 108, alive, abort_flag);
       tc_fence_after_sync();
-      float v[128];
-      tmem_load_128cols(t_s, v);
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(s_free);
-      if (j == n - 1 || window_masked(p, keys, j)) {
-        const int a = row.a - 128 * j, cc = row.c - 128 * j, d = row.d - 128 * j;
+      auto new_reference = [&](float rmax) {
+        if (m_ref == -INFINITY) {
+          m_ref = rmax;  // nothing accumulated so far: nothing to rescale
+        } else if ((rmax - m_ref) * c > kRescaleThreshold) {
+          alpha = fast_exp2((m_ref - rmax) * c);
+          m_ref = rmax;
+        }
+      };
+      if (s_tiles->open(j)) {
+        // Every row sees all 128 places: the scores once into registers, S free for the next product meanwhile.
+        float v[128];
+        tmem_load_128cols(t_s, v);
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free);
+        new_reference(fmaxf(fmaxf(max32(v), max32(v + 32)), fmaxf(max32(v + 64), max32(v + 96))));
+        const uint64_t c2 = splat2(c);
+        const uint64_t neg_mc2 = splat2(-m_ref * c);
+        uint64_t sum2 = 0;
+        uint32_t w[64];
 #pragma unroll
-        for (int k = 0; k < 128; ++k) v[k] = (k <= d && (k >= cc || k < a)) ? v[k] : -INFINITY;
-      }
-      const float rmax = fmaxf(fmaxf(max32(v), max32(v + 32)), fmaxf(max32(v + 64), max32(v + 96)));
-      if (m_ref == -INFINITY) {
-        m_ref = rmax;  // nothing accumulated so far: nothing to rescale
-      } else if ((rmax - m_ref) * c > kRescaleThreshold) {
-        alpha = fast_exp2((m_ref - rmax) * c);
-        m_ref = rmax;
-      }
-      const uint64_t c2 = splat2(c);
-      const uint64_t neg_mc2 = splat2(m_ref == -INFINITY ? 0.f : -m_ref * c);
-      uint64_t sum2 = 0;
-      uint32_t w[64];
+        for (int k = 0; k < 64; ++k) {
+          float x0 = v[2 * k], x1 = v[2 * k + 1];
+          fma2_inplace(x0, x1, c2, neg_mc2);
+          const float e0 = fast_exp2(x0);
+          const float e1 = fast_exp2(x1);
+          sum2 = add2f(sum2, pack2f(e0, e1));
+          w[k] = pack_bf16x2(e0, e1);
+        }
+        float sum0, sum1;
+        unpack2f(sum2, sum0, sum1);
+        l_sum = l_sum * alpha + (sum0 + sum1);
+        if (j > 0) {
+          softmax_wait(o_full, (j - 1) & 1, 109, alive, abort_flag);
+          tc_fence_after_sync();
+        }
 #pragma unroll
-      for (int k = 0; k < 64; ++k) {
-        float x0 = v[2 * k], x1 = v[2 * k + 1];
-        fma2_inplace(x0, x1, c2, neg_mc2);
-        const float e0 = fast_exp2(x0);
-        const float e1 = fast_exp2(x1);
-        sum2 = add2f(sum2, pack2f(e0, e1));
-        w[k] = pack_bf16x2(e0, e1);
-      }
-      float sum0, sum1;
-      unpack2f(sum2, sum0, sum1);
-      l_sum = l_sum * alpha + (sum0 + sum1);
-      if (j > 0) {
-        softmax_wait(o_full, (j - 1) & 1, 109, alive, abort_flag);
-        tc_fence_after_sync();
-      }
+        for (int g = 0; g < 4; ++g) tmem_store_16cols_async(t_p + 16 * g, w + 16 * g);
+      } else {
+        // Some row does not see some place: 32 places at a time, as far as there are keys, the scores read twice (maximum,
+        // then weights), so that the masks cost no registers that the other path needs.
+        const RowKeys row = s_tiles->row(p, s_tiles->i0 + (r >> p.group_shift));
+        const int groups = (min(128, s_tiles->rows - 128 * j) + 31) >> 5;
+        float rmax = -INFINITY;
+#pragma unroll 1
+        for (int g = 0; g < groups; ++g) {
+          float v[32];
+          tmem_load_32cols(t_s + 32 * g, v);
+          window_hide(v, window_bits(row, 128 * j + 32 * g));
+          rmax = fmaxf(rmax, max32(v));
+        }
+        new_reference(rmax);
+        if (j > 0) {
+          softmax_wait(o_full, (j - 1) & 1, 109, alive, abort_flag);
+          tc_fence_after_sync();
+        }
+        const uint64_t c2 = splat2(c);
+        const uint64_t neg_mc2 = splat2(m_ref == -INFINITY ? 0.f : -m_ref * c);
+        uint64_t sum2 = 0;
+#pragma unroll 1
+        for (int g = 0; g < groups; ++g) {
+          float v[32];
+          uint32_t w[16];
+          tmem_load_32cols(t_s + 32 * g, v);
+          window_hide(v, window_bits(row, 128 * j + 32 * g));
 #pragma unroll
-      for (int g = 0; g < 4; ++g) tmem_store_16cols_async(t_p + 16 * g, w + 16 * g);
+          for (int k = 0; k < 16; ++k) {
+            float x0 = v[2 * k], x1 = v[2 * k + 1];
+            fma2_inplace(x0, x1, c2, neg_mc2);
+            const float e0 = fast_exp2(x0);
+            const float e1 = fast_exp2(x1);
+            sum2 = add2f(sum2, pack2f(e0, e1));
+            w[k] = pack_bf16x2(e0, e1);
+          }
+          tmem_store_16cols_async(t_p + 16 * g, w);
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free);
+        float sum0, sum1;
+        unpack2f(sum2, sum0, sum1);
+        l_sum = l_sum * alpha + (sum0 + sum1);
+      }
       tmem_wait_st();
       if (__any_sync(0xffffffffu, alpha < 1.f)) {
 #pragma unroll 1
@@ -409,7 +478,7 @@ __global__ void __launch_bounds__(192, 2)
           tmem_store_32cols(t_o + cc * 32, o);
         }
       }
-      if (j == n - 1 && (last_rows & 15) != 0) {  // products stop at the next multiple of 16 rows
+      if (const int last_rows = s_tiles->rows - 128 * j; last_rows < 128 && (last_rows & 15) != 0) {  // products stop at the next multiple of 16 rows
         // (O += P(j-1) V has completed, so the stage's barrier is in this tile's phase)
         softmax_wait(&v_full[j % kStages], (j / kStages) & 1, 111, alive, abort_flag);
         window_clear_values<1>(s_v + (j % kStages) * kTileBytes, last_rows, threadIdx.x - 64, 128);
@@ -419,8 +488,9 @@ __global__ void __launch_bounds__(192, 2)
       if (lane == 0) mbar_arrive(p_full);
     }
 
-    softmax_wait(o_full, (n - 1) & 1, 110, alive, abort_flag);
+    softmax_wait(o_full, (s_tiles->count - 1) & 1, 110, alive, abort_flag);
     tc_fence_after_sync();
+    const int token = s_tiles->i0 + (r >> p.group_shift);
     const float inv = token < len && l_sum != 0.f ? 1.0f / l_sum : 0.f;
     const int head = head0 + (r & ((1 << p.group_shift) - 1));
     uint4* dst = reinterpret_cast<uint4*>(p.ctx + (static_cast<int64_t>(b) * p.S + token) * p.ld_ctx + head * HD);
@@ -663,15 +733,15 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
     float* red = reinterpret_cast<float*>(smem + Cfg::kOffRed);
     const uint32_t pair_bar = 1 + quad;
     const float c = p.scale_log2;
-    const RowKeys row = window_row(p, keys, token);
+    const WindowTiles tiles = window_tiles(p, keys);
     constexpr float kRescaleThreshold = 8.0f;
 
     float m_ref = -INFINITY;
     float l_sum = 0.f;
     bool alive = true;
 
-#pragma unroll 1
-    for (int j = 0; j < n; ++j) {
+    // One tile; `hide`: some row does not see some place of it.
+    auto softmax_tile = [&](int j, auto hide) {
       const int buf = j % Cfg::kBufs;
       const uint32_t t_s = t_lane + buf * 128;
       float alpha = 1.f;
@@ -679,11 +749,10 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
       tc_fence_after_sync();
       float v[64];
       tmem_load_64cols(t_s + 64 * half, v);
-      if (j == n - 1 || window_masked(p, keys, j)) {
-        const int v0 = 128 * j + 64 * half;
-        const int a = row.a - v0, cc = row.c - v0, d = row.d - v0;
+      if constexpr (decltype(hide)::value) {
+        const RowKeys row = tiles.row(p, token);
 #pragma unroll
-        for (int k = 0; k < 64; ++k) v[k] = (k <= d && (k >= cc || k < a)) ? v[k] : -INFINITY;
+        for (int g = 0; g < 2; ++g) window_hide(v + 32 * g, window_bits(row, 128 * j + 64 * half + 32 * g));
       }
       // Row maximum over both halves; after the barrier both warps have loaded their scores, so P may be written over
       // the buffer's first 64 columns (slots alternate by tile).
@@ -692,7 +761,7 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
       named_barrier_sync(pair_bar, 64);
       const float rmax = fmaxf(slot[r], slot[128 + r]);
       if (m_ref == -INFINITY) {
-        m_ref = rmax;
+        m_ref = rmax;  // nothing accumulated so far: nothing to rescale
       } else if ((rmax - m_ref) * c > kRescaleThreshold) {
         alpha = fast_exp2((m_ref - rmax) * c);
         m_ref = rmax;
@@ -734,17 +803,26 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
           tmem_store_32cols(t_o + cc * 32, o);
         }
       }
-      if (j == n - 1 && (last_rows & 15) != 0) {
-        const int st = j % Cfg::kVStages;
-        // First O += P(j-2) V, the stage's last reader: its barrier is then in this tile's phase.
-        const int jv = j - Cfg::kVStages;
-        if (jv >= 0) softmax_wait(&o_done[jv % Cfg::kBufs], (jv / Cfg::kBufs) & 1, 132, alive, abort_flag);
-        softmax_wait(&v_full[st], (j / Cfg::kVStages) & 1, 131, alive, abort_flag);
-        window_clear_values<2>(s_v + st * Cfg::kTileBytes, last_rows, threadIdx.x - 64, 256);
+      if constexpr (decltype(hide)::value) {
+        if (j == n - 1 && (last_rows & 15) != 0) {
+          const int st = j % Cfg::kVStages;
+          // First O += P(j-2) V, the stage's last reader: its barrier is then in this tile's phase.
+          const int jv = j - Cfg::kVStages;
+          if (jv >= 0) softmax_wait(&o_done[jv % Cfg::kBufs], (jv / Cfg::kBufs) & 1, 132, alive, abort_flag);
+          softmax_wait(&v_full[st], (j / Cfg::kVStages) & 1, 131, alive, abort_flag);
+          window_clear_values<2>(s_v + st * Cfg::kTileBytes, last_rows, threadIdx.x - 64, 256);
+        }
       }
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[buf]);
+    };
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      if (tiles.open(j))
+        softmax_tile(j, std::false_type{});
+      else
+        softmax_tile(j, std::true_type{});
     }
 
     red[2 * 256 + half * 128 + r] = l_sum;

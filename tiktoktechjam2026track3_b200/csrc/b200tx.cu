@@ -109,12 +109,17 @@ int device_sm_count(int device) {
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 static bool is_sm100(int* major_out) {
+  static int cache[64] = {0};  // 10 * major + minor by device, as device_sm_count keeps its answer
   int dev = 0, major = 0, minor = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
-  cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
-  if (major_out) *major_out = major * 10 + minor;
-  return major == 10 && minor == 0;
+  int& c = cache[dev & 63];
+  if (c == 0) {
+    cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+    cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
+    c = major * 10 + minor;
+  }
+  if (major_out) *major_out = c;
+  return c == 100;
 }
 
 }  // namespace b2

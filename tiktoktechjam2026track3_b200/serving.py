@@ -190,6 +190,8 @@ class KVCache:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         if workspace is None:
             workspace = self._workspace(q, q_len)
+        elif workspace.dtype != torch.uint8 or not workspace.is_cuda or not workspace.is_contiguous():
+            raise ValueError("workspace must be a contiguous uint8 CUDA tensor (see KVCache.workspace)")
         _capi.cache_attention(self._desc, q, q_len, page_table, kv_len, window, sinks,
                               self.head_dim**-0.5 if scale is None else scale, out, workspace)
         return out
@@ -198,7 +200,7 @@ class KVCache:
         """The current stream's workspace, kept between calls (those of one stream run one after the other) and made
         anew when a call is larger than all before it."""
         need = (q.shape[0] // q_len, q.shape[1] // self.head_dim, q_len)
-        stream = torch.cuda.current_stream(q.device).cuda_stream
+        stream = _capi._stream_ptr(q.device)
         kept = self._workspaces.get(stream)
         if kept is not None and need[0] <= kept[0][0] and need[1] <= kept[0][1] and need[2] <= kept[0][2]:
             return kept[1]
