@@ -110,12 +110,13 @@ __device__ __forceinline__ RowKeys window_row(const WindowParams& p, int lo, int
 // that hide nothing.
 struct WindowTiles {
   int i0, lo, sink_rows, rows, count;
-  int open_a, open_c, open_d;  // tiles below open_d that lie from open_c on or below open_a hide no key from any row
+  int open_a, open_c, open_d;  // tiles below open_d that lie from open_c on or below open_a hide no key from these rows
   __device__ __forceinline__ bool open(int t) const { return t < open_d && (t >= open_c || t < open_a); }
   __device__ __forceinline__ RowKeys row(const WindowParams& p, int i) const { return window_row(p, lo, sink_rows, i); }
 };
 
-__device__ __forceinline__ WindowTiles window_tiles(const WindowParams& p, const KeyList& l) {
+// For the rows of tokens first ... last of the query tile.
+__device__ __forceinline__ WindowTiles window_tiles(const WindowParams& p, const KeyList& l, int first, int last) {
   WindowTiles t;
   t.i0 = l.i0;
   t.count = l.tiles;
@@ -123,8 +124,8 @@ __device__ __forceinline__ WindowTiles window_tiles(const WindowParams& p, const
   t.sink_rows = l.sink_rows;
   t.rows = l.rows;
   t.open_a = p.sinks >> 7;
-  t.open_c = (window_row(p, l.lo, l.sink_rows, l.i1 - 1).c + 127) >> 7;
-  t.open_d = (window_row(p, l.lo, l.sink_rows, l.i0).d + 1) >> 7;
+  t.open_c = (window_row(p, l.lo, l.sink_rows, last).c + 127) >> 7;
+  t.open_d = min(window_row(p, l.lo, l.sink_rows, first).d + 1, l.rows) >> 7;
   return t;
 }
 
@@ -238,7 +239,10 @@ __global__ void __launch_bounds__(192, 2)
   }
   const int n = keys.tiles;
   const int last_rows = keys.rows - 128 * (n - 1);  // of the last tile
-  if (threadIdx.x == 0) *s_tiles = window_tiles(p, keys);
+  if (warp >= 2 && lane == 0) {
+    const int r0 = (warp & 3) * 32;
+    s_tiles[warp & 3] = window_tiles(p, keys, keys.i0 + (r0 >> p.group_shift), keys.i0 + ((r0 + 31) >> p.group_shift));
+  }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
@@ -367,6 +371,7 @@ __global__ void __launch_bounds__(192, 2)
     }
   } else {
     // ---------------- softmax: one row per thread ----------------
+    s_tiles += warp & 3;
     const int r = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t t_s = t_lane;
@@ -392,16 +397,21 @@ __global__ void __launch_bounds__(192, 2)
           m_ref = rmax;
         }
       };
-      if (s_tiles->open(j)) {
-        // Every row sees all 128 places: the scores once into registers, S free for the next product meanwhile.
+      auto whole_tile = [&](auto hide) {
+        // The scores once into registers, S free for the next product meanwhile.
         float v[128];
         tmem_load_128cols(t_s, v);
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free);
+        if constexpr (decltype(hide)::value) {
+          const RowKeys row = s_tiles->row(p, s_tiles->i0 + (r >> p.group_shift));
+#pragma unroll
+          for (int g = 0; g < 4; ++g) window_hide(v + 32 * g, window_bits(row, 128 * j + 32 * g));
+        }
         new_reference(fmaxf(fmaxf(max32(v), max32(v + 32)), fmaxf(max32(v + 64), max32(v + 96))));
         const uint64_t c2 = splat2(c);
-        const uint64_t neg_mc2 = splat2(-m_ref * c);
+        const uint64_t neg_mc2 = splat2(decltype(hide)::value && m_ref == -INFINITY ? 0.f : -m_ref * c);
         uint64_t sum2 = 0;
         uint32_t w[64];
 #pragma unroll
@@ -422,6 +432,11 @@ __global__ void __launch_bounds__(192, 2)
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) tmem_store_16cols_async(t_p + 16 * g, w + 16 * g);
+      };
+      if (s_tiles->open(j)) {
+        whole_tile(std::false_type{});
+      } else if (s_tiles->rows - 128 * j > 96) {
+        whole_tile(std::true_type{});
       } else {
         // Some row does not see some place: 32 places at a time, as far as there are keys, the scores read twice (maximum,
         // then weights), so that the masks cost no registers that the other path needs.
@@ -733,7 +748,8 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
     float* red = reinterpret_cast<float*>(smem + Cfg::kOffRed);
     const uint32_t pair_bar = 1 + quad;
     const float c = p.scale_log2;
-    const WindowTiles tiles = window_tiles(p, keys);
+    const WindowTiles tiles = window_tiles(p, keys, keys.i0 + ((quad * 32) >> p.group_shift),
+                                           keys.i0 + ((quad * 32 + 31) >> p.group_shift));
     constexpr float kRescaleThreshold = 8.0f;
 
     float m_ref = -INFINITY;
