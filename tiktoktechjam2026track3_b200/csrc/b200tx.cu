@@ -493,7 +493,8 @@ static int cache_pages(const b2_kv_cache* c, const char* what, CachePages* out, 
     return fail(2, "%s: page_size=%lld must be 16, 32, 64, 128 or 256", what, (long long)c->page_size);
   if (c->head_dim % 16 != 0 || c->head_dim < 16 || c->head_dim > 256)
     return fail(2, "%s: head_dim=%lld must be a multiple of 16 up to 256", what, (long long)c->head_dim);
-  if (c->kv_heads > 16384 || c->pages > 0x7fffffffLL) return fail(2, "%s: cache too large", what);
+  if (c->kv_heads > 16384 || c->pages > 0x7fffffffLL || c->page_stride > (0x7fffffffLL >> 1))
+    return fail(2, "%s: cache too large", what);
   const int64_t head = c->page_size * c->head_dim;
   if (c->head_stride < head || c->page_stride < c->head_stride * (c->kv_heads - 1) + head)
     return fail(1, "%s: page_stride or head_stride too small", what);
@@ -608,10 +609,10 @@ B2_API int b2_cache_attention_fwd(const b2_kv_cache* cache, const void* q, int64
   if (!(scale > 0.f)) return fail(1, "b2_cache_attention_fwd: scale must be positive");
   if (ld_q < num_heads * hd || ld_out < num_heads * hd || ld_q % 8 != 0 || ld_out % 8 != 0)
     return fail(2, "b2_cache_attention_fwd: row strides must be multiples of 8 and at least num_heads * head_dim");
-  const int64_t units = (table_pages << p.c.page_shift) / (16 * kCacheWarps) + 1;
+  const int64_t units = (table_pages << p.c.page_shift) / 64 + 1;  // at most one for 64 tokens
   const int64_t rows = q_len * (num_heads / hk);
   // Token positions stay below 2^30, so that sums of a position and a window do not leave 32 bits.
-  if (batch > 16384 || q_len > 1024 || num_heads > 65536 || table_pages > ((int64_t{1} << 30) >> p.c.page_shift) ||
+  if (batch > kCacheMaxBatch || q_len > 1024 || num_heads > 65536 || table_pages > ((int64_t{1} << 30) >> p.c.page_shift) ||
       batch * hk > 0x7fffffffLL / units)
     return fail(2, "b2_cache_attention_fwd: problem too large");
   if (batch == 0) return 0;

@@ -46,12 +46,13 @@ struct CacheAttnParams {
   const int32_t* kv_len;
   int batch, q_len, group, window, sinks;
   float scale_log2;
-  int* counters;    // [row blocks][batch * kv_heads], zero between calls
+  int* counters;        // [row blocks][batch * kv_heads], zero between calls
+  int* group_counters;  // [row blocks][groups of CTAs][2], likewise
   float* partials;  // [row blocks][CTAs][2][rows][head_dim + 2]
 };
 
-constexpr int kCacheWarps = 8;
-constexpr int kCacheThreads = 32 * kCacheWarps;
+constexpr int kCacheMaxBatch = 4096;
+constexpr int kCacheGroup = 16;  // parts of a (sequence, head) that one CTA joins at once
 constexpr float kCacheRescale = 8.f;   // log2: the maximum moves when a score exceeds it by more
 constexpr float kCacheHeadroom = 7.f;  // log2: weights are at most 2^(8 + 7), below fp16's largest
 
@@ -79,10 +80,6 @@ __device__ __forceinline__ int seq_length(const CacheAttnParams& p, int b) {
   const int most = p.table_pages << p.c.page_shift;
   if (len < 0 || len > most) record_status(kKernelCacheAttention, 1, kReasonBadIndex);
   return min(max(len, 0), most);
-}
-
-__device__ __forceinline__ int seq_units(const CacheAttnParams& p, int b) {
-  return max(1, (seq_tiles(p, seq_length(p, b)).count + kCacheWarps - 1) / kCacheWarps);
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -164,20 +161,52 @@ struct CacheAttnCfg {
   static constexpr int kKWords = HD * kBytes / 16;  // of one token, per thread: 4 threads share a row of K,
   static constexpr int kVWords = HD * kBytes / 32;  // 8 a row of V
   static constexpr int kSteps = HD / 16;
-  static constexpr int kPartial = kRows * (HD + 2);  // floats of one partial result
-  static constexpr int kMergeFloats = kCacheWarps * kPartial;
+  // A warp takes kSub tiles of 16 tokens at a time, interleaved: 4 KB of keys and values on their way per warp.
+  static constexpr int kSub = 128 / (HD * kBytes * NT) > 1 ? 128 / (HD * kBytes * NT) : 1;
+  // Registers decide the warps: the loads' (32, or 64 for 256-byte rows), O's and Q's (6 per row block and 16 dims).
+  static constexpr bool kWide = HD == 128 && (!kFp8 || NT == 2);
+  static constexpr bool kSharedQ = NT == 2 || (HD == 128 && kFp8);
+  static constexpr int kCtasPerSm = kWide ? 2 : 4;
+  static constexpr int kWarps = kWide && (kFp8 || NT == 1) ? 6 : 4;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kLeast = 16 / kWarps;  // units of a CTA's stretch at least, where the call has fewer than fill it
+  static constexpr int kUnitTiles = kWarps * kSub;  // of 16 tokens: what a CTA takes at a time
+  // Twelve warps with 8 KB on their way each need no prefetch (183 us with it, 168 without: 32 x 8192 tokens, 8 heads).
+  static constexpr bool kPrefetch = !(kWide && !kFp8 && NT == 1);
+  static constexpr int kLines = kSub * 2 * 16 * HD * kBytes / 128;  // 128-byte lines of a warp's part of a unit
+  static constexpr int kPartial = kRows * (HD + 2);  // floats of one partial result: outputs, then maxima, then sums
+  // Shared memory: the join of the warps' results, or the factors of the join of CTAs; then (batch + 1) first units.
+  static constexpr int kSmemBytes = kWarps * kPartial * 4 > 24576 ? kWarps * kPartial * 4 : 24576;
 };
 
+// A stretch's part of one (sequence, head): units [u0, u1) of its `units`, the first of which is head_begin on the line.
+struct Part {
+  int b, h, head_begin, u0, u1, units;
+  SeqTiles seq;
+};
+
+template <class Cfg>
+__device__ __forceinline__ int seq_units(const CacheAttnParams& p, int b) {
+  return max(1, (seq_tiles(p, seq_length(p, b)).count + Cfg::kUnitTiles - 1) / Cfg::kUnitTiles);
+}
+
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 template <int HD, bool kFp8, int NT>
-__global__ void __launch_bounds__(kCacheThreads, NT == 1 ? 2 : 1) cache_attention_kernel(const CacheAttnParams p) {
+__global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT>::kThreads, CacheAttnCfg<HD, kFp8, NT>::kCtasPerSm)
+    cache_attention_kernel(const CacheAttnParams p) {
   using Cfg = CacheAttnCfg<HD, kFp8, NT>;
   using KPieces = RowPieces<Cfg::kKWords, 4>;
   using VPieces = RowPieces<Cfg::kVWords, 8>;
   constexpr int R = Cfg::kRows;
-  extern __shared__ float s_dyn[];
-  float* s_merge = s_dyn;                                            // [warps][R][HD + 2]
-  int* s_first = reinterpret_cast<int*>(s_dyn + Cfg::kMergeFloats);  // [batch + 1] first unit of each sequence
-  __shared__ int s_scan[kCacheWarps];
+  constexpr int kSub = Cfg::kSub;
+  constexpr int kWarps = Cfg::kWarps;
+  extern __shared__ __align__(16) uint8_t s_dyn[];
+  float* s_merge = reinterpret_cast<float*>(s_dyn);
+  int* s_first = reinterpret_cast<int*>(s_dyn + Cfg::kSmemBytes);  // [batch + 1] first unit of each sequence
+  __shared__ uint2 s_q[Cfg::kSharedQ ? NT * Cfg::kSteps * 32 : 1];
+  __shared__ int s_scan[kWarps];
+  __shared__ Part s_part;  // what the join needs of `now`, out of the registers of the loop
   __shared__ int s_last;
 
   const int tid = threadIdx.x;
@@ -194,9 +223,9 @@ __global__ void __launch_bounds__(kCacheThreads, NT == 1 ? 2 : 1) cache_attentio
 
   // First unit of each sequence on the line of all units.
   int base = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += kCacheThreads) {
+  for (int b0 = 0; b0 < p.batch; b0 += Cfg::kThreads) {
     const int b = b0 + tid;
-    int v = b < p.batch ? seq_units(p, b) * kv_heads : 0;
+    int v = b < p.batch ? seq_units<Cfg>(p, b) * kv_heads : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -207,7 +236,7 @@ __global__ void __launch_bounds__(kCacheThreads, NT == 1 ? 2 : 1) cache_attentio
     int before = base;
     int all = 0;
 #pragma unroll
-    for (int i = 0; i < kCacheWarps; ++i) {
+    for (int i = 0; i < kWarps; ++i) {
       if (i < warp) before += s_scan[i];
       all += s_scan[i];
     }
@@ -218,32 +247,85 @@ __global__ void __launch_bounds__(kCacheThreads, NT == 1 ? 2 : 1) cache_attentio
   if (tid == 0) s_first[0] = 0;
   __syncthreads();
   const int64_t total = base;
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);
+  const int64_t ctas = min(static_cast<int64_t>(gridDim.x),
+                           max(static_cast<int64_t>(p.batch) * kv_heads, (total + Cfg::kLeast - 1) / Cfg::kLeast));
   const int64_t cta = blockIdx.x;
   if (cta >= ctas) return;
   const int w_begin = static_cast<int>(cta * total / ctas);
   const int w_end = static_cast<int>((cta + 1) * total / ctas);
 
-  int b = 0;
-  {
-    int hi = p.batch;  // s_first[b] <= w_begin < s_first[hi]
-    while (hi - b > 1) {
-      const int mid = (b + hi) >> 1;
-      if (s_first[mid] <= w_begin) b = mid; else hi = mid;
-    }
-  }
+  constexpr int kNoTile = 1 << 30;         // a first token that no row sees
+  constexpr int kIds = 32 / kSub;          // units whose page numbers the lanes hold
+  constexpr int kAhead = kIds > 4 ? 3 : 2;  // units that the prefetch into L2 runs ahead
+  const int page_bytes = static_cast<int>(p.c.page_stride) * Cfg::kBytes;  // below 2^31 (checked by the host)
+  const int slot_mask = (1 << p.c.page_shift) - 1;
 
-  for (int w = w_begin; w < w_end;) {
+  auto part_from = [&](int w, int b) {
+    Part x;
     while (s_first[b + 1] <= w) ++b;
-    const SeqTiles seq = seq_tiles(p, seq_length(p, b));
-    const int units = (s_first[b + 1] - s_first[b]) / kv_heads;
-    const int h = (w - s_first[b]) / units;
-    const int head_begin = s_first[b] + h * units;  // of the line
-    const int u0 = w - head_begin;
-    const int u1 = min(units, w_end - head_begin);
+    x.b = b;
+    x.seq = seq_tiles(p, seq_length(p, b));
+    x.units = (s_first[b + 1] - s_first[b]) / kv_heads;
+    x.h = (w - s_first[b]) / x.units;
+    x.head_begin = s_first[b] + x.h * x.units;
+    x.u0 = w - x.head_begin;
+    x.u1 = min(x.units, w_end - x.head_begin);
+    return x;
+  };
+  // Lane l: the first token (kNoTile: none) and the page of this warp's tile l % kSub in unit ids_from + l / kSub.
+  int my_tok = kNoTile, my_page = 0, ids_from = 0;
+  auto read_ids = [&](const Part& x, int u) {
+    ids_from = u;
+    const int i = ((u + lane / kSub) * kWarps + warp) * kSub + lane % kSub;
+    my_tok = kNoTile;
+    my_page = 0;
+    if (i < x.seq.count) {
+      my_tok = 16 * (i < x.seq.sink_tiles ? i : i - x.seq.sink_tiles + x.seq.first_win);
+      my_page = p.page_table[x.b * p.ld_table + (my_tok >> p.c.page_shift)];
+      if (my_page < 0 || my_page >= p.c.pages) {
+        record_status(kKernelCacheAttention, 2, kReasonBadIndex);
+        my_tok = kNoTile;
+        my_page = 0;
+      }
+    }
+  };
+  // The lines of the warp's part of unit u into L2, a lane each.
+  auto prefetch = [&](const Part& x, int u) {
+    constexpr int kTileLines = Cfg::kLines / kSub;  // K's, then V's
+#pragma unroll
+    for (int line0 = 0; line0 < Cfg::kLines; line0 += 32) {
+      const int line = line0 + lane;
+      const int src = min((u - ids_from) * kSub + line / kTileLines, 31);
+      const int tok = __shfl_sync(0xffffffffu, my_tok, src);
+      const int page = __shfl_sync(0xffffffffu, my_page, src);
+      const int in = line % kTileLines;
+      const bool keys = in < kTileLines / 2;
+      if (u < x.u1 && (Cfg::kLines % 32 == 0 || line < Cfg::kLines) && tok != kNoTile)
+        prefetch_l2((keys ? p.c.k : p.c.v) + static_cast<int64_t>(page) * page_bytes + x.h * p.c.head_stride * Cfg::kBytes +
+                    (tok & slot_mask) * (HD * Cfg::kBytes) + (keys ? in : in - kTileLines / 2) * 128);
+    }
+  };
+  Part now;
+  {
+    int lo = 0, hi = p.batch;  // s_first[lo] <= w_begin < s_first[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_first[mid] <= w_begin) lo = mid; else hi = mid;
+    }
+    now = part_from(w_begin, lo);
+  }
+  while (true) {
+    read_ids(now, now.u0);
+    if (Cfg::kPrefetch) {
+#pragma unroll
+      for (int d = 0; d < kAhead; ++d) prefetch(now, now.u0 + d);
+    }
+    if (tid == 0) s_part = now;
+    const SeqTiles seq = now.seq;
+    const int64_t head_bytes = now.h * p.c.head_stride * Cfg::kBytes;
 
     // Q: fragments of the 8-row operand(s), and the factor of its rows' scores.
-    uint32_t qf[NT][Cfg::kSteps][2];
+    uint32_t qf[NT][Cfg::kSteps][2];  // (in shared memory where registers are short: it is alike for every warp)
     float row_scale[NT][2];
     int limit[NT][2];  // position of the rows 2t, 2t + 1 of each operand, -1: no such row
 #pragma unroll
@@ -251,8 +333,8 @@ __global__ void __launch_bounds__(kCacheThreads, NT == 1 ? 2 : 1) cache_attentio
       const int row = row_block + 8 * nt + g;
       const bool real = row < rows_total;
       const __nv_bfloat16* src =
-          p.q + (static_cast<int64_t>(b) * p.q_len + (real ? row / p.group : 0)) * p.ld_q +
-          (h * p.group + (real ? row % p.group : 0)) * HD;
+          p.q + (static_cast<int64_t>(now.b) * p.q_len + (real ? row / p.group : 0)) * p.ld_q +
+          (now.h * p.group + (real ? row % p.group : 0)) * HD;
       if constexpr (kFp8) {
         float f[Cfg::kSteps][4];
         float amax = 0.f;
@@ -294,6 +376,17 @@ __global__ void __launch_bounds__(kCacheThreads, NT == 1 ? 2 : 1) cache_attentio
       }
     }
 
+    if constexpr (Cfg::kSharedQ) {
+      if (warp == 0) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int st = 0; st < Cfg::kSteps; ++st)
+            s_q[(nt * Cfg::kSteps + st) * 32 + lane] = make_uint2(qf[nt][st][0], qf[nt][st][1]);
+      }
+      __syncthreads();
+    }
+
     float o[NT][Cfg::kSteps][4];
     float m[NT][2], l[NT][2];
 #pragma unroll
@@ -306,104 +399,131 @@ __global__ void __launch_bounds__(kCacheThreads, NT == 1 ? 2 : 1) cache_attentio
         for (int i = 0; i < 4; ++i) o[nt][j][i] = 0.f;
     }
 
-    const uint8_t* k_head = p.c.k + h * p.c.head_stride * Cfg::kBytes;
-    const uint8_t* v_head = p.c.v + h * p.c.head_stride * Cfg::kBytes;
-    const int32_t* pages = p.page_table + b * p.ld_table;
     // Tokens that every row sees lie below `all_see`, and (with a window) from `all_from` on or below the sinks.
     const int all_see = seq.len - p.q_len + 1;
     const int all_from = p.window > 0 ? max(0, seq.len - p.window) : 0;
 
-    for (int u = u0; u < u1; ++u) {
-      const int i = u * kCacheWarps + warp;
-      if (i >= seq.count) break;
-      const int tok0 = 16 * (i < seq.sink_tiles ? i : i - seq.sink_tiles + seq.first_win);
-      const int page = pages[tok0 >> p.c.page_shift];
-      if (page < 0 || page >= p.c.pages) {
-        record_status(kKernelCacheAttention, 2, kReasonBadIndex);
-        continue;
-      }
-      const int slot0 = tok0 & ((1 << p.c.page_shift) - 1);
-      const int64_t at = (page * p.c.page_stride + slot0 * HD) * Cfg::kBytes;
-      uint32_t kr[2][Cfg::kKWords], vr[4][Cfg::kVWords];
+#pragma unroll 1
+    for (int u = now.u0; u < now.u1; ++u) {
+      if ((u * kWarps + warp) * kSub >= seq.count) break;
+      if (u + kAhead >= ids_from + kIds && ids_from + kIds < now.u1) read_ids(now, u);
+      uint32_t kr[kSub][2][Cfg::kKWords], vr[kSub][4][Cfg::kVWords];
+      float ks[kSub], vs[kSub];
+      int tok[kSub];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) KPieces::load(k_head + at + (g + 8 * x) * (HD * Cfg::kBytes), t, kr[x]);
+      for (int c = 0; c < kSub; ++c) {
+        const int src = (u - ids_from) * kSub + c;
+        tok[c] = __shfl_sync(0xffffffffu, my_tok, src);
+        const int page = __shfl_sync(0xffffffffu, my_page, src);
+        // (a tile that is missing reads page 0, slot 0, and is masked)
+        const int64_t at = static_cast<int64_t>(page) * page_bytes + head_bytes + (tok[c] & slot_mask) * (HD * Cfg::kBytes);
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        VPieces::load(v_head + at + (2 * t + (x & 1) + 4 * (x & 2)) * (HD * Cfg::kBytes), g, vr[x]);
-      float k_scale = 1.f, ev = 0.f, inv_v = 1.f;
-      if (kFp8) {
-        k_scale = __ldg(p.c.k_scale + static_cast<int64_t>(page) * kv_heads + h);
-        const float vs = __ldg(p.c.v_scale + static_cast<int64_t>(page) * kv_heads + h);
-        ev = static_cast<float>(static_cast<int>(__float_as_uint(vs) >> 23) - 127);
-        inv_v = exp2_int(-static_cast<int>(ev));
-      }
-
-      float s[NT][4];
+        for (int x = 0; x < 2; ++x) KPieces::load(p.c.k + at + (g + 8 * x) * (HD * Cfg::kBytes), t, kr[c][x]);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-      for (int st = 0; st < Cfg::kSteps; ++st) {
-        uint32_t a0, a1, a2, a3;
-        if constexpr (kFp8) {
-          a0 = e4m3x2_to_f16x2(kr[0][st]);
-          a1 = e4m3x2_to_f16x2(kr[1][st]);
-          a2 = e4m3x2_to_f16x2(kr[0][st] >> 16);
-          a3 = e4m3x2_to_f16x2(kr[1][st] >> 16);
-        } else {
-          a0 = kr[0][2 * st];
-          a1 = kr[1][2 * st];
-          a2 = kr[0][2 * st + 1];
-          a3 = kr[1][2 * st + 1];
+        for (int x = 0; x < 4; ++x)
+          VPieces::load(p.c.v + at + (2 * t + (x & 1) + 4 * (x & 2)) * (HD * Cfg::kBytes), g, vr[c][x]);
+        ks[c] = vs[c] = 1.f;
+        if (kFp8) {
+          ks[c] = __ldg(p.c.k_scale + static_cast<int64_t>(page) * kv_heads + now.h);
+          vs[c] = __ldg(p.c.v_scale + static_cast<int64_t>(page) * kv_heads + now.h);
         }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) cache_mma<kFp8>(s[nt], a0, a1, a2, a3, qf[nt][st][0], qf[nt][st][1]);
       }
+      if (Cfg::kPrefetch) prefetch(now, u + kAhead);
+
+      float s[kSub][NT][4];
+#pragma unroll
+      for (int c = 0; c < kSub; ++c)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[c][nt][0] = s[c][nt][1] = s[c][nt][2] = s[c][nt][3] = 0.f;
+#pragma unroll
+      for (int st = 0; st < Cfg::kSteps; ++st)
+#pragma unroll
+        for (int c = 0; c < kSub; ++c) {
+          uint32_t a0, a1, a2, a3;
+          if constexpr (kFp8) {
+            a0 = e4m3x2_to_f16x2(kr[c][0][st]);
+            a1 = e4m3x2_to_f16x2(kr[c][1][st]);
+            a2 = e4m3x2_to_f16x2(kr[c][0][st] >> 16);
+            a3 = e4m3x2_to_f16x2(kr[c][1][st] >> 16);
+          } else {
+            a0 = kr[c][0][2 * st];
+            a1 = kr[c][1][2 * st];
+            a2 = kr[c][0][2 * st + 1];
+            a3 = kr[c][1][2 * st + 1];
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            uint2 q2 = make_uint2(qf[nt][st][0], qf[nt][st][1]);
+            if constexpr (Cfg::kSharedQ) q2 = s_q[(nt * Cfg::kSteps + st) * 32 + lane];
+            cache_mma<kFp8>(s[c][nt], a0, a1, a2, a3, q2.x, q2.y);
+          }
+        }
 
       // Tokens g and g + 8 of rows 2t and 2t + 1, in exponents of 2 with V's scale in.
+      float inv_v[kSub];
+      bool edge = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) s[nt][x] = fmaf(s[nt][x], row_scale[nt][x & 1] * k_scale, ev);
-      const bool edge = tok0 + 16 > all_see || (tok0 < all_from && tok0 + 16 > p.sinks);
-      if (edge) {
+      for (int c = 0; c < kSub; ++c) {
+        float ev = 0.f;
+        inv_v[c] = 1.f;
+        if (kFp8) {
+          const int e = static_cast<int>(__float_as_uint(vs[c]) >> 23) - 127;
+          ev = static_cast<float>(e);
+          inv_v[c] = exp2_int(-e);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int j = tok0 + g + 8 * (x >> 1);
-            const int pos = limit[nt][x & 1];
-            if (j > pos || (p.window > 0 && pos - j >= p.window && j >= p.sinks)) s[nt][x] = -INFINITY;
-          }
-        // Values of tokens that no row sees may be anything (0 times a NaN is a NaN).
-        const int see = seq.len;
+          for (int x = 0; x < 4; ++x) s[c][nt][x] = fmaf(s[c][nt][x], row_scale[nt][x & 1] * ks[c], ev);
+        edge |= tok[c] + 16 > all_see || (tok[c] < all_from && tok[c] + 16 > p.sinks);
+      }
+      if (edge) {
         const int from = max(0, seq.len - p.q_len - p.window + 1);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int j = tok0 + 2 * t + (x & 1) + 4 * (x & 2);
-          if (j >= see || (p.window > 0 && j < from && j >= p.sinks)) {
+        for (int c = 0; c < kSub; ++c) {
 #pragma unroll
-            for (int i2 = 0; i2 < Cfg::kVWords; ++i2) vr[x][i2] = 0u;
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int j = tok[c] + g + 8 * (x >> 1);
+              const int pos = limit[nt][x & 1];
+              if (j > pos || (p.window > 0 && pos - j >= p.window && j >= p.sinks)) s[c][nt][x] = -INFINITY;
+            }
+          // Values of tokens that no row sees may be anything (0 times a NaN is a NaN).
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int j = tok[c] + 2 * t + (x & 1) + 4 * (x & 2);
+            if (j >= seq.len || (p.window > 0 && j < from && j >= p.sinks)) {
+#pragma unroll
+              for (int i2 = 0; i2 < Cfg::kVWords; ++i2) vr[c][x][i2] = 0u;
+            }
           }
         }
       }
 
       bool grew = false;
+      float top[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) grew |= fmaxf(s[nt][x], s[nt][x + 2]) > m[nt][x] + kCacheRescale;
+        for (int x = 0; x < 2; ++x) {
+          top[nt][x] = fmaxf(s[0][nt][x], s[0][nt][x + 2]);
+#pragma unroll
+          for (int c = 1; c < kSub; ++c) top[nt][x] = max3f(top[nt][x], s[c][nt][x], s[c][nt][x + 2]);
+          grew |= top[nt][x] > m[nt][x] + kCacheRescale;
+        }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            float top = fmaxf(s[nt][x], s[nt][x + 2]);
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            if (top > m[nt][x]) {
-              const float alpha = fast_exp2(m[nt][x] - top);  // 0 the first time
-              m[nt][x] = top;
+            float best = top[nt][x];
+            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
+            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 8));
+            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
+            if (best > m[nt][x]) {
+              const float alpha = fast_exp2(m[nt][x] - best);  // 0 the first time
+              m[nt][x] = best;
               l[nt][x] *= alpha;
 #pragma unroll
               for (int j = 0; j < Cfg::kSteps; ++j) {
@@ -414,52 +534,54 @@ __global__ void __launch_bounds__(kCacheThreads, NT == 1 ? 2 : 1) cache_attentio
           }
       }
 
-      uint32_t pf[NT][2];
+      uint32_t pf[kSub][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float w4[4];
+        const float ref0 = m[nt][0] == -INFINITY ? -kCacheHeadroom : m[nt][0] - kCacheHeadroom;
+        const float ref1 = m[nt][1] == -INFINITY ? -kCacheHeadroom : m[nt][1] - kCacheHeadroom;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float ref = m[nt][x & 1] == -INFINITY ? 0.f : m[nt][x & 1];
-          w4[x] = fast_exp2(s[nt][x] - ref + kCacheHeadroom);
+        for (int c = 0; c < kSub; ++c) {
+          const float w0 = fast_exp2(s[c][nt][0] - ref0), w1 = fast_exp2(s[c][nt][1] - ref1);
+          const float w2 = fast_exp2(s[c][nt][2] - ref0), w3 = fast_exp2(s[c][nt][3] - ref1);
+          l[nt][0] = fmaf(w0 + w2, inv_v[c], l[nt][0]);
+          l[nt][1] = fmaf(w1 + w3, inv_v[c], l[nt][1]);
+          pf[c][nt][0] = movmatrix_trans(kFp8 ? pack_f16x2(w0, w1) : pack_bf16x2(w0, w1));
+          pf[c][nt][1] = movmatrix_trans(kFp8 ? pack_f16x2(w2, w3) : pack_bf16x2(w2, w3));
         }
-        l[nt][0] = fmaf(w4[0] + w4[2], inv_v, l[nt][0]);
-        l[nt][1] = fmaf(w4[1] + w4[3], inv_v, l[nt][1]);
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          pf[nt][x] = movmatrix_trans(kFp8 ? pack_f16x2(w4[2 * x], w4[2 * x + 1])
-                                           : pack_bf16x2(w4[2 * x], w4[2 * x + 1]));
       }
 
-      if constexpr (kFp8) {
 #pragma unroll
-        for (int i2 = 0; i2 < Cfg::kVWords; ++i2) {
+      for (int c = 0; c < kSub; ++c) {
+        if constexpr (kFp8) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t sel = half ? 0x7362u : 0x5140u;
-            const uint32_t lo = __byte_perm(vr[0][i2], vr[1][i2], sel);  // tokens 2t, 2t+1 of two dims
-            const uint32_t hi = __byte_perm(vr[2][i2], vr[3][i2], sel);  // tokens 2t+8, 2t+9
-            const uint32_t a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_to_f16x2(lo >> 16);
-            const uint32_t a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_to_f16x2(hi >> 16);
+          for (int i2 = 0; i2 < Cfg::kVWords; ++i2) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              cache_mma<kFp8>(o[nt][2 * i2 + half], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t sel = half ? 0x7362u : 0x5140u;
+              const uint32_t lo = __byte_perm(vr[c][0][i2], vr[c][1][i2], sel);  // tokens 2t, 2t+1 of two dims
+              const uint32_t hi = __byte_perm(vr[c][2][i2], vr[c][3][i2], sel);  // tokens 2t+8, 2t+9
+              const uint32_t a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_to_f16x2(lo >> 16);
+              const uint32_t a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_to_f16x2(hi >> 16);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                cache_mma<kFp8>(o[nt][2 * i2 + half], a0, a1, a2, a3, pf[c][nt][0], pf[c][nt][1]);
+            }
           }
-        }
-      } else {
+        } else {
 #pragma unroll
-        for (int i2 = 0; i2 < Cfg::kVWords; ++i2) {
-          const uint32_t a0 = __byte_perm(vr[0][i2], vr[1][i2], 0x5410u);
-          const uint32_t a1 = __byte_perm(vr[0][i2], vr[1][i2], 0x7632u);
-          const uint32_t a2 = __byte_perm(vr[2][i2], vr[3][i2], 0x5410u);
-          const uint32_t a3 = __byte_perm(vr[2][i2], vr[3][i2], 0x7632u);
+          for (int i2 = 0; i2 < Cfg::kVWords; ++i2) {
+            const uint32_t a0 = __byte_perm(vr[c][0][i2], vr[c][1][i2], 0x5410u);
+            const uint32_t a1 = __byte_perm(vr[c][0][i2], vr[c][1][i2], 0x7632u);
+            const uint32_t a2 = __byte_perm(vr[c][2][i2], vr[c][3][i2], 0x5410u);
+            const uint32_t a3 = __byte_perm(vr[c][2][i2], vr[c][3][i2], 0x7632u);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) cache_mma<kFp8>(o[nt][i2], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
+            for (int nt = 0; nt < NT; ++nt) cache_mma<kFp8>(o[nt][i2], a0, a1, a2, a3, pf[c][nt][0], pf[c][nt][1]);
+          }
         }
       }
     }
 
-    // The warps' results into shared memory, [warp][row][dims, maximum, sum].
+    // The warps' results into shared memory, each [row][dim], maxima, sums.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -467,87 +589,164 @@ __global__ void __launch_bounds__(kCacheThreads, NT == 1 ? 2 : 1) cache_attentio
         l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], 4);
         l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], 8);
         l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], 16);
-        float* dst = s_merge + (warp * R + 8 * nt + 2 * t + x) * (HD + 2);
+        const int r = 8 * nt + 2 * t + x;
+        float* dst = s_merge + warp * Cfg::kPartial;
 #pragma unroll
-        for (int j = 0; j < Cfg::kSteps; ++j)
-#pragma unroll
-          for (int hi = 0; hi < 2; ++hi) {
-            const int d = kFp8 ? VPieces::offset(j / 2, g) + 2 * (j & 1) + hi : VPieces::offset(j, g) / 2 + hi;
-            dst[d] = o[nt][j][x + 2 * hi];
-          }
+        for (int j = 0; j < Cfg::kSteps; ++j) {
+          const int d = kFp8 ? VPieces::offset(j / 2, g) + 2 * (j & 1) : VPieces::offset(j, g) / 2;
+          *reinterpret_cast<float2*>(dst + r * HD + d) = make_float2(o[nt][j][x], o[nt][j][x + 2]);
+        }
         if (g == 0) {
-          dst[HD] = m[nt][x];
-          dst[HD + 1] = l[nt][x];
+          dst[R * HD + r] = m[nt][x];
+          dst[R * HD + R + r] = l[nt][x];
         }
       }
     __syncthreads();
 
-    // Join `count` results of the rows, in order; into the output or a partial result.
+    const volatile Part& part_now = s_part;
+    const int b = part_now.b, h = part_now.h, head_begin = part_now.head_begin, units = part_now.units;
+    const int u0 = part_now.u0, u1 = part_now.u1;
+    // One row's output, joined: into `out` as bf16, or with its maximum and sum into a partial result.
     const int rows = min(R, rows_total - row_block);
-    auto join = [&](const float* from, auto read, int64_t count, auto slot_of, float* partial) {
-      for (int i = tid; i < rows * HD; i += kCacheThreads) {
-        const int r = i / HD, d = i - r * HD;
-        float top = -INFINITY;
-        for (int64_t k = 0; k < count; ++k) top = fmaxf(top, read(from + slot_of(k) * Cfg::kPartial + r * (HD + 2) + HD));
-        const float ref = top == -INFINITY ? 0.f : top;
-        float acc = 0.f, sum = 0.f;
-        for (int64_t k = 0; k < count; ++k) {
-          const float* one = from + slot_of(k) * Cfg::kPartial + r * (HD + 2);
-          const float f = fast_exp2(read(one + HD) - ref);
-          acc = fmaf(read(one + d), f, acc);
-          sum = fmaf(read(one + HD + 1), f, sum);
-        }
-        if (partial != nullptr) {
-          partial[r * (HD + 2) + d] = acc;
-          if (d == 0) {
-            partial[r * (HD + 2) + HD] = top;
-            partial[r * (HD + 2) + HD + 1] = sum;
-          }
-        } else {
-          const int row = row_block + r;
-          // sum is 0 only where nothing is visible; a NaN stays one.
-          p.out[(static_cast<int64_t>(b) * p.q_len + row / p.group) * p.ld_out + (h * p.group + row % p.group) * HD + d] =
-              __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);
-        }
-      }
+    auto finish = [&](int r, int d, float2 acc, float sum) {
+      const int row = row_block + r;
+      // sum is 0 only where nothing is visible; a NaN stays one.
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      if (sum == 0.f) acc = make_float2(0.f, 0.f);
+      *reinterpret_cast<uint32_t*>(
+          p.out + (static_cast<int64_t>(b) * p.q_len + row / p.group) * p.ld_out + (h * p.group + row % p.group) * HD + d) =
+          pack_bf16x2(acc.x * inv, acc.y * inv);
     };
-    auto same = [](int64_t k) { return k; };
-    auto shared = [](const float* x) { return *x; };
-    auto other = [](const float* x) { return __ldcg(x); };  // another SM's: not from this one's L1
-    if (u1 - u0 == units) {
-      join(s_merge, shared, kCacheWarps, same, nullptr);
-    } else {
-      float* mine = p.partials + static_cast<int64_t>(blockIdx.y) * gridDim.x * 2 * Cfg::kPartial;
-      const int64_t c_first = ((head_begin + 1) * ctas - 1) / total;
-      const int64_t c_last = (static_cast<int64_t>(head_begin + units) * ctas - 1) / total;
-      // Slot 0 of a CTA: the stretch's part of a head that began before it (or with it); slot 1: of one that begins inside.
-      join(s_merge, shared, kCacheWarps, same,
-           mine + (cta * 2 + (w_begin >= head_begin ? 0 : 1)) * Cfg::kPartial);
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        int* counter = p.counters + static_cast<int64_t>(blockIdx.y) * p.batch * kv_heads + b * kv_heads + h;
-        const int last = atomicAdd(counter, 1) == static_cast<int>(c_last - c_first);
-        if (last) *counter = 0;
-        s_last = last;
+    const bool whole = u1 - u0 == units;
+    const int64_t mine = static_cast<int64_t>(blockIdx.y) * gridDim.x * 2;
+    // Slot 0 of a CTA: the part of a head that began before its stretch (or with it); slot 1: of one that begins inside.
+    float* partial = p.partials + (mine + cta * 2 + (w_begin >= head_begin ? 0 : 1)) * Cfg::kPartial;
+    for (int i = tid; i < rows * (HD / 2); i += Cfg::kThreads) {
+      const int r = i / (HD / 2), d = 2 * (i - r * (HD / 2));
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) top = fmaxf(top, s_merge[k * Cfg::kPartial + R * HD + r]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float2 acc = make_float2(0.f, 0.f);
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float* one = s_merge + k * Cfg::kPartial;
+        const float f = fast_exp2(one[R * HD + r] - ref);
+        const float2 v = *reinterpret_cast<const float2*>(one + r * HD + d);
+        acc.x = fmaf(v.x, f, acc.x);
+        acc.y = fmaf(v.y, f, acc.y);
+        sum = fmaf(one[R * HD + R + r], f, sum);
       }
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        auto slot = [&](int64_t k) {
-          const int64_t c = c_first + k;
-          return c * 2 + (c * total / ctas >= head_begin ? 0 : 1);
-        };
-        join(mine, other, c_last - c_first + 1, slot, nullptr);
+      if (whole) {
+        finish(r, d, acc, sum);
+      } else {
+        *reinterpret_cast<float2*>(partial + r * HD + d) = acc;
+        if (d == 0) {
+          partial[R * HD + r] = top;
+          partial[R * HD + R + r] = sum;
+        }
       }
     }
+    if (!whole) {
+      // Joins of CTAs' parts, in their order on the line. Up to kCacheGroup parts at once; more (few sequences with few
+      // key heads) first in groups of kCacheGroup CTAs, whose result takes the place of its first part.
+      const int64_t c_first = ((static_cast<int64_t>(head_begin) + 1) * ctas - 1) / total;
+      const int64_t c_last = (static_cast<int64_t>(head_begin + units) * ctas - 1) / total;
+      auto part = [&](int64_t c) {
+        return p.partials + (mine + c * 2 + (c * total / ctas >= head_begin ? 0 : 1)) * Cfg::kPartial;
+      };
+      // True (in every thread) for the last of n arrivals; all their writes are then visible past this SM's L1.
+      auto last_of = [&](int* counter, int n) {
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+          const int last = atomicAdd(counter, 1) == n - 1;
+          if (last) *counter = 0;
+          s_last = last;
+        }
+        __syncthreads();
+        const bool last = s_last != 0;
+        if (last) __threadfence();
+        return last;
+      };
+      // Parts of the CTAs c_from(k), k < n <= kCacheGroup (+ 3 groups' results).
+      auto join = [&](auto c_from, int n, float* into) {
+        const float** s_at = reinterpret_cast<const float**>(s_merge);  // [n]
+        float* s_f = reinterpret_cast<float*>(s_at + n);                // [n][R] maxima, then factors
+        float* s_l = s_f + n * R;                                       // [n][R] sums
+        float* s_row = s_l + n * R;                                     // [2][R] joined sums and maxima
+        if (tid < n) s_at[tid] = part(c_from(tid));
+        __syncthreads();
+        for (int i = tid; i < n * 2 * R; i += Cfg::kThreads) {
+          const int k = i / (2 * R), x = i - k * 2 * R;
+          (x < R ? s_f + k * R + x : s_l + k * R + x - R)[0] = __ldcg(s_at[k] + R * HD + x);
+        }
+        __syncthreads();
+        if (tid < rows) {
+          float top = -INFINITY;
+          for (int k = 0; k < n; ++k) top = fmaxf(top, s_f[k * R + tid]);
+          const float ref = top == -INFINITY ? 0.f : top;
+          float sum = 0.f;
+          for (int k = 0; k < n; ++k) {
+            const float f = fast_exp2(s_f[k * R + tid] - ref);
+            s_f[k * R + tid] = f;
+            sum = fmaf(s_l[k * R + tid], f, sum);
+          }
+          s_row[tid] = sum;
+          s_row[R + tid] = top;
+        }
+        __syncthreads();
+        for (int i = tid; i < rows * (HD / 2); i += Cfg::kThreads) {
+          const int r = i / (HD / 2), d = 2 * (i - r * (HD / 2));
+          float2 acc = make_float2(0.f, 0.f);
+#pragma unroll 8
+          for (int k = 0; k < n; ++k) {
+            const float2 v = __ldcg(reinterpret_cast<const float2*>(s_at[k] + r * HD + d));
+            const float f = s_f[k * R + r];
+            acc.x = fmaf(v.x, f, acc.x);
+            acc.y = fmaf(v.y, f, acc.y);
+          }
+          if (into == nullptr) {
+            finish(r, d, acc, s_row[r]);
+          } else {
+            *reinterpret_cast<float2*>(into + r * HD + d) = acc;
+            if (d == 0) {
+              into[R * HD + r] = s_row[R + r];
+              into[R * HD + R + r] = s_row[r];
+            }
+          }
+        }
+        __syncthreads();
+      };
+      const int n = static_cast<int>(c_last - c_first) + 1;
+      int* head_counter = p.counters + static_cast<int64_t>(blockIdx.y) * p.batch * kv_heads + b * kv_heads + h;
+      if (n <= kCacheGroup) {
+        if (last_of(head_counter, n)) join([&](int k) { return c_first + k; }, n, nullptr);
+      } else {
+        const int64_t group = cta / kCacheGroup;
+        const int64_t g_first = max(c_first, group * kCacheGroup), g_last = min(c_last, group * kCacheGroup + kCacheGroup - 1);
+        // Of the heads that cross a border of the group, one crosses its first (or both), one only its last.
+        int* group_counter = p.group_counters + ((static_cast<int64_t>(blockIdx.y) * gridDim.x / kCacheGroup + blockIdx.y + group) * 2 +
+                                                 (c_first < group * kCacheGroup ? 0 : 1));
+        const int members = static_cast<int>(g_last - g_first) + 1;
+        const int64_t groups_from = c_first / kCacheGroup;
+        const int groups = static_cast<int>(c_last / kCacheGroup - groups_from) + 1;
+        if (last_of(group_counter, members)) {
+          join([&](int k) { return g_first + k; }, members, part(g_first));
+          if (last_of(head_counter, groups))
+            join([&](int k) { return max(c_first, (groups_from + k) * kCacheGroup); }, groups, nullptr);
+        }
+      }
+    }
+    if (head_begin + u1 >= w_end) break;
     __syncthreads();
-    w = head_begin + u1;
+    now = part_from(head_begin + u1, b);
   }
 }
 
 // CTAs of a launch, and the bytes of its workspace.
-static int cache_attention_ctas(int sm_count) { return 2 * sm_count; }
+static int cache_attention_ctas(int sm_count) { return 4 * sm_count; }
 
 // Rows of a block: 8, or 16 where there are more than 8 rows (a block reads the keys and values anew).
 static int64_t cache_attention_row_blocks(int64_t rows, int* nt) {
@@ -559,6 +758,10 @@ static int64_t cache_attention_counter_bytes(int64_t batch, int64_t kv_heads, in
   return (batch * kv_heads * row_blocks * 4 + 255) / 256 * 256;
 }
 
+static int64_t cache_attention_group_bytes(int64_t row_blocks, int sm_count) {
+  return (row_blocks * (cache_attention_ctas(sm_count) / kCacheGroup + 1) * 8 + 255) / 256 * 256;
+}
+
 static int64_t cache_attention_partial_bytes(int64_t head_dim, int64_t rows, int sm_count) {
   int nt = 1;
   const int64_t blocks = cache_attention_row_blocks(rows, &nt);
@@ -568,23 +771,25 @@ static int64_t cache_attention_partial_bytes(int64_t head_dim, int64_t rows, int
 static int64_t cache_attention_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t rows,
                                                int sm_count) {
   int nt = 1;
-  return cache_attention_counter_bytes(batch, kv_heads, cache_attention_row_blocks(rows, &nt)) +
+  const int64_t blocks = cache_attention_row_blocks(rows, &nt);
+  return cache_attention_group_bytes(blocks, sm_count) + cache_attention_counter_bytes(batch, kv_heads, blocks) +
          cache_attention_partial_bytes(head_dim, rows, sm_count);
 }
 
 template <int HD, bool kFp8, int NT>
 static cudaError_t launch_cache_attention_t(const CacheAttnParams& p, dim3 grid, cudaStream_t stream) {
   using Cfg = CacheAttnCfg<HD, kFp8, NT>;
-  const size_t smem = Cfg::kMergeFloats * 4 + (static_cast<size_t>(p.batch) + 1) * 4;
+  grid.x = grid.x / 4 * Cfg::kCtasPerSm;
+  const size_t smem = Cfg::kSmemBytes + (static_cast<size_t>(p.batch) + 1) * 4;
   static std::once_flag once[64];
   int dev = 0;
   cudaGetDevice(&dev);
   cudaError_t e = cudaSuccess;
   std::call_once(once[dev & 63], [&] {
-    e = cudaFuncSetAttribute(cache_attention_kernel<HD, kFp8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    e = cudaFuncSetAttribute(cache_attention_kernel<HD, kFp8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes + 4 * (kCacheMaxBatch + 1));
   });
   if (e != cudaSuccess) return e;
-  return launch_pdl(cache_attention_kernel<HD, kFp8, NT>, grid, dim3(kCacheThreads), smem, stream, p);
+  return launch_pdl(cache_attention_kernel<HD, kFp8, NT>, grid, dim3(Cfg::kThreads), smem, stream, p);
 }
 
 template <int HD>
@@ -603,7 +808,8 @@ static cudaError_t launch_cache_attention(CacheAttnParams p, void* workspace, in
   int nt = 1;
   const int64_t rows = static_cast<int64_t>(p.q_len) * p.group;
   const int64_t blocks = cache_attention_row_blocks(rows, &nt);
-  p.counters = static_cast<int*>(workspace);
+  p.group_counters = static_cast<int*>(workspace);
+  p.counters = p.group_counters + cache_attention_group_bytes(blocks, sm_count) / 4;
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + workspace_bytes / 256 * 256 -
                                         cache_attention_partial_bytes(p.c.head_dim, rows, sm_count));
   const dim3 grid(static_cast<unsigned>(cache_attention_ctas(sm_count)), static_cast<unsigned>(blocks));
