@@ -476,7 +476,10 @@ B2_API int b2_rotary_fwd(const void* x, int64_t ld_x, int64_t tokens, int64_t he
   p.head_dim = static_cast<int>(head_dim);
   p.rotary_dim = static_cast<int>(rotary_dim);
   p.inverse = inverse != 0;
-  return check_launch(launch_rotary(p, interleaved, static_cast<cudaStream_t>(stream)), "b2_rotary_fwd");
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return check_launch(launch_rotary(p, interleaved, device_sm_count(dev), static_cast<cudaStream_t>(stream)),
+                      "b2_rotary_fwd");
 }
 
 // The pages of a cache as the kernels take them, or a status.

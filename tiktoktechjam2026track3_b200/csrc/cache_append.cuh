@@ -11,10 +11,14 @@
 // then multiplied by 2^(e_old - e). The bounds on e keep the attention's sums of 2^e-weighted terms
 // inside fp32; magnitudes above 448 * 2^40 saturate, and values that are not finite become the NaN code.
 //
-// One CTA takes one page of one sequence and one head of K, of V, or (with a rotation) the query heads
-// of one key head for the page's tokens. Two passes over the new tokens of K and V in 8 bits: the page's
-// maximum has to be known before the first code is written.
+// Bound by HBM (the projection's rows in, codes or bf16 and rotated queries out), and nearly as much by the number of
+// instructions per element, so each is kept short: a thread holds up to two chunks of 16 elements, whose place in the
+// page is worked out once. A team of 1 to 16 warps, as many as hold the page's new tokens, takes one head of K or of
+// V (in 8 bits the page's maximum is then known before the first code is written, without reading twice; pages with
+// more than 1024 chunks are read twice), or the query heads of one key head, whose rows of the table stay in registers.
 #pragma once
+#include <cuda_fp16.h>
+
 #include "b2_common.cuh"
 #include "rotary.cuh"
 
@@ -71,16 +75,18 @@ __device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
 
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// 8 values as codes of the scale whose inverse is `inv`; a value that is not finite becomes NaN.
-__device__ __forceinline__ uint2 e4m3x8(const float (&f)[8], float inv) {
+// 8 values as codes of the scale whose inverse is `inv`; a NaN becomes the NaN code, and with `check` an infinity
+// does too (it would saturate).
+__device__ __forceinline__ uint2 e4m3x8(const float (&f)[8], float inv, bool check) {
   uint32_t w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     float y[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float x = f[4 * i + k];
-      y[k] = is_finite(x) ? x * inv : __uint_as_float(0x7fffffffu);
+    for (int k = 0; k < 4; ++k) y[k] = f[4 * i + k] * inv;
+    if (check) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) y[k] = is_finite(f[4 * i + k]) ? y[k] : __uint_as_float(0x7fffffffu);
     }
     w[i] = static_cast<uint32_t>(e4m3x2(y[0], y[1])) | (static_cast<uint32_t>(e4m3x2(y[2], y[3])) << 16);
   }
@@ -100,31 +106,28 @@ __device__ __forceinline__ uint32_t e4m3x4_scale(uint32_t w, float f) {
   return out;
 }
 
-constexpr int kAppendThreads = 128;
-
-__device__ __forceinline__ float append_block_max(float v, float* s_red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float m = s_red[0];
-#pragma unroll
-  for (int i = 1; i < kAppendThreads / 32; ++i) m = fmaxf(m, s_red[i]);
-  return m;
-}
+constexpr int kAppendMaxThreads = 512;
+constexpr int kAppendItems = 2;  // chunks that a thread holds
 
 template <bool kFp8, bool kInterleaved>
-__global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const AppendParams p) {
-  __shared__ float s_red[kAppendThreads / 32];
+__global__ void __launch_bounds__(kAppendMaxThreads, 2)
+    cache_append_kernel(const AppendParams p, const int team_shift, const unsigned role_blocks) {
+  __shared__ float s_red[kAppendMaxThreads / 32];
+  const unsigned block_page = blockIdx.x / role_blocks;
+  const unsigned team_threads = 32u << team_shift;
+  const unsigned tt = threadIdx.x & (team_threads - 1);
+  const unsigned team = threadIdx.x >> (5 + team_shift);
+  const int kv_heads = p.c.kv_heads;
+  const int role = static_cast<int>((blockIdx.x - block_page * role_blocks) * (blockDim.x >> (5 + team_shift)) + team);
+  if (role >= kv_heads * (p.rotary_dim > 0 ? 3 : 2)) return;  // the whole team: its barrier is its own
   pdl_wait_previous_grid();
   pdl_allow_next_grid();
   const int b = blockIdx.z;
   const int past = p.past_len[b];
   const int count = p.new_len[b];
+  const int first = p.new_start[b];
   if (count <= 0) return;
   const int shift = p.c.page_shift;
-  const int page_size = 1 << shift;
-  const int first = p.new_start[b];
   // Every index comes from device memory: one that does not fit is recorded and nothing is written.
   if (past < 0 || first < 0 || count > p.max_new || static_cast<int64_t>(first) + count > p.tokens ||
       static_cast<int64_t>(past) + count > (static_cast<int64_t>(p.table_pages) << shift) ||
@@ -132,33 +135,37 @@ __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const Appe
     record_status(kKernelCacheAppend, 1, kReasonBadIndex);
     return;
   }
-  const int page_index = (past >> shift) + static_cast<int>(blockIdx.x);
+  const int page_index = (past >> shift) + static_cast<int>(block_page);
   const int page0 = page_index << shift;  // first position of the page
   const int t0 = max(past, page0);
-  const int t1 = min(past + count, page0 + page_size);
+  const int t1 = min(past + count, page0 + (1 << shift));
   if (t0 >= t1) return;
-  const int n = t1 - t0;
+  const int held = t0 - page0;  // earlier tokens of the sequence in this page
+  const int hd = p.c.head_dim;
+  const unsigned chunks = static_cast<unsigned>(hd) >> 4;
+  const unsigned items = (t1 - t0) * chunks;
   const int64_t row0 = static_cast<int64_t>(first) + (t0 - past);
-  const unsigned chunks = static_cast<unsigned>(p.c.head_dim) >> 4;
-  const unsigned items = n * chunks;
-  const int kv_heads = p.c.kv_heads;
-  const int role = blockIdx.y;
-
-  auto load_table = [&](int token, int pair0, float (&c)[8], float (&s)[8]) {
-    rotary_load_table(p.table + static_cast<int64_t>(t0 + token) * (p.rotary_dim >> 1) + pair0, c, s);
+  const int ld = static_cast<int>(p.ld);
+  const bool is_v = role >= kv_heads && role < 2 * kv_heads;
+  const int rotary_dim = is_v ? 0 : p.rotary_dim;
+  auto angles_of = [&](unsigned token, int pair0, float (&c)[8], float (&s)[8]) {
+    rotary_load_table(p.table + static_cast<int64_t>(t0 + static_cast<int>(token)) * (rotary_dim >> 1) + pair0, c, s);
   };
 
   if (role >= 2 * kv_heads) {
-    // Query heads of one key head.
+    // The query heads of one key head.
     const int h0 = (role - 2 * kv_heads) * p.group;
-    for (unsigned i = threadIdx.x; i < items; i += kAppendThreads) {
+    const __nv_bfloat16* rows = p.qkv + row0 * p.ld + p.q_col + h0 * hd;
+    __nv_bfloat16* out = p.q_out + row0 * p.ld_q_out + h0 * hd;
+    for (unsigned i = tt; i < items; i += team_threads) {
       const unsigned token = i / chunks;
-      const RotaryChunk ch = rotary_chunk<kInterleaved>(i - token * chunks, p.rotary_dim);
+      const RotaryChunk ch = rotary_chunk<kInterleaved>(i - token * chunks, rotary_dim);
       float c[8], s[8];
-      if (ch.pair0 >= 0) load_table(token, ch.pair0, c, s);
-      const __nv_bfloat16* x = p.qkv + (row0 + token) * p.ld + p.q_col + h0 * p.c.head_dim;
-      __nv_bfloat16* y = p.q_out + (row0 + token) * p.ld_q_out + h0 * p.c.head_dim;
-      for (int g = 0; g < p.group; ++g, x += p.c.head_dim, y += p.c.head_dim) {
+      if (ch.pair0 >= 0) angles_of(token, ch.pair0, c, s);
+      const __nv_bfloat16* x = rows + token * static_cast<int64_t>(ld);
+      __nv_bfloat16* y = out + token * p.ld_q_out;
+#pragma unroll 2
+      for (int g = 0; g < p.group; ++g, x += hd, y += hd) {
         uint4 ua = *reinterpret_cast<const uint4*>(x + ch.off0);
         uint4 ub = *reinterpret_cast<const uint4*>(x + ch.off1);
         if (ch.pair0 >= 0) {
@@ -176,80 +183,153 @@ __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const Appe
     return;
   }
 
-  const bool is_v = role >= kv_heads;
   const int h = is_v ? role - kv_heads : role;
-  const int64_t page = p.page_table[b * p.ld_table + page_index];
-  if (page < 0 || page >= p.c.pages) {
-    record_status(kKernelCacheAppend, 2, kReasonBadIndex);
-    return;
-  }
-  const int rotary_dim = is_v ? 0 : p.rotary_dim;
-  const __nv_bfloat16* src = p.qkv + row0 * p.ld + (is_v ? p.v_col : p.k_col) + h * p.c.head_dim;
-  uint8_t* dst = (is_v ? p.c.v : p.c.k) + (page * p.c.page_stride + h * p.c.head_stride) * (kFp8 ? 1 : 2);
-
-  auto load = [&](unsigned i, unsigned& token, RotaryChunk& ch, float (&a)[8], float (&bb)[8]) {
-    token = i / chunks;
-    ch = rotary_chunk<kInterleaved>(i - token * chunks, rotary_dim);
-    const __nv_bfloat16* x = src + token * p.ld;
-    unpack_bf16x8(*reinterpret_cast<const uint4*>(x + ch.off0), a);
-    unpack_bf16x8(*reinterpret_cast<const uint4*>(x + ch.off1), bb);
+  // Looked at once the rows' loads are on their way; a page that does not exist is not written.
+  int64_t page = p.page_table[b * p.ld_table + page_index];
+  const __nv_bfloat16* rows = p.qkv + row0 * p.ld + (is_v ? p.v_col : p.k_col) + h * hd;
+  // The page, and where K goes besides.
+  uint8_t* dst = nullptr;
+  float* scale = nullptr;
+  auto find_page = [&]() {
+    if (page < 0 || page >= p.c.pages) {
+      record_status(kKernelCacheAppend, 2, kReasonBadIndex);
+      return false;
+    }
+    dst = (is_v ? p.c.v : p.c.k) + (page * p.c.page_stride + h * p.c.head_stride) * (kFp8 ? 1 : 2);
+    if (kFp8) scale = (is_v ? p.c.v_scale : p.c.k_scale) + page * kv_heads + h;
+    return true;
+  };
+  __nv_bfloat16* copy = !is_v && p.k_out != nullptr ? p.k_out + row0 * p.ld_k_out + h * hd : nullptr;
+  auto team_sync = [&]() {
+    if (team_shift > 0)
+      named_barrier_sync(1 + team, team_threads);
+    else
+      __syncwarp();
+  };
+  auto load = [&](unsigned token, const RotaryChunk& ch, float (&a)[8], float (&bb)[8]) {
+    const __nv_bfloat16* x = rows + token * static_cast<int64_t>(ld);
+    const uint4 ua = *reinterpret_cast<const uint4*>(x + ch.off0);
+    const uint4 ub = *reinterpret_cast<const uint4*>(x + ch.off1);
     if (ch.pair0 >= 0) {
       float c[8], s[8];
-      load_table(token, ch.pair0, c, s);
+      angles_of(token, ch.pair0, c, s);
+      unpack_bf16x8(ua, a);
+      unpack_bf16x8(ub, bb);
       rotary_apply<kInterleaved>(a, bb, c, s);
+    } else {
+      unpack_bf16x8(ua, a);
+      unpack_bf16x8(ub, bb);
     }
   };
-
-  float inv = 1.f;
-  if (kFp8) {
-    float amax = 0.f;
-    for (unsigned i = threadIdx.x; i < items; i += kAppendThreads) {
-      unsigned token;
-      RotaryChunk ch;
-      float a[8], bb[8];
-      load(i, token, ch, a, bb);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (is_finite(a[k])) amax = fmaxf(amax, fabsf(a[k]));
-        if (is_finite(bb[k])) amax = fmaxf(amax, fabsf(bb[k]));
-      }
-    }
-    int e = scale_exponent(append_block_max(amax, s_red));
-    float* scale = (is_v ? p.c.v_scale : p.c.k_scale) + page * kv_heads + h;
-    const int held = t0 - page0;  // earlier tokens of the sequence in this page
-    if (held > 0) {
-      const float old = *scale;
-      const int e_old = min(static_cast<int>((__float_as_uint(old) >> 23) & 0xffu) - 127, kScaleExpMax);
-      if (e > e_old) {
-        const float f = exp2_int(max(e_old - e, -126));
-        uint32_t* w = reinterpret_cast<uint32_t*>(dst);
-        for (int i = threadIdx.x; i < held * p.c.head_dim / 4; i += kAppendThreads) w[i] = e4m3x4_scale(w[i], f);
-      } else {
-        e = e_old;
-      }
-    }
-    __syncthreads();  // every thread has read the old scale
-    if (threadIdx.x == 0) *scale = exp2_int(e);
-    inv = exp2_int(-e);
-  }
-  for (unsigned i = threadIdx.x; i < items; i += kAppendThreads) {
-    unsigned token;
-    RotaryChunk ch;
-    float a[8], bb[8];
-    load(i, token, ch, a, bb);
-    const int64_t at = static_cast<int64_t>(t0 - page0 + token) * p.c.head_dim;
+  auto write = [&](unsigned token, const RotaryChunk& ch, const float (&a)[8], const float (&bb)[8], float inv, bool check) {
+    uint8_t* at = dst + (held + static_cast<int>(token)) * hd * (kFp8 ? 1 : 2);
     if (kFp8) {
-      *reinterpret_cast<uint2*>(dst + at + ch.off0) = e4m3x8(a, inv);
-      *reinterpret_cast<uint2*>(dst + at + ch.off1) = e4m3x8(bb, inv);
+      *reinterpret_cast<uint2*>(at + ch.off0) = e4m3x8(a, inv, check);
+      *reinterpret_cast<uint2*>(at + ch.off1) = e4m3x8(bb, inv, check);
     } else {
-      *reinterpret_cast<uint4*>(dst + 2 * (at + ch.off0)) = pack_bf16x8(a);
-      *reinterpret_cast<uint4*>(dst + 2 * (at + ch.off1)) = pack_bf16x8(bb);
+      *reinterpret_cast<uint4*>(at + 2 * ch.off0) = pack_bf16x8(a);
+      *reinterpret_cast<uint4*>(at + 2 * ch.off1) = pack_bf16x8(bb);
     }
-    if (!is_v && p.k_out != nullptr) {
-      __nv_bfloat16* y = p.k_out + (row0 + token) * p.ld_k_out + h * p.c.head_dim;
+    if (copy != nullptr) {
+      __nv_bfloat16* y = copy + token * p.ld_k_out;
       *reinterpret_cast<uint4*>(y + ch.off0) = pack_bf16x8(a);
       *reinterpret_cast<uint4*>(y + ch.off1) = pack_bf16x8(bb);
     }
+  };
+  // Largest magnitude (infinity if there is one; a NaN is passed over), and with `check` that of the finite values.
+  auto largest = [&](float amax, const float (&a)[8], const float (&bb)[8], bool check) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (check)
+        amax = fmaxf(amax, fmaxf(is_finite(a[k]) ? fabsf(a[k]) : 0.f, is_finite(bb[k]) ? fabsf(bb[k]) : 0.f));
+      else
+        amax = max3f(amax, fabsf(a[k]), fabsf(bb[k]));
+    }
+    return amax;
+  };
+  auto team_max = [&](float amax) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (team_shift > 0) {
+      if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = amax;
+      team_sync();
+      const int warp0 = static_cast<int>(team) << team_shift;
+      for (int i = 0; i < (1 << team_shift); ++i) amax = fmaxf(amax, s_red[warp0 + i]);
+    }
+    return amax;
+  };
+  // The page's scale from the team's largest value; earlier codes are rounded again if it grew. Returns its inverse.
+  auto settle_scale = [&](float amax) {
+    int e = scale_exponent(amax);
+    if (held > 0) {
+      const int e_old = min(static_cast<int>((__float_as_uint(*scale) >> 23) & 0xffu) - 127, kScaleExpMax);
+      if (e > e_old) {
+        const float f = exp2_int(max(e_old - e, -126));
+        uint32_t* w = reinterpret_cast<uint32_t*>(dst);
+        for (int i = tt; i < held * hd / 4; i += team_threads) w[i] = e4m3x4_scale(w[i], f);
+      } else {
+        e = e_old;
+      }
+      team_sync();  // every thread of the team has read the old scale
+    }
+    if (tt == 0) *scale = exp2_int(e);
+    return exp2_int(-e);
+  };
+
+  if (items <= kAppendItems * team_threads) {
+    float a[kAppendItems][8], bb[kAppendItems][8];
+    RotaryChunk ch[kAppendItems];
+    unsigned token[kAppendItems];
+    float amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < kAppendItems; ++k) {
+      const unsigned i = tt + k * team_threads;
+      token[k] = i / chunks;
+      ch[k] = rotary_chunk<kInterleaved>(i - token[k] * chunks, rotary_dim);
+      if (i < items) load(token[k], ch[k], a[k], bb[k]);
+    }
+    if (!find_page()) return;  // the whole team
+    float inv = 1.f;
+    bool check = false;
+    if (kFp8) {
+#pragma unroll
+      for (int k = 0; k < kAppendItems; ++k)
+        if (tt + k * team_threads < items) amax = largest(amax, a[k], bb[k], false);
+      amax = team_max(amax);
+      if (!is_finite(amax)) {  // an infinity among them: the scale goes by the finite values
+        check = true;
+        amax = 0.f;
+#pragma unroll
+        for (int k = 0; k < kAppendItems; ++k)
+          if (tt + k * team_threads < items) amax = largest(amax, a[k], bb[k], true);
+        team_sync();  // the first maxima have been read
+        amax = team_max(amax);
+      }
+      inv = settle_scale(amax);
+    }
+#pragma unroll
+    for (int k = 0; k < kAppendItems; ++k)
+      if (tt + k * team_threads < items) write(token[k], ch[k], a[k], bb[k], inv, check);
+  } else {
+    if (!find_page()) return;
+    auto each = [&](auto f) {
+      for (unsigned i = tt; i < items; i += team_threads) {
+        const unsigned token = i / chunks;
+        const RotaryChunk ch = rotary_chunk<kInterleaved>(i - token * chunks, rotary_dim);
+        float a[8], bb[8];
+        load(token, ch, a, bb);
+        f(token, ch, a, bb);
+      }
+    };
+    float inv = 1.f;
+    if (kFp8) {
+      float amax = 0.f;
+      each([&](unsigned, const RotaryChunk&, const float(&a)[8], const float(&bb)[8]) { amax = largest(amax, a, bb, true); });
+      inv = settle_scale(team_max(amax));  // between reading and writing: k_out may be the projection's own columns
+    }
+    each([&](unsigned token, const RotaryChunk& ch, const float(&a)[8], const float(&bb)[8]) {
+      write(token, ch, a, bb, inv, true);
+    });
   }
 }
 
@@ -257,15 +337,22 @@ static cudaError_t launch_cache_append(const AppendParams& p, int64_t max_new, b
                                        cudaStream_t stream) {
   // max_new tokens touch at most this many pages, wherever in a page they begin.
   const int64_t page_size = int64_t{1} << p.c.page_shift;
-  const unsigned pages = static_cast<unsigned>((max_new + page_size - 2) / page_size + 1);
-  const unsigned roles = static_cast<unsigned>(p.c.kv_heads * (p.rotary_dim > 0 ? 3 : 2));
-  const dim3 grid(pages, roles, static_cast<unsigned>(p.batch));
-  const dim3 block(kAppendThreads);
+  const int64_t pages = (max_new + page_size - 2) / page_size + 1;
+  const int64_t chunks = (max_new < page_size ? max_new : page_size) * (p.c.head_dim / 16);
+  int team_shift = 0;
+  while (team_shift < 4 && chunks > (int64_t{32 * kAppendItems} << team_shift)) ++team_shift;
+  const int threads = team_shift == 4 ? kAppendMaxThreads : 256;
+  const int64_t roles = static_cast<int64_t>(p.c.kv_heads) * (p.rotary_dim > 0 ? 3 : 2);
+  const int64_t teams = (threads / 32) >> team_shift;
+  const int64_t role_blocks = (roles + teams - 1) / teams;
+  if (role_blocks * pages > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  const dim3 grid(static_cast<unsigned>(role_blocks * pages), 1, static_cast<unsigned>(p.batch));
+  const unsigned rb = static_cast<unsigned>(role_blocks);
   if (fp8)
-    return interleaved ? launch_pdl(cache_append_kernel<true, true>, grid, block, 0, stream, p)
-                       : launch_pdl(cache_append_kernel<true, false>, grid, block, 0, stream, p);
-  return interleaved ? launch_pdl(cache_append_kernel<false, true>, grid, block, 0, stream, p)
-                     : launch_pdl(cache_append_kernel<false, false>, grid, block, 0, stream, p);
+    return interleaved ? launch_pdl(cache_append_kernel<true, true>, grid, dim3(threads), 0, stream, p, team_shift, rb)
+                       : launch_pdl(cache_append_kernel<true, false>, grid, dim3(threads), 0, stream, p, team_shift, rb);
+  return interleaved ? launch_pdl(cache_append_kernel<false, true>, grid, dim3(threads), 0, stream, p, team_shift, rb)
+                     : launch_pdl(cache_append_kernel<false, false>, grid, dim3(threads), 0, stream, p, team_shift, rb);
 }
 
 }  // namespace b2

@@ -100,9 +100,9 @@ __device__ __forceinline__ void rotary_apply(float (&a)[8], float (&b)[8], const
   }
 }
 
-constexpr int kRotaryThreads = 256;
+constexpr int kRotaryThreads = 128;
 
-template <bool kInterleaved>
+template <bool kInterleaved, int kHeads>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryParams p) {
   const unsigned chunks = static_cast<unsigned>(p.head_dim) >> 4;
   const unsigned columns = chunks * p.head_splits;
@@ -132,32 +132,53 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
     }
     const __nv_bfloat16* x = p.x + token * p.ld_x;
     __nv_bfloat16* y = p.out + token * p.ld_out;
-    for (int h = hs; h < p.heads; h += p.head_splits) {
-      const int base = h * p.head_dim;
-      uint4 ua = *reinterpret_cast<const uint4*>(x + base + ch.off0);
-      uint4 ub = *reinterpret_cast<const uint4*>(x + base + ch.off1);
-      if (ch.pair0 >= 0) {
-        float a[8], b[8];
-        unpack_bf16x8(ua, a);
-        unpack_bf16x8(ub, b);
-        rotary_apply<kInterleaved>(a, b, c, s);
-        ua = pack_bf16x8(a);
-        ub = pack_bf16x8(b);
+    // kHeads heads at a time: all their loads, then all their stores (out may be x, so the compiler cannot move them).
+    for (int h0 = hs; h0 < p.heads; h0 += kHeads * p.head_splits) {
+      uint4 ua[kHeads], ub[kHeads];
+#pragma unroll
+      for (int k = 0; k < kHeads; ++k) {
+        const int h = h0 + k * p.head_splits;
+        if (h < p.heads) {
+          ua[k] = __ldcs(reinterpret_cast<const uint4*>(x + h * p.head_dim + ch.off0));
+          ub[k] = __ldcs(reinterpret_cast<const uint4*>(x + h * p.head_dim + ch.off1));
+        }
       }
-      *reinterpret_cast<uint4*>(y + base + ch.off0) = ua;
-      *reinterpret_cast<uint4*>(y + base + ch.off1) = ub;
+#pragma unroll
+      for (int k = 0; k < kHeads; ++k) {
+        const int h = h0 + k * p.head_splits;
+        if (h < p.heads) {
+          if (ch.pair0 >= 0) {
+            float a[8], b[8];
+            unpack_bf16x8(ua[k], a);
+            unpack_bf16x8(ub[k], b);
+            rotary_apply<kInterleaved>(a, b, c, s);
+            ua[k] = pack_bf16x8(a);
+            ub[k] = pack_bf16x8(b);
+          }
+          __stcs(reinterpret_cast<uint4*>(y + h * p.head_dim + ch.off0), ua[k]);
+          __stcs(reinterpret_cast<uint4*>(y + h * p.head_dim + ch.off1), ub[k]);
+        }
+      }
     }
   }
 }
 
-static cudaError_t launch_rotary(RotaryParams p, int interleaved, cudaStream_t stream) {
+static cudaError_t launch_rotary(RotaryParams p, int interleaved, int sm_count, cudaStream_t stream) {
   const int chunks = p.head_dim / 16;
-  p.head_splits = p.heads;
+  // Four heads to a thread, which then loads its part of the table once for the four, where that still leaves each SM
+  // 2048 threads eight times over; else one, so that a small call has all its loads in flight at once.
+  const int64_t work = static_cast<int64_t>(p.tokens) * p.heads * chunks;
+  const bool four = p.heads >= 4 && work >= int64_t{4 * 8 * 2048} * sm_count;
+  p.head_splits = four ? (p.heads + 3) / 4 : p.heads;
   const int columns = chunks * p.head_splits;
   p.tokens_per_cta = columns >= kRotaryThreads ? 1 : kRotaryThreads / columns;
-  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(p.tokens) + p.tokens_per_cta - 1) / p.tokens_per_cta);
-  if (interleaved) return launch_pdl(rotary_kernel<true>, dim3(grid), dim3(kRotaryThreads), 0, stream, p);
-  return launch_pdl(rotary_kernel<false>, dim3(grid), dim3(kRotaryThreads), 0, stream, p);
+  const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(p.tokens) + p.tokens_per_cta - 1) / p.tokens_per_cta);
+  const dim3 grid(blocks), block(kRotaryThreads);
+  if (four)
+    return interleaved ? launch_pdl(rotary_kernel<true, 4>, grid, block, 0, stream, p)
+                       : launch_pdl(rotary_kernel<false, 4>, grid, block, 0, stream, p);
+  return interleaved ? launch_pdl(rotary_kernel<true, 1>, grid, block, 0, stream, p)
+                     : launch_pdl(rotary_kernel<false, 1>, grid, block, 0, stream, p);
 }
 
 }  // namespace b2
