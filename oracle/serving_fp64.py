@@ -82,3 +82,31 @@ def visible_keys(positions, keys, window, sinks):
     if window:
         seen &= (p - j < window) | (j < sinks)
     return seen
+
+
+def stack(state, num_heads, num_layers, x, table=None, rotary_dim=0, interleaved=False, window=0, sinks=0):
+    """A causal stack (the reference's block, models.py:727-738, with rotary positions and a window) in float64.
+
+    x [tokens, d_model]: one sequence from position 0. Returns [tokens, d_model].
+    """
+    n, d = x.shape
+    hd = d // num_heads
+    par = {k: v.double() for k, v in state.items()}
+    norm = torch.nn.functional.layer_norm
+    seen = visible_keys(torch.arange(n), n, window, sinks)
+    r = x.double()
+    for i in range(num_layers):
+        p = f"layers.{i}."
+
+        def lin(y, name):
+            return y @ par[p + name + ".weight"].T + par[p + name + ".bias"]
+
+        y = norm(r, (d,), par[p + "norm1.weight"], par[p + "norm1.bias"], 1e-5)
+        q, k, v = (lin(y, f"attention.{z}_proj").view(n, num_heads, hd) for z in "qkv")
+        if table is not None:
+            q, k = (rotate(z, table[:n], rotary_dim, interleaved) for z in (q, k))
+        ctx = torch.stack([attend(q[:, h], k[:, h], v[:, h], seen, hd**-0.5)[0] for h in range(num_heads)], 1)
+        r = r + lin(ctx.reshape(n, d), "attention.out_proj")
+        y = norm(r, (d,), par[p + "norm2.weight"], par[p + "norm2.bias"], 1e-5)
+        r = r + lin(torch.nn.functional.gelu(lin(y, "ffn_in")), "ffn_out")
+    return norm(r, (d,), par["final_norm.weight"], par["final_norm.bias"], 1e-5)

@@ -154,3 +154,22 @@ def test_wrappers_refuse_cpu_tensors():
         serving.rotary(x, torch.zeros(4, dtype=torch.int32), serving.rotary_table(8, 64, device="cpu"), 64)
     with pytest.raises(ValueError, match="CUDA"):
         serving.KVCache(torch.zeros(2, 1, 16, 16, dtype=torch.bfloat16), torch.zeros(2, 1, 16, 16, dtype=torch.bfloat16))
+
+
+def test_streaming_refusals():
+    from tiktoktechjam2026track3_b200 import StreamingTransformer, TransformerConfig, UserOptimizedTransformer
+
+    def model(heads=4, causal=True):
+        return UserOptimizedTransformer(TransformerConfig(1, 8, 64, heads, 64, 1, causal))
+
+    with pytest.raises(ValueError, match="causal"):
+        StreamingTransformer(model(1, causal=False), 1, 8)
+    with pytest.raises(NotImplementedError, match="head_dim"):
+        StreamingTransformer(model(4), 1, 8)  # head_dim 16
+    for bad in (dict(window=-1), dict(sinks=2), dict(window=2, sinks=-1)):
+        with pytest.raises(ValueError):
+            StreamingTransformer(model(1), 1, 8, **bad)
+    with pytest.raises(ValueError, match="table"):
+        StreamingTransformer(model(1), 1, 8, table=serving.rotary_table(4, 64, device="cpu"))
+    with pytest.raises(RuntimeError, match="GPU"):
+        StreamingTransformer(model(1), 1, 8)

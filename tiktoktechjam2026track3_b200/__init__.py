@@ -9,12 +9,14 @@ from .cases import BASELINE_CONFIGS, TransformerConfig, Workload, config_from
 from .correctness import AccuracyResult, GateResult, baseline_gate, compare_outputs
 from .models import UserOptimizedTransformer, copy_model_weights
 from .serving import KVCache, rotary, rotary_table, window_attention
+from .streaming import StreamingTransformer
 
 __all__ = [
     "AccuracyResult",
     "BASELINE_CONFIGS",
     "GateResult",
     "KVCache",
+    "StreamingTransformer",
     "TransformerConfig",
     "UserOptimizedTransformer",
     "Workload",
