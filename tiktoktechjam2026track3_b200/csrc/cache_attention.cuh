@@ -52,7 +52,8 @@ struct CacheAttnParams {
 };
 
 constexpr int kCacheMaxBatch = 4096;
-constexpr int kCacheGroup = 16;  // parts of a (sequence, head) that one CTA joins at once
+constexpr int kCacheAtOnce = 40;  // parts of a (sequence, head) that one CTA joins in one go;
+constexpr int kCacheGroup = 16;   // of more, so many in a first go
 constexpr float kCacheRescale = 8.f;   // log2: the maximum moves when a score exceeds it by more
 constexpr float kCacheHeadroom = 7.f;  // log2: weights are at most 2^(8 + 7), below fp16's largest
 
@@ -316,10 +317,6 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT>::kThreads, CacheAtt
   }
   while (true) {
     read_ids(now, now.u0);
-    if (Cfg::kPrefetch) {
-#pragma unroll
-      for (int d = 0; d < kAhead; ++d) prefetch(now, now.u0 + d);
-    }
     if (tid == 0) s_part = now;
     const SeqTiles seq = now.seq;
     const int64_t head_bytes = now.h * p.c.head_stride * Cfg::kBytes;
@@ -397,6 +394,12 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT>::kThreads, CacheAtt
       for (int j = 0; j < Cfg::kSteps; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[nt][j][i] = 0.f;
+    }
+
+    // (behind Q's loads, which need not wait for the page numbers; the first unit's own loads come next)
+    if (Cfg::kPrefetch) {
+#pragma unroll
+      for (int d = 1; d < kAhead; ++d) prefetch(now, now.u0 + d);
     }
 
     // Tokens that every row sees lie below `all_see`, and (with a window) from `all_from` on or below the sinks.
@@ -649,7 +652,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT>::kThreads, CacheAtt
       }
     }
     if (!whole) {
-      // Joins of CTAs' parts, in their order on the line. Up to kCacheGroup parts at once; more (few sequences with few
+      // Joins of CTAs' parts, in their order on the line. Up to kCacheAtOnce parts in one go; more (few sequences with few
       // key heads) first in groups of kCacheGroup CTAs, whose result takes the place of its first part.
       const int64_t c_first = ((static_cast<int64_t>(head_begin) + 1) * ctas - 1) / total;
       const int64_t c_last = (static_cast<int64_t>(head_begin + units) * ctas - 1) / total;
@@ -670,7 +673,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT>::kThreads, CacheAtt
         if (last) __threadfence();
         return last;
       };
-      // Parts of the CTAs c_from(k), k < n <= kCacheGroup (+ 3 groups' results).
+      // Parts of the CTAs c_from(k), k < n.
       auto join = [&](auto c_from, int n, float* into) {
         const float** s_at = reinterpret_cast<const float**>(s_merge);  // [n]
         float* s_f = reinterpret_cast<float*>(s_at + n);                // [n][R] maxima, then factors
@@ -697,23 +700,46 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT>::kThreads, CacheAtt
           s_row[R + tid] = top;
         }
         __syncthreads();
-        for (int i = tid; i < rows * (HD / 2); i += Cfg::kThreads) {
-          const int r = i / (HD / 2), d = 2 * (i - r * (HD / 2));
-          float2 acc = make_float2(0.f, 0.f);
+        // Four dims to a thread; where that leaves threads over, they share the parts.
+        const int quads = rows * (HD / 4);
+        const int shares = max(1, Cfg::kThreads / quads);
+        float4* s_acc = reinterpret_cast<float4*>(s_merge + (n * (2 * R + 2) + 2 * R + 3) / 4 * 4);  // [shares][quads]
+        for (int i0 = 0; i0 < quads; i0 += Cfg::kThreads) {
+          const int share = shares > 1 ? tid / quads : 0;
+          const int i = shares > 1 ? tid - share * quads : i0 + tid;
+          const int r = i / (HD / 4), d = 4 * (i - r * (HD / 4));
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i < quads && share < shares) {
 #pragma unroll 8
-          for (int k = 0; k < n; ++k) {
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(s_at[k] + r * HD + d));
-            const float f = s_f[k * R + r];
-            acc.x = fmaf(v.x, f, acc.x);
-            acc.y = fmaf(v.y, f, acc.y);
+            for (int k = share; k < n; k += shares) {
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(s_at[k] + r * HD + d));
+              const float f = s_f[k * R + r];
+              acc.x = fmaf(v.x, f, acc.x);
+              acc.y = fmaf(v.y, f, acc.y);
+              acc.z = fmaf(v.z, f, acc.z);
+              acc.w = fmaf(v.w, f, acc.w);
+            }
           }
-          if (into == nullptr) {
-            finish(r, d, acc, s_row[r]);
-          } else {
-            *reinterpret_cast<float2*>(into + r * HD + d) = acc;
-            if (d == 0) {
-              into[R * HD + r] = s_row[R + r];
-              into[R * HD + R + r] = s_row[r];
+          if (shares > 1) {
+            if (share < shares) s_acc[share * quads + i] = acc;
+            __syncthreads();
+            if (share == 0) {
+              for (int x = 1; x < shares; ++x) {
+                const float4 v = s_acc[x * quads + i];
+                acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+              }
+            }
+          }
+          if (i < quads && share == 0) {
+            if (into == nullptr) {
+              finish(r, d, make_float2(acc.x, acc.y), s_row[r]);
+              finish(r, d + 2, make_float2(acc.z, acc.w), s_row[r]);
+            } else {
+              *reinterpret_cast<float4*>(into + r * HD + d) = acc;
+              if (d == 0) {
+                into[R * HD + r] = s_row[R + r];
+                into[R * HD + R + r] = s_row[r];
+              }
             }
           }
         }
@@ -721,7 +747,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT>::kThreads, CacheAtt
       };
       const int n = static_cast<int>(c_last - c_first) + 1;
       int* head_counter = p.counters + static_cast<int64_t>(blockIdx.y) * p.batch * kv_heads + b * kv_heads + h;
-      if (n <= kCacheGroup) {
+      if (n <= kCacheAtOnce) {
         if (last_of(head_counter, n)) join([&](int k) { return c_first + k; }, n, nullptr);
       } else {
         const int64_t group = cta / kCacheGroup;
