@@ -324,11 +324,11 @@ int b2_cache_attention_fwd(const b2_kv_cache* cache, const void* q, int64_t ld_q
                            int64_t workspace_bytes, void* stream);
 
 /*
- * Causal attention of whole prompts with a sliding window and first tokens that stay visible: query i of sequence b sees
- * key j <= i iff window == 0, i - j < window or j < sinks; out = softmax(scale * q k^T) v. Rows i >= kv_len[b] (kv_len
- * NULL: seq_len) are written as zeros, and what their keys and values hold does not reach the others. A
- * value that is not finite at a valid position reaches the queries that see it and may reach others whose
- * position is less than 128 away from one that does. The reference's attention
+ * Causal attention of whole prompts with a sliding window and first tokens that stay visible: query i of
+ * sequence b sees key j <= i iff window == 0, i - j < window or j < sinks; out = softmax(scale * q k^T) v.
+ * Rows i >= kv_len[b] (kv_len NULL: seq_len) are written as zeros, and what their keys and values hold does
+ * not reach the others. A value that is not finite at a valid position reaches the queries that see it and
+ * may reach others whose position is less than 128 away from one that does. The reference's attention
  * (models.py:55-75) is the case without a window and with one key head per query head.
  *   q    [batch * seq_len, ld_q] bf16, num_heads heads side by side; k, v likewise with kv_heads heads: query head
  *        i reads key head i / (num_heads / kv_heads). All may be column ranges of one packed projection

@@ -17,6 +17,13 @@
 //   - In list places v, row i sees v <= d and (v >= c or v < a), with a = sinks, d the place of key i and c that of key
 //     i - window + 1; only tiles where these cut are masked.
 //   - Values behind the band's last key are cleared in shared memory: a weight of zero does not remove a NaN there.
+// Measured on one B200 (us a call back to back; floor, the larger of products at the measured GEMM rate and bytes at the copy
+// rate, in brackets): 32768 tokens, 16 heads of 128 on 4 key heads, window 4096: 1000 to 1150 as the 1000 W limit lets it
+// (627); 16 ragged sequences of up to 2048, 16 heads of 64, window 512: 152 (28); the same on 4 key heads, not ragged: 155
+// (37); causal without a window, 16 x 2048 x 16 heads of 64: 247 (83; attention_solo_kernel 229), 8192 x 16 heads
+// of 128: 270 (167; attention_wide_kernel 260). Per tile of 128 x 128 the exponential unit needs 1024 cycles at head_dim
+// 64 and the issue of twelve products as many; a masked tile costs about half as much again as an open one,
+// and of the six tiles of a window of 512 four are masked.
 #pragma once
 #include <mutex>
 #include <type_traits>
@@ -493,8 +500,9 @@ __global__ void __launch_bounds__(192, 2)
           tmem_store_32cols(t_o + cc * 32, o);
         }
       }
-      if (const int last_rows = s_tiles->rows - 128 * j; last_rows < 128 && (last_rows & 15) != 0) {  // products stop at the next multiple of 16 rows
-        // (O += P(j-1) V has completed, so the stage's barrier is in this tile's phase)
+      // Products stop at the next multiple of 16 rows. (O += P(j-1) V has completed, so the stage's barrier is in this
+      // tile's phase.)
+      if (const int last_rows = s_tiles->rows - 128 * j; last_rows < 128 && (last_rows & 15) != 0) {
         softmax_wait(&v_full[j % kStages], (j / kStages) & 1, 111, alive, abort_flag);
         window_clear_values<1>(s_v + (j % kStages) * kTileBytes, last_rows, threadIdx.x - 64, 128);
       }

@@ -616,7 +616,7 @@ B2_API int b2_cache_attention_fwd(const b2_kv_cache* cache, const void* q, int64
   const int64_t rows = q_len * (num_heads / hk);
   // Token positions stay below 2^30, so that sums of a position and a window do not leave 32 bits.
   if (batch > kCacheMaxBatch || q_len > 1024 || num_heads > 65536 || table_pages > ((int64_t{1} << 30) >> p.c.page_shift) ||
-      batch * hk > 0x7fffffffLL / units)
+      batch * hk > 0x7fffffffLL / units || rows > 16 * 65535)
     return fail(2, "b2_cache_attention_fwd: problem too large");
   if (batch == 0) return 0;
   if (q == nullptr || page_table == nullptr || kv_len == nullptr || out == nullptr || workspace == nullptr)

@@ -16,6 +16,11 @@
 // page is worked out once. A team of 1 to 16 warps, as many as hold the page's new tokens, takes one head of K or of
 // V (in 8 bits the page's maximum is then known before the first code is written, without reading twice; pages with
 // more than 1024 chunks are read twice), or the query heads of one key head, whose rows of the table stay in registers.
+// Measured on one B200 (us a call, floor in brackets): ragged prompts of 16 sequences of up to 2048 tokens, 16 heads of
+// 64, 8-bit pages of 32: 71 (43; 94 with a CTA of 128 threads per head that read its rows twice); 32768 tokens of 16
+// query and 4 key heads of 128: 82 (64; 92); bf16 chunks of three documents 30 (20); one token in each of 64 sequences
+// 3.9, a launch. Issue slots are 55 % busy and the L1 data pipe (the table, 64 bytes a thread) 54 %: more warps do not
+// fit their registers, and going through several heads with the table in registers cost more instructions than it saved.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -335,7 +340,8 @@ __global__ void __launch_bounds__(kAppendMaxThreads, 2)
 
 static cudaError_t launch_cache_append(const AppendParams& p, int64_t max_new, bool fp8, int interleaved,
                                        cudaStream_t stream) {
-  // max_new tokens touch at most this many pages, wherever in a page they begin.
+  // max_new tokens touch at most this many pages, wherever in a page they begin. 256 threads a CTA (ragged prompts as
+  // above: 71 us, 78 with 512, 106 with 128), 512 where one team needs them.
   const int64_t page_size = int64_t{1} << p.c.page_shift;
   const int64_t pages = (max_new + page_size - 2) / page_size + 1;
   const int64_t chunks = (max_new < page_size ? max_new : page_size) * (p.c.head_dim / 16);
