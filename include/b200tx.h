@@ -246,6 +246,12 @@ int b2_layernorm_gather_fwd(const float* x, const void* gamma, const void* beta,
 int b2_peer_barrier(void* const* pads, int world, int rank, int channel, void* stream);
 
 /*
+ * The entry points from here on serve single steps, whose calls are short next to their launches. Each takes its
+ * arguments as one struct whose members are all 8 bytes wide, so that a binding fills one block of memory instead of
+ * converting two dozen arguments (1.6 us of a call through ctypes).
+ */
+
+/*
  * Rotary positions, in place or into `out`: of each head's first rotary_dim elements the pairs
  * (x[i], x[i + rotary_dim / 2]), or with interleaved != 0 (x[2i], x[2i + 1]), become
  *   (x1 c - x2 s, x2 c + x1 s),  (c, s) = table[positions[token]][i]   (inverse != 0: s -> -s, the
@@ -256,9 +262,17 @@ int b2_peer_barrier(void* const* pads, int world, int rank, int channel, void* s
  *   table      [max_positions, rotary_dim / 2, 2] fp32 (cos, sin)
  * head_dim: a multiple of 16 up to 256; rotary_dim: a multiple of 16 up to head_dim.
  */
-int b2_rotary_fwd(const void* x, int64_t ld_x, int64_t tokens, int64_t heads, int64_t head_dim, int64_t rotary_dim,
-                  int interleaved, int inverse, const int32_t* positions, const float* table, int64_t max_positions,
-                  void* out, int64_t ld_out, void* stream);
+typedef struct b2_rotary_args {
+  const void* x;
+  int64_t ld_x, tokens, heads, head_dim, rotary_dim, interleaved, inverse;
+  const int32_t* positions;
+  const float* table;
+  int64_t max_positions;
+  void* out;
+  int64_t ld_out;
+} b2_rotary_args;
+
+int b2_rotary_fwd(const b2_rotary_args* args, void* stream);
 
 /* Element type of a cache's pages. */
 #define B2_CACHE_BF16 0
@@ -294,12 +308,21 @@ typedef struct b2_kv_cache {
  *   q_out  [tokens, ld_q_out] bf16: rotated Q (rotary_dim > 0 only; may be qkv's own columns)
  *   k_out  [tokens, ld_k_out] bf16: K as it was before rounding to the cache's type, or NULL
  */
-int b2_cache_append_fwd(const b2_kv_cache* cache, const void* qkv, int64_t ld_qkv, int64_t q_col, int64_t k_col,
-                        int64_t v_col, int64_t tokens, int64_t num_heads, int64_t batch, const int32_t* new_start,
-                        const int32_t* new_len, const int32_t* past_len, const int32_t* page_table,
-                        int64_t table_pages, int64_t max_new, const float* table, int64_t max_positions,
-                        int64_t rotary_dim, int interleaved, void* q_out, int64_t ld_q_out, void* k_out,
-                        int64_t ld_k_out, void* stream);
+typedef struct b2_cache_append_args {
+  const b2_kv_cache* cache;
+  const void* qkv;
+  int64_t ld_qkv, q_col, k_col, v_col, tokens, num_heads, batch;
+  const int32_t *new_start, *new_len, *past_len, *page_table;
+  int64_t table_pages, max_new;
+  const float* table;
+  int64_t max_positions, rotary_dim, interleaved;
+  void* q_out;
+  int64_t ld_q_out;
+  void* k_out;
+  int64_t ld_k_out;
+} b2_cache_append_args;
+
+int b2_cache_append_fwd(const b2_cache_append_args* args, void* stream);
 
 /* Bytes of b2_cache_attention_fwd's workspace. sm_count 0 asks the current device. */
 int b2_cache_attention_workspace(int64_t batch, int64_t q_len, int64_t num_heads, int64_t kv_heads, int64_t head_dim,
@@ -318,10 +341,22 @@ int b2_cache_attention_workspace(int64_t batch, int64_t q_len, int64_t num_heads
  *              counters zero. One made for the largest batch, q_len and num_heads serves smaller calls too;
  *              calls that may run at the same time need one each
  */
-int b2_cache_attention_fwd(const b2_kv_cache* cache, const void* q, int64_t ld_q, int64_t batch, int64_t q_len,
-                           int64_t num_heads, const int32_t* page_table, int64_t table_pages, const int32_t* kv_len,
-                           int64_t window, int64_t sinks, float scale, void* out, int64_t ld_out, void* workspace,
-                           int64_t workspace_bytes, void* stream);
+typedef struct b2_cache_attention_args {
+  const b2_kv_cache* cache;
+  const void* q;
+  int64_t ld_q, batch, q_len, num_heads;
+  const int32_t* page_table;
+  int64_t table_pages;
+  const int32_t* kv_len;
+  int64_t window, sinks;
+  double scale;
+  void* out;
+  int64_t ld_out;
+  void* workspace;
+  int64_t workspace_bytes;
+} b2_cache_attention_args;
+
+int b2_cache_attention_fwd(const b2_cache_attention_args* args, void* stream);
 
 /*
  * Causal attention of whole prompts with a sliding window and first tokens that stay visible: query i of
@@ -334,10 +369,21 @@ int b2_cache_attention_fwd(const b2_kv_cache* cache, const void* q, int64_t ld_q
  *        i reads key head i / (num_heads / kv_heads). All may be column ranges of one packed projection
  *   out  [batch * seq_len, ld_out] bf16. head_dim 32, 64 or 128
  */
-int b2_window_attention_fwd(const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* v, int64_t ld_v,
-                            int64_t batch, int64_t seq_len, int64_t num_heads, int64_t kv_heads, int64_t head_dim,
-                            const int32_t* kv_len, int64_t window, int64_t sinks, float scale, void* out,
-                            int64_t ld_out, void* stream);
+typedef struct b2_window_attention_args {
+  const void* q;
+  int64_t ld_q;
+  const void* k;
+  int64_t ld_k;
+  const void* v;
+  int64_t ld_v, batch, seq_len, num_heads, kv_heads, head_dim;
+  const int32_t* kv_len;
+  int64_t window, sinks;
+  double scale;
+  void* out;
+  int64_t ld_out;
+} b2_window_attention_args;
+
+int b2_window_attention_fwd(const b2_window_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -496,3 +496,42 @@ def test_window_attention_long_sequence_tail():
         ref, absum, size = oracle.attend(q.cpu().double().view(n, 4, d)[rows, h], k.cpu().double(), v.cpu().double(), seen,
                                          d**-0.5)
         _close(out.view(n, 4, d)[rows.cuda(), h], ref, 2**-8 * ref.abs() + (2**-8 + 2**-12 + 2 * d * 2**-23 * size) * absum)
+
+
+# ---------------------------------------------------------------------------------- refusals of the wrappers
+def test_wrappers_refuse_what_does_not_fit():
+    table = serving.rotary_table(16, 32)
+    x = torch.zeros(4, 64, dtype=BF16, device="cuda")
+    pos = _i32([0, 1, 2, 3])
+    for bad in (dict(x=x.float()), dict(x=x.t()), dict(x=x[:, :40]), dict(positions=pos[:3]), dict(positions=pos.long()),
+                dict(table=table.double()), dict(table=table[:, :, :1]), dict(out=x[:3]), dict(x=x.view(2, 2, 64))):
+        with pytest.raises((ValueError, IndexError)):
+            serving.rotary(**(dict(x=x, positions=pos, table=table, head_dim=32, out=torch.empty_like(x)) | bad))
+    cache = serving.KVCache.allocate(4, 2, 32, 16)
+    qkv = torch.zeros(4, 8 * 32, dtype=BF16, device="cuda")
+    pages = _i32([[0, 1], [2, 3]])
+    good = dict(qkv=qkv, num_heads=4, new_start=_i32([0, 2]), new_len=_i32([2, 2]), past_len=_i32([0, 0]),
+                page_table=pages, max_new=2)
+    for bad in (dict(num_heads=2), dict(new_start=_i32([0])), dict(page_table=pages[:1]), dict(page_table=pages.repeat(1, 2)[:, ::2]),
+                dict(past_len=torch.zeros(2, device="cuda")), dict(q_out=qkv[:, :128]), dict(table=table, q_out=qkv[:, :96]),
+                dict(k_out=qkv[:2, :64])):
+        with pytest.raises((ValueError, RuntimeError)):
+            cache.append(**(good | bad))
+    q = torch.zeros(2, 4 * 32, dtype=BF16, device="cuda")
+    good = dict(q=q, page_table=pages, kv_len=_i32([1, 1]))
+    for bad in (dict(q_len=2), dict(q=q[:, :48]), dict(q=q[:, :96]), dict(kv_len=_i32([1])), dict(sinks=2), dict(scale=0.0),
+                dict(workspace=torch.zeros(256, dtype=torch.uint8, device="cuda")),
+                dict(workspace=torch.zeros(1 << 20, device="cuda")), dict(out=q[:, :64])):
+        with pytest.raises((ValueError, RuntimeError)):
+            cache.attend(**(good | bad))
+    for bad in ((q, q[:, :64], q, 1, 2), (q, q, q, 2, 2), (q, q[:, :40], q[:, :40], 1, 2)):
+        with pytest.raises(ValueError):
+            serving.window_attention(*bad, 32)
+    with pytest.raises(RuntimeError, match="sinks"):
+        serving.window_attention(q, q, q, 1, 2, 32, sinks=1)
+    k = torch.zeros(4, 2, 16, 32, dtype=BF16, device="cuda")
+    for bad in ((k, k[:2]), (k, k.float()), (k.half(), k.half()), (k[:, :, :8], k[:, :, :8]),
+                (k, k, torch.ones(4, 2, device="cuda"), torch.ones(4, 2, device="cuda")), (k.to(E4M3), k.to(E4M3)),
+                (k.transpose(2, 3), k.transpose(2, 3))):
+        with pytest.raises(ValueError):
+            serving.KVCache(*bad)

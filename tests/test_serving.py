@@ -2,12 +2,16 @@
 
 import ctypes
 import math
+import re
+from pathlib import Path
 
 import pytest
 import torch
 
 from tiktoktechjam2026track3_b200 import _capi, serving
 from tiktoktechjam2026track3_b200.build import build
+
+HEADER = Path(__file__).resolve().parents[1] / "include" / "b200tx.h"
 
 
 @pytest.fixture(scope="module")
@@ -52,20 +56,26 @@ def test_rotary_table_refusals(args):
 
 
 # ---------------------------------------------------------------------------------- refusals
-P = ctypes.c_void_p(256)
-ODD = ctypes.c_void_p(264)
+P = 256  # addresses that no refused call looks at
+ODD = 264
+
+
+def _call(fn, layout, *args):
+    """An entry point that takes its arguments as a struct; None is a null pointer."""
+    return fn(layout.pack(*(0 if a is None else a for a in args)), None)
 
 
 def test_rotary_rejects_bad_arguments(lib):
     def call(x=P, ld_x=128, tokens=4, heads=2, head_dim=64, rotary_dim=64, pos=P, table=P, most=10, out=P, ld_out=128):
-        return lib.b2_rotary_fwd(x, ld_x, tokens, heads, head_dim, rotary_dim, 0, 0, pos, table, most, out, ld_out, None)
+        return _call(lib.b2_rotary_fwd, _capi.ROTARY_ARGS, x, ld_x, tokens, heads, head_dim, rotary_dim, 0, 0, pos, table,
+                     most, out, ld_out)
 
     assert call(x=None) == 1 and call(pos=None) == 1 and call(table=None) == 1 and call(out=None) == 1
     assert call(tokens=-1) == 1 and call(heads=0) == 1 and call(most=0) == 1
     assert call(head_dim=24) == 2 and call(head_dim=512, ld_x=1024, ld_out=1024) == 2
     assert call(rotary_dim=80) == 2 and call(rotary_dim=8) == 2 and call(rotary_dim=0) == 2
     assert b"rotary_dim" in lib.b2_last_error()
-    assert call(ld_x=120) == 2 and call(ld_out=132) == 2 and call(x=ctypes.c_void_p(8)) == 2
+    assert call(ld_x=120) == 2 and call(ld_out=132) == 2 and call(x=8) == 2
     assert call(tokens=0, x=None) == 0  # empty is a no-op
 
 
@@ -86,17 +96,44 @@ BAD_CACHES = [
 @pytest.mark.parametrize("change,status", BAD_CACHES)
 def test_bad_caches_are_rejected(lib, change, status):
     c = _desc(**change)
-    assert lib.b2_cache_append_fwd(c, P, 512, 0, 256, 384, 4, 4, 1, P, P, P, P, 2, 4, P, 64, 64, 0, P, 256, None, 0,
-                                   None) == status
-    assert lib.b2_cache_attention_fwd(c, P, 256, 1, 1, 4, P, 2, P, 0, 0, 0.125, P, 256, P, 1 << 30, None) == status
-    assert lib.b2_cache_attention_fwd(None, P, 256, 1, 1, 4, P, 2, P, 0, 0, 0.125, P, 256, P, 1 << 30, None) == 1
+
+    def append(cache):
+        return _call(lib.b2_cache_append_fwd, _capi.CACHE_APPEND_ARGS, cache, P, 512, 0, 256, 384, 4, 4, 1, P, P, P, P, 2, 4,
+                     P, 64, 64, 0, P, 256, None, 0)
+
+    def attend(cache):
+        return _call(lib.b2_cache_attention_fwd, _capi.CACHE_ATTENTION_ARGS, cache, P, 256, 1, 1, 4, P, 2, P, 0, 0, 0.125, P,
+                     256, P, 1 << 30)
+
+    assert append(ctypes.addressof(c)) == status and attend(ctypes.addressof(c)) == status
+    assert append(None) == 1 and attend(None) == 1
+
+
+def test_a_missing_argument_struct_is_rejected(lib):
+    for fn in (lib.b2_rotary_fwd, lib.b2_cache_append_fwd, lib.b2_cache_attention_fwd, lib.b2_window_attention_fwd):
+        assert fn(None, None) == 1 and b"null" in lib.b2_last_error()
+
+
+def test_argument_structs_have_the_headers_layout():
+    """Members of each struct in the header, all 8 bytes wide, against what the binding packs."""
+    text = re.sub(r"/\*.*?\*/", "", HEADER.read_text(), flags=re.S)
+    for name, layout in (("rotary", _capi.ROTARY_ARGS), ("cache_append", _capi.CACHE_APPEND_ARGS),
+                         ("cache_attention", _capi.CACHE_ATTENTION_ARGS), ("window_attention", _capi.WINDOW_ATTENTION_ARGS)):
+        body = re.search(r"typedef struct b2_%s_args \{(.*?)\}" % name, text, flags=re.S).group(1)
+        kinds = ""
+        for line in filter(None, (part.strip() for part in body.split(";"))):
+            kinds += ("d" if line.startswith("double") else "q") * len(line.split(","))
+        packed = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([qd])", layout.format))
+        assert kinds == packed, name
 
 
 def test_cache_append_rejects_bad_arguments(lib):
     def call(qkv=P, ld=512, cols=(0, 256, 384), tokens=4, heads=4, batch=1, start=P, count=P, past=P, pages=P,
              table_pages=2, most=4, table=P, positions=64, rotary_dim=64, q_out=P, ld_q=256, k_out=None, ld_k=0):
-        return lib.b2_cache_append_fwd(_desc(), qkv, ld, *cols, tokens, heads, batch, start, count, past, pages,
-                                       table_pages, most, table, positions, rotary_dim, 0, q_out, ld_q, k_out, ld_k, None)
+        cache = _desc()
+        return _call(lib.b2_cache_append_fwd, _capi.CACHE_APPEND_ARGS, ctypes.addressof(cache), qkv, ld, *cols, tokens, heads,
+                     batch, start, count, past, pages, table_pages, most, table, positions, rotary_dim, 0, q_out, ld_q, k_out,
+                     ld_k)
 
     for name in ("qkv", "start", "count", "past", "pages", "table", "q_out"):
         assert call(**{name: None}) == 1, name
@@ -114,8 +151,9 @@ def test_cache_attention_rejects_bad_arguments(lib):
 
     def call(cache=None, q=P, ld_q=256, batch=3, q_len=1, heads=4, pages=P, table_pages=2, kv=P, window=0, sinks=0,
              scale=0.125, out=P, ld_out=256, ws=P, ws_bytes=1 << 30):
-        return lib.b2_cache_attention_fwd(cache or _desc(), q, ld_q, batch, q_len, heads, pages, table_pages, kv, window,
-                                          sinks, scale, out, ld_out, ws, ws_bytes, None)
+        desc = cache or _desc()
+        return _call(lib.b2_cache_attention_fwd, _capi.CACHE_ATTENTION_ARGS, ctypes.addressof(desc), q, ld_q, batch, q_len,
+                     heads, pages, table_pages, kv, window, sinks, scale, out, ld_out, ws, ws_bytes)
 
     for name in ("q", "pages", "kv", "out", "ws"):
         assert call(**{name: None}) == 1, name
@@ -134,12 +172,12 @@ def test_cache_attention_rejects_bad_arguments(lib):
 def test_window_attention_rejects_bad_arguments(lib):
     def call(q=P, ld_q=256, k=P, ld_k=128, v=P, ld_v=128, batch=2, seq=100, heads=4, kv_heads=2, head_dim=64, kv_len=None,
              window=10, sinks=2, scale=0.125, out=P, ld_out=256):
-        return lib.b2_window_attention_fwd(q, ld_q, k, ld_k, v, ld_v, batch, seq, heads, kv_heads, head_dim, kv_len, window,
-                                           sinks, scale, out, ld_out, None)
+        return _call(lib.b2_window_attention_fwd, _capi.WINDOW_ATTENTION_ARGS, q, ld_q, k, ld_k, v, ld_v, batch, seq, heads,
+                     kv_heads, head_dim, kv_len, window, sinks, scale, out, ld_out)
 
     for name in ("q", "k", "v", "out"):
         assert call(**{name: None}) == 1, name
-        assert call(**{name: ctypes.c_void_p(8)}) == 2, name
+        assert call(**{name: 8}) == 2, name
     assert call(heads=3) == 1 and call(kv_heads=0) == 1 and call(batch=-1) == 1 and call(scale=-1.0) == 1
     assert call(window=-1) == 1 and call(sinks=-1) == 1 and call(window=0) == 1  # sinks without a window
     assert call(head_dim=48) == 2 and call(head_dim=256, ld_q=1024, ld_k=512, ld_v=512, ld_out=1024) == 2

@@ -13,6 +13,7 @@ CUDA stream; all arithmetic happens in the CUDA kernels.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 from typing import Optional, Tuple
@@ -45,7 +46,11 @@ class KVCacheDesc(ctypes.Structure):
                 ("dtype", ctypes.c_int)]
 
 
-_cache_p = ctypes.POINTER(KVCacheDesc)
+# The argument structs of the serving entry points: every member is 8 bytes wide, pointers as integers.
+ROTARY_ARGS = struct.Struct("13q")
+CACHE_APPEND_ARGS = struct.Struct("23q")
+CACHE_ATTENTION_ARGS = struct.Struct("11qd4q")
+WINDOW_ATTENTION_ARGS = struct.Struct("14qd2q")
 SIGNATURES = {
     "b2_abi_version": (ctypes.c_int, []),
     "b2_last_error": (ctypes.c_char_p, []),
@@ -98,25 +103,12 @@ SIGNATURES = {
     "b2_layernorm_gather_fwd": (
         ctypes.c_int, [_vp, _vp, _vp, ctypes.c_float, ctypes.POINTER(_vp), ctypes.c_int, _vp, _i64, _i64, _vp],
     ),
-    "b2_rotary_fwd": (
-        ctypes.c_int,
-        [_vp, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, _vp, _vp, _i64, _vp, _i64, _vp],
-    ),
-    "b2_cache_append_fwd": (
-        ctypes.c_int,
-        [_cache_p, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64,
-         ctypes.c_int, _vp, _i64, _vp, _i64, _vp],
-    ),
-    "b2_window_attention_fwd": (
-        ctypes.c_int,
-        [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, ctypes.c_float, _vp, _i64, _vp],
-    ),
+    "b2_rotary_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
+    "b2_cache_append_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
+    "b2_cache_attention_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
+    "b2_window_attention_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
     "b2_cache_attention_workspace": (
         ctypes.c_int, [_i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.POINTER(_i64)],
-    ),
-    "b2_cache_attention_fwd": (
-        ctypes.c_int,
-        [_cache_p, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, ctypes.c_float, _vp, _i64, _vp, _i64, _vp],
     ),
 }
 
@@ -535,32 +527,34 @@ def linear_bcast(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
     _check(status, "b2_linear_bcast_fwd")
 
 
+_BF16, _INT32 = torch.bfloat16, torch.int32
+
+
 def _rows(t: torch.Tensor, name: str) -> int:
     """Row stride of a bf16 CUDA matrix whose rows are contiguous (a column slice of packed rows is one)."""
     stride = t.stride()
-    if len(stride) != 2 or stride[1] != 1 or t.dtype is not torch.bfloat16 or not t.is_cuda:
+    if len(stride) != 2 or stride[1] != 1 or t.dtype is not _BF16 or not t.is_cuda:
         if not t.is_cuda:
             raise ValueError(f"{name} must be a CUDA tensor (this package has no CPU path)")
         if t.dtype != torch.bfloat16:
             raise ValueError(f"{name} must be {torch.bfloat16}, got {t.dtype}")
         raise ValueError(f"{name} must be 2-D with contiguous rows")
     # A single row's stride may be anything: its length takes the place.
-    return stride[0] if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
+    return stride[0] if t.size(0) > 1 else (t.size(1) + 7) // 8 * 8
 
 
 def _table(t: torch.Tensor) -> Tuple[int, int]:
     """(positions, rotary_dim) of a rotary table [positions, rotary_dim / 2, 2]."""
-    shape = t.shape
-    if len(shape) != 3 or shape[2] != 2:
+    if t.dim() != 3 or t.size(2) != 2:
         raise ValueError("table must be [positions, rotary_dim / 2, 2]")
     _require(t, torch.float32, "table")
-    return shape[0], 2 * shape[1]
+    return t.size(0), 2 * t.size(1)
 
 
 def _indices(t: torch.Tensor, n: int, name: str) -> int:
     """Pointer of n contiguous int32 entries on the GPU."""
-    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous():
-        _require(t, torch.int32, name)
+    if t.dtype is not _INT32 or not t.is_cuda or not t.is_contiguous():
+        _require(t, _INT32, name)
     if t.numel() != n:
         raise ValueError(f"{name} must have {n} entries, got {t.numel()}")
     return t.data_ptr()
@@ -568,25 +562,24 @@ def _indices(t: torch.Tensor, n: int, name: str) -> int:
 
 def _page_table(t: torch.Tensor, batch: int) -> Tuple[int, int]:
     """(pointer, pages per sequence) of an int32 page table."""
-    shape = t.shape
-    if len(shape) != 2 or shape[0] != batch:
-        raise ValueError(f"page_table must be [{batch}, pages], got {tuple(shape)}")
-    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous():
-        _require(t, torch.int32, "page_table")
-    return t.data_ptr(), shape[1]
+    if t.dim() != 2 or t.size(0) != batch:
+        raise ValueError(f"page_table must be [{batch}, pages], got {tuple(t.shape)}")
+    if t.dtype is not _INT32 or not t.is_cuda or not t.is_contiguous():
+        _require(t, _INT32, "page_table")
+    return t.data_ptr(), t.size(1)
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, head_dim: int, out: torch.Tensor,
            interleaved: bool = False, inverse: bool = False) -> None:
     """out = the rows of x with every head turned by its row's position (see b2_rotary_fwd)."""
     ld_x, ld_out = _rows(x, "x"), _rows(out, "out")
-    tokens, width = x.shape
-    if width % head_dim or out.shape != x.shape:
+    tokens, width = x.size(0), x.size(1)
+    if width % head_dim or out.size(0) != tokens or out.size(1) != width:
         raise ValueError(f"x and out must both be [tokens, heads * {head_dim}]")
     most, rotary_dim = _table(table)
-    status = load_library().b2_rotary_fwd(
+    status = load_library().b2_rotary_fwd(ROTARY_ARGS.pack(
         x.data_ptr(), ld_x, tokens, width // head_dim, head_dim, rotary_dim, interleaved, inverse,
-        _indices(positions, tokens, "positions"), table.data_ptr(), most, out.data_ptr(), ld_out, _stream_ptr(x.device))
+        _indices(positions, tokens, "positions"), table.data_ptr(), most, out.data_ptr(), ld_out), _stream_ptr(x.device))
     if status:
         _check(status, "b2_rotary_fwd")
 
@@ -597,7 +590,7 @@ def cache_append(cache: KVCacheDesc, qkv: torch.Tensor, num_heads: int, q_col: i
                  q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None) -> None:
     """Stores (and with `table` rotates) the new tokens of packed rows qkv (see b2_cache_append_fwd)."""
     ld = _rows(qkv, "qkv")
-    batch, tokens = new_len.numel(), qkv.shape[0]
+    batch, tokens = new_len.numel(), qkv.size(0)
     pages, table_pages = _page_table(page_table, batch)
     positions = rotary_dim = ld_q = ld_k = 0
     if table is not None:
@@ -606,16 +599,18 @@ def cache_append(cache: KVCacheDesc, qkv: torch.Tensor, num_heads: int, q_col: i
             raise ValueError("a rotation needs q_out")
     if q_out is not None:
         ld_q = _rows(q_out, "q_out")
-        if table is None or q_out.shape != (tokens, num_heads * cache.head_dim):
+        if table is None or q_out.size(0) != tokens or q_out.size(1) != num_heads * cache.head_dim:
             raise ValueError("q_out needs a table and the shape [tokens, num_heads * head_dim]")
     if k_out is not None:
         ld_k = _rows(k_out, "k_out")
-        if k_out.shape != (tokens, cache.kv_heads * cache.head_dim):
+        if k_out.size(0) != tokens or k_out.size(1) != cache.kv_heads * cache.head_dim:
             raise ValueError("k_out must be [tokens, kv_heads * head_dim]")
-    status = load_library().b2_cache_append_fwd(
-        cache, qkv.data_ptr(), ld, q_col, k_col, v_col, tokens, num_heads, batch, _indices(new_start, batch, "new_start"),
-        _indices(new_len, batch, "new_len"), _indices(past_len, batch, "past_len"), pages, table_pages, max_new,
-        _ptr(table), positions, rotary_dim, interleaved, _ptr(q_out), ld_q, _ptr(k_out), ld_k, _stream_ptr(qkv.device))
+    status = load_library().b2_cache_append_fwd(CACHE_APPEND_ARGS.pack(
+        ctypes.addressof(cache), qkv.data_ptr(), ld, q_col, k_col, v_col, tokens, num_heads, batch,
+        _indices(new_start, batch, "new_start"), _indices(new_len, batch, "new_len"),
+        _indices(past_len, batch, "past_len"), pages, table_pages, max_new, 0 if table is None else table.data_ptr(),
+        positions, rotary_dim, interleaved, 0 if q_out is None else q_out.data_ptr(), ld_q,
+        0 if k_out is None else k_out.data_ptr(), ld_k), _stream_ptr(qkv.device))
     if status:
         _check(status, "b2_cache_append_fwd")
 
@@ -633,17 +628,18 @@ def cache_attention(cache: KVCacheDesc, q: torch.Tensor, q_len: int, page_table:
                     window: int, sinks: int, scale: float, out: torch.Tensor, workspace: torch.Tensor) -> None:
     """out = attention of the q_len newest tokens of each sequence over the cache (see b2_cache_attention_fwd)."""
     ld_q, ld_out = _rows(q, "q"), _rows(out, "out")
-    rows, width = q.shape
+    rows, width = q.size(0), q.size(1)
     batch = kv_len.numel()
     pages, table_pages = _page_table(page_table, batch)
     if rows != batch * q_len:
         raise ValueError("q needs q_len rows and kv_len an entry per sequence")
-    if width % cache.head_dim or out.shape != q.shape:
+    head_dim = cache.head_dim
+    if width % head_dim or out.size(0) != rows or out.size(1) != width:
         raise ValueError("q and out must both be [batch * q_len, heads * head_dim]")
-    status = load_library().b2_cache_attention_fwd(
-        cache, q.data_ptr(), ld_q, batch, q_len, width // cache.head_dim, pages, table_pages,
+    status = load_library().b2_cache_attention_fwd(CACHE_ATTENTION_ARGS.pack(
+        ctypes.addressof(cache), q.data_ptr(), ld_q, batch, q_len, width // head_dim, pages, table_pages,
         _indices(kv_len, batch, "kv_len"), window, sinks, scale, out.data_ptr(), ld_out, workspace.data_ptr(),
-        workspace.numel(), _stream_ptr(q.device))
+        workspace.numel()), _stream_ptr(q.device))
     if status:
         _check(status, "b2_cache_attention_fwd")
 
@@ -652,14 +648,15 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: i
                      window: int, sinks: int, kv_len: Optional[torch.Tensor], scale: float, out: torch.Tensor) -> None:
     """out = causal attention with a sliding window and sinks (see b2_window_attention_fwd)."""
     ld_q, ld_k, ld_v, ld_out = _rows(q, "q"), _rows(k, "k"), _rows(v, "v"), _rows(out, "out")
-    (rows, width), (k_rows, k_width) = q.shape, k.shape
-    if rows != batch * seq_len or k_rows != rows or v.shape != k.shape or out.shape != q.shape:
+    rows, width, k_width = q.size(0), q.size(1), k.size(1)
+    if (rows != batch * seq_len or k.size(0) != rows or v.size(0) != rows or out.size(0) != rows or v.size(1) != k_width
+            or out.size(1) != width):
         raise ValueError("q, k, v and out must have batch * seq_len rows, k and v alike, out like q")
     if width % head_dim or k_width % head_dim:
         raise ValueError(f"q and k must be whole heads of {head_dim}")
-    status = load_library().b2_window_attention_fwd(
+    status = load_library().b2_window_attention_fwd(WINDOW_ATTENTION_ARGS.pack(
         q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(), ld_v, batch, seq_len, width // head_dim,
-        k_width // head_dim, head_dim, None if kv_len is None else _indices(kv_len, batch, "kv_len"), window, sinks, scale,
-        out.data_ptr(), ld_out, _stream_ptr(q.device))
+        k_width // head_dim, head_dim, 0 if kv_len is None else _indices(kv_len, batch, "kv_len"), window, sinks, scale,
+        out.data_ptr(), ld_out), _stream_ptr(q.device))
     if status:
         _check(status, "b2_window_attention_fwd")

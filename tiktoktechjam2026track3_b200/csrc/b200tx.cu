@@ -445,9 +445,10 @@ B2_API int b2_linear_bcast_fwd(const void* a, const void* w, const void* bias, i
                       "b2_linear_bcast_fwd");
 }
 
-B2_API int b2_rotary_fwd(const void* x, int64_t ld_x, int64_t tokens, int64_t heads, int64_t head_dim,
-                         int64_t rotary_dim, int interleaved, int inverse, const int32_t* positions,
-                         const float* table, int64_t max_positions, void* out, int64_t ld_out, void* stream) {
+B2_API int b2_rotary_fwd(const b2_rotary_args* args, void* stream) {
+  if (args == nullptr) return fail(1, "b2_rotary_fwd: null pointer argument");
+  const auto [x, ld_x, tokens, heads, head_dim, rotary_dim, interleaved, inverse, positions, table, max_positions, out,
+              ld_out] = *args;
   if (tokens < 0 || heads <= 0 || max_positions <= 0)
     return fail(1, "b2_rotary_fwd: invalid shape tokens=%lld heads=%lld max_positions=%lld", (long long)tokens,
                 (long long)heads, (long long)max_positions);
@@ -478,7 +479,7 @@ B2_API int b2_rotary_fwd(const void* x, int64_t ld_x, int64_t tokens, int64_t he
   p.inverse = inverse != 0;
   int dev = 0;
   cudaGetDevice(&dev);
-  return check_launch(launch_rotary(p, interleaved, device_sm_count(dev), static_cast<cudaStream_t>(stream)),
+  return check_launch(launch_rotary(p, interleaved != 0, device_sm_count(dev), static_cast<cudaStream_t>(stream)),
                       "b2_rotary_fwd");
 }
 
@@ -516,12 +517,10 @@ static int cache_pages(const b2_kv_cache* c, const char* what, CachePages* out, 
   return 0;
 }
 
-B2_API int b2_cache_append_fwd(const b2_kv_cache* cache, const void* qkv, int64_t ld_qkv, int64_t q_col,
-                               int64_t k_col, int64_t v_col, int64_t tokens, int64_t num_heads, int64_t batch,
-                               const int32_t* new_start, const int32_t* new_len, const int32_t* past_len,
-                               const int32_t* page_table, int64_t table_pages, int64_t max_new, const float* table,
-                               int64_t max_positions, int64_t rotary_dim, int interleaved, void* q_out,
-                               int64_t ld_q_out, void* k_out, int64_t ld_k_out, void* stream) {
+B2_API int b2_cache_append_fwd(const b2_cache_append_args* args, void* stream) {
+  if (args == nullptr) return fail(1, "b2_cache_append_fwd: null pointer argument");
+  const auto [cache, qkv, ld_qkv, q_col, k_col, v_col, tokens, num_heads, batch, new_start, new_len, past_len, page_table,
+              table_pages, max_new, table, max_positions, rotary_dim, interleaved, q_out, ld_q_out, k_out, ld_k_out] = *args;
   AppendParams p{};
   bool fp8 = false;
   if (const int rc = cache_pages(cache, "b2_cache_append_fwd", &p.c, &fp8)) return rc;
@@ -574,7 +573,7 @@ B2_API int b2_cache_append_fwd(const b2_kv_cache* cache, const void* qkv, int64_
   p.k_out = static_cast<__nv_bfloat16*>(k_out);
   p.ld_q_out = ld_q_out;
   p.ld_k_out = ld_k_out;
-  return check_launch(launch_cache_append(p, max_new, fp8, interleaved, static_cast<cudaStream_t>(stream)),
+  return check_launch(launch_cache_append(p, max_new, fp8, interleaved != 0, static_cast<cudaStream_t>(stream)),
                       "b2_cache_append_fwd");
 }
 
@@ -593,10 +592,11 @@ B2_API int b2_cache_attention_workspace(int64_t batch, int64_t q_len, int64_t nu
   return 0;
 }
 
-B2_API int b2_cache_attention_fwd(const b2_kv_cache* cache, const void* q, int64_t ld_q, int64_t batch, int64_t q_len,
-                                  int64_t num_heads, const int32_t* page_table, int64_t table_pages,
-                                  const int32_t* kv_len, int64_t window, int64_t sinks, float scale, void* out,
-                                  int64_t ld_out, void* workspace, int64_t workspace_bytes, void* stream) {
+B2_API int b2_cache_attention_fwd(const b2_cache_attention_args* args, void* stream) {
+  if (args == nullptr) return fail(1, "b2_cache_attention_fwd: null pointer argument");
+  const auto [cache, q, ld_q, batch, q_len, num_heads, page_table, table_pages, kv_len, window, sinks, scale64, out, ld_out,
+              workspace, workspace_bytes] = *args;
+  const float scale = static_cast<float>(scale64);
   CacheAttnParams p{};
   bool fp8 = false;
   if (const int rc = cache_pages(cache, "b2_cache_attention_fwd", &p.c, &fp8)) return rc;
@@ -647,10 +647,11 @@ B2_API int b2_cache_attention_fwd(const b2_kv_cache* cache, const void* q, int64
                       "b2_cache_attention_fwd");
 }
 
-B2_API int b2_window_attention_fwd(const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* v,
-                                   int64_t ld_v, int64_t batch, int64_t seq_len, int64_t num_heads, int64_t kv_heads,
-                                   int64_t head_dim, const int32_t* kv_len, int64_t window, int64_t sinks, float scale,
-                                   void* out, int64_t ld_out, void* stream) {
+B2_API int b2_window_attention_fwd(const b2_window_attention_args* args, void* stream) {
+  if (args == nullptr) return fail(1, "b2_window_attention_fwd: null pointer argument");
+  const auto [q, ld_q, k, ld_k, v, ld_v, batch, seq_len, num_heads, kv_heads, head_dim, kv_len, window, sinks, scale64, out,
+              ld_out] = *args;
+  const float scale = static_cast<float>(scale64);
   if (batch < 0 || seq_len < 0 || num_heads <= 0 || kv_heads <= 0) return fail(1, "b2_window_attention_fwd: invalid shape");
   if (num_heads % kv_heads != 0)
     return fail(1, "b2_window_attention_fwd: num_heads=%lld must be a multiple of kv_heads=%lld", (long long)num_heads,

@@ -163,7 +163,7 @@ class KVCache:
         qkv's own columns. max_new (host) is at least every new_len.
         """
         d, hk = self.head_dim, self.kv_heads
-        if qkv.shape[-1] != (num_heads + 2 * hk) * d:
+        if qkv.size(-1) != (num_heads + 2 * hk) * d:
             raise ValueError(f"qkv must be [tokens, {(num_heads + 2 * hk) * d}], got {tuple(qkv.shape)}")
         if table is not None and q_out is None:
             q_out = torch.empty(qkv.shape[0], num_heads * d, dtype=qkv.dtype, device=qkv.device)
@@ -199,7 +199,7 @@ class KVCache:
     def _workspace(self, q: torch.Tensor, q_len: int) -> torch.Tensor:
         """The current stream's workspace, kept between calls (those of one stream run one after the other) and made
         anew when a call is larger than all before it."""
-        need = (q.shape[0] // q_len, q.shape[1] // self.head_dim, q_len)
+        need = (q.size(0) // q_len, q.size(1) // self.head_dim, q_len)
         stream = _capi._stream_ptr(q.device)
         kept = self._workspaces.get(stream)
         if kept is not None and need[0] <= kept[0][0] and need[1] <= kept[0][1] and need[2] <= kept[0][2]:
