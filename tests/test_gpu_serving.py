@@ -309,8 +309,12 @@ ATTENDS = [
 
 @pytest.mark.parametrize("lengths,page,heads,kv_heads,head_dim,q_len,window,sinks", ATTENDS)
 @pytest.mark.parametrize("dtype", [E4M3, BF16])
-def test_attend(lengths, page, heads, kv_heads, head_dim, q_len, window, sinks, dtype):
+@pytest.mark.parametrize("room", [0, 1 << 17])
+def test_attend(lengths, page, heads, kv_heads, head_dim, q_len, window, sinks, dtype, room):
+    """`room`: tokens that the page table has columns for. Short tables give each head to one CTA, long ones (without a
+    window) cut the heads into stretches."""
     cache, seqs = _filled(lengths, page, kv_heads, head_dim, dtype, sum(lengths) + heads)
+    seqs.table = torch.nn.functional.pad(seqs.table, (0, max(0, room // page - seqs.table.shape[1])), value=-1)
     g = _gen(heads)
     rows = len(lengths) * q_len
     packed = torch.randn(rows, heads * head_dim + 16, generator=g).bfloat16().cuda()
@@ -339,11 +343,12 @@ def test_attend_scores_far_apart(dtype):
     _check_attend(cache, seqs, [n], 4, 1, 0, 0, q, out, d**-0.5)
 
 
-def test_attend_many_sequences_and_workspace_reuse():
+@pytest.mark.parametrize("room", [0, 1 << 17])
+def test_attend_many_sequences_and_workspace_reuse(room):
     """More sequences than threads of a CTA, then a smaller and a larger call on the same stream's workspace."""
     lengths = [(37 * b) % 90 for b in range(300)]
     cache, seqs = _filled([max(1, n) for n in lengths], 16, 2, 32, E4M3, 9)
-    table = seqs.table.cuda()
+    table = torch.nn.functional.pad(seqs.table, (0, max(0, room // 16 - seqs.table.shape[1])), value=-1).cuda()
     q = torch.randn(300, 4 * 32, generator=_gen(3)).bfloat16().cuda()
     out = cache.attend(q, table, _i32(lengths))
     _check_attend(cache, seqs, lengths, 4, 1, 0, 0, q, out, 32**-0.5)
@@ -354,10 +359,25 @@ def test_attend_many_sequences_and_workspace_reuse():
     assert torch.equal(cache.attend(q, table, _i32(lengths)), out)
 
 
-def test_attend_on_another_stream_and_in_a_graph():
+@pytest.mark.parametrize("head_dim,heads,dtype", [(64, 3, E4M3), (128, 12, E4M3), (128, 4, E4M3), (128, 10, BF16),
+                                                  (64, 16, BF16), (32, 1, BF16), (128, 8, BF16)])
+@pytest.mark.parametrize("room", [0, 1 << 17])
+def test_attend_more_sequences_than_sms(head_dim, heads, dtype, room):
+    """A quarter of an SM to each sequence, or stretches that hold several of them."""
+    lengths = [(53 * b) % 211 for b in range(160)]
+    cache, seqs = _filled([max(1, n) for n in lengths], 32, 1, head_dim, dtype, 3)
+    table = torch.nn.functional.pad(seqs.table, (0, max(0, room // 32 - seqs.table.shape[1])), value=-1)
+    q = torch.randn(160, heads * head_dim, generator=_gen(3)).bfloat16().cuda()
+    out = cache.attend(q, table.cuda(), _i32(lengths))
+    _check_attend(cache, seqs, lengths, heads, 1, 0, 0, q, out, head_dim**-0.5)
+
+
+@pytest.mark.parametrize("room", [0, 1 << 17])
+def test_attend_on_another_stream_and_in_a_graph(room):
     lengths = [3000, 11]
     cache, seqs = _filled(lengths, 32, 2, 64, E4M3, 4)
-    table, n = seqs.table.cuda(), _i32(lengths)
+    table = torch.nn.functional.pad(seqs.table, (0, max(0, room // 32 - seqs.table.shape[1])), value=-1).cuda()
+    n = _i32(lengths)
     q = torch.randn(2, 8 * 64, generator=_gen(3)).bfloat16().cuda()
     want = cache.attend(q, table, n)
     side = torch.cuda.Stream()
@@ -380,7 +400,9 @@ def test_attend_indices_outside_their_tables():
     cache, seqs = _filled([40], 16, 1, 32, E4M3, 1)
     q = torch.randn(1, 32, generator=_gen(1)).bfloat16().cuda()
     table = seqs.table.cuda()
-    for bad_table, n, site in ((table, 49, 1), (table, -1, 1), (torch.full_like(table, 1000), 40, 2)):
+    wide = torch.nn.functional.pad(table, (0, 8192), value=1000)
+    for bad_table, n, site in ((table, 49, 1), (table, -1, 1), (torch.full_like(table, 1000), 40, 2), (wide, 60, 2),
+                               (wide, 1 << 20, 1), (wide, -1, 1)):
         cache.attend(q, bad_table, _i32([n]))
         torch.cuda.synchronize()
         assert _capi.device_status(clear=True) == (7 << 16) | (site << 8) | 3

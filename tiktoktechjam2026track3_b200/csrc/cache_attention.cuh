@@ -23,10 +23,11 @@
 // The maximum moves only when a score exceeds it by 2^8 (the weights keep 2^7 of headroom below fp16's
 // subnormals); sums, maxima and outputs are fp32.
 //
-// Split: every (sequence, key head) is cut into units of 16 tokens per warp, all units of the call are laid on one line
-// and the CTAs take equal stretches of it, so that one long sequence among short ones, and few sequences on 148 SMs, fill the
-// machine alike. A CTA whose stretch holds only part of a (sequence, head) leaves its maximum, sum and
-// output in the workspace; the last one to arrive (a counter) joins them, in the order of the stretches.
+// Split: short calls give every (sequence, key head) to one CTA. Else each is cut into units of 16 tokens per warp, all
+// units of the call are laid on one line and the CTAs take equal stretches of it, so that one long sequence among short
+// ones, and few sequences on 148 SMs, fill the machine alike. A CTA whose stretch holds only part of a (sequence, head)
+// leaves its maximum, sum and output in the workspace; the last one to arrive (a counter) joins them, in the order of
+// the stretches.
 //
 // What bounds a warp is the chain of one tile (loads, 8 dependent products, maximum, exponentials, products: about
 // 1500 cycles besides the loads), so the loads' latency is kept out of it: the lanes hold the page numbers of the
@@ -36,10 +37,12 @@
 // page number in the loop and joined element by element): 8 x 131072 8-bit tokens, 8 key heads of 128, 4 query heads
 // each: 327 (328; 355); 64 sequences of up to 8192: 116 (100; 129); one of 131072: 59 (41; 111), one of 8192: 17 (2.6; 22);
 // bf16, 32 x 8192: 166 (164; 181); 32 windows of 4096 bf16 tokens, 10 rows: 64 (41; 104); 16 key heads of 64: 186 (165;
-// 265), of 32: 121 (82; 226); 12 heads of 1001 tokens: 10.9 (0.2; 12.6). At the 1000 W limit the clock drops and the
-// first two take 368 and 125. A short call is 6 us of dependent steps (lengths, page numbers, keys, join of the warps),
+// 265), of 32: 121 (82; 226); 12 heads of 1001 tokens: 6.7 (0.2; 12.6). At the 1000 W limit the clock drops and the
+// first two take 368 and 125. A short call is 5 us of dependent steps (lengths, page numbers, keys, join of the warps),
 // a join of CTAs 3 to 5 more.
 #pragma once
+#include <algorithm>
+
 #include <cuda_fp16.h>
 
 #include "b2_common.cuh"
@@ -167,7 +170,7 @@ struct RowPieces {
   }
 };
 
-template <int HD, bool kFp8, int NT>
+template <int HD, bool kFp8, int NT, int kShare>
 struct CacheAttnCfg {
   static constexpr int kRows = 8 * NT;
   static constexpr int kBytes = kFp8 ? 1 : 2;
@@ -181,8 +184,10 @@ struct CacheAttnCfg {
   // sequences of up to 8192 tokens: 116 us, 122 in CTAs of 8), or of 6 where 12 is the number.
   static constexpr bool kWide = HD == 128 && (!kFp8 || NT == 2);
   static constexpr bool kSharedQ = NT == 2 || (HD == 128 && kFp8);
-  static constexpr int kCtasPerSm = kWide ? 2 : 4;
-  static constexpr int kWarps = kWide && (kFp8 || NT == 1) ? 6 : 4;
+  // kShare 1 or 4: a CTA takes a whole (sequence, head) with all the warps of an SM, or a quarter; 0: a stretch of the line.
+  static constexpr int kWarpsPerSm = !kWide ? 16 : kFp8 || NT == 1 ? 12 : 8;
+  static constexpr int kWarps = kShare > 0 ? kWarpsPerSm / kShare : kWarpsPerSm == 12 ? 6 : 4;
+  static constexpr int kCtasPerSm = kWarpsPerSm / kWarps;
   static constexpr int kThreads = 32 * kWarps;
   // Units of a CTA's stretch at least (not of a head's): shorter ones cost more in the join than they save.
   static constexpr int kLeast = 16 / kWarps;
@@ -208,10 +213,12 @@ __device__ __forceinline__ int seq_units(const CacheAttnParams& p, int b) {
 
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
-template <int HD, bool kFp8, int NT>
-__global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT>::kThreads, CacheAttnCfg<HD, kFp8, NT>::kCtasPerSm)
+template <int HD, bool kFp8, int NT, int kShare>
+__global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
+                                  CacheAttnCfg<HD, kFp8, NT, kShare>::kCtasPerSm)
     cache_attention_kernel(const CacheAttnParams p) {
-  using Cfg = CacheAttnCfg<HD, kFp8, NT>;
+  using Cfg = CacheAttnCfg<HD, kFp8, NT, kShare>;
+  constexpr bool kWhole = kShare > 0;
   using KPieces = RowPieces<Cfg::kKWords, 4>;
   using VPieces = RowPieces<Cfg::kVWords, 8>;
   constexpr int R = Cfg::kRows;
@@ -237,38 +244,42 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT>::kThreads, CacheAtt
   pdl_wait_previous_grid();
   pdl_allow_next_grid();
 
-  // First unit of each sequence on the line of all units.
-  int base = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += Cfg::kThreads) {
-    const int b = b0 + tid;
-    int v = b < p.batch ? seq_units<Cfg>(p, b) * kv_heads : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
-    }
-    if (lane == 31) s_scan[warp] = v;
-    __syncthreads();
-    int before = base;
-    int all = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      if (i < warp) before += s_scan[i];
-      all += s_scan[i];
-    }
-    if (b < p.batch) s_first[b + 1] = before + v;
-    base += all;
-    __syncthreads();
-  }
-  if (tid == 0) s_first[0] = 0;
-  __syncthreads();
-  const int64_t total = base;
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x),
-                           max(static_cast<int64_t>(p.batch) * kv_heads, (total + Cfg::kLeast - 1) / Cfg::kLeast));
   const int64_t cta = blockIdx.x;
-  if (cta >= ctas) return;
-  const int w_begin = static_cast<int>(cta * total / ctas);
-  const int w_end = static_cast<int>((cta + 1) * total / ctas);
+  int64_t total = 0, ctas = 0;    // of units; of the CTAs that take some
+  int w_begin = 0, w_end = 0;  // this one's stretch
+  if constexpr (!kWhole) {
+    // First unit of each sequence on the line of all units.
+    int base = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += Cfg::kThreads) {
+      const int b = b0 + tid;
+      int v = b < p.batch ? seq_units<Cfg>(p, b) * kv_heads : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      if (lane == 31) s_scan[warp] = v;
+      __syncthreads();
+      int before = base;
+      int all = 0;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+        if (i < warp) before += s_scan[i];
+        all += s_scan[i];
+      }
+      if (b < p.batch) s_first[b + 1] = before + v;
+      base += all;
+      __syncthreads();
+    }
+    if (tid == 0) s_first[0] = 0;
+    __syncthreads();
+    total = base;
+    ctas = min(static_cast<int64_t>(gridDim.x),
+               max(static_cast<int64_t>(p.batch) * kv_heads, (total + Cfg::kLeast - 1) / Cfg::kLeast));
+    if (cta >= ctas) return;
+    w_begin = static_cast<int>(cta * total / ctas);
+    w_end = static_cast<int>((cta + 1) * total / ctas);
+  }
 
   constexpr int kNoTile = 1 << 30;         // a first token that no row sees
   constexpr int kIds = 32 / kSub;          // units whose page numbers the lanes hold
@@ -322,7 +333,14 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT>::kThreads, CacheAtt
     }
   };
   Part now;
-  {
+  if constexpr (kWhole) {
+    now.b = static_cast<int>(blockIdx.x) / kv_heads;
+    now.h = static_cast<int>(blockIdx.x) - now.b * kv_heads;
+    now.seq = seq_tiles(p, seq_length(p, now.b));
+    now.units = max(1, (now.seq.count + Cfg::kUnitTiles - 1) / Cfg::kUnitTiles);
+    now.head_begin = now.u0 = 0;
+    now.u1 = now.units;
+  } else {
     int lo = 0, hi = p.batch;  // s_first[lo] <= w_begin < s_first[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -635,7 +653,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT>::kThreads, CacheAtt
           p.out + (static_cast<int64_t>(b) * p.q_len + row / p.group) * p.ld_out + (h * p.group + row % p.group) * HD + d) =
           pack_bf16x2(acc.x * inv, acc.y * inv);
     };
-    const bool whole = u1 - u0 == units;
+    const bool whole = kWhole || u1 - u0 == units;
     const int64_t mine = static_cast<int64_t>(blockIdx.y) * gridDim.x * 2;
     // Slot 0 of a CTA: the part of a head that began before its stretch (or with it); slot 1: of one that begins inside.
     float* partial = p.partials + (mine + cta * 2 + (w_begin >= head_begin ? 0 : 1)) * Cfg::kPartial;
@@ -666,7 +684,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT>::kThreads, CacheAtt
         }
       }
     }
-    if (!whole) {
+    if constexpr (!kWhole) if (!whole) {
       // Joins of CTAs' parts, in their order on the line. Up to kCacheAtOnce parts in one go; more (few sequences with few
       // key heads) first in groups of kCacheGroup CTAs, whose result takes the place of its first part.
       const int64_t c_first = ((static_cast<int64_t>(head_begin) + 1) * ctas - 1) / total;
@@ -780,7 +798,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT>::kThreads, CacheAtt
         }
       }
     }
-    if (head_begin + u1 >= w_end) break;
+    if (kWhole || head_begin + u1 >= w_end) break;
     __syncthreads();
     now = part_from(head_begin + u1, b);
   }
@@ -817,29 +835,58 @@ static int64_t cache_attention_workspace_bytes(int64_t batch, int64_t kv_heads, 
          cache_attention_partial_bytes(head_dim, rows, sm_count);
 }
 
-template <int HD, bool kFp8, int NT>
-static cudaError_t launch_cache_attention_t(const CacheAttnParams& p, dim3 grid, cudaStream_t stream) {
-  using Cfg = CacheAttnCfg<HD, kFp8, NT>;
-  grid.x = grid.x / 4 * Cfg::kCtasPerSm;
-  const size_t smem = Cfg::kSmemBytes + (static_cast<size_t>(p.batch) + 1) * 4;
+template <int HD, bool kFp8, int NT, int kShare>
+static cudaError_t launch_cache_attention_t(const CacheAttnParams& p, int64_t row_blocks, int sm_count, cudaStream_t stream) {
+  using Cfg = CacheAttnCfg<HD, kFp8, NT, kShare>;
+  const size_t smem = Cfg::kSmemBytes + (kShare > 0 ? 0 : (static_cast<size_t>(p.batch) + 1) * 4);
   static std::once_flag once[64];
   int dev = 0;
   cudaGetDevice(&dev);
   cudaError_t e = cudaSuccess;
   std::call_once(once[dev & 63], [&] {
-    e = cudaFuncSetAttribute(cache_attention_kernel<HD, kFp8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes + 4 * (kCacheMaxBatch + 1));
+    e = cudaFuncSetAttribute(cache_attention_kernel<HD, kFp8, NT, kShare>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Cfg::kSmemBytes + (kShare > 0 ? 0 : 4 * (kCacheMaxBatch + 1)));
   });
   if (e != cudaSuccess) return e;
-  return launch_pdl(cache_attention_kernel<HD, kFp8, NT>, grid, dim3(Cfg::kThreads), smem, stream, p);
+  const int ctas = kShare > 0 ? p.batch * p.c.kv_heads : sm_count * Cfg::kCtasPerSm;
+  return launch_pdl(cache_attention_kernel<HD, kFp8, NT, kShare>, dim3(ctas, static_cast<unsigned>(row_blocks)),
+                    dim3(Cfg::kThreads), smem, stream, p);
+}
+
+template <int HD, bool kFp8, int NT>
+static cudaError_t launch_cache_attention_nt(const CacheAttnParams& p, int64_t row_blocks, int sm_count, cudaStream_t stream) {
+  // The most tokens that a sequence can see (the host does not know their lengths), in units of a CTA.
+  int64_t tokens = static_cast<int64_t>(p.table_pages) << p.c.page_shift;
+  if (p.window > 0) tokens = std::min<int64_t>(tokens, static_cast<int64_t>(p.window) + p.sinks + p.q_len + 32);
+  const int64_t heads = static_cast<int64_t>(p.batch) * p.c.kv_heads * row_blocks;
+  // A head to a CTA saves the line's sums and the joins, about 5 us; a stretch saves what long or unlike heads would leave
+  // idle. Up to as many heads as SMs, a head gets an SM's warps while they are done with it in four rounds, or in 16
+  // where the heads leave at most two thirds of the SMs idle (us, heads / stretches, 8-bit heads of 128: 8 heads of 500
+  // tokens 7.7 / 10.9, of 1000 10.0 / 11.3, of 2000 14.2 / 11.8; 64 heads of 500 8.2 / 13.7, of 4000 25.8 / 27.9, of 8000
+  // 43.7 / 39.5). More heads get a quarter of an SM, in up to 16 rounds, or 32 where they are three times the SMs (256
+  // heads of 1000 tokens 20.8 / 28.0, of 4000 62.6 / 58.7; 512 heads of 1000 28.7 / 38.9, of 2000 47.8 / 57.2, of up to
+  // 4000 77.4 / 74.3).
+  if (heads <= sm_count) {
+    constexpr int kTokens = 16 * CacheAttnCfg<HD, kFp8, NT, 1>::kUnitTiles;
+    const int64_t rounds = (tokens + kTokens - 1) / kTokens;
+    if (rounds <= 4 || (rounds <= 16 && 3 * heads >= sm_count))
+      return launch_cache_attention_t<HD, kFp8, NT, 1>(p, row_blocks, sm_count, stream);
+  } else {
+    constexpr int kTokens = 16 * CacheAttnCfg<HD, kFp8, NT, 4>::kUnitTiles;
+    if (tokens <= (heads >= 3 * static_cast<int64_t>(sm_count) ? 32 : 16) * kTokens)
+      return launch_cache_attention_t<HD, kFp8, NT, 4>(p, row_blocks, sm_count, stream);
+  }
+  return launch_cache_attention_t<HD, kFp8, NT, 0>(p, row_blocks, sm_count, stream);
 }
 
 template <int HD>
-static cudaError_t launch_cache_attention_hd(const CacheAttnParams& p, bool fp8, int nt, dim3 grid, cudaStream_t stream) {
+static cudaError_t launch_cache_attention_hd(const CacheAttnParams& p, bool fp8, int nt, int64_t row_blocks, int sm_count,
+                                             cudaStream_t stream) {
   if (fp8)
-    return nt == 1 ? launch_cache_attention_t<HD, true, 1>(p, grid, stream)
-                   : launch_cache_attention_t<HD, true, 2>(p, grid, stream);
-  return nt == 1 ? launch_cache_attention_t<HD, false, 1>(p, grid, stream)
-                 : launch_cache_attention_t<HD, false, 2>(p, grid, stream);
+    return nt == 1 ? launch_cache_attention_nt<HD, true, 1>(p, row_blocks, sm_count, stream)
+                   : launch_cache_attention_nt<HD, true, 2>(p, row_blocks, sm_count, stream);
+  return nt == 1 ? launch_cache_attention_nt<HD, false, 1>(p, row_blocks, sm_count, stream)
+                 : launch_cache_attention_nt<HD, false, 2>(p, row_blocks, sm_count, stream);
 }
 
 // Counters from the start of the workspace, partial results up to its end: a workspace made for the largest batch and
@@ -853,14 +900,13 @@ static cudaError_t launch_cache_attention(CacheAttnParams p, void* workspace, in
   p.counters = p.group_counters + cache_attention_group_bytes(blocks, sm_count) / 4;
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + workspace_bytes / 256 * 256 -
                                         cache_attention_partial_bytes(p.c.head_dim, rows, sm_count));
-  const dim3 grid(static_cast<unsigned>(cache_attention_ctas(sm_count)), static_cast<unsigned>(blocks));
   switch (p.c.head_dim) {
     case 32:
-      return launch_cache_attention_hd<32>(p, fp8, nt, grid, stream);
+      return launch_cache_attention_hd<32>(p, fp8, nt, blocks, sm_count, stream);
     case 64:
-      return launch_cache_attention_hd<64>(p, fp8, nt, grid, stream);
+      return launch_cache_attention_hd<64>(p, fp8, nt, blocks, sm_count, stream);
     case 128:
-      return launch_cache_attention_hd<128>(p, fp8, nt, grid, stream);
+      return launch_cache_attention_hd<128>(p, fp8, nt, blocks, sm_count, stream);
     default:
       return cudaErrorInvalidValue;
   }
