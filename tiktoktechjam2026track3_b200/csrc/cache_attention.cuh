@@ -36,7 +36,7 @@
 // Measured on one B200 (us a call back to back, floor at the measured copy rate in brackets; first form, which read each
 // page number in the loop and joined element by element): 8 x 131072 8-bit tokens, 8 key heads of 128, 4 query heads
 // each: 327 (328; 355); 64 sequences of up to 8192: 116 (100; 129); one of 131072: 59 (41; 111), one of 8192: 17 (2.6; 22);
-// bf16, 32 x 8192: 166 (164; 181); 32 windows of 4096 bf16 tokens, 10 rows: 64 (41; 104); 16 key heads of 64: 186 (165;
+// bf16, 32 x 8192: 166 (164; 181); 32 windows of 4096 bf16 tokens, 10 rows: 52 (41; 104); 16 key heads of 64: 186 (165;
 // 265), of 32: 121 (82; 226); 12 heads of 1001 tokens: 6.7 (0.2; 12.6). At the 1000 W limit the clock drops and the
 // first two take 368 and 125. A short call is 5 us of dependent steps (lengths, page numbers, keys, join of the warps),
 // a join of CTAs 3 to 5 more.
@@ -855,26 +855,31 @@ static cudaError_t launch_cache_attention_t(const CacheAttnParams& p, int64_t ro
 
 template <int HD, bool kFp8, int NT>
 static cudaError_t launch_cache_attention_nt(const CacheAttnParams& p, int64_t row_blocks, int sm_count, cudaStream_t stream) {
-  // The most tokens that a sequence can see (the host does not know their lengths), in units of a CTA.
-  int64_t tokens = static_cast<int64_t>(p.table_pages) << p.c.page_shift;
-  if (p.window > 0) tokens = std::min<int64_t>(tokens, static_cast<int64_t>(p.window) + p.sinks + p.q_len + 32);
+  // The most tokens that a sequence can see; the host does not know their lengths.
+  const int64_t room = static_cast<int64_t>(p.table_pages) << p.c.page_shift;
+  const int64_t band = static_cast<int64_t>(p.window) + p.sinks + p.q_len + 32;
+  const bool windowed = p.window > 0 && band < room;
+  const int64_t tokens = windowed ? band : room;
+  // A head to a CTA saves the line's sums, the start of a second part and the joins, 5 to 15 us; a stretch saves what
+  // long or unlike heads leave idle. With s CTAs an SM (1 up to as many heads as SMs, else 4), heads fill some of their
+  // last s x 148 places. So each gets a CTA while that is done in at most (us: heads / stretches, 8-bit heads of 128)
+  //   32 rounds of its warps where two thirds are filled: 128 heads of 4096 tokens 28.9 / 39.4, of 8192 47.8 / 60.9, of
+  //      up to 8192 46.0 / 42.5, of up to 16384 83 / 73;
+  //   72 there behind a window, which makes lengths alike: windows of 4096, 100 heads 29.0 / 35.7, 512 heads 90.9 / 99.3
+  //      (of 8192 165.5 / 164.3), bf16 with 10 rows, 128 heads 51.6 / 64.0;
+  //   20 where one third is, or with 4 an SM: 64 heads of 4096 26.1 / 28.7, of up to 8192 43.2 / 30.6; 256 heads of 1000
+  //      20.8 / 28.0, of 4000 62.6 / 58.7;
+  //   4 else: 8 heads of 1000 10.0 / 11.3, of 2000 14.2 / 11.8.
   const int64_t heads = static_cast<int64_t>(p.batch) * p.c.kv_heads * row_blocks;
-  // A head to a CTA saves the line's sums and the joins, about 5 us; a stretch saves what long or unlike heads would leave
-  // idle. Up to as many heads as SMs, a head gets an SM's warps while they are done with it in four rounds, or in 16
-  // where the heads leave at most two thirds of the SMs idle (us, heads / stretches, 8-bit heads of 128: 8 heads of 500
-  // tokens 7.7 / 10.9, of 1000 10.0 / 11.3, of 2000 14.2 / 11.8; 64 heads of 500 8.2 / 13.7, of 4000 25.8 / 27.9, of 8000
-  // 43.7 / 39.5). More heads get a quarter of an SM, in up to 16 rounds, or 32 where they are three times the SMs (256
-  // heads of 1000 tokens 20.8 / 28.0, of 4000 62.6 / 58.7; 512 heads of 1000 28.7 / 38.9, of 2000 47.8 / 57.2, of up to
-  // 4000 77.4 / 74.3).
-  if (heads <= sm_count) {
-    constexpr int kTokens = 16 * CacheAttnCfg<HD, kFp8, NT, 1>::kUnitTiles;
-    const int64_t rounds = (tokens + kTokens - 1) / kTokens;
-    if (rounds <= 4 || (rounds <= 16 && 3 * heads >= sm_count))
+  const bool sm_each = heads <= sm_count;
+  const int64_t places = sm_each ? sm_count : 4 * static_cast<int64_t>(sm_count);
+  const int64_t thirds = 3 * heads / ((heads + places - 1) / places * places);
+  const int64_t most = thirds >= 2 ? (windowed ? 72 : 32) : thirds == 1 || !sm_each ? 20 : 4;
+  if (sm_each) {
+    if (tokens <= most * 16 * CacheAttnCfg<HD, kFp8, NT, 1>::kUnitTiles)
       return launch_cache_attention_t<HD, kFp8, NT, 1>(p, row_blocks, sm_count, stream);
-  } else {
-    constexpr int kTokens = 16 * CacheAttnCfg<HD, kFp8, NT, 4>::kUnitTiles;
-    if (tokens <= (heads >= 3 * static_cast<int64_t>(sm_count) ? 32 : 16) * kTokens)
-      return launch_cache_attention_t<HD, kFp8, NT, 4>(p, row_blocks, sm_count, stream);
+  } else if (tokens <= most * 16 * CacheAttnCfg<HD, kFp8, NT, 4>::kUnitTiles) {
+    return launch_cache_attention_t<HD, kFp8, NT, 4>(p, row_blocks, sm_count, stream);
   }
   return launch_cache_attention_t<HD, kFp8, NT, 0>(p, row_blocks, sm_count, stream);
 }
