@@ -372,6 +372,20 @@ def test_attend_more_sequences_than_sms(head_dim, heads, dtype, room):
     _check_attend(cache, seqs, lengths, heads, 1, 0, 0, q, out, head_dim**-0.5)
 
 
+@pytest.mark.parametrize("batch", [1, 2, 3, 6, 9])  # clusters of 8 for 2 ... 12 heads, of 4 up to 32, of 2 up to 64
+@pytest.mark.parametrize("kv_heads,head_dim,heads,q_len,window,sinks,dtype", [
+    (2, 128, 8, 1, 0, 0, E4M3), (7, 64, 7, 1, 0, 0, BF16), (6, 128, 18, 3, 0, 0, BF16), (4, 32, 4, 2, 0, 0, E4M3),
+    (4, 64, 20, 2, 1500, 20, E4M3), (1, 128, 20, 1, 0, 0, E4M3), (7, 128, 14, 1, 2000, 4, BF16)])
+def test_attend_clusters(batch, kv_heads, head_dim, heads, q_len, window, sinks, dtype):
+    lengths = [2700, 0, 17, 1301, 640, 1, 2499, 128, 3][:batch]
+    cache, seqs = _filled([max(1, n) for n in lengths], 64, kv_heads, head_dim, dtype, batch)
+    q = torch.randn(batch * q_len, heads * head_dim, generator=_gen(5)).bfloat16().cuda()
+    args = dict(q_len=q_len, window=window, sinks=sinks)
+    out = cache.attend(q, seqs.table.cuda(), _i32(lengths), **args)
+    _check_attend(cache, seqs, lengths, heads, q_len, window, sinks, q, out, head_dim**-0.5)
+    assert torch.equal(cache.attend(q, seqs.table.cuda(), _i32(lengths), **args), out)
+
+
 @pytest.mark.parametrize("room", [0, 1 << 17])
 def test_attend_on_another_stream_and_in_a_graph(room):
     lengths = [3000, 11]

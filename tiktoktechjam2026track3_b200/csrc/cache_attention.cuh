@@ -23,11 +23,11 @@
 // The maximum moves only when a score exceeds it by 2^8 (the weights keep 2^7 of headroom below fp16's
 // subnormals); sums, maxima and outputs are fp32.
 //
-// Split: short calls give every (sequence, key head) to one CTA. Else each is cut into units of 16 tokens per warp, all
+// Split: a (sequence, key head) is cut into units of 16 tokens per warp. Calls of moderate length give each to one CTA,
+// or to a cluster of CTAs that share its units and join their maxima, sums and outputs through shared memory. Else all
 // units of the call are laid on one line and the CTAs take equal stretches of it, so that one long sequence among short
 // ones, and few sequences on 148 SMs, fill the machine alike. A CTA whose stretch holds only part of a (sequence, head)
-// leaves its maximum, sum and output in the workspace; the last one to arrive (a counter) joins them, in the order of
-// the stretches.
+// leaves its results in the workspace; the last one to arrive (a counter) joins them, in the order of the stretches.
 //
 // What bounds a warp is the chain of one tile (loads, 8 dependent products, maximum, exponentials, products: about
 // 1500 cycles besides the loads), so the loads' latency is kept out of it: the lanes hold the page numbers of the
@@ -35,7 +35,7 @@
 // or shared memory. Heads of 64 and 32 take 2 and 4 tiles of 16 tokens at a time, interleaved.
 // Measured on one B200 (us a call back to back, floor at the measured copy rate in brackets; first form, which read each
 // page number in the loop and joined element by element): 8 x 131072 8-bit tokens, 8 key heads of 128, 4 query heads
-// each: 327 (328; 355); 64 sequences of up to 8192: 116 (100; 129); one of 131072: 59 (41; 111), one of 8192: 17 (2.6; 22);
+// each: 327 (328; 355); 64 sequences of up to 8192: 116 (100; 129); one of 131072: 58 (41; 111), one of 8192: 13 (2.6; 22);
 // bf16, 32 x 8192: 166 (164; 181); 32 windows of 4096 bf16 tokens, 10 rows: 52 (41; 104); 16 key heads of 64: 186 (165;
 // 265), of 32: 121 (82; 226); 12 heads of 1001 tokens: 6.7 (0.2; 12.6). At the 1000 W limit the clock drops and the
 // first two take 368 and 125. A short call is 5 us of dependent steps (lengths, page numbers, keys, join of the warps),
@@ -69,6 +69,7 @@ struct CacheAttnParams {
 constexpr int kCacheMaxBatch = 4096;
 constexpr int kCacheAtOnce = 40;  // parts of a (sequence, head) that one CTA joins in one go;
 constexpr int kCacheGroup = 16;   // of more, so many in a first go
+constexpr int kCacheCluster = 8;  // CTAs of a cluster, at most
 constexpr float kCacheRescale = 8.f;   // log2: the maximum moves when a score exceeds it by more
 constexpr float kCacheHeadroom = 7.f;  // log2: weights are at most 2^(8 + 7), below fp16's largest
 
@@ -170,6 +171,23 @@ struct RowPieces {
   }
 };
 
+__device__ __forceinline__ int cluster_nctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return static_cast<int>(r);
+}
+// From a shared::cluster address.
+__device__ __forceinline__ float cluster_load(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+
 template <int HD, bool kFp8, int NT, int kShare>
 struct CacheAttnCfg {
   static constexpr int kRows = 8 * NT;
@@ -184,9 +202,10 @@ struct CacheAttnCfg {
   // sequences of up to 8192 tokens: 116 us, 122 in CTAs of 8), or of 6 where 12 is the number.
   static constexpr bool kWide = HD == 128 && (!kFp8 || NT == 2);
   static constexpr bool kSharedQ = NT == 2 || (HD == 128 && kFp8);
-  // kShare 1 or 4: a CTA takes a whole (sequence, head) with all the warps of an SM, or a quarter; 0: a stretch of the line.
+  // kShare 1 or 4: a CTA takes a whole (sequence, head) with all the warps of an SM, or a quarter; kCacheCluster: a
+  // cluster does, each CTA with those of an SM; 0: a stretch of the line.
   static constexpr int kWarpsPerSm = !kWide ? 16 : kFp8 || NT == 1 ? 12 : 8;
-  static constexpr int kWarps = kShare > 0 ? kWarpsPerSm / kShare : kWarpsPerSm == 12 ? 6 : 4;
+  static constexpr int kWarps = kShare > 0 ? kWarpsPerSm / (kShare == 4 ? 4 : 1) : kWarpsPerSm == 12 ? 6 : 4;
   static constexpr int kCtasPerSm = kWarpsPerSm / kWarps;
   static constexpr int kThreads = 32 * kWarps;
   // Units of a CTA's stretch at least (not of a head's): shorter ones cost more in the join than they save.
@@ -219,6 +238,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
     cache_attention_kernel(const CacheAttnParams p) {
   using Cfg = CacheAttnCfg<HD, kFp8, NT, kShare>;
   constexpr bool kWhole = kShare > 0;
+  constexpr bool kCluster = kShare == kCacheCluster;
   using KPieces = RowPieces<Cfg::kKWords, 4>;
   using VPieces = RowPieces<Cfg::kVWords, 8>;
   constexpr int R = Cfg::kRows;
@@ -333,13 +353,18 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
     }
   };
   Part now;
+  const int rank = kCluster ? static_cast<int>(cluster_ctarank()) : 0;
+  const int ranks = kCluster ? cluster_nctarank() : 1;  // a power of two
+  const int ranks_shift = __ffs(ranks) - 1;
   if constexpr (kWhole) {
-    now.b = static_cast<int>(blockIdx.x) / kv_heads;
-    now.h = static_cast<int>(blockIdx.x) - now.b * kv_heads;
+    const int head = static_cast<int>(blockIdx.x) >> ranks_shift;
+    now.b = head / kv_heads;
+    now.h = head - now.b * kv_heads;
     now.seq = seq_tiles(p, seq_length(p, now.b));
     now.units = max(1, (now.seq.count + Cfg::kUnitTiles - 1) / Cfg::kUnitTiles);
-    now.head_begin = now.u0 = 0;
-    now.u1 = now.units;
+    now.head_begin = 0;
+    now.u0 = static_cast<int>(static_cast<int64_t>(rank) * now.units >> ranks_shift);
+    now.u1 = static_cast<int>(static_cast<int64_t>(rank + 1) * now.units >> ranks_shift);
   } else {
     int lo = 0, hi = p.batch;  // s_first[lo] <= w_begin < s_first[hi]
     while (hi - lo > 1) {
@@ -653,10 +678,12 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
           p.out + (static_cast<int64_t>(b) * p.q_len + row / p.group) * p.ld_out + (h * p.group + row % p.group) * HD + d) =
           pack_bf16x2(acc.x * inv, acc.y * inv);
     };
-    const bool whole = kWhole || u1 - u0 == units;
+    const bool whole = kWhole ? !kCluster : u1 - u0 == units;
     const int64_t mine = static_cast<int64_t>(blockIdx.y) * gridDim.x * 2;
     // Slot 0 of a CTA: the part of a head that began before its stretch (or with it); slot 1: of one that begins inside.
-    float* partial = p.partials + (mine + cta * 2 + (w_begin >= head_begin ? 0 : 1)) * Cfg::kPartial;
+    // (Of a cluster: in shared memory.)
+    float* const s_partial = reinterpret_cast<float*>(s_dyn + Cfg::kSmemBytes);
+    float* partial = kWhole ? s_partial : p.partials + (mine + cta * 2 + (w_begin >= head_begin ? 0 : 1)) * Cfg::kPartial;
     for (int i = tid; i < rows * (HD / 2); i += Cfg::kThreads) {
       const int r = i / (HD / 2), d = 2 * (i - r * (HD / 2));
       float top = -INFINITY;
@@ -683,6 +710,40 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
           partial[R * HD + R + r] = sum;
         }
       }
+    }
+    if constexpr (kCluster) {
+      // The cluster's partial results, in the order of its CTAs, each of which joins a share of the outputs.
+      cluster_sync_all();
+      for (int i = rank * Cfg::kThreads + tid; i < rows * (HD / 2); i += ranks * Cfg::kThreads) {
+        const int r = i / (HD / 2), d = 2 * (i - r * (HD / 2));
+        float m_of[kCacheCluster], l_of[kCacheCluster];
+        float2 v_of[kCacheCluster];
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kCacheCluster; ++k) {
+          if (k < ranks) {
+            const uint32_t at = cluster_map_to_rank(s_partial, k);
+            m_of[k] = cluster_load(at + 4 * (R * HD + r));
+            l_of[k] = cluster_load(at + 4 * (R * HD + R + r));
+            v_of[k] = cluster_load2(at + 4 * (r * HD + d));
+            top = fmaxf(top, m_of[k]);
+          }
+        }
+        const float ref = top == -INFINITY ? 0.f : top;
+        float2 acc = make_float2(0.f, 0.f);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kCacheCluster; ++k) {
+          if (k < ranks) {
+            const float f = fast_exp2(m_of[k] - ref);
+            acc.x = fmaf(v_of[k].x, f, acc.x);
+            acc.y = fmaf(v_of[k].y, f, acc.y);
+            sum = fmaf(l_of[k], f, sum);
+          }
+        }
+        finish(r, d, acc, sum);
+      }
+      cluster_sync_all();  // nobody leaves while others read from it
     }
     if constexpr (!kWhole) if (!whole) {
       // Joins of CTAs' parts, in their order on the line. Up to kCacheAtOnce parts in one go; more (few sequences with few
@@ -835,20 +896,46 @@ static int64_t cache_attention_workspace_bytes(int64_t batch, int64_t kv_heads, 
          cache_attention_partial_bytes(head_dim, rows, sm_count);
 }
 
+// launch_pdl in clusters of `cluster` CTAs along x.
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, int cluster, size_t smem,
+                                      cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 2;
+  return cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...);
+}
+
 template <int HD, bool kFp8, int NT, int kShare>
-static cudaError_t launch_cache_attention_t(const CacheAttnParams& p, int64_t row_blocks, int sm_count, cudaStream_t stream) {
+static cudaError_t launch_cache_attention_t(const CacheAttnParams& p, int64_t row_blocks, int sm_count, cudaStream_t stream,
+                                            int cluster = 1) {
   using Cfg = CacheAttnCfg<HD, kFp8, NT, kShare>;
-  const size_t smem = Cfg::kSmemBytes + (kShare > 0 ? 0 : (static_cast<size_t>(p.batch) + 1) * 4);
+  constexpr int kClusterBytes = kShare == kCacheCluster ? Cfg::kPartial * 4 : 0;
+  const size_t smem = Cfg::kSmemBytes + (kShare > 0 ? kClusterBytes : (static_cast<size_t>(p.batch) + 1) * 4);
   static std::once_flag once[64];
   int dev = 0;
   cudaGetDevice(&dev);
   cudaError_t e = cudaSuccess;
   std::call_once(once[dev & 63], [&] {
     e = cudaFuncSetAttribute(cache_attention_kernel<HD, kFp8, NT, kShare>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Cfg::kSmemBytes + (kShare > 0 ? 0 : 4 * (kCacheMaxBatch + 1)));
+                             Cfg::kSmemBytes + (kShare > 0 ? kClusterBytes : 4 * (kCacheMaxBatch + 1)));
   });
   if (e != cudaSuccess) return e;
-  const int ctas = kShare > 0 ? p.batch * p.c.kv_heads : sm_count * Cfg::kCtasPerSm;
+  const int ctas = kShare > 0 ? p.batch * p.c.kv_heads * cluster : sm_count * Cfg::kCtasPerSm;
+  if (kShare == kCacheCluster)
+    return launch_pdl_cluster(cache_attention_kernel<HD, kFp8, NT, kShare>, dim3(ctas, static_cast<unsigned>(row_blocks)),
+                              dim3(Cfg::kThreads), cluster, smem, stream, p);
   return launch_pdl(cache_attention_kernel<HD, kFp8, NT, kShare>, dim3(ctas, static_cast<unsigned>(row_blocks)),
                     dim3(Cfg::kThreads), smem, stream, p);
 }
@@ -860,25 +947,37 @@ static cudaError_t launch_cache_attention_nt(const CacheAttnParams& p, int64_t r
   const int64_t band = static_cast<int64_t>(p.window) + p.sinks + p.q_len + 32;
   const bool windowed = p.window > 0 && band < room;
   const int64_t tokens = windowed ? band : room;
-  // A head to a CTA saves the line's sums, the start of a second part and the joins, 5 to 15 us; a stretch saves what
-  // long or unlike heads leave idle. With s CTAs an SM (1 up to as many heads as SMs, else 4), heads fill some of their
-  // last s x 148 places. So each gets a CTA while that is done in at most (us: heads / stretches, 8-bit heads of 128)
-  //   32 rounds of its warps where two thirds are filled: 128 heads of 4096 tokens 28.9 / 39.4, of 8192 47.8 / 60.9, of
-  //      up to 8192 46.0 / 42.5, of up to 16384 83 / 73;
-  //   72 there behind a window, which makes lengths alike: windows of 4096, 100 heads 29.0 / 35.7, 512 heads 90.9 / 99.3
-  //      (of 8192 165.5 / 164.3), bf16 with 10 rows, 128 heads 51.6 / 64.0;
-  //   20 where one third is, or with 4 an SM: 64 heads of 4096 26.1 / 28.7, of up to 8192 43.2 / 30.6; 256 heads of 1000
-  //      20.8 / 28.0, of 4000 62.6 / 58.7;
-  //   4 else: 8 heads of 1000 10.0 / 11.3, of 2000 14.2 / 11.8.
+  // A head to itself saves the line's sums, the start of a second part and the joins through global memory, 5 to 15 us;
+  // a stretch saves what long or unlike heads leave idle. Up to as many heads as SMs, each gets an SM; of more than two
+  // rounds of its warps, a cluster of 2, 4 or 8 SMs, up to one a round (8 heads of 1000 tokens: 8.3 us, 10.0 on one SM
+  // each). That leaves an eighth of the SMs over, or a quarter with eights, as clusters need theirs side by side (16 heads
+  // in eights ran in two turns: 15.5 us, 9.9 in fours). More heads get a quarter of an SM each. How many rounds
+  // are taken so depends on the share of the places, SMs or quarters, that the heads fill in their last turn.
+  // Measured, us, heads / stretches, 8-bit heads of 128 unless said:
+  //   two thirds, up to 32 rounds: 32 heads of 2000 tokens 10.2 / 14.7, of 16000 31.0 / 39.1, of up to 32000 48 / 47; 128 heads
+  //     of 4096 28.9 / 39.4, of up to 8192 46.0 / 42.5, of up to 16384 83 / 73; 512 heads of 2000 47.8 / 57.2;
+  //   two thirds behind a window, which makes lengths alike, up to 72: windows of 4096 of 100 heads 29.0 / 35.7, of 512
+  //     heads 90.9 / 99.3 (of 8192 165.5 / 164.3), of 128 bf16 heads with 10 rows 51.6 / 64.0;
+  //   a third, or in quarters, up to 20: 8 heads of 8000 12.5 / 19.5, of 32000 28.2 / 29.4, of 64000 47 / 39; 256 heads
+  //     of 1000 20.8 / 28.0, of 4000 62.6 / 58.7;
+  //   else up to 8: 4 heads of 8000 12.3 / 18.0, of 32000 25.5 / 20.3; 1 of 8000 11.7 / 13.4, of 16000 16.2 / 16.4.
   const int64_t heads = static_cast<int64_t>(p.batch) * p.c.kv_heads * row_blocks;
   const bool sm_each = heads <= sm_count;
+  const int64_t round = 16 * (sm_each ? CacheAttnCfg<HD, kFp8, NT, 1>::kUnitTiles : CacheAttnCfg<HD, kFp8, NT, 4>::kUnitTiles);
+  int cluster = 1;
+  if (sm_each && tokens > 2 * round) {
+    while (cluster < kCacheCluster && tokens > cluster * round &&
+           2 * cluster * heads * 8 <= (cluster == 4 ? 6 : 7) * static_cast<int64_t>(sm_count))
+      cluster *= 2;
+  }
   const int64_t places = sm_each ? sm_count : 4 * static_cast<int64_t>(sm_count);
-  const int64_t thirds = 3 * heads / ((heads + places - 1) / places * places);
-  const int64_t most = thirds >= 2 ? (windowed ? 72 : 32) : thirds == 1 || !sm_each ? 20 : 4;
-  if (sm_each) {
-    if (tokens <= most * 16 * CacheAttnCfg<HD, kFp8, NT, 1>::kUnitTiles)
-      return launch_cache_attention_t<HD, kFp8, NT, 1>(p, row_blocks, sm_count, stream);
-  } else if (tokens <= most * 16 * CacheAttnCfg<HD, kFp8, NT, 4>::kUnitTiles) {
+  const int64_t ctas = heads * cluster;
+  const int64_t thirds = 3 * ctas / ((ctas + places - 1) / places * places);
+  const int64_t most = thirds >= 2 ? (windowed ? 72 : 32) : thirds == 1 || !sm_each ? 20 : 8;
+  if (tokens <= most * cluster * round) {
+    if (cluster > 1)
+      return launch_cache_attention_t<HD, kFp8, NT, kCacheCluster>(p, row_blocks, sm_count, stream, cluster);
+    if (sm_each) return launch_cache_attention_t<HD, kFp8, NT, 1>(p, row_blocks, sm_count, stream);
     return launch_cache_attention_t<HD, kFp8, NT, 4>(p, row_blocks, sm_count, stream);
   }
   return launch_cache_attention_t<HD, kFp8, NT, 0>(p, row_blocks, sm_count, stream);
