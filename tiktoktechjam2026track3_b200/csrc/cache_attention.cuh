@@ -37,7 +37,7 @@
 // page number in the loop and joined element by element): 8 x 131072 8-bit tokens, 8 key heads of 128, 4 query heads
 // each: 327 (328; 355); 64 sequences of up to 8192: 116 (100; 129); one of 131072: 58 (41; 111), one of 8192: 13 (2.6; 22);
 // bf16, 32 x 8192: 166 (164; 181); 32 windows of 4096 bf16 tokens, 10 rows: 52 (41; 104); 16 key heads of 64: 186 (165;
-// 265), of 32: 121 (82; 226); 12 heads of 1001 tokens: 6.7 (0.2; 12.6). At the 1000 W limit the clock drops and the
+// 265), of 32: 112 (82; 226); 12 heads of 1001 tokens: 6.9 (0.2; 12.6). At the 1000 W limit the clock drops and the
 // first two take 368 and 125. A short call is 5 us of dependent steps (lengths, page numbers, keys, join of the warps),
 // a join of CTAs 3 to 5 more.
 #pragma once
