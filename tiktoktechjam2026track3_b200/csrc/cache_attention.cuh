@@ -69,7 +69,7 @@ struct CacheAttnParams {
 constexpr int kCacheMaxBatch = 4096;
 constexpr int kCacheAtOnce = 40;  // parts of a (sequence, head) that one CTA joins in one go;
 constexpr int kCacheGroup = 16;   // of more, so many in a first go
-constexpr int kCacheCluster = 8;  // CTAs of a cluster, at most
+constexpr int kCacheCluster = 16;  // CTAs of a cluster, at most (a power of two)
 constexpr float kCacheRescale = 8.f;   // log2: the maximum moves when a score exceeds it by more
 constexpr float kCacheHeadroom = 7.f;  // log2: weights are at most 2^(8 + 7), below fp16's largest
 
@@ -896,46 +896,76 @@ static int64_t cache_attention_workspace_bytes(int64_t batch, int64_t kv_heads, 
          cache_attention_partial_bytes(head_dim, rows, sm_count);
 }
 
-// launch_pdl in clusters of `cluster` CTAs along x.
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, int cluster, size_t smem,
-                                      cudaStream_t stream, Args&&... args) {
+// A launch with programmatic dependence in clusters of `cluster` CTAs along x.
+struct CacheClusterLaunch {
   cudaLaunchConfig_t config = {};
-  config.gridDim = grid;
-  config.blockDim = block;
-  config.dynamicSmemBytes = smem;
-  config.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attr;
-  config.numAttrs = 2;
-  return cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...);
+  CacheClusterLaunch(dim3 grid, int threads, int cluster, size_t smem, cudaStream_t stream) {
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attr;
+    config.numAttrs = 2;
+  }
+};
+
+// How many clusters of `cluster` CTAs run side by side on the current device. (It depends on which SMs a GPU has in each
+// of its parts: 16 SMs next to each other were found for 6 clusters, not for 8.)
+template <int HD, bool kFp8, int NT>
+static cudaError_t cache_attention_clusters(int cluster, int* side_by_side) {
+  using Cfg = CacheAttnCfg<HD, kFp8, NT, kCacheCluster>;
+  const auto kernel = cache_attention_kernel<HD, kFp8, NT, kCacheCluster>;
+  constexpr int kSmem = Cfg::kSmemBytes + Cfg::kPartial * 4;
+  static std::once_flag once[64];
+  static int fit[64][kCacheCluster + 1];
+  static cudaError_t result[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  dev &= 63;
+  std::call_once(once[dev], [&] {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    for (int c = 2; e == cudaSuccess && c <= kCacheCluster; c *= 2) {
+      const CacheClusterLaunch launch(dim3(c), Cfg::kThreads, c, kSmem, nullptr);
+      e = cudaOccupancyMaxActiveClusters(&fit[dev][c], kernel, &launch.config);
+    }
+    result[dev] = e;
+  });
+  *side_by_side = fit[dev][cluster];
+  return result[dev];
+}
+
+template <int HD, bool kFp8, int NT>
+static cudaError_t launch_cache_attention_cluster(const CacheAttnParams& p, int64_t row_blocks, int cluster,
+                                                  cudaStream_t stream) {
+  using Cfg = CacheAttnCfg<HD, kFp8, NT, kCacheCluster>;
+  const CacheClusterLaunch launch(dim3(p.batch * p.c.kv_heads * cluster, static_cast<unsigned>(row_blocks)), Cfg::kThreads,
+                                  cluster, Cfg::kSmemBytes + Cfg::kPartial * 4, stream);
+  return cudaLaunchKernelEx(&launch.config, cache_attention_kernel<HD, kFp8, NT, kCacheCluster>, p);
 }
 
 template <int HD, bool kFp8, int NT, int kShare>
-static cudaError_t launch_cache_attention_t(const CacheAttnParams& p, int64_t row_blocks, int sm_count, cudaStream_t stream,
-                                            int cluster = 1) {
+static cudaError_t launch_cache_attention_t(const CacheAttnParams& p, int64_t row_blocks, int sm_count, cudaStream_t stream) {
   using Cfg = CacheAttnCfg<HD, kFp8, NT, kShare>;
-  constexpr int kClusterBytes = kShare == kCacheCluster ? Cfg::kPartial * 4 : 0;
-  const size_t smem = Cfg::kSmemBytes + (kShare > 0 ? kClusterBytes : (static_cast<size_t>(p.batch) + 1) * 4);
+  const size_t smem = Cfg::kSmemBytes + (kShare > 0 ? 0 : (static_cast<size_t>(p.batch) + 1) * 4);
   static std::once_flag once[64];
   int dev = 0;
   cudaGetDevice(&dev);
   cudaError_t e = cudaSuccess;
   std::call_once(once[dev & 63], [&] {
     e = cudaFuncSetAttribute(cache_attention_kernel<HD, kFp8, NT, kShare>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Cfg::kSmemBytes + (kShare > 0 ? kClusterBytes : 4 * (kCacheMaxBatch + 1)));
+                             Cfg::kSmemBytes + (kShare > 0 ? 0 : 4 * (kCacheMaxBatch + 1)));
   });
   if (e != cudaSuccess) return e;
-  const int ctas = kShare > 0 ? p.batch * p.c.kv_heads * cluster : sm_count * Cfg::kCtasPerSm;
-  if (kShare == kCacheCluster)
-    return launch_pdl_cluster(cache_attention_kernel<HD, kFp8, NT, kShare>, dim3(ctas, static_cast<unsigned>(row_blocks)),
-                              dim3(Cfg::kThreads), cluster, smem, stream, p);
+  const int ctas = kShare > 0 ? p.batch * p.c.kv_heads : sm_count * Cfg::kCtasPerSm;
   return launch_pdl(cache_attention_kernel<HD, kFp8, NT, kShare>, dim3(ctas, static_cast<unsigned>(row_blocks)),
                     dim3(Cfg::kThreads), smem, stream, p);
 }
@@ -949,10 +979,10 @@ static cudaError_t launch_cache_attention_nt(const CacheAttnParams& p, int64_t r
   const int64_t tokens = windowed ? band : room;
   // A head to itself saves the line's sums, the start of a second part and the joins through global memory, 5 to 15 us;
   // a stretch saves what long or unlike heads leave idle. Up to as many heads as SMs, each gets an SM; of more than two
-  // rounds of its warps, a cluster of 2, 4 or 8 SMs, up to one a round (8 heads of 1000 tokens: 8.3 us, 10.0 on one SM
-  // each). That leaves an eighth of the SMs over, or a quarter with eights, as clusters need theirs side by side (16 heads
-  // in eights ran in two turns: 15.5 us, 9.9 in fours). More heads get a quarter of an SM each. How many rounds
-  // are taken so depends on the share of the places, SMs or quarters, that the heads fill in their last turn.
+  // rounds of its warps, a cluster of 2, 4, 8 or 16 SMs, up to one a round (8 heads of 1000 tokens: 8.3 us, 10.0 on one SM
+  // each; 4 of 16000 12.9 in sixteens, 16.4 in eights), as far as all heads' clusters run side by side (16 heads in eights
+  // took two turns, 15.5 us, 9.9 in fours). More heads get a quarter of an SM each. How many rounds are taken
+  // so depends on the share of the places, SMs or quarters, that the heads fill in their last turn.
   // Measured, us, heads / stretches, 8-bit heads of 128 unless said:
   //   two thirds, up to 32 rounds: 32 heads of 2000 tokens 10.2 / 14.7, of 16000 31.0 / 39.1, of up to 32000 48 / 47; 128 heads
   //     of 4096 28.9 / 39.4, of up to 8192 46.0 / 42.5, of up to 16384 83 / 73; 512 heads of 2000 47.8 / 57.2;
@@ -960,15 +990,19 @@ static cudaError_t launch_cache_attention_nt(const CacheAttnParams& p, int64_t r
   //     heads 90.9 / 99.3 (of 8192 165.5 / 164.3), of 128 bf16 heads with 10 rows 51.6 / 64.0;
   //   a third, or in quarters, up to 20: 8 heads of 8000 12.5 / 19.5, of 32000 28.2 / 29.4, of 64000 47 / 39; 256 heads
   //     of 1000 20.8 / 28.0, of 4000 62.6 / 58.7;
-  //   else up to 8: 4 heads of 8000 12.3 / 18.0, of 32000 25.5 / 20.3; 1 of 8000 11.7 / 13.4, of 16000 16.2 / 16.4.
+  //   else up to 8: 4 heads of 8000 10.4 / 18.0, of 32000 17.4 / 20.2; 1 of 8000 9.9 / 13.5, of 32000 16.7 / 17.1.
   const int64_t heads = static_cast<int64_t>(p.batch) * p.c.kv_heads * row_blocks;
   const bool sm_each = heads <= sm_count;
   const int64_t round = 16 * (sm_each ? CacheAttnCfg<HD, kFp8, NT, 1>::kUnitTiles : CacheAttnCfg<HD, kFp8, NT, 4>::kUnitTiles);
   int cluster = 1;
   if (sm_each && tokens > 2 * round) {
-    while (cluster < kCacheCluster && tokens > cluster * round &&
-           2 * cluster * heads * 8 <= (cluster == 4 ? 6 : 7) * static_cast<int64_t>(sm_count))
+    while (cluster < kCacheCluster && tokens > cluster * round) {
+      int side_by_side = 0;
+      const cudaError_t e = cache_attention_clusters<HD, kFp8, NT>(2 * cluster, &side_by_side);
+      if (e != cudaSuccess) return e;
+      if (heads > side_by_side) break;
       cluster *= 2;
+    }
   }
   const int64_t places = sm_each ? sm_count : 4 * static_cast<int64_t>(sm_count);
   const int64_t ctas = heads * cluster;
@@ -976,7 +1010,7 @@ static cudaError_t launch_cache_attention_nt(const CacheAttnParams& p, int64_t r
   const int64_t most = thirds >= 2 ? (windowed ? 72 : 32) : thirds == 1 || !sm_each ? 20 : 8;
   if (tokens <= most * cluster * round) {
     if (cluster > 1)
-      return launch_cache_attention_t<HD, kFp8, NT, kCacheCluster>(p, row_blocks, sm_count, stream, cluster);
+      return launch_cache_attention_cluster<HD, kFp8, NT>(p, row_blocks, cluster, stream);
     if (sm_each) return launch_cache_attention_t<HD, kFp8, NT, 1>(p, row_blocks, sm_count, stream);
     return launch_cache_attention_t<HD, kFp8, NT, 4>(p, row_blocks, sm_count, stream);
   }
