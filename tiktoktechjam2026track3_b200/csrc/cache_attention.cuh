@@ -716,25 +716,32 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
       cluster_sync_all();
       for (int i = rank * Cfg::kThreads + tid; i < rows * (HD / 2); i += ranks * Cfg::kThreads) {
         const int r = i / (HD / 2), d = 2 * (i - r * (HD / 2));
-        float m_of[kCacheCluster], l_of[kCacheCluster];
-        float2 v_of[kCacheCluster];
-        float top = -INFINITY;
+        float top = -INFINITY, sum = 0.f;
+        float2 acc = make_float2(0.f, 0.f);
+#pragma unroll 1
+        for (int k0 = 0; k0 < ranks; k0 += 8) {
+          float m_of[8], l_of[8];
+          float2 v_of[8];
+          const float before = top;
 #pragma unroll
-        for (int k = 0; k < kCacheCluster; ++k) {
-          if (k < ranks) {
-            const uint32_t at = cluster_map_to_rank(s_partial, k);
-            m_of[k] = cluster_load(at + 4 * (R * HD + r));
-            l_of[k] = cluster_load(at + 4 * (R * HD + R + r));
-            v_of[k] = cluster_load2(at + 4 * (r * HD + d));
+          for (int k = 0; k < 8; ++k) {
+            m_of[k] = -INFINITY;
+            l_of[k] = 0.f;
+            v_of[k] = make_float2(0.f, 0.f);
+            if (k0 + k < ranks) {
+              const uint32_t at = cluster_map_to_rank(s_partial, k0 + k);
+              m_of[k] = cluster_load(at + 4 * (R * HD + r));
+              l_of[k] = cluster_load(at + 4 * (R * HD + R + r));
+              v_of[k] = cluster_load2(at + 4 * (r * HD + d));
+            }
             top = fmaxf(top, m_of[k]);
           }
-        }
-        const float ref = top == -INFINITY ? 0.f : top;
-        float2 acc = make_float2(0.f, 0.f);
-        float sum = 0.f;
+          const float ref = top == -INFINITY ? 0.f : top;
+          const float old = fast_exp2(before - ref);
+          acc = make_float2(acc.x * old, acc.y * old);
+          sum *= old;
 #pragma unroll
-        for (int k = 0; k < kCacheCluster; ++k) {
-          if (k < ranks) {
+          for (int k = 0; k < 8; ++k) {
             const float f = fast_exp2(m_of[k] - ref);
             acc.x = fmaf(v_of[k].x, f, acc.x);
             acc.y = fmaf(v_of[k].y, f, acc.y);
