@@ -1,0 +1,43 @@
+"""What the serving operators' Python side decides before a launch (no GPU)."""
+
+import pytest
+import torch
+
+from tiktoktechjam2026track3_b200 import _capi, serving
+
+
+class _Queries:
+    """Stands for q: [rows, width] on the GPU."""
+
+    device = torch.device("cuda", 0)
+
+    def __init__(self, rows, width):
+        self.shape = (rows, width)
+
+    def size(self, i):
+        return self.shape[i]
+
+
+def _cache(monkeypatch, capturing):
+    """A cache without tensors whose workspaces are plain lists, on stream 7."""
+    cache = object.__new__(serving.KVCache)
+    cache.head_dim, cache._workspaces = 64, {}
+    monkeypatch.setattr(_capi, "_stream_ptr", lambda device: 7)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(cache, "workspace", lambda *size: list(size), raising=False)
+    return cache
+
+
+def test_a_captured_call_has_a_workspace_of_its_own(monkeypatch):
+    """A graph may outlive the workspace that its stream keeps, and run next to the stream's other calls."""
+    capturing = [False]
+    cache = _cache(monkeypatch, capturing)
+    kept = cache._workspace(_Queries(2, 256), 1)
+    assert cache._workspace(_Queries(1, 256), 1) is kept  # smaller calls of the stream share it
+    capturing[0] = True
+    first, second = cache._workspace(_Queries(2, 256), 1), cache._workspace(_Queries(2, 256), 1)
+    assert first is not kept and second is not kept and first is not second
+    larger = cache._workspace(_Queries(64, 256), 1)
+    assert all(larger is not w for _, w in cache._workspaces.values())
+    capturing[0] = False
+    assert cache._workspace(_Queries(2, 256), 1) is kept

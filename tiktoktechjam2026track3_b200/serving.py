@@ -198,14 +198,15 @@ class KVCache:
 
     def _workspace(self, q: torch.Tensor, q_len: int) -> torch.Tensor:
         """The current stream's workspace, kept between calls (those of one stream run one after the other) and made
-        anew when a call is larger than all before it."""
+        anew when a call is larger than all before it. A call that is being captured gets one of its own: its memory
+        and its zeroing are part of the graph, which may run next to the stream's other calls and outlive the kept one."""
         need = (q.size(0) // q_len, q.size(1) // self.head_dim, q_len)
+        if torch.cuda.is_current_stream_capturing():
+            return self.workspace(*need)
         stream = _capi._stream_ptr(q.device)
         kept = self._workspaces.get(stream)
         if kept is not None and need[0] <= kept[0][0] and need[1] <= kept[0][1] and need[2] <= kept[0][2]:
             return kept[1]
-        if torch.cuda.is_current_stream_capturing():
-            return self.workspace(*need)  # its zeroing is part of the graph, and so is its memory
         size = tuple(map(max, need, kept[0])) if kept is not None else need
         size = (1 << (size[0] - 1).bit_length() if size[0] > 0 else 1, size[1], size[2])
         made = self.workspace(*size)
