@@ -3,7 +3,6 @@
 Tolerances are those of test_gpu_serving.py, by the same arithmetic.
 """
 
-
 import pytest
 import torch
 
@@ -53,3 +52,31 @@ def test_graph_captured_on_its_warm_up_stream_outlives_the_streams_workspace():
     torch.cuda.synchronize()
     assert torch.equal(out, want[:1]) and torch.equal(again, want)
     assert all(bool((x == 7).all()) for x in others)
+
+
+@pytest.mark.parametrize("heads", [1, 8])
+@pytest.mark.parametrize("room", [0, 1 << 17])
+def test_steps_enqueued_at_once_are_those_waited_for_one_by_one(heads, room):
+    """Append and attend in turn without a wait between, with magnitudes that make the page's scale grow every few
+    steps (neighbouring heads' scales lie in one sector): the same bits as with a wait after every call."""
+    steps, d = 40, 64
+    g = _gen(11)
+    grow = torch.exp2(torch.arange(steps) / 3.0)[:, None]
+    rows = (torch.randn(steps, 3 * heads * d, generator=g) * grow).bfloat16().cuda()
+    got = []
+    for wait in (False, True):
+        cache = serving.KVCache.allocate(4, heads, d, 16)
+        table = torch.nn.functional.pad(_i32([[2, 0, 3]]), (0, max(0, room // 16 - 3)), value=-1)
+        past, lens = [_i32([i]) for i in range(steps)], [_i32([i + 1]) for i in range(steps)]
+        zero, one = _i32([0]), _i32([1])
+        torch.cuda.synchronize()
+        outs = []
+        for i in range(steps):
+            cache.append(rows[i:i + 1], heads, zero, one, past[i], table, 1)
+            if wait:
+                torch.cuda.synchronize()
+            outs.append(cache.attend(rows[i:i + 1, :heads * d], table, lens[i]))
+            if wait:
+                torch.cuda.synchronize()
+        got.append(torch.cat(outs))
+    assert torch.equal(*got)

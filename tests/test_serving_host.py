@@ -1,5 +1,8 @@
 """What the serving operators' Python side decides before a launch (no GPU)."""
 
+import re
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -41,3 +44,10 @@ def test_a_captured_call_has_a_workspace_of_its_own(monkeypatch):
     assert all(larger is not w for _, w in cache._workspaces.values())
     capturing[0] = False
     assert cache._workspace(_Queries(2, 256), 1) is kept
+
+
+def test_cache_attention_reads_its_pages_past_the_read_only_path():
+    """The launch that writes pages and scales may still run when the attention's first CTAs are resident."""
+    text = (Path(serving.__file__).parent / "csrc" / "cache_attention.cuh").read_text()
+    assert "pdl_wait_previous_grid" in text
+    assert not re.search(r"__ldg|ld\.global(\.\w+)*\.nc", text)

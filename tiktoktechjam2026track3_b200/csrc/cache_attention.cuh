@@ -141,7 +141,9 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 }
 
 // 32-bit words of a token that one thread holds, and where they lie: vectors of up to 4 words; a thread's vectors are
-// `lanes` vectors apart, so that each load of the warp covers consecutive bytes of a row.
+// `lanes` vectors apart, so that each load of the warp covers consecutive bytes of a row. Plain loads: pages and scales
+// may be written by the launch before this one, which is still running when this grid's first CTAs are resident, so
+// that they are not constant for the grid's time as the read-only path asks.
 template <int kWords, int kLanes>
 struct RowPieces {
   static constexpr int kVec = kWords < 4 ? kWords : 4;
@@ -155,17 +157,17 @@ struct RowPieces {
     for (int v = 0; v < kVectors; ++v) {
       const uint8_t* src = row + v * (4 * kVec * kLanes) + at * 4 * kVec;
       if constexpr (kVec == 4) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(src));
+        const uint4 u = *reinterpret_cast<const uint4*>(src);
         w[4 * v] = u.x;
         w[4 * v + 1] = u.y;
         w[4 * v + 2] = u.z;
         w[4 * v + 3] = u.w;
       } else if constexpr (kVec == 2) {
-        const uint2 u = __ldg(reinterpret_cast<const uint2*>(src));
+        const uint2 u = *reinterpret_cast<const uint2*>(src);
         w[2 * v] = u.x;
         w[2 * v + 1] = u.y;
       } else {
-        w[v] = __ldg(reinterpret_cast<const uint32_t*>(src));
+        w[v] = *reinterpret_cast<const uint32_t*>(src);
       }
     }
   }
@@ -485,8 +487,8 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
           VPieces::load(p.c.v + at + (2 * t + (x & 1) + 4 * (x & 2)) * (HD * Cfg::kBytes), g, vr[c][x]);
         ks[c] = vs[c] = 1.f;
         if (kFp8) {
-          ks[c] = __ldg(p.c.k_scale + static_cast<int64_t>(page) * kv_heads + now.h);
-          vs[c] = __ldg(p.c.v_scale + static_cast<int64_t>(page) * kv_heads + now.h);
+          ks[c] = p.c.k_scale[static_cast<int64_t>(page) * kv_heads + now.h];
+          vs[c] = p.c.v_scale[static_cast<int64_t>(page) * kv_heads + now.h];
         }
       }
       if (Cfg::kPrefetch) prefetch(now, u + kAhead);

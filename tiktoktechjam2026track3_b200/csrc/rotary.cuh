@@ -79,6 +79,8 @@ __device__ __forceinline__ RotaryChunk rotary_chunk(int chunk, int rotary_dim) {
   return c;
 }
 
+// (The read-only path: no kernel of this library writes a table, and a grid that lets its successor start early is one
+// of them, so a table is constant for as long as any CTA of its reader runs.)
 __device__ __forceinline__ void rotary_load_table(const float2* row, float (&c)[8], float (&s)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
