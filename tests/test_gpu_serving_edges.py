@@ -6,7 +6,7 @@ Tolerances are those of test_gpu_serving.py, by the same arithmetic.
 import pytest
 import torch
 
-from test_gpu_serving import _filled, _gen, _i32
+from test_gpu_serving import _check_attend, _filled, _gen, _i32
 from tiktoktechjam2026track3_b200 import _capi, serving
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +80,15 @@ def test_steps_enqueued_at_once_are_those_waited_for_one_by_one(heads, room):
                 torch.cuda.synchronize()
         got.append(torch.cat(outs))
     assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("heads,kv_heads,head_dim,q_len,dtype", [
+    (16, 1, 64, 5, E4M3), (40, 2, 128, 4, BF16), (12, 1, 32, 11, E4M3), (16, 2, 128, 17, E4M3)])
+def test_attend_with_more_row_blocks_than_one_launch_takes(heads, kv_heads, head_dim, q_len, dtype):
+    lengths = [1100, 30, 3000]
+    cache, seqs = _filled(lengths, 64, kv_heads, head_dim, dtype, 8)
+    q = torch.randn(len(lengths) * q_len, heads * head_dim, generator=_gen(2)).bfloat16().cuda()
+    outs = [cache.attend(q, table, _i32(lengths), q_len=q_len) for table in (seqs.table.cuda(), _wide(seqs, 64)) for _ in range(2)]
+    for out in outs[::2]:
+        _check_attend(cache, seqs, lengths, heads, q_len, 0, 0, q, out, head_dim**-0.5)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[2], outs[3])

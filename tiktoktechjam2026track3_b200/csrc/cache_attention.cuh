@@ -60,6 +60,7 @@ struct CacheAttnParams {
   int table_pages;
   const int32_t* kv_len;
   int batch, q_len, group, window, sinks;
+  int block0;  // first row block of this launch
   float scale_log2;
   int* counters;        // [row blocks][batch * kv_heads], zero between calls
   int* group_counters;  // [row blocks][groups of CTAs][2], likewise
@@ -70,6 +71,9 @@ constexpr int kCacheMaxBatch = 4096;
 constexpr int kCacheAtOnce = 40;  // parts of a (sequence, head) that one CTA joins in one go;
 constexpr int kCacheGroup = 16;   // of more, so many in a first go
 constexpr int kCacheCluster = 16;  // CTAs of a cluster, at most (a power of two)
+// Row blocks that one launch of the line form takes: more take turns over the same partial results, so that the workspace
+// does not grow with them (20 MB at most; 128 blocks of 16 rows would be 630). Each launch fills the machine by itself.
+constexpr int kCacheBlocksAtOnce = 4;
 constexpr float kCacheRescale = 8.f;   // log2: the maximum moves when a score exceeds it by more
 constexpr float kCacheHeadroom = 7.f;  // log2: weights are at most 2^(8 + 7), below fp16's largest
 
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
   const int t = lane & 3;
   const int kv_heads = p.c.kv_heads;
   const int rows_total = p.q_len * p.group;
-  const int row_block = blockIdx.y * R;
+  const int row_block = (p.block0 + static_cast<int>(blockIdx.y)) * R;
 
   pdl_wait_previous_grid();
   pdl_allow_next_grid();
@@ -874,8 +878,10 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
   }
 }
 
-// CTAs of a launch, and the bytes of its workspace.
-static int cache_attention_ctas(int sm_count) { return 4 * sm_count; }
+// CTAs of a launch of the line form, at most (CacheAttnCfg::kCtasPerSm of both types), and the bytes of its workspace.
+static int cache_attention_ctas(int64_t head_dim, int nt, int sm_count) {
+  return (head_dim == 128 && nt == 2 ? 2 : 4) * sm_count;
+}
 
 // Rows of a block: 8, or 16 where there are more than 8 rows (a block reads the keys and values anew).
 static int64_t cache_attention_row_blocks(int64_t rows, int* nt) {
@@ -884,17 +890,17 @@ static int64_t cache_attention_row_blocks(int64_t rows, int* nt) {
 }
 
 static int64_t cache_attention_counter_bytes(int64_t batch, int64_t kv_heads, int64_t row_blocks) {
-  return (batch * kv_heads * row_blocks * 4 + 255) / 256 * 256;
+  return (batch * kv_heads * std::min<int64_t>(row_blocks, kCacheBlocksAtOnce) * 4 + 255) / 256 * 256;
 }
 
 static int64_t cache_attention_group_bytes(int64_t row_blocks, int sm_count) {
-  return (row_blocks * (cache_attention_ctas(sm_count) / kCacheGroup + 1) * 8 + 255) / 256 * 256;
+  return (std::min<int64_t>(row_blocks, kCacheBlocksAtOnce) * (4 * sm_count / kCacheGroup + 1) * 8 + 255) / 256 * 256;
 }
 
 static int64_t cache_attention_partial_bytes(int64_t head_dim, int64_t rows, int sm_count) {
   int nt = 1;
-  const int64_t blocks = cache_attention_row_blocks(rows, &nt);
-  return (blocks * cache_attention_ctas(sm_count) * 2 * (8 * nt) * (head_dim + 2) * 4 + 255) / 256 * 256;
+  const int64_t blocks = std::min<int64_t>(cache_attention_row_blocks(rows, &nt), kCacheBlocksAtOnce);
+  return (blocks * cache_attention_ctas(head_dim, nt, sm_count) * 2 * (8 * nt) * (head_dim + 2) * 4 + 255) / 256 * 256;
 }
 
 static int64_t cache_attention_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t rows,
@@ -974,9 +980,20 @@ static cudaError_t launch_cache_attention_t(const CacheAttnParams& p, int64_t ro
                              Cfg::kSmemBytes + (kShare > 0 ? 0 : 4 * (kCacheMaxBatch + 1)));
   });
   if (e != cudaSuccess) return e;
-  const int ctas = kShare > 0 ? p.batch * p.c.kv_heads : sm_count * Cfg::kCtasPerSm;
-  return launch_pdl(cache_attention_kernel<HD, kFp8, NT, kShare>, dim3(ctas, static_cast<unsigned>(row_blocks)),
-                    dim3(Cfg::kThreads), smem, stream, p);
+  if constexpr (kShare > 0) {
+    return launch_pdl(cache_attention_kernel<HD, kFp8, NT, kShare>,
+                      dim3(p.batch * p.c.kv_heads, static_cast<unsigned>(row_blocks)), dim3(Cfg::kThreads), smem, stream, p);
+  } else {
+    static_assert(Cfg::kCtasPerSm <= (HD == 128 && NT == 2 ? 2 : 4), "as cache_attention_ctas says");
+    CacheAttnParams turn = p;
+    for (int64_t block = 0; block < row_blocks && e == cudaSuccess; block += kCacheBlocksAtOnce) {
+      turn.block0 = static_cast<int>(block);
+      const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(row_blocks - block, kCacheBlocksAtOnce));
+      e = launch_pdl(cache_attention_kernel<HD, kFp8, NT, kShare>, dim3(sm_count * Cfg::kCtasPerSm, blocks),
+                     dim3(Cfg::kThreads), smem, stream, turn);
+    }
+    return e;
+  }
 }
 
 template <int HD, bool kFp8, int NT>
