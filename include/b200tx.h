@@ -339,8 +339,8 @@ int b2_cache_attention_workspace(int64_t batch, int64_t q_len, int64_t num_heads
  *              query head i reads key head i / (num_heads / kv_heads). head_dim 32, 64 or 128
  *   kv_len     [batch] int32, the tokens in the cache, the q_len newest included
  *   workspace  at least b2_cache_attention_workspace bytes, zeroed by the caller once; the kernel leaves its
- *              counters zero. One made for the largest batch, q_len and num_heads serves smaller calls too;
- *              calls that may run at the same time need one each
+ *              counters, which lie at the same place for every call, zero. Any call that it is large enough for may
+ *              use it; calls that may run at the same time need one each
  */
 typedef struct b2_cache_attention_args {
   const b2_kv_cache* cache;

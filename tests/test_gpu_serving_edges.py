@@ -36,7 +36,8 @@ def test_graph_captured_on_its_warm_up_stream_outlives_the_streams_workspace():
     cache, seqs = _filled(lengths, 32, 2, 64, E4M3, 4)
     table, n = _wide(seqs, 32), _i32(lengths)
     q = torch.randn(4, 8 * 64, generator=_gen(3)).bfloat16().cuda()
-    want = cache.attend(q, table, n)
+    more = torch.randn(16, 8 * 64, generator=_gen(4)).bfloat16().cuda()  # four tokens each: a larger workspace
+    want, larger = cache.attend(q[:1], table[:1], n[:1]), cache.attend(more, table, n, q_len=4)
     out = torch.empty_like(q[:1])
     side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
     side.wait_stream(torch.cuda.current_stream())
@@ -44,13 +45,13 @@ def test_graph_captured_on_its_warm_up_stream_outlives_the_streams_workspace():
         cache.attend(q[:1], table[:1], n[:1], out=out)
         with torch.cuda.graph(graph, stream=side):
             cache.attend(q[:1], table[:1], n[:1], out=out)
-        assert torch.equal(cache.attend(q, table, n), want)
+        assert torch.equal(cache.attend(more, table, n, q_len=4), larger)
         others = [torch.full((1 << 20,), 7, dtype=torch.uint8, device="cuda") for _ in range(40)]
         out.zero_()
         graph.replay()
-        again = cache.attend(q, table, n)
+        again = cache.attend(more, table, n, q_len=4)
     torch.cuda.synchronize()
-    assert torch.equal(out, want[:1]) and torch.equal(again, want)
+    assert torch.equal(out, want) and torch.equal(again, larger)
     assert all(bool((x == 7).all()) for x in others)
 
 
@@ -92,3 +93,22 @@ def test_attend_with_more_row_blocks_than_one_launch_takes(heads, kv_heads, head
     for out in outs[::2]:
         _check_attend(cache, seqs, lengths, heads, q_len, 0, 0, q, out, head_dim**-0.5)
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[2], outs[3])
+
+
+def test_one_workspace_for_calls_of_any_shape():
+    """Many newest tokens of one sequence, then one of many, on different caches, through one workspace of the caller's."""
+    lengths = [4000] + [70 + 5 * b for b in range(63)]
+    caches = [_filled(lengths, 64, 2, 64, E4M3, 1), _filled(lengths, 64, 1, 128, BF16, 2)]
+    calls = []
+    for cache, seqs in caches:
+        table = _wide(seqs, 64)
+        for batch, q_len in ((1, 16), (64, 1), (3, 4), (64, 2), (1, 1)):
+            q = torch.randn(batch * q_len, 4 * cache.head_dim, generator=_gen(batch)).bfloat16().cuda()
+            args = (q, table[:batch], _i32(lengths[:batch]))
+            fresh = cache.workspace(batch, 4, q_len)
+            calls.append((cache, args, q_len, cache.attend(*args, q_len=q_len, workspace=fresh)))
+    shared = max((c.workspace(1, 4, 16) for c, _ in caches), key=lambda w: w.numel())
+    for order in (calls, calls[::-1], calls[::2] + calls[1::2]):
+        for cache, args, q_len, want in order:
+            assert torch.equal(cache.attend(*args, q_len=q_len, workspace=shared), want)
+    _check_attend(*caches[0], lengths, 4, 1, 0, 0, calls[1][1][0], calls[1][3], 64**-0.5)

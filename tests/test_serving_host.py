@@ -63,3 +63,10 @@ def test_workspace_does_not_grow_with_the_row_blocks(head_dim):
         return _capi.cache_attention_workspace(batch, q_len, heads, 8, head_dim, sm_count=148)
 
     assert size(1, 8) <= size(2, 64) <= size(4, 64) <= size(8, 64) == size(1024, 64) <= 21 << 20
+
+
+def test_workspace_is_alike_for_every_batch():
+    """Its counters lie at one place for every call: a workspace is either too small, and refused, or right."""
+    build()
+    sizes = {_capi.cache_attention_workspace(batch, 2, 4 * kv, kv, 64, sm_count=148) for batch in (1, 64, 4096) for kv in (1, 8)}
+    assert len(sizes) == 1

@@ -588,7 +588,7 @@ B2_API int b2_cache_attention_workspace(int64_t batch, int64_t q_len, int64_t nu
     if (cudaGetDevice(&dev) != cudaSuccess) return fail(2, "b2_cache_attention_workspace: no CUDA device and no sm_count");
     sms = device_sm_count(dev);
   }
-  *bytes = cache_attention_workspace_bytes(batch, kv_heads, head_dim, q_len * (num_heads / kv_heads), sms);
+  *bytes = cache_attention_workspace_bytes(head_dim, q_len * (num_heads / kv_heads), sms);
   return 0;
 }
 
@@ -627,7 +627,7 @@ B2_API int b2_cache_attention_fwd(const b2_cache_attention_args* args, void* str
   int dev = 0;
   cudaGetDevice(&dev);
   const int sms = device_sm_count(dev);
-  if (workspace_bytes < cache_attention_workspace_bytes(batch, hk, hd, rows, sms))
+  if (workspace_bytes < cache_attention_workspace_bytes(hd, rows, sms))
     return fail(1, "b2_cache_attention_fwd: the workspace is smaller than b2_cache_attention_workspace says");
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.out = static_cast<__nv_bfloat16*>(out);
@@ -643,7 +643,7 @@ B2_API int b2_cache_attention_fwd(const b2_cache_attention_args* args, void* str
   p.window = static_cast<int>(window < (int64_t{1} << 30) ? window : 0);  // beyond every position: none
   p.sinks = static_cast<int>(sinks < (int64_t{1} << 30) ? sinks : (int64_t{1} << 30));
   p.scale_log2 = scale * 1.4426950408889634f;
-  return check_launch(launch_cache_attention(p, workspace, workspace_bytes, fp8, sms, static_cast<cudaStream_t>(stream)),
+  return check_launch(launch_cache_attention(p, workspace, fp8, sms, static_cast<cudaStream_t>(stream)),
                       "b2_cache_attention_fwd");
 }
 

@@ -62,7 +62,7 @@ struct CacheAttnParams {
   int batch, q_len, group, window, sinks;
   int block0;  // first row block of this launch
   float scale_log2;
-  int* counters;        // [row blocks][batch * kv_heads], zero between calls
+  int* counters;        // [row blocks][CTAs]: of the head that begins in a CTA's stretch and goes on; zero between calls
   int* group_counters;  // [row blocks][groups of CTAs][2], likewise
   float* partials;      // [row blocks][CTAs][2][rows][head_dim + 2]
 };
@@ -853,7 +853,8 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
         __syncthreads();
       };
       const int n = static_cast<int>(c_last - c_first) + 1;
-      int* head_counter = p.counters + static_cast<int64_t>(blockIdx.y) * p.batch * kv_heads + b * kv_heads + h;
+      // Of the heads that a stretch holds, only its last one can go on behind it: one counter a CTA is enough.
+      int* head_counter = p.counters + static_cast<int64_t>(blockIdx.y) * gridDim.x + c_first;
       if (n <= kCacheAtOnce) {
         if (last_of(head_counter, n)) join([&](int k) { return c_first + k; }, n, nullptr);
       } else {
@@ -889,12 +890,13 @@ static int64_t cache_attention_row_blocks(int64_t rows, int* nt) {
   return (rows + 8 * *nt - 1) / (8 * *nt);
 }
 
-static int64_t cache_attention_counter_bytes(int64_t batch, int64_t kv_heads, int64_t row_blocks) {
-  return (batch * kv_heads * std::min<int64_t>(row_blocks, kCacheBlocksAtOnce) * 4 + 255) / 256 * 256;
-}
+// Counters of the heads, then of the groups, at the start of a workspace: as many for every call, so that no call's
+// partial results lie where another's counters do, whatever their sizes and in whatever order they come.
+static int64_t cache_attention_head_counters(int sm_count) { return kCacheBlocksAtOnce * 4 * static_cast<int64_t>(sm_count); }
 
-static int64_t cache_attention_group_bytes(int64_t row_blocks, int sm_count) {
-  return (std::min<int64_t>(row_blocks, kCacheBlocksAtOnce) * (4 * sm_count / kCacheGroup + 1) * 8 + 255) / 256 * 256;
+static int64_t cache_attention_counter_bytes(int sm_count) {
+  const int64_t groups = kCacheBlocksAtOnce * (4 * static_cast<int64_t>(sm_count) / kCacheGroup + 1) * 2;
+  return ((cache_attention_head_counters(sm_count) + groups) * 4 + 255) / 256 * 256;
 }
 
 static int64_t cache_attention_partial_bytes(int64_t head_dim, int64_t rows, int sm_count) {
@@ -903,12 +905,8 @@ static int64_t cache_attention_partial_bytes(int64_t head_dim, int64_t rows, int
   return (blocks * cache_attention_ctas(head_dim, nt, sm_count) * 2 * (8 * nt) * (head_dim + 2) * 4 + 255) / 256 * 256;
 }
 
-static int64_t cache_attention_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t rows,
-                                               int sm_count) {
-  int nt = 1;
-  const int64_t blocks = cache_attention_row_blocks(rows, &nt);
-  return cache_attention_group_bytes(blocks, sm_count) + cache_attention_counter_bytes(batch, kv_heads, blocks) +
-         cache_attention_partial_bytes(head_dim, rows, sm_count);
+static int64_t cache_attention_workspace_bytes(int64_t head_dim, int64_t rows, int sm_count) {
+  return cache_attention_counter_bytes(sm_count) + cache_attention_partial_bytes(head_dim, rows, sm_count);
 }
 
 // A launch with programmatic dependence in clusters of `cluster` CTAs along x.
@@ -1053,17 +1051,13 @@ static cudaError_t launch_cache_attention_hd(const CacheAttnParams& p, bool fp8,
                  : launch_cache_attention_nt<HD, false, 2>(p, row_blocks, sm_count, stream);
 }
 
-// Counters from the start of the workspace, partial results up to its end: a workspace made for the largest batch and
-// the most rows then serves smaller calls in turn, whose partial results never lie over a larger call's counters.
-static cudaError_t launch_cache_attention(CacheAttnParams p, void* workspace, int64_t workspace_bytes, bool fp8,
-                                          int sm_count, cudaStream_t stream) {
+static cudaError_t launch_cache_attention(CacheAttnParams p, void* workspace, bool fp8, int sm_count, cudaStream_t stream) {
   int nt = 1;
   const int64_t rows = static_cast<int64_t>(p.q_len) * p.group;
   const int64_t blocks = cache_attention_row_blocks(rows, &nt);
-  p.group_counters = static_cast<int*>(workspace);
-  p.counters = p.group_counters + cache_attention_group_bytes(blocks, sm_count) / 4;
-  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + workspace_bytes / 256 * 256 -
-                                        cache_attention_partial_bytes(p.c.head_dim, rows, sm_count));
+  p.counters = static_cast<int*>(workspace);
+  p.group_counters = p.counters + cache_attention_head_counters(sm_count);
+  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + cache_attention_counter_bytes(sm_count));
   switch (p.c.head_dim) {
     case 32:
       return launch_cache_attention_hd<32>(p, fp8, nt, blocks, sm_count, stream);

@@ -139,7 +139,7 @@ class KVCache:
             k.stride(0) if pages > 1 else kv_heads * page_size * head_dim if kv_heads == 1 else kv_heads * k.stride(1),
             k.stride(1) if kv_heads > 1 else page_size * head_dim,
             _capi.CACHE_E4M3 if self.quantised else _capi.CACHE_BF16)
-        self._workspaces: Dict[int, Tuple[tuple, torch.Tensor]] = {}  # by stream
+        self._workspaces: Dict[int, Tuple[int, torch.Tensor]] = {}  # by stream: width times q_len, and what it needs
 
     @classmethod
     def allocate(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64,
@@ -172,8 +172,8 @@ class KVCache:
         return q_out
 
     def workspace(self, batch: int, num_heads: int, q_len: int = 1) -> torch.Tensor:
-        """A zeroed workspace for `attend` calls of up to this batch, heads and q_len, for callers that keep their
-        own: calls that may run at the same time (other streams, CUDA graphs) need one each."""
+        """A zeroed workspace for `attend` calls of up to this many heads times q_len (any batch), for callers that keep
+        their own: calls that may run at the same time (other streams, CUDA graphs) need one each."""
         n = _capi.cache_attention_workspace(batch, q_len, num_heads, self.kv_heads, self.head_dim)
         return torch.zeros(n, dtype=torch.uint8, device=self.k.device)
 
@@ -200,15 +200,11 @@ class KVCache:
         """The current stream's workspace, kept between calls (those of one stream run one after the other) and made
         anew when a call is larger than all before it. A call that is being captured gets one of its own: its memory
         and its zeroing are part of the graph, which may run next to the stream's other calls and outlive the kept one."""
-        need = (q.size(0) // q_len, q.size(1) // self.head_dim, q_len)
         if torch.cuda.is_current_stream_capturing():
-            return self.workspace(*need)
-        stream = _capi._stream_ptr(q.device)
+            return self.workspace(q.size(0) // q_len, q.size(1) // self.head_dim, q_len)
+        stream, need = _capi._stream_ptr(q.device), q.size(1) * q_len
         kept = self._workspaces.get(stream)
-        if kept is not None and need[0] <= kept[0][0] and need[1] <= kept[0][1] and need[2] <= kept[0][2]:
-            return kept[1]
-        size = tuple(map(max, need, kept[0])) if kept is not None else need
-        size = (1 << (size[0] - 1).bit_length() if size[0] > 0 else 1, size[1], size[2])
-        made = self.workspace(*size)
-        self._workspaces[stream] = (size, made)
-        return made
+        if kept is None or need > kept[0]:
+            kept = need, self.workspace(q.size(0) // q_len, q.size(1) // self.head_dim, q_len)
+            self._workspaces[stream] = kept
+        return kept[1]
