@@ -3,10 +3,13 @@
 Tolerances are those of test_gpu_serving.py, by the same arithmetic.
 """
 
+import math
+
 import pytest
 import torch
 
-from test_gpu_serving import _check_attend, _filled, _gen, _i32
+from oracle import serving_fp64 as oracle
+from test_gpu_serving import _check_attend, _close, _filled, _gen, _i32
 from tiktoktechjam2026track3_b200 import _capi, serving
 
 pytestmark = pytest.mark.gpu
@@ -112,3 +115,29 @@ def test_one_workspace_for_calls_of_any_shape():
         for cache, args, q_len, want in order:
             assert torch.equal(cache.attend(*args, q_len=q_len, workspace=shared), want)
     _check_attend(*caches[0], lengths, 4, 1, 0, 0, calls[1][1][0], calls[1][3], 64**-0.5)
+
+
+# ---------------------------------------------------------------------------------- values that are not finite
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("heads,kv_heads,window,sinks,at", [
+    (2, 2, 100, 4, [4, 5, 15]), (4, 1, 33, 20, [20, 31]), (2, 1, 64, 130, [130, 143]), (1, 1, 100, 4, [16, 17]),
+    (16, 1, 50, 1, [1, 15]), (3, 3, 40, 270, [271])])
+def test_values_behind_the_sinks_reach_only_the_rows_near_those_that_see_them(d, heads, kv_heads, window, sinks, at):
+    """Infinities and NaN in the values of tokens right behind the sinks: at most the rows less than 128 from one that
+    sees them may be touched (the tokens lie in the same 16 rows as the last sink, which every later row sees)."""
+    n = 900
+    g = _gen(d + sinks)
+    q = torch.randn(n, heads * d, generator=g).bfloat16()
+    k, v = (torch.randn(n, kv_heads * d, generator=g).bfloat16() for _ in range(2))
+    for i, j in enumerate(at):
+        v[j] = (math.nan, math.inf, -math.inf)[i]
+    out = serving.window_attention(q.cuda(), k.cuda(), v.cuda(), 1, n, d, window=window, sinks=sinks).cpu().view(n, heads, d)
+    rows = torch.cat([torch.arange(min(at) // 128 * 128), torch.arange(max(at) + window + 127, n)])
+    seen = oracle.visible_keys(rows, n, window, sinks)
+    assert not bool(seen[:, at].any())
+    q, k, v = (x.double().view(n, -1, d) for x in (q, k, v))
+    v[at] = 0.0
+    for h in range(heads):
+        kv = h * kv_heads // heads
+        ref, absum, size = oracle.attend(q[rows, h], k[:, kv], v[:, kv], seen, d**-0.5)
+        _close(out[rows, h], ref, 2**-8 * ref.abs() + (2**-8 + 2**-12 + 2 * d * 2**-23 * size) * absum)

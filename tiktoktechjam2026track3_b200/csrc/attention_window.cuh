@@ -16,7 +16,8 @@
 //     exponentials stop at its last key.
 //   - In list places v, row i sees v <= d and (v >= c or v < a), with a = sinks, d the place of key i and c that of key
 //     i - window + 1; only tiles where these cut are masked.
-//   - Values behind the band's last key are cleared in shared memory: a weight of zero does not remove a NaN there.
+//   - Values behind the band's last key are cleared in shared memory: a weight of zero does not remove a NaN there. Those
+//     between the last sink and the next multiple of 16 come from a map that ends with the sinks: its rows behind read as zeros.
 // Measured on one B200 (us a call back to back; floor, the larger of products at the measured GEMM rate and bytes at the copy
 // rate, in brackets): 32768 tokens, 16 heads of 128 on 4 key heads, window 4096: 1000 to 1150 as the 1000 W limit lets it
 // (627); 16 ragged sequences of up to 2048, 16 heads of 64, window 512: 152 (28); the same on 4 key heads, not ragged: 155
@@ -48,6 +49,7 @@ struct WindowParams {
 // Keys and values [B][S][kv_heads][head_dim] in boxes of 64 columns and 128 or 16 rows; Q in boxes of a query tile.
 struct WindowMaps {
   CUtensorMap q, k, v, k16, v16;
+  CUtensorMap v_sinks, v16_sinks;  // the sequence's first `sinks` rows only
 };
 
 // The list of keys of one query tile.
@@ -64,12 +66,11 @@ __device__ __forceinline__ KeyList window_keys(const WindowParams& p, int tile, 
   l.i0 = tile * tokens;
   l.i1 = min(l.i0 + tokens, len);
   l.lo = p.window > 0 ? max(0, l.i0 - p.window + 1) : 0;
-  const int rounded = (min(p.sinks, l.lo) + 15) & ~15;
-  if (p.sinks > 0 && rounded >= l.lo) {
+  if (p.sinks >= l.lo) {
     l.lo = 0;  // the sinks reach the band: one piece
     l.sink_rows = 0;
   } else {
-    l.sink_rows = rounded;
+    l.sink_rows = (p.sinks + 15) & ~15;
   }
   l.rows = l.sink_rows + l.i1 - l.lo;
   l.tiles = (l.rows + 127) >> 7;
@@ -86,17 +87,24 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
 }
 
 // Tile t of the list, 64 columns from `col` on: one box, or eight across the seam. Every box counts its full bytes.
+// `sinks`, `sinks16`: the maps for the part in front of the band.
 __device__ __forceinline__ void window_load_tile(uint8_t* dst, const CUtensorMap* map, const CUtensorMap* map16,
-                                                 uint64_t* bar, const KeyList& l, int t, int col, int head, int b) {
+                                                 const CUtensorMap* sinks, const CUtensorMap* sinks16, uint64_t* bar,
+                                                 const KeyList& l, int t, int col, int head, int b) {
   const int v0 = 128 * t;
-  if (v0 >= l.sink_rows || v0 + 128 <= l.sink_rows) {
-    tma_load_4d(dst, map, bar, col, head, v0 >= l.sink_rows ? l.lo + v0 - l.sink_rows : v0, b);
+  if (v0 >= l.sink_rows) {
+    tma_load_4d(dst, map, bar, col, head, l.lo + v0 - l.sink_rows, b);
+    return;
+  }
+  if (v0 + 128 <= l.sink_rows) {
+    tma_load_4d(dst, sinks, bar, col, head, v0, b);
     return;
   }
 #pragma unroll 1
   for (int r = 0; r < 128; r += 16) {
     const int v = v0 + r;
-    tma_load_4d(dst + r * 128, map16, bar, col, head, v < l.sink_rows ? v : l.lo + v - l.sink_rows, b);
+    const bool sink = v < l.sink_rows;
+    tma_load_4d(dst + r * 128, sink ? sinks16 : map16, bar, col, head, sink ? v : l.lo + v - l.sink_rows, b);
   }
 }
 
@@ -274,14 +282,14 @@ __global__ void __launch_bounds__(192, 2)
         if (k_next < n && mbar_test_wait(&k_empty[k_next % kStages], ((k_next / kStages) & 1) ^ 1u)) {
           const int st = k_next % kStages;
           mbar_arrive_expect_tx(&k_full[st], kTileBytes);
-          window_load_tile(s_k + st * kTileBytes, &maps.k, &maps.k16, &k_full[st], keys, k_next, 0, kv_head, b);
+          window_load_tile(s_k + st * kTileBytes, &maps.k, &maps.k16, &maps.k, &maps.k16, &k_full[st], keys, k_next, 0, kv_head, b);
           ++k_next;
           progress = true;
         }
         if (v_next < n && mbar_test_wait(&v_empty[v_next % kStages], ((v_next / kStages) & 1) ^ 1u)) {
           const int st = v_next % kStages;
           mbar_arrive_expect_tx(&v_full[st], kTileBytes);
-          window_load_tile(s_v + st * kTileBytes, &maps.v, &maps.v16, &v_full[st], keys, v_next, 0, kv_head, b);
+          window_load_tile(s_v + st * kTileBytes, &maps.v, &maps.v16, &maps.v_sinks, &maps.v16_sinks, &v_full[st], keys, v_next, 0, kv_head, b);
           ++v_next;
           progress = true;
         }
@@ -646,8 +654,8 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
           const int st = k_next % Cfg::kStages;
           uint8_t* dst = s_k + st * Cfg::kTileBytes;
           mbar_arrive_expect_tx(&k_full[st], Cfg::kTileBytes);
-          window_load_tile(dst, &maps.k, &maps.k16, &k_full[st], keys, k_next, 0, kv_head, b);
-          window_load_tile(dst + Cfg::kBoxBytes, &maps.k, &maps.k16, &k_full[st], keys, k_next, 64, kv_head, b);
+          window_load_tile(dst, &maps.k, &maps.k16, &maps.k, &maps.k16, &k_full[st], keys, k_next, 0, kv_head, b);
+          window_load_tile(dst + Cfg::kBoxBytes, &maps.k, &maps.k16, &maps.k, &maps.k16, &k_full[st], keys, k_next, 64, kv_head, b);
           ++k_next;
           progress = true;
         }
@@ -655,8 +663,8 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
           const int st = v_next % Cfg::kVStages;
           uint8_t* dst = s_v + st * Cfg::kTileBytes;
           mbar_arrive_expect_tx(&v_full[st], Cfg::kTileBytes);
-          window_load_tile(dst, &maps.v, &maps.v16, &v_full[st], keys, v_next, 0, kv_head, b);
-          window_load_tile(dst + Cfg::kBoxBytes, &maps.v, &maps.v16, &v_full[st], keys, v_next, 64, kv_head, b);
+          window_load_tile(dst, &maps.v, &maps.v16, &maps.v_sinks, &maps.v16_sinks, &v_full[st], keys, v_next, 0, kv_head, b);
+          window_load_tile(dst + Cfg::kBoxBytes, &maps.v, &maps.v16, &maps.v_sinks, &maps.v16_sinks, &v_full[st], keys, v_next, 64, kv_head, b);
           ++v_next;
           progress = true;
         }
@@ -913,18 +921,22 @@ static cudaError_t launch_window_attention(const __nv_bfloat16* q, int64_t ld_q,
   if (p.head_major && bh > 65535) return cudaErrorInvalidConfiguration;
   WindowMaps maps;
   const uint64_t h = static_cast<uint64_t>(hd), S = static_cast<uint64_t>(p.S), B = static_cast<uint64_t>(p.B);
-  auto make = [&](CUtensorMap* m, const __nv_bfloat16* base, int64_t ld, int heads, uint32_t box_heads, uint32_t box_rows) {
+  auto make = [&](CUtensorMap* m, const __nv_bfloat16* base, int64_t ld, int heads, uint32_t box_heads, uint32_t box_rows,
+                  uint64_t rows) {
     const uint64_t row = static_cast<uint64_t>(ld) * 2;
-    const uint64_t dims[4] = {h, static_cast<uint64_t>(heads), S, B};
+    const uint64_t dims[4] = {h, static_cast<uint64_t>(heads), rows, B};
     const uint64_t strides[3] = {h * 2, row, row * S};
     const uint32_t box[4] = {64, box_heads, box_rows, 1};
     return make_tmap_bf16_4d(m, base, dims, strides, box);
   };
-  cudaError_t e = make(&maps.q, q, ld_q, p.heads, 1u << p.group_shift, tokens);
-  if (e == cudaSuccess) e = make(&maps.k, k, ld_k, p.kv_heads, 1, 128);
-  if (e == cudaSuccess) e = make(&maps.v, v, ld_v, p.kv_heads, 1, 128);
-  if (e == cudaSuccess) e = make(&maps.k16, k, ld_k, p.kv_heads, 1, 16);
-  if (e == cudaSuccess) e = make(&maps.v16, v, ld_v, p.kv_heads, 1, 16);
+  const uint64_t sinks = p.sinks > 0 ? static_cast<uint64_t>(p.sinks) : 1;
+  cudaError_t e = make(&maps.q, q, ld_q, p.heads, 1u << p.group_shift, tokens, S);
+  if (e == cudaSuccess) e = make(&maps.k, k, ld_k, p.kv_heads, 1, 128, S);
+  if (e == cudaSuccess) e = make(&maps.v, v, ld_v, p.kv_heads, 1, 128, S);
+  if (e == cudaSuccess) e = make(&maps.k16, k, ld_k, p.kv_heads, 1, 16, S);
+  if (e == cudaSuccess) e = make(&maps.v16, v, ld_v, p.kv_heads, 1, 16, S);
+  if (e == cudaSuccess) e = make(&maps.v_sinks, v, ld_v, p.kv_heads, 1, 128, sinks);
+  if (e == cudaSuccess) e = make(&maps.v16_sinks, v, ld_v, p.kv_heads, 1, 16, sinks);
   if (e != cudaSuccess) return e;
   static std::once_flag once32[64], once64[64], once128[64];
   constexpr int kSoloSmem = 5 * 128 * 128 + 256 + 1024;
