@@ -141,3 +141,35 @@ def test_values_behind_the_sinks_reach_only_the_rows_near_those_that_see_them(d,
         kv = h * kv_heads // heads
         ref, absum, size = oracle.attend(q[rows, h], k[:, kv], v[:, kv], seen, d**-0.5)
         _close(out[rows, h], ref, 2**-8 * ref.abs() + (2**-8 + 2**-12 + 2 * d * 2**-23 * size) * absum)
+
+
+@pytest.mark.parametrize("junk", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads,kv_heads,head_dim,page,lengths", [
+    (4, 2, 32, 16, [1, 17, 33, 500]), (3, 3, 64, 32, [16, 49, 1000]), (20, 2, 32, 64, [5, 130]), (8, 1, 128, 16, [47]),
+    (1, 1, 64, 16, [0, 3])])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3)])
+@pytest.mark.parametrize("room", [0, 1 << 17])
+def test_scales_of_pages_that_no_row_sees_are_not_used(junk, heads, kv_heads, head_dim, page, lengths, window, sinks, room):
+    """Scales as an allocation leaves them in pages that nobody owns, page 0 among them (tiles that are missing at a
+    sequence's end read it)."""
+    cache, seqs = _filled(lengths, page, kv_heads, head_dim, E4M3, 6)
+    last = seqs.pages - 1
+    used = sorted(int(i) for i in seqs.table.flatten() if i >= 0)
+    if 0 in used:  # the owner of page 0 takes an unused page instead
+        free = next(i for i in range(last, 0, -1) if i not in used)
+        for x in (cache.k, cache.v):
+            x.view(torch.uint8)[free] = x.view(torch.uint8)[0]
+            x.view(torch.uint8)[0] = 0x7f  # the code of a NaN
+        for x in (cache.k_scale, cache.v_scale):
+            x[free] = x[0]
+        seqs.table[seqs.table == 0] = free
+        used[used.index(0)] = free
+    unowned = [i for i in range(seqs.pages) if i not in used]
+    assert 0 in unowned
+    cache.k_scale[unowned] = junk
+    cache.v_scale[unowned] = junk
+    table = _wide(seqs, page, room) if room else seqs.table.cuda()
+    q = torch.randn(len(lengths), heads * head_dim, generator=_gen(1)).bfloat16().cuda()
+    out = cache.attend(q, table, _i32(lengths), window=window, sinks=sinks)
+    kept = serving.KVCache(cache.k, cache.v, cache.k_scale.nan_to_num(1.0, 1.0, 1.0), cache.v_scale.nan_to_num(1.0, 1.0, 1.0))
+    _check_attend(kept, seqs, lengths, heads, 1, window, sinks, q, out, head_dim**-0.5)

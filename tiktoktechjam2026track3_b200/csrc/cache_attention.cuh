@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
         const int src = (u - ids_from) * kSub + c;
         tok[c] = __shfl_sync(0xffffffffu, my_tok, src);
         const int page = __shfl_sync(0xffffffffu, my_page, src);
-        // (a tile that is missing reads page 0, slot 0, and is masked)
+        // (a tile that is missing reads page 0, slot 0, whosever it is, and is masked)
         const int64_t at = static_cast<int64_t>(page) * page_bytes + head_bytes + (tok[c] & slot_mask) * (HD * Cfg::kBytes);
 #pragma unroll
         for (int x = 0; x < 2; ++x) KPieces::load(p.c.k + at + (g + 8 * x) * (HD * Cfg::kBytes), t, kr[c][x]);
@@ -548,6 +548,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
         const int from = max(0, seq.len - p.q_len - p.window + 1);
 #pragma unroll
         for (int c = 0; c < kSub; ++c) {
+          if (tok[c] == kNoTile) inv_v[c] = 1.f;  // of a scale that may be anything: its weights are 0, but 0 times a NaN is a NaN
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
