@@ -52,19 +52,23 @@ int b2_abi_version(void);
 /* Message describing the last failed call on this thread ("" if none). */
 const char* b2_last_error(void);
 
-/* Reads (and with clear != 0 resets) the current device's pipeline status word:
- * 0 = no kernel gave up waiting since the last clear; otherwise (kernel << 16) | (site << 8) |
- * reason, kernel 2 = linear, 3 = attention, 5 = rotary, 6 = cache append, 7 = cache attention;
- * reason 1 = a wait ran out, 3 = a position, length or page number read from device memory lay
- * outside its table (what it names was skipped). Synchronous: it waits for the device. */
+/* Reads (and with clear != 0 resets) the current device's status words: the pipelines' (a kernel gave up
+ * waiting), or where that is 0 the indices' (a position, length or page number read from device memory lay
+ * outside its table; what it names was skipped, other results are valid). 0 = neither since the last clear;
+ * otherwise (kernel << 16) | (site << 8) | reason, kernel 2 = linear, 3 = attention, 5 = rotary,
+ * 6 = cache append, 7 = cache attention; reason 1 = a wait ran out, 3 = an index. Synchronous: it
+ * waits for the device. */
 int b2_device_status(uint32_t* out_status, int clear);
 
-/* Enqueues a copy of the current device's status word (the value b2_device_status reads, not
- * cleared) into host_dst on `stream`, behind the work already enqueued there; host_dst should be
+/* Enqueues a copy of the current device's pipeline status word (not cleared; never reason 3, so that
+ * one caller's wrong index does not stop another's) into host_dst on `stream`, behind the work already enqueued there; host_dst should be
  * pinned host memory, valid until the copy completes. Lets a caller check every forward pass for
  * a pipeline timeout without synchronising: read *host_dst once an event recorded after this call
  * has completed. No counterpart in the reference (its kernels have no bounded waits). */
 int b2_device_status_async(uint32_t* host_dst, void* stream);
+
+/* The same for the word of the indices, for callers of the serving entry points below. */
+int b2_index_status_async(uint32_t* host_dst, void* stream);
 
 /* Sets the current device's limit for one pipeline wait (mbarrier, peer flag) in nanoseconds;
  * 0 restores the default of 4 s, values below 1 ms are rejected. Applies to kernels launched after

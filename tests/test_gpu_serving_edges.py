@@ -10,7 +10,7 @@ import torch
 
 from oracle import serving_fp64 as oracle
 from test_gpu_serving import _check_attend, _close, _filled, _gen, _i32
-from tiktoktechjam2026track3_b200 import _capi, serving
+from tiktoktechjam2026track3_b200 import TransformerConfig, UserOptimizedTransformer, _capi, serving
 
 pytestmark = pytest.mark.gpu
 
@@ -173,3 +173,26 @@ def test_scales_of_pages_that_no_row_sees_are_not_used(junk, heads, kv_heads, he
     out = cache.attend(q, table, _i32(lengths), window=window, sinks=sinks)
     kept = serving.KVCache(cache.k, cache.v, cache.k_scale.nan_to_num(1.0, 1.0, 1.0), cache.v_scale.nan_to_num(1.0, 1.0, 1.0))
     _check_attend(kept, seqs, lengths, heads, 1, window, sinks, q, out, head_dim**-0.5)
+
+
+# ---------------------------------------------------------------------------------- wrong indices
+def test_a_wrong_index_does_not_stop_other_callers():
+    """One caller's position past its table is reported to those who ask for indices; a model's forward goes on."""
+    model = UserOptimizedTransformer(TransformerConfig(1, 16, 64, 1, 64, 1, True)).to("cuda", BF16).eval()
+    x = torch.randn(1, 16, 64, generator=_gen(1)).bfloat16().cuda()
+    rows = torch.randn(2, 64, generator=_gen(2)).bfloat16().cuda()
+    watch = _capi.StatusWatch(indices=True)
+    with torch.inference_mode():
+        before = model(x)
+        model.check_device_status()
+        serving.rotary(rows, _i32([0, 16]), serving.rotary_table(16, 64), 64)
+        after = model(x)
+        model.check_device_status()
+        assert torch.equal(model(x), before) and torch.equal(after, before)
+        model.check_device_status()
+    watch.after_forward(rows.device)
+    with pytest.raises(RuntimeError, match="rotary kernel met an index outside its table.*skipped"):
+        watch.check(wait=True)
+    assert _capi.device_status(clear=True) == (5 << 16) | (1 << 8) | 3
+    watch.after_forward(rows.device)
+    assert watch.check(wait=True) == 0

@@ -56,6 +56,7 @@ SIGNATURES = {
     "b2_last_error": (ctypes.c_char_p, []),
     "b2_device_status": (ctypes.c_int, [ctypes.POINTER(ctypes.c_uint32), ctypes.c_int]),
     "b2_device_status_async": (ctypes.c_int, [_vp, _vp]),
+    "b2_index_status_async": (ctypes.c_int, [_vp, _vp]),
     "b2_set_wait_limit": (ctypes.c_int, [ctypes.c_uint64]),
     "b2_mask_lengths": (ctypes.c_int, [_vp, _i64, _i64, _vp, _vp, _vp, _vp]),
     "b2_test_set_fault": (ctypes.c_int, [ctypes.c_int]),
@@ -172,7 +173,7 @@ def _require(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
 
 
 def device_status(clear: bool = True) -> int:
-    """Pipeline status word of the current device (0 = no kernel gave up waiting)."""
+    """Status of the current device (0 = no kernel gave up waiting or met an index outside its table)."""
     lib = load_library()
     out = ctypes.c_uint32(0)
     _check(lib.b2_device_status(ctypes.byref(out), 1 if clear else 0), "b2_device_status")
@@ -216,9 +217,13 @@ class StatusWatch:
     raises RuntimeError if a kernel gave up waiting, so a timed-out pass is reported at the latest
     by the next call. The status word is sticky until cleared (b2_device_status(clear=1)), so a
     timeout is never missed, only reported one call late when its copy has not landed yet.
+
+    With `indices` it watches the word of the serving operators' indices too (b2_index_status_async): a position,
+    length or page number of any caller on the device that lay outside its table.
     """
 
-    def __init__(self) -> None:
+    def __init__(self, indices: bool = False) -> None:
+        self._indices = indices
         self._host: Optional[torch.Tensor] = None
         self._event: Optional[torch.cuda.Event] = None
         self.status = 0
@@ -231,27 +236,30 @@ class StatusWatch:
             return 0
         ev.synchronize()
         self._event = None
-        value = int(self._host[0].item())
+        value = int(self._host[0].item()) or int(self._host[1].item())
         if value:
             self.status = value
             kernel, site, reason = value >> 16, (value >> 8) & 0xFF, value & 0xFF
             names = {1: "layernorm", 2: "linear", 3: "attention", 4: "peer barrier", 5: "rotary", 6: "cache append",
                      7: "cache attention"}
-            what = "met an index outside its table" if reason == REASON_BAD_INDEX else "gave up waiting"
+            what, so = "gave up waiting", "outputs computed since then are not valid"
+            if reason == REASON_BAD_INDEX:
+                what, so = "met an index outside its table", "what it names was skipped"
             raise RuntimeError(
                 f"a {names.get(kernel, kernel)} kernel {what} (status {value:#x}: site {site}, reason "
-                f"{reason}); outputs computed since then are not valid. Clear the status with "
-                "_capi.device_status(clear=True) after handling it")
+                f"{reason}); {so}. Clear the status with _capi.device_status(clear=True) after handling it")
         return 0
 
     def after_forward(self, device: torch.device) -> None:
         if self._host is None:
-            self._host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+            self._host = torch.zeros(2, dtype=torch.int32, pin_memory=True)
         if self._event is not None and not self._event.query():
             return  # the previous copy is still in flight: it will report the same sticky word
         self._event = None
         lib = load_library()
         _check(lib.b2_device_status_async(self._host.data_ptr(), _stream_ptr(device)), "b2_device_status_async")
+        if self._indices:
+            _check(lib.b2_index_status_async(self._host.data_ptr() + 4, _stream_ptr(device)), "b2_index_status_async")
         ev = torch.cuda.Event()
         ev.record(torch.cuda.current_stream(device))
         self._event = ev

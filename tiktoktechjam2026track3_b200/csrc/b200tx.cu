@@ -132,15 +132,17 @@ B2_API const char* b2_last_error(void) { return g_last_error; }
 
 B2_API int b2_device_status(uint32_t* out_status, int clear) {
   if (out_status == nullptr) return fail(1, "b2_device_status: out_status is null");
-  uint32_t v = 0;
+  uint32_t v = 0, index = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, g_device_status, sizeof(v));
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&index, g_index_status, sizeof(index));
   if (e != cudaSuccess) return check_launch(e, "b2_device_status");
-  if (clear && v != 0) {
+  if (clear) {
     const uint32_t zero = 0;
-    e = cudaMemcpyToSymbol(g_device_status, &zero, sizeof(zero));
+    if (v != 0) e = cudaMemcpyToSymbol(g_device_status, &zero, sizeof(zero));
+    if (e == cudaSuccess && index != 0) e = cudaMemcpyToSymbol(g_index_status, &zero, sizeof(zero));
     if (e != cudaSuccess) return check_launch(e, "b2_device_status(clear)");
   }
-  *out_status = v;
+  *out_status = v != 0 ? v : index;
   return 0;
 }
 
@@ -149,6 +151,13 @@ B2_API int b2_device_status_async(uint32_t* host_dst, void* stream) {
   return check_launch(cudaMemcpyFromSymbolAsync(host_dst, g_device_status, sizeof(uint32_t), 0,
                                                 cudaMemcpyDeviceToHost, static_cast<cudaStream_t>(stream)),
                       "b2_device_status_async");
+}
+
+B2_API int b2_index_status_async(uint32_t* host_dst, void* stream) {
+  if (host_dst == nullptr) return fail(1, "b2_index_status_async: host_dst is null");
+  return check_launch(cudaMemcpyFromSymbolAsync(host_dst, g_index_status, sizeof(uint32_t), 0, cudaMemcpyDeviceToHost,
+                                                static_cast<cudaStream_t>(stream)),
+                      "b2_index_status_async");
 }
 
 B2_API int b2_set_wait_limit(uint64_t limit_ns) {

@@ -17,8 +17,9 @@
 namespace b2 {
 
 // ---------------------------------------------------------------------------------------------
-// Status word shared by all kernels of the library (one per device; lives until process exit).
-// Encoding: (kernel_id << 16) | (site << 8) | reason. 0 = no error since the last read.
+// Status words shared by all kernels of the library (one of each per device; they live until process exit).
+// Encoding: (kernel_id << 16) | (site << 8) | reason. 0 = no error since the last read. An index that its caller got
+// wrong has a word of its own: it says nothing about other callers' results, as a pipeline that gave up does.
 // ---------------------------------------------------------------------------------------------
 enum : uint32_t {
   kKernelLayerNorm = 1,
@@ -37,9 +38,11 @@ enum : uint32_t {
 
 // Defined once: the library is a single translation unit (b200tx.cu includes every kernel).
 __device__ uint32_t g_device_status = 0;
+__device__ uint32_t g_index_status = 0;  // reason kReasonBadIndex
 
 __device__ __forceinline__ void record_status(uint32_t kernel_id, uint32_t site, uint32_t reason) {
-  atomicCAS(&g_device_status, 0u, (kernel_id << 16) | (site << 8) | reason);
+  atomicCAS(reason == kReasonBadIndex ? &g_index_status : &g_device_status, 0u,
+            (kernel_id << 16) | (site << 8) | reason);
 }
 
 // Bounded polling loops (several barriers serviced by one thread) count idle spins and read the

@@ -12,8 +12,8 @@ that a causal stack needs next to it to go on from what it has read:
 
 Everything runs in libb200tx.so on the current CUDA stream (include/b200tx.h says what each call takes);
 there is no CPU or PyTorch fallback. Lengths, positions and page tables stay on the device and are not read
-back: an entry outside its table is skipped by the kernel and reported by the device's status word
-(`_capi.device_status`, `_capi.StatusWatch`).
+back: an entry outside its table is skipped by the kernel and reported by a status word of the device
+(`_capi.device_status`, `_capi.StatusWatch(indices=True)`); it does not stop other callers.
 """
 
 from __future__ import annotations

@@ -91,7 +91,7 @@ class StreamingTransformer:
         self.lengths = [0] * self.batch
 
     def check_device_status(self) -> None:
-        """Waits for the last pass and raises RuntimeError if a kernel of it gave up or met a bad index."""
+        """Waits for the last pass and raises RuntimeError if a kernel of it, or an earlier one, gave up waiting."""
         self._status.check(wait=True)
 
     # ------------------------------------------------------------------ passes
