@@ -1,5 +1,6 @@
 """What the serving operators' Python side decides before a launch (no GPU)."""
 
+import math
 import re
 from pathlib import Path
 
@@ -25,7 +26,8 @@ class _Queries:
 def _cache(monkeypatch, capturing):
     """A cache without tensors whose workspaces are plain lists, on stream 7."""
     cache = object.__new__(serving.KVCache)
-    cache.head_dim, cache._workspaces = 64, {}
+    cache.head_dim, cache._workspaces, cache._desc = 64, {}, _capi.KVCacheDesc()
+    monkeypatch.setattr(_capi, "_current_device", lambda: 0)
     monkeypatch.setattr(_capi, "_stream_ptr", lambda device: 7)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
     monkeypatch.setattr(cache, "workspace", lambda *size: list(size), raising=False)
@@ -70,3 +72,111 @@ def test_workspace_is_alike_for_every_batch():
     build()
     sizes = {_capi.cache_attention_workspace(batch, 2, 4 * kv, kv, 64, sm_count=148) for batch in (1, 64, 4096) for kv in (1, 8)}
     assert len(sizes) == 1
+
+
+# ---------------------------------------------------------------------------------- where tensors lie
+class _On:
+    """What a wrapper asks of a contiguous CUDA tensor, on a device that need not be there."""
+
+    is_cuda = True
+
+    def __init__(self, device, shape, dtype=torch.bfloat16):
+        self.device, self.shape, self.dtype = torch.device("cuda", device), tuple(shape), dtype
+
+    def size(self, i=None):
+        return self.shape if i is None else self.shape[i]
+
+    def stride(self):
+        return tuple(math.prod(self.shape[i + 1:]) for i in range(len(self.shape)))
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return math.prod(self.shape)
+
+    def get_device(self):
+        return self.device.index
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return 256
+
+
+class _Library:
+    """Takes every entry point and keeps (its name, the device that was current, the stream)."""
+
+    def __init__(self, current):
+        self.calls, self._current = [], current
+
+    def __getattr__(self, name):
+        def entry(args, stream):
+            self.calls.append((name, self._current[0], stream))
+            return 0
+        return entry
+
+
+@pytest.fixture
+def library(monkeypatch):
+    current = [0]
+
+    class Device:
+        def __init__(self, device):
+            self.index = device if isinstance(device, int) else device.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    fake = _Library(current)
+    monkeypatch.setattr(_capi, "_lib", fake)
+    monkeypatch.setattr(_capi, "_raw_stream", lambda device: 100 + device)
+    monkeypatch.setattr(_capi, "_current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    return fake
+
+
+def _calls(device):
+    """name -> (wrapper, its tensors on `device`, its other arguments)."""
+    i32 = torch.int32
+    desc = _capi.KVCacheDesc(pages=4, kv_heads=2, page_size=16, head_dim=64)
+    desc.device = device
+
+    def on(*shape, dtype=torch.bfloat16):
+        return _On(device, shape, dtype)
+
+    return {
+        "b2_rotary_fwd": (_capi.rotary, dict(
+            x=on(4, 128), positions=on(4, dtype=i32), table=on(9, 32, 2, dtype=torch.float32), out=on(4, 128)),
+            dict(head_dim=64)),
+        "b2_cache_append_fwd": (_capi.cache_append, dict(
+            qkv=on(4, 512), new_start=on(2, dtype=i32), new_len=on(2, dtype=i32), past_len=on(2, dtype=i32),
+            page_table=on(2, 3, dtype=i32), table=on(9, 32, 2, dtype=torch.float32), q_out=on(4, 256), k_out=on(4, 128)),
+            dict(cache=desc, num_heads=4, q_col=0, k_col=256, v_col=384, max_new=2)),
+        "b2_cache_attention_fwd": (_capi.cache_attention, dict(
+            q=on(2, 256), page_table=on(2, 3, dtype=i32), kv_len=on(2, dtype=i32), out=on(2, 256),
+            workspace=on(1 << 20, dtype=torch.uint8)), dict(cache=desc, q_len=1, window=0, sinks=0, scale=0.1)),
+        "b2_window_attention_fwd": (_capi.window_attention, dict(
+            q=on(6, 256), k=on(6, 128), v=on(6, 128), kv_len=on(2, dtype=i32), out=on(6, 256)),
+            dict(batch=2, seq_len=3, head_dim=64, window=0, sinks=0, scale=0.1)),
+    }
+
+
+@pytest.mark.parametrize("device", [0, 1])
+def test_calls_run_on_the_gpu_of_their_tensors(library, device):
+    for name, (call, tensors, rest) in _calls(device).items():
+        call(**tensors, **rest)
+        assert library.calls.pop() == (name, device, 100 + device)
+    assert _capi._current_device() == 0
+
+
+def test_tensors_of_another_gpu_are_refused(library):
+    for call, tensors, rest in _calls(0).values():
+        for name, t in tensors.items():
+            with pytest.raises(ValueError, match="must be on cuda"):
+                call(**(tensors | {name: _On(1, t.shape, t.dtype)}), **rest)
+    assert not library.calls

@@ -44,6 +44,7 @@ class KVCacheDesc(ctypes.Structure):
     _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", _i64), ("kv_heads", _i64),
                 ("page_size", _i64), ("head_dim", _i64), ("page_stride", _i64), ("head_stride", _i64),
                 ("dtype", ctypes.c_int)]
+    device = 0  # index of the GPU that holds them (not part of the C struct)
 
 
 # The argument structs of the serving entry points: every member is 8 bytes wide, pointers as integers.
@@ -151,6 +152,7 @@ def _check(status: int, what: str) -> None:
 # The current stream's handle without making a torch.cuda.Stream object for it (0.15 us against 2.3 us of host time a
 # call, a quarter of a small kernel's launch); the object's way where this build of torch lacks the query.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # without its check for a first use
 
 
 def _stream_ptr(device: torch.device) -> int:
@@ -538,12 +540,30 @@ def linear_bcast(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
 _BF16, _INT32 = torch.bfloat16, torch.int32
 
 
-def _rows(t: torch.Tensor, name: str) -> int:
-    """Row stride of a bf16 CUDA matrix whose rows are contiguous (a column slice of packed rows is one)."""
+def _elsewhere(t: torch.Tensor, name: str, device: int) -> ValueError:
+    if not t.is_cuda:
+        return ValueError(f"{name} must be a CUDA tensor (this package has no CPU path)")
+    return ValueError(f"{name} must be on cuda:{device} as the call's other tensors, got {t.device}")
+
+
+def _launch(entry: str, args: bytes, device: int) -> None:
+    """One serving entry point on the current stream of the GPU that holds the call's tensors, made current for it."""
+    fn = getattr(_lib or load_library(), entry)
+    if _current_device() == device:
+        status = fn(args, _raw_stream(device) if _raw_stream is not None else _stream_ptr(torch.device("cuda", device)))
+    else:
+        with torch.cuda.device(device):
+            status = fn(args, _stream_ptr(torch.device("cuda", device)))
+    if status:
+        _check(status, entry)
+
+
+def _rows(t: torch.Tensor, name: str, device: int) -> int:
+    """Row stride of a bf16 matrix on `device` whose rows are contiguous (a column slice of packed rows is one)."""
     stride = t.stride()
-    if len(stride) != 2 or stride[1] != 1 or t.dtype is not _BF16 or not t.is_cuda:
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor (this package has no CPU path)")
+    if len(stride) != 2 or stride[1] != 1 or t.dtype is not _BF16 or t.get_device() != device or device < 0:
+        if t.get_device() != device or device < 0:
+            raise _elsewhere(t, name, device)
         if t.dtype != torch.bfloat16:
             raise ValueError(f"{name} must be {torch.bfloat16}, got {t.dtype}")
         raise ValueError(f"{name} must be 2-D with contiguous rows")
@@ -551,28 +571,34 @@ def _rows(t: torch.Tensor, name: str) -> int:
     return stride[0] if t.size(0) > 1 else (t.size(1) + 7) // 8 * 8
 
 
-def _table(t: torch.Tensor) -> Tuple[int, int]:
+def _table(t: torch.Tensor, device: int) -> Tuple[int, int]:
     """(positions, rotary_dim) of a rotary table [positions, rotary_dim / 2, 2]."""
     if t.dim() != 3 or t.size(2) != 2:
         raise ValueError("table must be [positions, rotary_dim / 2, 2]")
+    if t.get_device() != device:
+        raise _elsewhere(t, "table", device)
     _require(t, torch.float32, "table")
     return t.size(0), 2 * t.size(1)
 
 
-def _indices(t: torch.Tensor, n: int, name: str) -> int:
-    """Pointer of n contiguous int32 entries on the GPU."""
-    if t.dtype is not _INT32 or not t.is_cuda or not t.is_contiguous():
+def _indices(t: torch.Tensor, n: int, name: str, device: int) -> int:
+    """Pointer of n contiguous int32 entries on `device`."""
+    if t.get_device() != device:
+        raise _elsewhere(t, name, device)
+    if t.dtype is not _INT32 or not t.is_contiguous():
         _require(t, _INT32, name)
     if t.numel() != n:
         raise ValueError(f"{name} must have {n} entries, got {t.numel()}")
     return t.data_ptr()
 
 
-def _page_table(t: torch.Tensor, batch: int) -> Tuple[int, int]:
+def _page_table(t: torch.Tensor, batch: int, device: int) -> Tuple[int, int]:
     """(pointer, pages per sequence) of an int32 page table."""
     if t.dim() != 2 or t.size(0) != batch:
         raise ValueError(f"page_table must be [{batch}, pages], got {tuple(t.shape)}")
-    if t.dtype is not _INT32 or not t.is_cuda or not t.is_contiguous():
+    if t.get_device() != device:
+        raise _elsewhere(t, "page_table", device)
+    if t.dtype is not _INT32 or not t.is_contiguous():
         _require(t, _INT32, "page_table")
     return t.data_ptr(), t.size(1)
 
@@ -580,16 +606,15 @@ def _page_table(t: torch.Tensor, batch: int) -> Tuple[int, int]:
 def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, head_dim: int, out: torch.Tensor,
            interleaved: bool = False, inverse: bool = False) -> None:
     """out = the rows of x with every head turned by its row's position (see b2_rotary_fwd)."""
-    ld_x, ld_out = _rows(x, "x"), _rows(out, "out")
+    device = x.get_device()
+    ld_x, ld_out = _rows(x, "x", device), _rows(out, "out", device)
     tokens, width = x.size(0), x.size(1)
     if width % head_dim or out.size(0) != tokens or out.size(1) != width:
         raise ValueError(f"x and out must both be [tokens, heads * {head_dim}]")
-    most, rotary_dim = _table(table)
-    status = load_library().b2_rotary_fwd(ROTARY_ARGS.pack(
+    most, rotary_dim = _table(table, device)
+    _launch("b2_rotary_fwd", ROTARY_ARGS.pack(
         x.data_ptr(), ld_x, tokens, width // head_dim, head_dim, rotary_dim, interleaved, inverse,
-        _indices(positions, tokens, "positions"), table.data_ptr(), most, out.data_ptr(), ld_out), _stream_ptr(x.device))
-    if status:
-        _check(status, "b2_rotary_fwd")
+        _indices(positions, tokens, "positions", device), table.data_ptr(), most, out.data_ptr(), ld_out), device)
 
 
 def cache_append(cache: KVCacheDesc, qkv: torch.Tensor, num_heads: int, q_col: int, k_col: int, v_col: int,
@@ -597,30 +622,29 @@ def cache_append(cache: KVCacheDesc, qkv: torch.Tensor, num_heads: int, q_col: i
                  max_new: int, table: Optional[torch.Tensor] = None, interleaved: bool = False,
                  q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None) -> None:
     """Stores (and with `table` rotates) the new tokens of packed rows qkv (see b2_cache_append_fwd)."""
-    ld = _rows(qkv, "qkv")
+    device = cache.device
+    ld = _rows(qkv, "qkv", device)
     batch, tokens = new_len.numel(), qkv.size(0)
-    pages, table_pages = _page_table(page_table, batch)
+    pages, table_pages = _page_table(page_table, batch, device)
     positions = rotary_dim = ld_q = ld_k = 0
     if table is not None:
-        positions, rotary_dim = _table(table)
+        positions, rotary_dim = _table(table, device)
         if q_out is None:
             raise ValueError("a rotation needs q_out")
     if q_out is not None:
-        ld_q = _rows(q_out, "q_out")
+        ld_q = _rows(q_out, "q_out", device)
         if table is None or q_out.size(0) != tokens or q_out.size(1) != num_heads * cache.head_dim:
             raise ValueError("q_out needs a table and the shape [tokens, num_heads * head_dim]")
     if k_out is not None:
-        ld_k = _rows(k_out, "k_out")
+        ld_k = _rows(k_out, "k_out", device)
         if k_out.size(0) != tokens or k_out.size(1) != cache.kv_heads * cache.head_dim:
             raise ValueError("k_out must be [tokens, kv_heads * head_dim]")
-    status = load_library().b2_cache_append_fwd(CACHE_APPEND_ARGS.pack(
+    _launch("b2_cache_append_fwd", CACHE_APPEND_ARGS.pack(
         ctypes.addressof(cache), qkv.data_ptr(), ld, q_col, k_col, v_col, tokens, num_heads, batch,
-        _indices(new_start, batch, "new_start"), _indices(new_len, batch, "new_len"),
-        _indices(past_len, batch, "past_len"), pages, table_pages, max_new, 0 if table is None else table.data_ptr(),
-        positions, rotary_dim, interleaved, 0 if q_out is None else q_out.data_ptr(), ld_q,
-        0 if k_out is None else k_out.data_ptr(), ld_k), _stream_ptr(qkv.device))
-    if status:
-        _check(status, "b2_cache_append_fwd")
+        _indices(new_start, batch, "new_start", device), _indices(new_len, batch, "new_len", device),
+        _indices(past_len, batch, "past_len", device), pages, table_pages, max_new,
+        0 if table is None else table.data_ptr(), positions, rotary_dim, interleaved,
+        0 if q_out is None else q_out.data_ptr(), ld_q, 0 if k_out is None else k_out.data_ptr(), ld_k), device)
 
 
 def cache_attention_workspace(batch: int, q_len: int, num_heads: int, kv_heads: int, head_dim: int,
@@ -635,36 +659,37 @@ def cache_attention_workspace(batch: int, q_len: int, num_heads: int, kv_heads: 
 def cache_attention(cache: KVCacheDesc, q: torch.Tensor, q_len: int, page_table: torch.Tensor, kv_len: torch.Tensor,
                     window: int, sinks: int, scale: float, out: torch.Tensor, workspace: torch.Tensor) -> None:
     """out = attention of the q_len newest tokens of each sequence over the cache (see b2_cache_attention_fwd)."""
-    ld_q, ld_out = _rows(q, "q"), _rows(out, "out")
+    device = cache.device
+    ld_q, ld_out = _rows(q, "q", device), _rows(out, "out", device)
+    if workspace.get_device() != device:
+        raise _elsewhere(workspace, "workspace", device)
     rows, width = q.size(0), q.size(1)
     batch = kv_len.numel()
-    pages, table_pages = _page_table(page_table, batch)
+    pages, table_pages = _page_table(page_table, batch, device)
     if rows != batch * q_len:
         raise ValueError("q needs q_len rows and kv_len an entry per sequence")
     head_dim = cache.head_dim
     if width % head_dim or out.size(0) != rows or out.size(1) != width:
         raise ValueError("q and out must both be [batch * q_len, heads * head_dim]")
-    status = load_library().b2_cache_attention_fwd(CACHE_ATTENTION_ARGS.pack(
+    _launch("b2_cache_attention_fwd", CACHE_ATTENTION_ARGS.pack(
         ctypes.addressof(cache), q.data_ptr(), ld_q, batch, q_len, width // head_dim, pages, table_pages,
-        _indices(kv_len, batch, "kv_len"), window, sinks, scale, out.data_ptr(), ld_out, workspace.data_ptr(),
-        workspace.numel()), _stream_ptr(q.device))
-    if status:
-        _check(status, "b2_cache_attention_fwd")
+        _indices(kv_len, batch, "kv_len", device), window, sinks, scale, out.data_ptr(), ld_out, workspace.data_ptr(),
+        workspace.numel()), device)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: int, seq_len: int, head_dim: int,
                      window: int, sinks: int, kv_len: Optional[torch.Tensor], scale: float, out: torch.Tensor) -> None:
     """out = causal attention with a sliding window and sinks (see b2_window_attention_fwd)."""
-    ld_q, ld_k, ld_v, ld_out = _rows(q, "q"), _rows(k, "k"), _rows(v, "v"), _rows(out, "out")
+    device = q.get_device()
+    ld_q, ld_k = _rows(q, "q", device), _rows(k, "k", device)
+    ld_v, ld_out = _rows(v, "v", device), _rows(out, "out", device)
     rows, width, k_width = q.size(0), q.size(1), k.size(1)
     if (rows != batch * seq_len or k.size(0) != rows or v.size(0) != rows or out.size(0) != rows or v.size(1) != k_width
             or out.size(1) != width):
         raise ValueError("q, k, v and out must have batch * seq_len rows, k and v alike, out like q")
     if width % head_dim or k_width % head_dim:
         raise ValueError(f"q and k must be whole heads of {head_dim}")
-    status = load_library().b2_window_attention_fwd(WINDOW_ATTENTION_ARGS.pack(
+    _launch("b2_window_attention_fwd", WINDOW_ATTENTION_ARGS.pack(
         q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(), ld_v, batch, seq_len, width // head_dim,
-        k_width // head_dim, head_dim, 0 if kv_len is None else _indices(kv_len, batch, "kv_len"), window, sinks, scale,
-        out.data_ptr(), ld_out), _stream_ptr(q.device))
-    if status:
-        _check(status, "b2_window_attention_fwd")
+        k_width // head_dim, head_dim, 0 if kv_len is None else _indices(kv_len, batch, "kv_len", device), window, sinks,
+        scale, out.data_ptr(), ld_out), device)

@@ -139,6 +139,7 @@ class KVCache:
             k.stride(0) if pages > 1 else kv_heads * page_size * head_dim if kv_heads == 1 else kv_heads * k.stride(1),
             k.stride(1) if kv_heads > 1 else page_size * head_dim,
             _capi.CACHE_E4M3 if self.quantised else _capi.CACHE_BF16)
+        self._desc.device = k.get_device()
         self._workspaces: Dict[int, Tuple[int, torch.Tensor]] = {}  # by stream: width times q_len, and what it needs
 
     @classmethod
@@ -174,7 +175,8 @@ class KVCache:
     def workspace(self, batch: int, num_heads: int, q_len: int = 1) -> torch.Tensor:
         """A zeroed workspace for `attend` calls of up to this many heads times q_len (any batch), for callers that keep
         their own: calls that may run at the same time (other streams, CUDA graphs) need one each."""
-        n = _capi.cache_attention_workspace(batch, q_len, num_heads, self.kv_heads, self.head_dim)
+        with torch.cuda.device(self.k.device):  # whose SMs it goes by
+            n = _capi.cache_attention_workspace(batch, q_len, num_heads, self.kv_heads, self.head_dim)
         return torch.zeros(n, dtype=torch.uint8, device=self.k.device)
 
     def attend(self, q: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor, *, q_len: int = 1,
@@ -200,6 +202,9 @@ class KVCache:
         """The current stream's workspace, kept between calls (those of one stream run one after the other) and made
         anew when a call is larger than all before it. A call that is being captured gets one of its own: its memory
         and its zeroing are part of the graph, which may run next to the stream's other calls and outlive the kept one."""
+        if _capi._current_device() != self._desc.device:  # the streams meant are those of the cache's GPU
+            with torch.cuda.device(self._desc.device):
+                return self._workspace(q, q_len)
         if torch.cuda.is_current_stream_capturing():
             return self.workspace(q.size(0) // q_len, q.size(1) // self.head_dim, q_len)
         stream, need = _capi._stream_ptr(q.device), q.size(1) * q_len

@@ -155,8 +155,8 @@ class StreamingTransformer:
     def _check(self, x: torch.Tensor) -> None:
         if x.dim() != 3 or x.shape[0] != self.batch or x.shape[2] != self.config.d_model or x.shape[1] == 0:
             raise ValueError(f"x must be [{self.batch}, tokens, {self.config.d_model}], got {tuple(x.shape)}")
-        if not x.is_cuda or x.dtype != torch.bfloat16:
-            raise RuntimeError("StreamingTransformer computes in bfloat16 on the GPU")
+        if x.device != self.device or x.dtype != torch.bfloat16:
+            raise RuntimeError(f"StreamingTransformer computes in bfloat16 on the GPU of its weights, {self.device}")
 
     def _start(self, rows: int) -> torch.Tensor:
         """First row of every sequence, `rows` rows each."""
