@@ -15,7 +15,7 @@ Without a table, a window and 8 bits it computes what the model's own causal for
 
 from __future__ import annotations
 
-from typing import List, Optional, Sequence
+from typing import Callable, List, Optional, Sequence
 
 import torch
 
@@ -41,7 +41,8 @@ class StreamingTransformer:
 
     table, interleaved: rotary positions (`rotary_table`; None: none, as the model's own forward). window, sinks: each
     token sees the `window` newest tokens and the first `sinks` ones (0: all). dtype: of the cache, float8_e4m3fn
-    or bfloat16. The weights are read when the object is made and again by `refresh()`.
+    or bfloat16. Every pass uses the model's weights as they are: a change since the last one is seen by the parameters'
+    storage and version, as in the model's own forward. What is in the cache stays as it was computed.
     """
 
     def __init__(self, model: UserOptimizedTransformer, batch: int, max_tokens: int, *,
@@ -78,10 +79,12 @@ class StreamingTransformer:
         self.use_cuda_graph = True
 
     def refresh(self) -> None:
-        """Reads the model's weights again (after an update)."""
+        """Reads the model's weights again; a pass does so by itself where a parameter has changed."""
         self.packed = self.model.packed_weights()
         if not self.packed[0].w_qkv.is_cuda or self.packed[0].w_qkv.dtype != torch.bfloat16:
             raise RuntimeError("model weights must be bfloat16 on the GPU: call .to(device, torch.bfloat16)")
+        # Their storage, kept until the next refresh: a pass launched before a change is noticed reads it.
+        self._held = [p.detach() for p in self.model.parameters()]
         self._graphs = {}
 
     def reset(self) -> None:
@@ -126,7 +129,8 @@ class StreamingTransformer:
 
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
         self._status.check()
-        self._pass(x.contiguous().view(-1, cfg.d_model), rows, attend, mask, out.view(-1, cfg.d_model))
+        self._with_weights(lambda: self._pass(x.contiguous().view(-1, cfg.d_model), rows, attend, mask,
+                                              out.view(-1, cfg.d_model)))
         self.past.copy_(count)
         self.lengths = new
         self._status.after_forward(self.device)
@@ -140,18 +144,44 @@ class StreamingTransformer:
             raise ValueError(f"{max(self.lengths)} + {t} tokens do not fit max_tokens {self.max_tokens}")
         self._status.check()
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        if self.use_cuda_graph:
-            static_x, static_out, graph = self._graph(t)
-            static_x.copy_(x)
-            graph.replay()
-            out.copy_(static_out)
-        else:
-            self._step(x.contiguous(), out, _Rows(self.config, self.batch * t, self.device))
+
+        def launch() -> None:
+            if self.use_cuda_graph:
+                static_x, static_out, graph = self._graph(t)
+                static_x.copy_(x)
+                graph.replay()
+                out.copy_(static_out)
+            else:
+                self._step(x.contiguous(), out, _Rows(self.config, self.batch * t, self.device))
+
+        self._with_weights(launch, lambda: self.past.sub_(t))
         self.lengths = [n + t for n in self.lengths]
         self._status.after_forward(self.device)
         return out
 
     # ------------------------------------------------------------------ inside
+    def _with_weights(self, launch: Callable[[], None], undo: Callable[[], object] = lambda: None) -> None:
+        """launch() with the model's weights as they are (the packed projections are copies, and graphs hold addresses).
+
+        As in the model's forward the launches come first and the comparison of every parameter with the last pass's
+        after them (40 us of host time at 12 layers); where one has changed, undo() and launch() again with the new
+        ones. The tokens of the first attempt are overwritten, like drafts that were not taken.
+        """
+        key = self.model._packed_key
+        if self.model._packed is not self.packed or key is None or key[0] == "storage":  # known to differ, or not told
+            self._follow_weights()
+        launch()
+        if self.model._weights_key() != self.model._packed_key and self.model.packed_weights() is not self.packed:
+            undo()
+            self._follow_weights()
+            launch()
+
+    def _follow_weights(self) -> None:
+        if self.model.packed_weights() is not self.packed:
+            self.refresh()
+            if self.packed[0].w_qkv.device != self.device:
+                raise RuntimeError(f"the model's weights have left {self.device}, where this object's cache is")
+
     def _check(self, x: torch.Tensor) -> None:
         if x.dim() != 3 or x.shape[0] != self.batch or x.shape[2] != self.config.d_model or x.shape[1] == 0:
             raise ValueError(f"x must be [{self.batch}, tokens, {self.config.d_model}], got {tuple(x.shape)}")
