@@ -75,3 +75,22 @@ def test_a_step_sees_weights_changed_in_the_middle_of_a_conversation(cuda_device
         got.append(outs)
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+@torch.no_grad()
+def test_passes_refuse_to_be_captured(cuda_device):
+    """A first pass would leave buffers that only the graph's replay fills; the conversation goes on as if not asked."""
+    model, _ = _model(256, 4)
+    want = _talk(_make(model, True))
+    for graphs in (True, False):
+        stream = _make(model, graphs)
+        x = _x(2, 40, 256, 1).cuda()
+        for call in (lambda: stream.prompt(x, [40, 11]), lambda: stream.step(x[:, :1])):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                with pytest.raises(RuntimeError, match="captured"):
+                    call()
+                x.add(1)  # a graph of something
+            assert stream.lengths == [0, 0] and not stream._starts and not stream._workspaces
+        for a, b in zip(_talk(stream), want):
+            assert torch.equal(a, b)

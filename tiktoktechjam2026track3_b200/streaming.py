@@ -187,6 +187,9 @@ class StreamingTransformer:
             raise ValueError(f"x must be [{self.batch}, tokens, {self.config.d_model}], got {tuple(x.shape)}")
         if x.device != self.device or x.dtype != torch.bfloat16:
             raise RuntimeError(f"StreamingTransformer computes in bfloat16 on the GPU of its weights, {self.device}")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a pass cannot be captured: it counts tokens on the host and makes buffers that later passes "
+                               "use (steps are replayed from graphs of the object's own)")
 
     def _start(self, rows: int) -> torch.Tensor:
         """First row of every sequence, `rows` rows each."""
