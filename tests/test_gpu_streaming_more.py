@@ -94,3 +94,23 @@ def test_passes_refuse_to_be_captured(cuda_device):
             assert stream.lengths == [0, 0] and not stream._starts and not stream._workspaces
         for a, b in zip(_talk(stream), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_any_autograd_mode_may_make_and_use_it(cuda_device, graphs):
+    """Made or first used under inference mode and then without it, and the other way round; inputs that need gradients
+    (the passes have none: their outputs do not, and nothing of a conversation is kept for them)."""
+    model, _ = _model(256, 4)
+    want = _talk(_make(model, graphs))
+    for make, first, then in ((True, True, False), (False, True, False), (True, False, True), (False, False, True)):
+        with torch.inference_mode(make):
+            stream = _make(model, graphs)
+        for mode in (first, then):
+            with torch.inference_mode(mode):
+                for a, b in zip(_talk(stream), want):
+                    assert torch.equal(a, b)
+    x = _x(2, 40, 256, 1).cuda().requires_grad_()
+    y = stream.prompt(x, [40, 11])
+    z = stream.step(x[:, :1] * 1.0)
+    assert torch.equal(y, want[0]) and not y.requires_grad and not z.requires_grad
+    assert not any(t.requires_grad for g in stream._graphs.values() for t in g[:2])

@@ -15,6 +15,7 @@ Without a table, a window and 8 bits it computes what the model's own causal for
 
 from __future__ import annotations
 
+import functools
 from typing import Callable, List, Optional, Sequence
 
 import torch
@@ -36,6 +37,15 @@ class _Rows:
         self.hidden = torch.empty(rows, f, device=device, dtype=torch.bfloat16)
 
 
+def _plain_tensors(f):
+    """f without gradients and with tensors that every autograd mode may write, whatever mode its caller is in."""
+    @functools.wraps(f)
+    def g(*args, **kwargs):
+        with torch.inference_mode(False), torch.no_grad():
+            return f(*args, **kwargs)
+    return g
+
+
 class StreamingTransformer:
     """Prompt and step passes of a causal UserOptimizedTransformer over `batch` sequences of up to `max_tokens`.
 
@@ -45,6 +55,7 @@ class StreamingTransformer:
     storage and version, as in the model's own forward. What is in the cache stays as it was computed.
     """
 
+    @_plain_tensors
     def __init__(self, model: UserOptimizedTransformer, batch: int, max_tokens: int, *,
                  table: Optional[torch.Tensor] = None, interleaved: bool = False, window: int = 0, sinks: int = 0,
                  page_size: int = 64, dtype: torch.dtype = torch.float8_e4m3fn) -> None:
@@ -78,6 +89,7 @@ class StreamingTransformer:
         self._status = _capi.StatusWatch()
         self.use_cuda_graph = True
 
+    @_plain_tensors
     def refresh(self) -> None:
         """Reads the model's weights again; a pass does so by itself where a parameter has changed."""
         self.packed = self.model.packed_weights()
@@ -98,6 +110,7 @@ class StreamingTransformer:
         self._status.check(wait=True)
 
     # ------------------------------------------------------------------ passes
+    @torch.no_grad()
     def prompt(self, x: torch.Tensor, lengths: Optional[Sequence[int]] = None) -> torch.Tensor:
         """The prompts of fresh sequences: x [batch, S, D] bf16, rows past lengths[b] padding (outputs there are zero)."""
         self._check(x)
@@ -136,6 +149,7 @@ class StreamingTransformer:
         self._status.after_forward(self.device)
         return out
 
+    @torch.no_grad()
     def step(self, x: torch.Tensor) -> torch.Tensor:
         """The next t tokens of every sequence: x [batch, t, D] bf16 -> [batch, t, D]."""
         self._check(x)
@@ -226,21 +240,25 @@ class StreamingTransformer:
     def _graph(self, t: int):
         """Static input, output and the CUDA graph of a step of t tokens."""
         if t not in self._graphs:
-            x = torch.zeros(self.batch, t, self.config.d_model, device=self.device, dtype=torch.bfloat16)
-            out = torch.empty_like(x)
-            rows = _Rows(self.config, self.batch * t, self.device)
-            self._start(t), self._counts(t)
-            self._workspaces[(t, True)] = self.caches[0].workspace(self.batch, self.config.num_heads, t)
-            # One eager pass (first use of each kernel sets its attributes outside capture) that stores no token.
-            before = self.past.clone()
-            self._step(x, out, rows, torch.zeros_like(self.past))
-            self.past.copy_(before)
-            torch.cuda.current_stream(self.device).synchronize()
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
-                self._step(x, out, rows)
-            self._graphs[t] = (x, out, graph, rows)  # the graph writes rows: they live as long as it does
+            self._capture(t)
         return self._graphs[t][:3]
+
+    @_plain_tensors
+    def _capture(self, t: int) -> None:
+        x = torch.zeros(self.batch, t, self.config.d_model, device=self.device, dtype=torch.bfloat16)
+        out = torch.empty_like(x)
+        rows = _Rows(self.config, self.batch * t, self.device)
+        self._start(t), self._counts(t)
+        self._workspaces[(t, True)] = self.caches[0].workspace(self.batch, self.config.num_heads, t)
+        # One eager pass (first use of each kernel sets its attributes outside capture) that stores no token.
+        before = self.past.clone()
+        self._step(x, out, rows, torch.zeros_like(self.past))
+        self.past.copy_(before)
+        torch.cuda.current_stream(self.device).synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            self._step(x, out, rows)
+        self._graphs[t] = (x, out, graph, rows)  # the graph writes rows: they live as long as it does
 
     def _pass(self, x: torch.Tensor, rows: _Rows, attend, mask: Optional[torch.Tensor], out: torch.Tensor) -> None:
         first = self.packed[0]
