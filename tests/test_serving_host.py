@@ -1,5 +1,6 @@
 """What the serving operators' Python side decides before a launch (no GPU)."""
 
+import ctypes
 import math
 import re
 from pathlib import Path
@@ -72,6 +73,58 @@ def test_workspace_is_alike_for_every_batch():
     build()
     sizes = {_capi.cache_attention_workspace(batch, 2, 4 * kv, kv, 64, sm_count=148) for batch in (1, 64, 4096) for kv in (1, 8)}
     assert len(sizes) == 1
+
+
+# ---------------------------------------------------------------------------------- arguments at their types' ends
+HUGE, P = (1 << 63) - 8, 256  # a multiple of 8; an address that nobody looks at: the calls have no rows
+
+
+def _refused(lib, entry, layout, args):
+    """Whether a call without rows, which does nothing if it passes the checks, is refused."""
+    status = getattr(lib, entry)(layout.pack(*args), None)
+    assert status in (0, 1, 2)
+    return status != 0
+
+
+def _desc(**changes):
+    fields = dict(k=256, v=256, k_scale=256, v_scale=256, pages=8, kv_heads=5, page_size=32, head_dim=64,
+                  page_stride=5 * 32 * 64, head_stride=32 * 64, dtype=_capi.CACHE_E4M3)
+    return _capi.KVCacheDesc(**(fields | changes))
+
+
+def _append_args(cache, ld=1024, cols=(0, 320, 640), heads=5, table_pages=2, most=4):
+    return (ctypes.addressof(cache), P, ld, *cols, 0, heads, 1, P, P, P, P, table_pages, most, P, 64, 64, 0, P, 320, 0, 0)
+
+
+def _attend_args(cache, heads=5, q_len=1, table_pages=2, scale=0.125):
+    return (ctypes.addressof(cache), P, 320, 0, q_len, heads, P, table_pages, P, 0, 0, scale, P, 320, P, 1 << 30)
+
+
+def test_sums_and_products_of_arguments_do_not_wrap():
+    """Strides, columns and counts near 2^63, whose sums and products with a head's size would look small."""
+    build()
+    lib = _capi.load_library()
+    good = _desc()
+    assert not _refused(lib, "b2_cache_append_fwd", _capi.CACHE_APPEND_ARGS, _append_args(good))
+    assert not _refused(lib, "b2_cache_attention_fwd", _capi.CACHE_ATTENTION_ARGS, _attend_args(good))
+    for bad in (dict(head_stride=1 << 62), dict(head_stride=(1 << 62) + 32 * 64), dict(page_stride=-(1 << 63))):
+        cache = _desc(**bad)
+        assert _refused(lib, "b2_cache_append_fwd", _capi.CACHE_APPEND_ARGS, _append_args(cache)), bad
+        assert _refused(lib, "b2_cache_attention_fwd", _capi.CACHE_ATTENTION_ARGS, _attend_args(cache)), bad
+    for bad in (dict(cols=(HUGE, 320, 640)), dict(cols=(0, HUGE, 640)), dict(cols=(0, 320, HUGE)), dict(ld=-(1 << 63)),
+                dict(ld=HUGE), dict(heads=5 << 58), dict(table_pages=1 << 60), dict(most=HUGE)):
+        assert _refused(lib, "b2_cache_append_fwd", _capi.CACHE_APPEND_ARGS, _append_args(good, **bad)), bad
+    for bad in (dict(heads=5 << 58), dict(q_len=1 << 62), dict(table_pages=(1 << 60) - 4),
+                dict(scale=math.inf), dict(scale=1e300), dict(scale=1e-300)):
+        assert _refused(lib, "b2_cache_attention_fwd", _capi.CACHE_ATTENTION_ARGS, _attend_args(good, **bad)), bad
+    for heads, scale in ((1 << 58, 0.125), (1 << 62, 0.125), (1, math.inf)):
+        args = (P, 64, P, 64, P, 64, 0, 5, heads, 1, 64, 0, 0, 0, scale, P, 64)
+        assert _refused(lib, "b2_window_attention_fwd", _capi.WINDOW_ATTENTION_ARGS, args)
+    for args in ((1, 1 << 62, 8, 8, 64), (1, 1, 1 << 62, 1, 64), (1, 1, 8, 8, 48), (1, 1, 8, 8, HUGE)):
+        with pytest.raises(RuntimeError):
+            _capi.cache_attention_workspace(*args, sm_count=148)
+    with pytest.raises(RuntimeError):
+        _capi.cache_attention_workspace(1, 1, 8, 8, 64, sm_count=1 << 30)
 
 
 # ---------------------------------------------------------------------------------- where tensors lie

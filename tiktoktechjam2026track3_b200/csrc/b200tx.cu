@@ -10,6 +10,7 @@
 //   * on failure, b2_last_error() returns a message for the calling thread.
 #include <cudaTypedefs.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -509,7 +510,7 @@ static int cache_pages(const b2_kv_cache* c, const char* what, CachePages* out, 
   if (c->kv_heads > 16384 || c->pages > 0x7fffffffLL || c->page_stride > (0x7fffffffLL >> 1))
     return fail(2, "%s: cache too large", what);
   const int64_t head = c->page_size * c->head_dim;
-  if (c->head_stride < head || c->page_stride < c->head_stride * (c->kv_heads - 1) + head)
+  if (c->head_stride < head || (c->kv_heads > 1 && c->head_stride > c->page_stride) || c->page_stride < c->head_stride * (c->kv_heads - 1) + head)
     return fail(1, "%s: page_stride or head_stride too small", what);
   if (c->head_stride % 16 != 0 || c->page_stride % 16 != 0 || !aligned16(c->k) || !aligned16(c->v))
     return fail(2, "%s: cache pointers must be 16-byte aligned, strides multiples of 16 elements", what);
@@ -539,16 +540,16 @@ B2_API int b2_cache_append_fwd(const b2_cache_append_args* args, void* stream) {
   if (num_heads % hk != 0)
     return fail(1, "b2_cache_append_fwd: num_heads=%lld must be a multiple of the cache's kv_heads=%lld",
                 (long long)num_heads, (long long)hk);
-  if (rotary_dim < 0 || rotary_dim > hd || rotary_dim % 16 != 0)
-    return fail(2, "b2_cache_append_fwd: rotary_dim=%lld must be 0 or a multiple of 16 up to head_dim", (long long)rotary_dim);
-  if (q_col < 0 || k_col < 0 || v_col < 0 || q_col % 8 != 0 || k_col % 8 != 0 || v_col % 8 != 0 || ld_qkv % 8 != 0)
-    return fail(2, "b2_cache_append_fwd: q/k/v columns and ld_qkv must be non-negative multiples of 8");
-  if (k_col + hk * hd > ld_qkv || v_col + hk * hd > ld_qkv || (rotary_dim > 0 && q_col + num_heads * hd > ld_qkv))
-    return fail(1, "b2_cache_append_fwd: q/k/v columns exceed ld_qkv");
-  if (rotary_dim > 0 && max_positions <= 0) return fail(1, "b2_cache_append_fwd: max_positions must be positive");
   if (batch > 65535 || tokens > 0x7fffffffLL || max_new > 0x7fffffffLL || num_heads > 65536 ||
       table_pages > (0x7fffffffLL >> p.c.page_shift) || ld_qkv > 0x7fffffffLL)
     return fail(2, "b2_cache_append_fwd: problem too large");
+  if (rotary_dim < 0 || rotary_dim > hd || rotary_dim % 16 != 0)
+    return fail(2, "b2_cache_append_fwd: rotary_dim=%lld must be 0 or a multiple of 16 up to head_dim", (long long)rotary_dim);
+  if (ld_qkv < 0 || q_col < 0 || k_col < 0 || v_col < 0 || q_col % 8 != 0 || k_col % 8 != 0 || v_col % 8 != 0 || ld_qkv % 8 != 0)
+    return fail(2, "b2_cache_append_fwd: q/k/v columns and ld_qkv must be non-negative multiples of 8");
+  if (k_col > ld_qkv - hk * hd || v_col > ld_qkv - hk * hd || (rotary_dim > 0 && q_col > ld_qkv - num_heads * hd))
+    return fail(1, "b2_cache_append_fwd: q/k/v columns exceed ld_qkv");
+  if (rotary_dim > 0 && max_positions <= 0) return fail(1, "b2_cache_append_fwd: max_positions must be positive");
   if (rotary_dim > 0 && (ld_q_out < num_heads * hd || ld_q_out % 8 != 0))
     return fail(2, "b2_cache_append_fwd: ld_q_out must be a multiple of 8 and at least num_heads * head_dim");
   if (k_out != nullptr && (ld_k_out < hk * hd || ld_k_out % 8 != 0))
@@ -591,6 +592,10 @@ B2_API int b2_cache_attention_workspace(int64_t batch, int64_t q_len, int64_t nu
   if (bytes == nullptr) return fail(1, "b2_cache_attention_workspace: null pointer argument");
   if (batch < 0 || q_len <= 0 || num_heads <= 0 || kv_heads <= 0 || num_heads % kv_heads != 0)
     return fail(1, "b2_cache_attention_workspace: invalid shape");
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128)
+    return fail(2, "b2_cache_attention_workspace: head_dim=%lld not supported (32, 64, 128)", (long long)head_dim);
+  if (q_len > 1024 || num_heads > 65536 || sm_count > 65536)
+    return fail(2, "b2_cache_attention_workspace: problem too large");
   int sms = sm_count;
   if (sms <= 0) {
     int dev = 0;
@@ -618,15 +623,16 @@ B2_API int b2_cache_attention_fwd(const b2_cache_attention_args* args, void* str
                 (long long)num_heads, (long long)hk);
   if (window < 0 || sinks < 0 || (window == 0 && sinks != 0))
     return fail(1, "b2_cache_attention_fwd: window and sinks must not be negative, and sinks need a window");
-  if (!(scale > 0.f)) return fail(1, "b2_cache_attention_fwd: scale must be positive");
-  if (ld_q < num_heads * hd || ld_out < num_heads * hd || ld_q % 8 != 0 || ld_out % 8 != 0)
-    return fail(2, "b2_cache_attention_fwd: row strides must be multiples of 8 and at least num_heads * head_dim");
+  if (!(scale > 0.f) || std::isinf(scale)) return fail(1, "b2_cache_attention_fwd: scale must be positive and finite");
+  // Token positions stay below 2^30, so that sums of a position and a window do not leave 32 bits.
+  if (batch > kCacheMaxBatch || q_len > 1024 || num_heads > 65536 || table_pages > ((int64_t{1} << 30) >> p.c.page_shift))
+    return fail(2, "b2_cache_attention_fwd: problem too large");
   const int64_t units = (table_pages << p.c.page_shift) / 64 + 1;  // at most one for 64 tokens
   const int64_t rows = q_len * (num_heads / hk);
-  // Token positions stay below 2^30, so that sums of a position and a window do not leave 32 bits.
-  if (batch > kCacheMaxBatch || q_len > 1024 || num_heads > 65536 || table_pages > ((int64_t{1} << 30) >> p.c.page_shift) ||
-      batch * hk > 0x7fffffffLL / units || rows > 16 * 65535)
+  if (batch * hk > 0x7fffffffLL / units || rows > 16 * 65535)
     return fail(2, "b2_cache_attention_fwd: problem too large");
+  if (ld_q < num_heads * hd || ld_out < num_heads * hd || ld_q % 8 != 0 || ld_out % 8 != 0)
+    return fail(2, "b2_cache_attention_fwd: row strides must be multiples of 8 and at least num_heads * head_dim");
   if (batch == 0) return 0;
   if (q == nullptr || page_table == nullptr || kv_len == nullptr || out == nullptr || workspace == nullptr)
     return fail(1, "b2_cache_attention_fwd: null pointer argument");
@@ -669,14 +675,15 @@ B2_API int b2_window_attention_fwd(const b2_window_attention_args* args, void* s
     return fail(2, "b2_window_attention_fwd: head_dim=%lld not supported (32, 64, 128)", (long long)head_dim);
   if (window < 0 || sinks < 0 || (window == 0 && sinks != 0))
     return fail(1, "b2_window_attention_fwd: window and sinks must not be negative, and sinks need a window");
-  if (!(scale > 0.f)) return fail(1, "b2_window_attention_fwd: scale must be positive");
+  if (!(scale > 0.f) || std::isinf(scale)) return fail(1, "b2_window_attention_fwd: scale must be positive and finite");
+  if (num_heads > 65535) return fail(2, "b2_window_attention_fwd: problem too large");
   const int64_t kv_width = kv_heads * head_dim;
   if (ld_q < num_heads * head_dim || ld_out < num_heads * head_dim || ld_k < kv_width || ld_v < kv_width)
     return fail(1, "b2_window_attention_fwd: row strides must be at least heads * head_dim");
   if (ld_q % 8 != 0 || ld_k % 8 != 0 || ld_v % 8 != 0 || ld_out % 8 != 0)
     return fail(2, "b2_window_attention_fwd: row strides must be multiples of 8");
   // List places (sinks + window + tokens) stay below 2^31; the tensor maps' strides below 2^40 bytes.
-  if (seq_len > (int64_t{1} << 28) || batch > 65535 || num_heads > 65535 || batch * num_heads > 0x7fffffffLL ||
+  if (seq_len > (int64_t{1} << 28) || batch > 65535 || batch * num_heads > 0x7fffffffLL ||
       ((seq_len > 0) && (ld_q | ld_k | ld_v) > ((int64_t{1} << 38) / seq_len)) ||
       (batch * num_heads > 65535 && seq_len >= (int64_t{1} << 18)))
     return fail(2, "b2_window_attention_fwd: problem too large");
