@@ -20,6 +20,9 @@ class _Queries:
     def __init__(self, rows, width):
         self.shape = (rows, width)
 
+    def dim(self):
+        return 2
+
     def size(self, i):
         return self.shape[i]
 
@@ -29,7 +32,7 @@ def _cache(monkeypatch, capturing):
     cache = object.__new__(serving.KVCache)
     cache.head_dim, cache._workspaces, cache._desc = 64, {}, _capi.KVCacheDesc()
     monkeypatch.setattr(_capi, "_current_device", lambda: 0)
-    monkeypatch.setattr(_capi, "_stream_ptr", lambda device: 7)
+    monkeypatch.setattr(_capi, "_stream_of", lambda device: 7)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
     monkeypatch.setattr(cache, "workspace", lambda *size: list(size), raising=False)
     return cache
@@ -232,4 +235,30 @@ def test_tensors_of_another_gpu_are_refused(library):
         for name, t in tensors.items():
             with pytest.raises(ValueError, match="must be on cuda"):
                 call(**(tensors | {name: _On(1, t.shape, t.dtype)}), **rest)
+    assert not library.calls
+
+
+# ---------------------------------------------------------------------------------- refusals by type
+@pytest.mark.parametrize("scaling", [("ntk",), ("linear", 2.0, 3.0), ("parts", 2.0), ("parts", 2.0, 64, 1.0),
+                                     ("parts", 2.0, 0), ("parts", 2.0, 64, 1.0, 32.0, 5.0)])
+def test_malformed_scalings_are_value_errors(scaling):
+    with pytest.raises(ValueError):
+        serving.rotary_table(8, 16, scaling=scaling, device="cpu")
+
+
+def test_attend_refuses_q_of_another_shape_before_it_makes_a_workspace(monkeypatch):
+    cache = _cache(monkeypatch, [False])
+    for q, q_len in ((_On(0, (4, 256)), 0), (_On(0, (4, 256)), -1), (_On(0, (256,)), 1), (_On(0, (2, 2, 64)), 1)):
+        with pytest.raises(ValueError, match="q must be"):
+            serving.KVCache.attend(cache, q, None, None, q_len=q_len, scale=0.1, out=q)
+    assert not cache._workspaces
+
+
+def test_numbers_that_are_not_integers_are_type_errors(library):
+    for call, tensors, rest in _calls(0).values():
+        for name in {"window", "sinks", "max_new", "q_col"} & set(rest):
+            with pytest.raises(TypeError, match="integers"):
+                call(**tensors, **(rest | {name: 4.0}))
+            with pytest.raises(TypeError, match="integers"):
+                call(**tensors, **(rest | {name: 1 << 70}))
     assert not library.calls

@@ -161,6 +161,11 @@ def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _stream_of(device: int) -> int:
+    """The current stream's handle of GPU `device`."""
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -546,14 +551,18 @@ def _elsewhere(t: torch.Tensor, name: str, device: int) -> ValueError:
     return ValueError(f"{name} must be on cuda:{device} as the call's other tensors, got {t.device}")
 
 
-def _launch(entry: str, args: bytes, device: int) -> None:
+def _launch(entry: str, layout: struct.Struct, device: int, *members) -> None:
     """One serving entry point on the current stream of the GPU that holds the call's tensors, made current for it."""
     fn = getattr(_lib or load_library(), entry)
+    try:
+        args = layout.pack(*members)
+    except struct.error as e:
+        raise TypeError(f"{entry}: sizes, windows and counts must be 64-bit integers, scales numbers ({e})") from None
     if _current_device() == device:
-        status = fn(args, _raw_stream(device) if _raw_stream is not None else _stream_ptr(torch.device("cuda", device)))
+        status = fn(args, _stream_of(device))
     else:
         with torch.cuda.device(device):
-            status = fn(args, _stream_ptr(torch.device("cuda", device)))
+            status = fn(args, _stream_of(device))
     if status:
         _check(status, entry)
 
@@ -612,9 +621,10 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, head_d
     if width % head_dim or out.size(0) != tokens or out.size(1) != width:
         raise ValueError(f"x and out must both be [tokens, heads * {head_dim}]")
     most, rotary_dim = _table(table, device)
-    _launch("b2_rotary_fwd", ROTARY_ARGS.pack(
-        x.data_ptr(), ld_x, tokens, width // head_dim, head_dim, rotary_dim, interleaved, inverse,
-        _indices(positions, tokens, "positions", device), table.data_ptr(), most, out.data_ptr(), ld_out), device)
+    _launch(
+        "b2_rotary_fwd", ROTARY_ARGS, device, x.data_ptr(), ld_x, tokens, width // head_dim, head_dim, rotary_dim,
+        interleaved, inverse, _indices(positions, tokens, "positions", device), table.data_ptr(), most, out.data_ptr(),
+        ld_out)
 
 
 def cache_append(cache: KVCacheDesc, qkv: torch.Tensor, num_heads: int, q_col: int, k_col: int, v_col: int,
@@ -639,12 +649,12 @@ def cache_append(cache: KVCacheDesc, qkv: torch.Tensor, num_heads: int, q_col: i
         ld_k = _rows(k_out, "k_out", device)
         if k_out.size(0) != tokens or k_out.size(1) != cache.kv_heads * cache.head_dim:
             raise ValueError("k_out must be [tokens, kv_heads * head_dim]")
-    _launch("b2_cache_append_fwd", CACHE_APPEND_ARGS.pack(
-        ctypes.addressof(cache), qkv.data_ptr(), ld, q_col, k_col, v_col, tokens, num_heads, batch,
-        _indices(new_start, batch, "new_start", device), _indices(new_len, batch, "new_len", device),
-        _indices(past_len, batch, "past_len", device), pages, table_pages, max_new,
-        0 if table is None else table.data_ptr(), positions, rotary_dim, interleaved,
-        0 if q_out is None else q_out.data_ptr(), ld_q, 0 if k_out is None else k_out.data_ptr(), ld_k), device)
+    _launch(
+        "b2_cache_append_fwd", CACHE_APPEND_ARGS, device, ctypes.addressof(cache), qkv.data_ptr(), ld, q_col, k_col,
+        v_col, tokens, num_heads, batch, _indices(new_start, batch, "new_start", device),
+        _indices(new_len, batch, "new_len", device), _indices(past_len, batch, "past_len", device), pages, table_pages,
+        max_new, 0 if table is None else table.data_ptr(), positions, rotary_dim, interleaved,
+        0 if q_out is None else q_out.data_ptr(), ld_q, 0 if k_out is None else k_out.data_ptr(), ld_k)
 
 
 def cache_attention_workspace(batch: int, q_len: int, num_heads: int, kv_heads: int, head_dim: int,
@@ -671,10 +681,10 @@ def cache_attention(cache: KVCacheDesc, q: torch.Tensor, q_len: int, page_table:
     head_dim = cache.head_dim
     if width % head_dim or out.size(0) != rows or out.size(1) != width:
         raise ValueError("q and out must both be [batch * q_len, heads * head_dim]")
-    _launch("b2_cache_attention_fwd", CACHE_ATTENTION_ARGS.pack(
-        ctypes.addressof(cache), q.data_ptr(), ld_q, batch, q_len, width // head_dim, pages, table_pages,
-        _indices(kv_len, batch, "kv_len", device), window, sinks, scale, out.data_ptr(), ld_out, workspace.data_ptr(),
-        workspace.numel()), device)
+    _launch(
+        "b2_cache_attention_fwd", CACHE_ATTENTION_ARGS, device, ctypes.addressof(cache), q.data_ptr(), ld_q, batch, q_len,
+        width // head_dim, pages, table_pages, _indices(kv_len, batch, "kv_len", device), window, sinks, scale,
+        out.data_ptr(), ld_out, workspace.data_ptr(), workspace.numel())
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: int, seq_len: int, head_dim: int,
@@ -689,7 +699,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: i
         raise ValueError("q, k, v and out must have batch * seq_len rows, k and v alike, out like q")
     if width % head_dim or k_width % head_dim:
         raise ValueError(f"q and k must be whole heads of {head_dim}")
-    _launch("b2_window_attention_fwd", WINDOW_ATTENTION_ARGS.pack(
-        q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(), ld_v, batch, seq_len, width // head_dim,
-        k_width // head_dim, head_dim, 0 if kv_len is None else _indices(kv_len, batch, "kv_len", device), window, sinks,
-        scale, out.data_ptr(), ld_out), device)
+    _launch(
+        "b2_window_attention_fwd", WINDOW_ATTENTION_ARGS, device, q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(),
+        ld_v, batch, seq_len, width // head_dim, k_width // head_dim, head_dim,
+        0 if kv_len is None else _indices(kv_len, batch, "kv_len", device), window, sinks, scale, out.data_ptr(), ld_out)

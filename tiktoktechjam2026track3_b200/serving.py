@@ -50,6 +50,8 @@ def rotary_table(max_positions: int, rotary_dim: int, base: float = 10000.0, sca
     kind = scaling[0] if scaling else None
     if kind not in (None, "linear", "ntk", "parts"):
         raise ValueError(f"unknown scaling {kind!r} (linear, ntk, parts)")
+    if scaling and len(scaling) not in ((3, 5) if kind == "parts" else (2,)):
+        raise ValueError(f"scaling {scaling!r} must be (kind, factor) or ('parts', factor, trained[, slow, fast])")
     factor = float(scaling[1]) if scaling else 1.0
     if not factor >= 1.0:
         raise ValueError("the scaling factor must be at least 1")
@@ -61,8 +63,8 @@ def rotary_table(max_positions: int, rotary_dim: int, base: float = 10000.0, sca
     elif kind == "parts":
         trained = float(scaling[2])
         slow, fast = (float(scaling[3]), float(scaling[4])) if len(scaling) > 3 else (1.0, 32.0)
-        if not 0 < slow < fast:
-            raise ValueError("0 < slow < fast turns are needed")
+        if not 0 < slow < fast or not trained > 0:
+            raise ValueError("a positive trained length and 0 < slow < fast turns are needed")
         turns = trained * rate / (2.0 * math.pi)
         keep = ((turns - slow) / (fast - slow)).clamp(0.0, 1.0)
         rate = rate * keep + rate / factor * (1.0 - keep)
@@ -202,12 +204,15 @@ class KVCache:
         """The current stream's workspace, kept between calls (those of one stream run one after the other) and made
         anew when a call is larger than all before it. A call that is being captured gets one of its own: its memory
         and its zeroing are part of the graph, which may run next to the stream's other calls and outlive the kept one."""
-        if _capi._current_device() != self._desc.device:  # the streams meant are those of the cache's GPU
-            with torch.cuda.device(self._desc.device):
+        if q_len < 1 or q.dim() != 2:
+            raise ValueError("q must be [batch * q_len, heads * head_dim], q_len at least 1")
+        device = self._desc.device
+        if _capi._current_device() != device:  # the streams meant are those of the cache's GPU
+            with torch.cuda.device(device):
                 return self._workspace(q, q_len)
         if torch.cuda.is_current_stream_capturing():
             return self.workspace(q.size(0) // q_len, q.size(1) // self.head_dim, q_len)
-        stream, need = _capi._stream_ptr(q.device), q.size(1) * q_len
+        stream, need = _capi._stream_of(device), q.size(1) * q_len
         kept = self._workspaces.get(stream)
         if kept is None or need > kept[0]:
             kept = need, self.workspace(q.size(0) // q_len, q.size(1) // self.head_dim, q_len)
