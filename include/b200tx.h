@@ -328,8 +328,9 @@ typedef struct b2_cache_append_args {
 
 int b2_cache_append_fwd(const b2_cache_append_args* args, void* stream);
 
-/* Bytes of b2_cache_attention_fwd's workspace, 1 to 20 MB on 148 SMs: up to 64 rows (q_len x query heads) of a key head
- * are taken at a time, more in turns over the same memory. sm_count 0 asks the current device. */
+/* Bytes of b2_cache_attention_fwd's workspace: on 148 SMs 1.4 to 5 MB for up to 16 rows (q_len x query heads) of a key
+ * head, as much again for every 16 more, up to 512 rows; still more are taken in turns over the same memory.
+ * sm_count 0 asks the current device. */
 int b2_cache_attention_workspace(int64_t batch, int64_t q_len, int64_t num_heads, int64_t kv_heads, int64_t head_dim,
                                  int sm_count, int64_t* bytes);
 

@@ -87,7 +87,7 @@ def test_steps_enqueued_at_once_are_those_waited_for_one_by_one(heads, room):
 
 
 @pytest.mark.parametrize("heads,kv_heads,head_dim,q_len,dtype", [
-    (16, 1, 64, 5, E4M3), (40, 2, 128, 4, BF16), (12, 1, 32, 11, E4M3), (16, 2, 128, 17, E4M3)])
+    (16, 1, 64, 5, E4M3), (40, 2, 128, 27, BF16), (12, 1, 32, 47, E4M3), (16, 2, 128, 65, E4M3)])
 def test_attend_with_more_row_blocks_than_one_launch_takes(heads, kv_heads, head_dim, q_len, dtype):
     lengths = [1100, 30, 3000]
     cache, seqs = _filled(lengths, 64, kv_heads, head_dim, dtype, 8)
