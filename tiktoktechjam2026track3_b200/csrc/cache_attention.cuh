@@ -73,7 +73,7 @@ constexpr int kCacheGroup = 16;   // of more, so many in a first go
 constexpr int kCacheCluster = 16;  // CTAs of a cluster, at most (a power of two)
 // Row blocks that one launch of the line form takes: more take turns over the same partial results, so that the workspace
 // does not grow with them (160 MB at most; 512 blocks of 16 rows would be 2.5 GB). A turn costs the end of one launch and the
-// start of the next, 28 us: 1024 rows over 100000 bf16 tokens 924 us in one launch, 951 in two, 1346 in sixteen.
+// start of the next, about 30 us: 1024 rows over 100000 bf16 tokens 925 us in one launch, 988 in two, 1346 in sixteen.
 constexpr int kCacheBlocksAtOnce = 32;
 constexpr float kCacheRescale = 8.f;   // log2: the maximum moves when a score exceeds it by more
 constexpr float kCacheHeadroom = 7.f;  // log2: weights are at most 2^(8 + 7), below fp16's largest
@@ -145,10 +145,29 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Pages and scales may be written by the launch before this one, which is still running when this grid's first CTAs are
+// resident: they are not constant for the grid's time, as the read-only path asks, so they come by coherent loads. These
+// leave no line in L1, where nothing would read it again, and are not volatile, so that the compiler may place them
+// freely (their addresses come from loads behind the wait for the grid before). Against plain loads: 64 query heads on 4
+// key heads, 32 x 8192 8-bit tokens, 78.8 -> 74.5 us; 64 x 8192 of 16 heads of 64, 187.6 -> 179.5.
+__device__ __forceinline__ uint4 load_once4(const void* p) {
+  uint4 u;
+  asm("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+  return u;
+}
+__device__ __forceinline__ uint2 load_once2(const void* p) {
+  uint2 u;
+  asm("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(u.x), "=r"(u.y) : "l"(p));
+  return u;
+}
+__device__ __forceinline__ uint32_t load_once(const void* p) {
+  uint32_t u;
+  asm("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(u) : "l"(p));
+  return u;
+}
+
 // 32-bit words of a token that one thread holds, and where they lie: vectors of up to 4 words; a thread's vectors are
-// `lanes` vectors apart, so that each load of the warp covers consecutive bytes of a row. Plain loads: pages and scales
-// may be written by the launch before this one, which is still running when this grid's first CTAs are resident, so
-// that they are not constant for the grid's time as the read-only path asks.
+// `lanes` vectors apart, so that each load of the warp covers consecutive bytes of a row.
 template <int kWords, int kLanes>
 struct RowPieces {
   static constexpr int kVec = kWords < 4 ? kWords : 4;
@@ -162,17 +181,17 @@ struct RowPieces {
     for (int v = 0; v < kVectors; ++v) {
       const uint8_t* src = row + v * (4 * kVec * kLanes) + at * 4 * kVec;
       if constexpr (kVec == 4) {
-        const uint4 u = *reinterpret_cast<const uint4*>(src);
+        const uint4 u = load_once4(src);
         w[4 * v] = u.x;
         w[4 * v + 1] = u.y;
         w[4 * v + 2] = u.z;
         w[4 * v + 3] = u.w;
       } else if constexpr (kVec == 2) {
-        const uint2 u = *reinterpret_cast<const uint2*>(src);
+        const uint2 u = load_once2(src);
         w[2 * v] = u.x;
         w[2 * v + 1] = u.y;
       } else {
-        w[v] = *reinterpret_cast<const uint32_t*>(src);
+        w[v] = load_once(src);
       }
     }
   }
