@@ -262,3 +262,12 @@ def test_numbers_that_are_not_integers_are_type_errors(library):
             with pytest.raises(TypeError, match="integers"):
                 call(**tensors, **(rest | {name: 1 << 70}))
     assert not library.calls
+
+
+def test_heads_of_no_width_are_value_errors(library):
+    for name in ("b2_rotary_fwd", "b2_window_attention_fwd"):
+        call, tensors, rest = _calls(0)[name]
+        for head_dim in (0, -64):
+            with pytest.raises(ValueError, match="heads"):
+                call(**tensors, **(rest | dict(head_dim=head_dim)))
+    assert not library.calls

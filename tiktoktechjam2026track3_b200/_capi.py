@@ -618,7 +618,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, head_d
     device = x.get_device()
     ld_x, ld_out = _rows(x, "x", device), _rows(out, "out", device)
     tokens, width = x.size(0), x.size(1)
-    if width % head_dim or out.size(0) != tokens or out.size(1) != width:
+    if head_dim < 1 or width % head_dim or out.size(0) != tokens or out.size(1) != width:
         raise ValueError(f"x and out must both be [tokens, heads * {head_dim}]")
     most, rotary_dim = _table(table, device)
     _launch(
@@ -697,7 +697,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: i
     if (rows != batch * seq_len or k.size(0) != rows or v.size(0) != rows or out.size(0) != rows or v.size(1) != k_width
             or out.size(1) != width):
         raise ValueError("q, k, v and out must have batch * seq_len rows, k and v alike, out like q")
-    if width % head_dim or k_width % head_dim:
+    if head_dim < 1 or width % head_dim or k_width % head_dim:
         raise ValueError(f"q and k must be whole heads of {head_dim}")
     _launch(
         "b2_window_attention_fwd", WINDOW_ATTENTION_ARGS, device, q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(),
