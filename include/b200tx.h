@@ -339,7 +339,8 @@ int b2_cache_attention_workspace(int64_t batch, int64_t q_len, int64_t num_heads
  * at p = kv_len[b] - q_len + t and sees the keys j <= p with window == 0, p - j < window or j < sinks;
  * out = softmax(scale * q k^T) v, zero where nothing is visible. What lies in pages and slots that no row
  * sees is not used, whatever it is. Of the tokens that some of the q_len rows see and others do not,
- * a value that is not finite reaches them all.
+ * a value that is not finite reaches them all. In 8 bits, tokens whose weight times the scale of their page of V is
+ * more than 2^32 below the largest count as if their values were zero.
  *   q, out     [batch * q_len, ld] bf16, num_heads heads side by side, a multiple of the cache's kv_heads:
  *              query head i reads key head i / (num_heads / kv_heads). head_dim 32, 64 or 128
  *   kv_len     [batch] int32, the tokens in the cache, the q_len newest included

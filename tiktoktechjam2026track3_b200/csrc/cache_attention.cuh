@@ -22,6 +22,12 @@
 // largest element to [2^14, 2^15): bf16's 8 bits then fit exactly down to 2^-28 of the largest.
 // The maximum moves only when a score exceeds it by 2^8 (the weights keep 2^7 of headroom below fp16's
 // subnormals); sums, maxima and outputs are fp32.
+// Roundings to fewer bits, for the products' sake: weights to the type of the values they meet, fp16 over 8 bits (11
+// bits, far below the codes' own 4) and bf16 over bf16 (one mma takes one type); the sums take them unrounded. Measured
+// over whole outputs against 64 bits, with the output's own rounding to bf16 in it: 0.0015 to 0.0017 of the norm over 8
+// bits, as with weights of 32 bits, and 0.0023 over bf16 (0.0017). fp16 bounds the range, too: a weight times its
+// page's scale of V loses bits from 2^21 below the largest on and is dropped from 2^32 on, even in dims where the page with the
+// large scale holds zeros.
 //
 // Split: a (sequence, key head) is cut into units of 16 tokens per warp. Calls of moderate length give each to one CTA,
 // or to a cluster of CTAs that share its units and join their maxima, sums and outputs through shared memory. Else all
@@ -35,10 +41,10 @@
 // or shared memory. Heads of 64 and 32 take 2 and 4 tiles of 16 tokens at a time, interleaved.
 // Measured on one B200 (us a call back to back, floor at the measured copy rate in brackets; first form, which read each
 // page number in the loop and joined element by element): 8 x 131072 8-bit tokens, 8 key heads of 128, 4 query heads
-// each: 327 (328; 355); 64 sequences of up to 8192: 116 (100; 129); one of 131072: 58 (41; 111), one of 8192: 13 (2.6; 22);
-// bf16, 32 x 8192: 166 (164; 181); 32 windows of 4096 bf16 tokens, 10 rows: 52 (41; 104); 16 key heads of 64: 186 (165;
-// 265), of 32: 112 (82; 226); 12 heads of 1001 tokens: 6.9 (0.2; 12.6). At the 1000 W limit the clock drops and the
-// first two take 368 and 125. A short call is 5 us of dependent steps (lengths, page numbers, keys, join of the warps),
+// each: 331 (328; 355); 64 sequences of up to 8192: 115 (100; 129); one of 131072: 59 (41; 111), one of 8192: 12 (2.6; 22);
+// bf16, 32 x 8192: 165 (164; 181); 32 windows of 4096 bf16 tokens, 10 rows: 52 (41; 104); 16 key heads of 64: 180 (165;
+// 265), of 32: 109 (82; 226); 12 heads of 1001 tokens: 6.8 (0.2; 12.6). At the 1000 W limit the clock drops and the
+// first two take 378 and 127. A short call is 5 us of dependent steps (lengths, page numbers, keys, join of the warps),
 // a join of CTAs 3 to 5 more.
 #pragma once
 #include <algorithm>
