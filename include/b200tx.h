@@ -56,7 +56,7 @@ const char* b2_last_error(void);
  * waiting), or where that is 0 the indices' (a position, length or page number read from device memory lay
  * outside its table; what it names was skipped, other results are valid). 0 = neither since the last clear;
  * otherwise (kernel << 16) | (site << 8) | reason, kernel 2 = linear, 3 = attention, 5 = rotary,
- * 6 = cache append, 7 = cache attention; reason 1 = a wait ran out, 3 = an index. Synchronous: it
+ * 6 = cache append, 7 = cache attention, 8 = cache read, 9 = packed attention; reason 1 = a wait ran out, 3 = an index. Synchronous: it
  * waits for the device. */
 int b2_device_status(uint32_t* out_status, int clear);
 
@@ -281,6 +281,7 @@ int b2_rotary_fwd(const b2_rotary_args* args, void* stream);
 /* Element type of a cache's pages. */
 #define B2_CACHE_BF16 0
 #define B2_CACHE_E4M3 1 /* e4m3 codes, one power-of-two fp32 scale per page and head */
+#define B2_CACHE_INT4 2 /* 4-bit codes, a bf16 step and middle for every 32 elements of a token and head */
 
 /*
  * A paged key/value cache: a page holds page_size (16, 32, 64, 128 or 256) consecutive tokens of one sequence for
@@ -288,7 +289,12 @@ int b2_rotary_fwd(const b2_rotary_args* args, void* stream);
  * slot * head_dim + dim (in elements; likewise V). Sequences own pages through a page table,
  * [batch, table_pages] int32: token j of sequence b is in slot j % page_size of page
  * page_table[b][j / page_size]. In 8 bits the value of a code is e4m3(code) * scale[page][head]. The scales are
- * powers of two between 2^-40 and 2^40; b2_cache_append_fwd writes them. The reference has no cache.
+ * powers of two between 2^-40 and 2^40; b2_cache_append_fwd writes them.
+ * In 4 bits (head_dim a multiple of 32, strides multiples of 32 elements; two elements to a byte) 32 neighbouring elements
+ * of a head of one token are a group; code c of 0 ... 15 stands for middle + (c - 8) * step. The head_dim / 2 bytes of a
+ * token and head hold, for i = 0 ... 7 and each group, two bytes with the codes of the group's elements 4 i ... 4 i + 3, the
+ * first in the lowest bits. k_group and v_group hold the groups' steps and middles,
+ * [pages][kv_heads][page_size][2][head_dim / 32] bf16, steps before middles. The reference has no cache.
  */
 typedef struct b2_kv_cache {
   void* k;
@@ -297,6 +303,8 @@ typedef struct b2_kv_cache {
   float* v_scale;
   int64_t pages, kv_heads, page_size, head_dim, page_stride, head_stride;
   int dtype;
+  void* k_group; /* 4 bits only: not read for the other types */
+  void* v_group;
 } b2_kv_cache;
 
 /*
@@ -307,6 +315,9 @@ typedef struct b2_kv_cache {
  * or the page's scale before where that is larger and the page holds earlier tokens of the sequence;
  * where it grows the earlier tokens' codes are rounded again. Codes are rounded to nearest even from
  * fp32, values that are not finite become NaN.
+ * 4-bit pages: of a group's values step = (most - least) / 15 (0 below 2^-100) and middle = least + 8 step, both rounded to
+ * bf16, and each code is 8 + the whole number in [-8, 7] nearest (the even one at a half) to (x - middle) * bf16(1 / step). A
+ * group with a value that is not finite, or whose range is not, reads as NaN. Earlier tokens are not touched.
  *   qkv    [tokens, ld_qkv] bf16, heads of Q at columns q_col ..., of K at k_col ..., of V at v_col ...
  *   table  as in b2_rotary_fwd
  *   q_out  [tokens, ld_q_out] bf16: rotated Q (rotary_dim > 0 only; may be qkv's own columns)
@@ -327,6 +338,27 @@ typedef struct b2_cache_append_args {
 } b2_cache_append_args;
 
 int b2_cache_append_fwd(const b2_cache_append_args* args, void* stream);
+
+/*
+ * Tokens of a cache as bf16 rows: row out_start[b] + i of k_out and v_out receives the key and the value (all heads side by
+ * side) of token start[b] + i of sequence b, for i < length[b]; max_len is at least every length. The values are those that
+ * the cache's codes stand for, rounded to bf16. Other rows are left as they are. The way from an 8- or 4-bit cache to
+ * b2_packed_attention_fwd.
+ *   k_out, v_out  [rows, ld] bf16; one of them may be NULL
+ */
+typedef struct b2_cache_read_args {
+  const b2_kv_cache* cache;
+  const int32_t *out_start, *length, *start;
+  int64_t batch;
+  const int32_t* page_table;
+  int64_t table_pages, max_len, rows;
+  void* k_out;
+  int64_t ld_k_out;
+  void* v_out;
+  int64_t ld_v_out;
+} b2_cache_read_args;
+
+int b2_cache_read_fwd(const b2_cache_read_args* args, void* stream);
 
 /* Bytes of b2_cache_attention_fwd's workspace: on 148 SMs 1.4 to 5 MB for up to 16 rows (q_len x query heads) of a key
  * head, as much again for every 16 more, up to 512 rows; still more are taken in turns over the same memory.
@@ -391,6 +423,32 @@ typedef struct b2_window_attention_args {
 } b2_window_attention_args;
 
 int b2_window_attention_fwd(const b2_window_attention_args* args, void* stream);
+
+/*
+ * The same for packed sequences of different lengths, whose queries may be the last of their keys: sequence b has the rows
+ * q_start[b] ... q_start[b + 1] - 1 of q and out and kv_start[b] ... kv_start[b + 1] - 1 of k and v, n_q and n_kv of them, and
+ * its query i stands at p = n_kv - n_q + i among its keys. It sees key j <= p iff window == 0, p - j < window or j < sinks;
+ * a row that sees none (p < 0, no keys) gives zeros. Rows of out that belong to no sequence are left as they are.
+ * What other sequences hold does not reach a sequence; what the previous entry point says of values that are not finite holds
+ * within one. A sequence that lies outside the rows, or ends before it begins, is skipped and recorded.
+ *   q_start, kv_start  [batch + 1] int32, ascending; the same pointer for whole prompts
+ *   q, out  [q_rows, ld] bf16; k, v  [kv_rows, ld] bf16. head_dim 32, 64 or 128
+ */
+typedef struct b2_packed_attention_args {
+  const void* q;
+  int64_t ld_q, q_rows;
+  const void* k;
+  int64_t ld_k;
+  const void* v;
+  int64_t ld_v, kv_rows;
+  const int32_t *q_start, *kv_start;
+  int64_t batch, num_heads, kv_heads, head_dim, window, sinks;
+  double scale;
+  void* out;
+  int64_t ld_out;
+} b2_packed_attention_args;
+
+int b2_packed_attention_fwd(const b2_packed_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }

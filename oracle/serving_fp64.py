@@ -54,6 +54,38 @@ def e4m3(x):
     return torch.where(torch.isfinite(x), y, math.nan)
 
 
+def int4_params(x):
+    """(step, middle) of each group of 32 neighbours of x [..., head_dim], float64 values that bf16 holds."""
+    y = x.double().reshape(*x.shape[:-1], -1, 32)
+    lo, hi = y.amin(-1), y.amax(-1)
+    step = ((hi - lo) / 15).bfloat16().double()
+    step = torch.where(step < 2.0**-100, 0.0, step)
+    mid = (lo + 8 * step).bfloat16().double()
+    bad = ~torch.isfinite(y).all(-1)
+    return torch.where(bad, math.nan, step), torch.where(bad, math.nan, mid)
+
+
+def int4(x):
+    """What 4 bits hold of x [..., head_dim], float64."""
+    step, mid = int4_params(x)
+    y = x.double().reshape(*x.shape[:-1], -1, 32)
+    inverse = torch.where(step > 0, (1 / step.clamp(min=2.0**-100)).bfloat16().double(), 0.0)
+    code = torch.round((y - mid[..., None]) * inverse[..., None]).clamp(-8, 7)
+    return (mid[..., None] + code * step[..., None]).reshape(x.shape)
+
+
+def int4_decode(codes, params):
+    """Values of codes [..., head_dim / 2] with params [..., 2, head_dim / 32]: every element looked up by its number."""
+    hd = 2 * codes.shape[-1]
+    out = torch.empty(*codes.shape[:-1], hd, dtype=torch.float64)
+    for d in range(hd):
+        group, i = divmod(d, 32)
+        byte = codes[..., 2 * ((i // 4) * (hd // 32) + group) + (i % 4) // 2].int()
+        c = (byte >> 4 if i % 2 else byte & 15) - 8
+        out[..., d] = params[..., 1, group].double() + c * params[..., 0, group].double()
+    return out
+
+
 def attend(q, k, v, visible, scale):
     """One head: q [rows, d], k and v [keys, d], visible bool [rows, keys], all float64.
 

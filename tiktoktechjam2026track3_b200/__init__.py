@@ -8,7 +8,7 @@ names, forward signature and mask semantics; computation in hand-written tcgen05
 from .cases import BASELINE_CONFIGS, TransformerConfig, Workload, config_from
 from .correctness import AccuracyResult, GateResult, baseline_gate, compare_outputs
 from .models import UserOptimizedTransformer, copy_model_weights
-from .serving import KVCache, rotary, rotary_table, window_attention
+from .serving import KVCache, packed_attention, rotary, rotary_table, window_attention
 from .streaming import StreamingTransformer
 
 __all__ = [
@@ -24,6 +24,7 @@ __all__ = [
     "compare_outputs",
     "config_from",
     "copy_model_weights",
+    "packed_attention",
     "rotary",
     "rotary_table",
     "window_attention",

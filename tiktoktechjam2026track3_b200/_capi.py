@@ -32,6 +32,7 @@ TILE_PAIR = 0x10000
 REASON_BAD_INDEX = 3  # of the status word: a position, length or page number lay outside its table
 CACHE_BF16 = 0
 CACHE_E4M3 = 1
+CACHE_INT4 = 2
 
 # Every symbol include/b200tx.h declares, with its ctypes signature.
 _i64 = ctypes.c_int64
@@ -43,7 +44,7 @@ class KVCacheDesc(ctypes.Structure):
 
     _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", _i64), ("kv_heads", _i64),
                 ("page_size", _i64), ("head_dim", _i64), ("page_stride", _i64), ("head_stride", _i64),
-                ("dtype", ctypes.c_int)]
+                ("dtype", ctypes.c_int), ("k_group", _vp), ("v_group", _vp)]
     device = 0  # index of the GPU that holds them (not part of the C struct)
 
 
@@ -51,7 +52,9 @@ class KVCacheDesc(ctypes.Structure):
 ROTARY_ARGS = struct.Struct("13q")
 CACHE_APPEND_ARGS = struct.Struct("23q")
 CACHE_ATTENTION_ARGS = struct.Struct("11qd4q")
+CACHE_READ_ARGS = struct.Struct("13q")
 WINDOW_ATTENTION_ARGS = struct.Struct("14qd2q")
+PACKED_ATTENTION_ARGS = struct.Struct("16qd2q")
 SIGNATURES = {
     "b2_abi_version": (ctypes.c_int, []),
     "b2_last_error": (ctypes.c_char_p, []),
@@ -108,7 +111,9 @@ SIGNATURES = {
     "b2_rotary_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
     "b2_cache_append_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
     "b2_cache_attention_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
+    "b2_cache_read_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
     "b2_window_attention_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
+    "b2_packed_attention_fwd": (ctypes.c_int, [ctypes.c_char_p, _vp]),
     "b2_cache_attention_workspace": (
         ctypes.c_int, [_i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.POINTER(_i64)],
     ),
@@ -248,7 +253,7 @@ class StatusWatch:
             self.status = value
             kernel, site, reason = value >> 16, (value >> 8) & 0xFF, value & 0xFF
             names = {1: "layernorm", 2: "linear", 3: "attention", 4: "peer barrier", 5: "rotary", 6: "cache append",
-                     7: "cache attention"}
+                     7: "cache attention", 8: "cache read", 9: "packed attention"}
             what, so = "gave up waiting", "outputs computed since then are not valid"
             if reason == REASON_BAD_INDEX:
                 what, so = "met an index outside its table", "what it names was skipped"
@@ -657,6 +662,27 @@ def cache_append(cache: KVCacheDesc, qkv: torch.Tensor, num_heads: int, q_col: i
         0 if q_out is None else q_out.data_ptr(), ld_q, 0 if k_out is None else k_out.data_ptr(), ld_k)
 
 
+def cache_read(cache: KVCacheDesc, out_start: torch.Tensor, length: torch.Tensor, start: torch.Tensor,
+               page_table: torch.Tensor, max_len: int, k_out: Optional[torch.Tensor], v_out: Optional[torch.Tensor]) -> None:
+    """Tokens of the cache as bf16 rows of k_out and v_out (see b2_cache_read_fwd)."""
+    device = cache.device
+    batch, width = length.numel(), cache.kv_heads * cache.head_dim
+    pages, table_pages = _page_table(page_table, batch, device)
+    if k_out is None and v_out is None:
+        raise ValueError("k_out or v_out is needed")
+    rows, strides = -1, [0, 0]
+    for i, (t, name) in enumerate(((k_out, "k_out"), (v_out, "v_out"))):
+        if t is not None:
+            strides[i] = _rows(t, name, device)
+            if t.size(1) != width or (rows >= 0 and t.size(0) != rows):
+                raise ValueError(f"k_out and v_out must be [rows, {width}], alike")
+            rows = t.size(0)
+    _launch(
+        "b2_cache_read_fwd", CACHE_READ_ARGS, device, ctypes.addressof(cache), _indices(out_start, batch, "out_start", device),
+        _indices(length, batch, "length", device), _indices(start, batch, "start", device), batch, pages, table_pages, max_len,
+        rows, 0 if k_out is None else k_out.data_ptr(), strides[0], 0 if v_out is None else v_out.data_ptr(), strides[1])
+
+
 def cache_attention_workspace(batch: int, q_len: int, num_heads: int, kv_heads: int, head_dim: int,
                               sm_count: int = 0) -> int:
     """Bytes of cache_attention's workspace (see b2_cache_attention_workspace)."""
@@ -703,3 +729,23 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: i
         "b2_window_attention_fwd", WINDOW_ATTENTION_ARGS, device, q.data_ptr(), ld_q, k.data_ptr(), ld_k, v.data_ptr(),
         ld_v, batch, seq_len, width // head_dim, k_width // head_dim, head_dim,
         0 if kv_len is None else _indices(kv_len, batch, "kv_len", device), window, sinks, scale, out.data_ptr(), ld_out)
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start: torch.Tensor, kv_start: torch.Tensor,
+                     head_dim: int, window: int, sinks: int, scale: float, out: torch.Tensor) -> None:
+    """out = causal attention of packed sequences (see b2_packed_attention_fwd)."""
+    device = q.get_device()
+    ld_q, ld_k = _rows(q, "q", device), _rows(k, "k", device)
+    ld_v, ld_out = _rows(v, "v", device), _rows(out, "out", device)
+    rows, width, k_width = q.size(0), q.size(1), k.size(1)
+    if out.size(0) != rows or out.size(1) != width or v.size(0) != k.size(0) or v.size(1) != k_width:
+        raise ValueError("out must be like q, and v like k")
+    if head_dim < 1 or width % head_dim or k_width % head_dim:
+        raise ValueError(f"q and k must be whole heads of {head_dim}")
+    batch = q_start.numel() - 1
+    if batch < 0:
+        raise ValueError("q_start must have an entry for every sequence and one behind the last")
+    _launch(
+        "b2_packed_attention_fwd", PACKED_ATTENTION_ARGS, device, q.data_ptr(), ld_q, rows, k.data_ptr(), ld_k, v.data_ptr(),
+        ld_v, k.size(0), _indices(q_start, batch + 1, "q_start", device), _indices(kv_start, batch + 1, "kv_start", device),
+        batch, width // head_dim, k_width // head_dim, head_dim, window, sinks, scale, out.data_ptr(), ld_out)

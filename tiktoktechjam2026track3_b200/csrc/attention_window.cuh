@@ -48,6 +48,11 @@ struct WindowParams {
   int window, sinks;  // window <= 0: none
   float scale_log2;
   int head_major;  // as in AttnParams
+  // Packed sequences (B = 1, S = 0): sequence b of `batch` has the rows q_start[b] ... q_start[b + 1] - 1 of q_rows queries and
+  // kv_start[b] ... kv_start[b + 1] - 1 of kv_rows keys.
+  const int32_t* q_start;
+  const int32_t* kv_start;
+  int batch, q_rows, kv_rows;
 };
 
 // Keys and values [B][S][kv_heads][head_dim] in boxes of 64 columns and 128 or 16 rows; Q in boxes of a query tile.
@@ -64,10 +69,11 @@ struct KeyList {
   int rows, tiles;
 };
 
-__device__ __forceinline__ KeyList window_keys(const WindowParams& p, int tile, int len) {
+// `first`: the position of the sequence's first query.
+__device__ __forceinline__ KeyList window_keys(const WindowParams& p, int tile, int len, int first = 0) {
   KeyList l;
   const int tokens = 128 >> p.group_shift;
-  l.i0 = tile * tokens;
+  l.i0 = first + tile * tokens;
   l.i1 = min(l.i0 + tokens, len);
   l.lo = p.window > 0 ? max(0, l.i0 - p.window + 1) : 0;
   if (p.sinks >= l.lo) {
@@ -94,21 +100,21 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
 // `sinks`, `sinks16`: the maps for the part in front of the band.
 __device__ __forceinline__ void window_load_tile(uint8_t* dst, const CUtensorMap* map, const CUtensorMap* map16,
                                                  const CUtensorMap* sinks, const CUtensorMap* sinks16, uint64_t* bar,
-                                                 const KeyList& l, int t, int col, int head, int b) {
+                                                 const KeyList& l, int t, int col, int head, int row0, int b) {
   const int v0 = 128 * t;
   if (v0 >= l.sink_rows) {
-    tma_load_4d(dst, map, bar, col, head, l.lo + v0 - l.sink_rows, b);
+    tma_load_4d(dst, map, bar, col, head, row0 + l.lo + v0 - l.sink_rows, b);
     return;
   }
   if (v0 + 128 <= l.sink_rows) {
-    tma_load_4d(dst, sinks, bar, col, head, v0, b);
+    tma_load_4d(dst, sinks, bar, col, head, row0 + v0, b);
     return;
   }
 #pragma unroll 1
   for (int r = 0; r < 128; r += 16) {
     const int v = v0 + r;
     const bool sink = v < l.sink_rows;
-    tma_load_4d(dst + r * 128, sink ? sinks16 : map16, bar, col, head, sink ? v : l.lo + v - l.sink_rows, b);
+    tma_load_4d(dst + r * 128, sink ? sinks16 : map16, bar, col, head, row0 + (sink ? v : l.lo + v - l.sink_rows), b);
   }
 }
 
@@ -129,6 +135,7 @@ __device__ __forceinline__ RowKeys window_row(const WindowParams& p, int lo, int
 // that hide nothing.
 struct WindowTiles {
   int i0, lo, sink_rows, rows, count;
+  int out_row, valid;  // packed: the row of the tile's first query, and how many it has
   int open_a, open_c, open_d;  // tiles below open_d that lie from open_c on or below open_a hide no key from these rows
   __device__ __forceinline__ bool open(int t) const { return t < open_d && (t >= open_c || t < open_a); }
   __device__ __forceinline__ RowKeys row(const WindowParams& p, int i) const { return window_row(p, lo, sink_rows, i); }
@@ -172,11 +179,23 @@ __device__ __forceinline__ void window_zero_rows(const WindowParams& p, int b, i
   }
 }
 
-// Clears rows [from, 128) of a value tile (128-byte rows, `boxes` boxes of 64 columns) and makes that visible to the
+// The same for `tokens` packed rows from `row0` on.
+template <int HD>
+__device__ __forceinline__ void window_zero_packed_rows(const WindowParams& p, int64_t row0, int tokens, int head0) {
+  const int group = 1 << p.group_shift;
+  constexpr int kPieces = HD / 8;
+  for (int i = threadIdx.x; i < tokens * group * kPieces; i += blockDim.x) {
+    const int token = i / (group * kPieces);
+    const int rest = i - token * (group * kPieces);
+    reinterpret_cast<uint4*>(p.ctx + (row0 + token) * p.ld_ctx + head0 * HD)[rest] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Clears rows [from, to) of a value tile (128-byte rows, `boxes` boxes of 64 columns) and makes that visible to the
 // tensor core; the threads of `warps` warps share it.
 template <int kBoxes>
-__device__ __forceinline__ void window_clear_values(uint8_t* tile, int from, int thread, int threads) {
-  for (int i = from * 8 + thread; i < 128 * 8; i += threads) {
+__device__ __forceinline__ void window_clear_values(uint8_t* tile, int from, int to, int thread, int threads) {
+  for (int i = from * 8 + thread; i < to * 8; i += threads) {
 #pragma unroll
     for (int box = 0; box < kBoxes; ++box) reinterpret_cast<uint4*>(tile + box * 128 * 128)[i] = make_uint4(0, 0, 0, 0);
   }
@@ -192,11 +211,64 @@ __device__ __forceinline__ void window_cta(const WindowParams& p, int& b, int& h
   tile = p.tiles - 1 - row;  // the longest lists first
 }
 
+// A packed call's CTA: which sequence and which of its query tiles.
+struct PackedTile {
+  int q0, n_q, k0, n_kv;  // rows of the sequence
+  int tile, rows;         // and of the tile
+};
+
+// Sequence b has places q_start[b] / tokens + b ... on the line of all query tiles: at least as many as it has tiles, since the
+// next one's first place lies a whole tile further than its rows do. A warp finds the sequence of a place in one turn for
+// every factor of 32 of the batch. False: no tile there (up to one place a sequence), or a sequence that lies outside
+// the rows.
+__device__ __forceinline__ bool packed_tile(const WindowParams& p, int place, PackedTile& t) {
+  const int lane = threadIdx.x & 31;
+  const int shift = 7 - p.group_shift;
+  int lo = 0, n = p.batch, first = 0;
+  while (true) {
+    const int step = (n + 31) >> 5;
+    const int b = lo + lane * step;
+    int at = 0;
+    bool below = false;
+    if (lane * step < n) {
+      at = (p.q_start[b] >> shift) + b;
+      below = at <= place;
+    }
+    const uint32_t seen = __ballot_sync(0xffffffffu, below);
+    if (seen == 0) return false;
+    const int k = 31 - __clz(seen);
+    first = __shfl_sync(0xffffffffu, at, k);
+    lo += k * step;
+    n = min(step, n - k * step);
+    if (step == 1) break;
+  }
+  t.q0 = p.q_start[lo];
+  const int q1 = p.q_start[lo + 1];
+  t.k0 = p.kv_start[lo];
+  const int k1 = p.kv_start[lo + 1];
+  if (t.q0 < 0 || q1 < t.q0 || q1 > p.q_rows || t.k0 < 0 || k1 < t.k0 || k1 > p.kv_rows) return false;
+  t.n_q = q1 - t.q0;
+  t.n_kv = k1 - t.k0;
+  t.tile = place - first;
+  const int row = t.tile << shift;
+  t.rows = min(1 << shift, t.n_q - row);
+  return t.rows > 0;
+}
+
+// One CTA of the call looks at all sequences, so that one that nobody finds is reported too.
+__device__ __forceinline__ void packed_check(const WindowParams& p) {
+  for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
+    const int q0 = p.q_start[b], q1 = p.q_start[b + 1], k0 = p.kv_start[b], k1 = p.kv_start[b + 1];
+    if (q0 < 0 || q1 < q0 || q1 > p.q_rows || k0 < 0 || k1 < k0 || k1 > p.kv_rows)
+      record_status(kKernelPackedAttention, 1, kReasonBadIndex);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
 // head_dim 32 and 64: the pipeline of attention_solo_kernel (two CTAs per SM). head_dim 32 is loaded in 64-column boxes
 // whose second half lies outside the head and reads as zeros.
 // ---------------------------------------------------------------------------------------------
-template <int HD>
+template <int HD, bool kPacked>
 __global__ void __launch_bounds__(192, 2)
     window_solo_kernel(const __grid_constant__ WindowMaps maps, const WindowParams p) {
   static_assert(HD == 32 || HD == 64, "head_dim 32 or 64");
@@ -250,10 +322,20 @@ __global__ void __launch_bounds__(192, 2)
   }
   pdl_wait_previous_grid();
   pdl_allow_next_grid();
-  const int len = p.kv_len != nullptr ? min(max(p.kv_len[b], 0), p.S) : p.S;
-  const KeyList keys = window_keys(p, tile, len);
-  if (keys.i0 >= len) {  // uniform for the CTA; no tensor memory allocated yet
-    window_zero_rows<HD>(p, b, head0, keys.i0);
+  PackedTile seq;
+  if constexpr (kPacked) {
+    if (blockIdx.x == 0 && blockIdx.y == 0) packed_check(p);
+    if (!packed_tile(p, tile, seq)) return;
+  }
+  const int len = kPacked ? seq.n_kv : p.kv_len != nullptr ? min(max(p.kv_len[b], 0), p.S) : p.S;
+  const KeyList keys = kPacked ? window_keys(p, seq.tile, len, len - seq.n_q) : window_keys(p, tile, len);
+  const int q_row = kPacked ? seq.q0 + seq.tile * (128 >> p.group_shift) : keys.i0;  // of the tile's first query
+  const int kv_row = kPacked ? seq.k0 : 0;
+  if (kPacked ? keys.i1 <= 0 : keys.i0 >= len) {  // uniform for the CTA; no tensor memory allocated yet
+    if constexpr (kPacked)
+      window_zero_packed_rows<HD>(p, q_row, seq.rows, head0);
+    else
+      window_zero_rows<HD>(p, b, head0, keys.i0);
     return;
   }
   const int n = keys.tiles;
@@ -261,6 +343,10 @@ __global__ void __launch_bounds__(192, 2)
   if (warp >= 2 && lane == 0) {
     const int r0 = (warp & 3) * 32;
     s_tiles[warp & 3] = window_tiles(p, keys, keys.i0 + (r0 >> p.group_shift), keys.i0 + ((r0 + 31) >> p.group_shift));
+    if constexpr (kPacked) {
+      s_tiles[warp & 3].out_row = q_row;
+      s_tiles[warp & 3].valid = seq.rows;
+    }
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 256);
@@ -276,7 +362,7 @@ __global__ void __launch_bounds__(192, 2)
     if (lane == 0) {
       const int kv_head = head0 / (p.heads / p.kv_heads);
       mbar_arrive_expect_tx(q_full, kTileBytes);
-      tma_load_4d(s_q, &maps.q, q_full, 0, head0, keys.i0, b);
+      tma_load_4d(s_q, &maps.q, q_full, 0, head0, q_row, b);
       int k_next = 0, v_next = 0;
       bool ok = true;
       PollTimeout poll;
@@ -286,14 +372,14 @@ __global__ void __launch_bounds__(192, 2)
         if (k_next < n && mbar_test_wait(&k_empty[k_next % kStages], ((k_next / kStages) & 1) ^ 1u)) {
           const int st = k_next % kStages;
           mbar_arrive_expect_tx(&k_full[st], kTileBytes);
-          window_load_tile(s_k + st * kTileBytes, &maps.k, &maps.k16, &maps.k, &maps.k16, &k_full[st], keys, k_next, 0, kv_head, b);
+          window_load_tile(s_k + st * kTileBytes, &maps.k, &maps.k16, &maps.k, &maps.k16, &k_full[st], keys, k_next, 0, kv_head, kv_row, b);
           ++k_next;
           progress = true;
         }
         if (v_next < n && mbar_test_wait(&v_empty[v_next % kStages], ((v_next / kStages) & 1) ^ 1u)) {
           const int st = v_next % kStages;
           mbar_arrive_expect_tx(&v_full[st], kTileBytes);
-          window_load_tile(s_v + st * kTileBytes, &maps.v, &maps.v16, &maps.v_sinks, &maps.v16_sinks, &v_full[st], keys, v_next, 0, kv_head, b);
+          window_load_tile(s_v + st * kTileBytes, &maps.v, &maps.v16, &maps.v_sinks, &maps.v16_sinks, &v_full[st], keys, v_next, 0, kv_head, kv_row, b);
           ++v_next;
           progress = true;
         }
@@ -516,7 +602,15 @@ __global__ void __launch_bounds__(192, 2)
       // tile's phase.)
       if (const int last_rows = s_tiles->rows - 128 * j; last_rows < 128 && (last_rows & 15) != 0) {
         softmax_wait(&v_full[j % kStages], (j / kStages) & 1, 111, alive, abort_flag);
-        window_clear_values<1>(s_v + (j % kStages) * kTileBytes, last_rows, threadIdx.x - 64, 128);
+        window_clear_values<1>(s_v + (j % kStages) * kTileBytes, last_rows, 128, threadIdx.x - 64, 128);
+      }
+      if constexpr (kPacked) {
+        // No map of one sequence's sinks: what lies between the last one and the next multiple of 16 is cleared, too.
+        if (s_tiles->sink_rows > p.sinks && j == p.sinks >> 7) {
+          softmax_wait(&v_full[j % kStages], (j / kStages) & 1, 112, alive, abort_flag);
+          window_clear_values<1>(s_v + (j % kStages) * kTileBytes, p.sinks & 127, s_tiles->sink_rows - 128 * j, threadIdx.x - 64,
+                                 128);
+        }
       }
       tc_fence_before_sync();
       __syncwarp();
@@ -526,16 +620,20 @@ __global__ void __launch_bounds__(192, 2)
     softmax_wait(o_full, (s_tiles->count - 1) & 1, 110, alive, abort_flag);
     tc_fence_after_sync();
     const int token = s_tiles->i0 + (r >> p.group_shift);
-    const float inv = token < len && l_sum != 0.f ? 1.0f / l_sum : 0.f;
+    const bool some = kPacked ? l_sum != 0.f : token < len;  // a row that no key is left for gives zeros
+    const bool stored = kPacked ? (r >> p.group_shift) < s_tiles->valid : token < p.S;
+    const float inv = some && l_sum != 0.f ? 1.0f / l_sum : 0.f;
     const int head = head0 + (r & ((1 << p.group_shift) - 1));
-    uint4* dst = reinterpret_cast<uint4*>(p.ctx + (static_cast<int64_t>(b) * p.S + token) * p.ld_ctx + head * HD);
+    const int64_t out_row = kPacked ? static_cast<int64_t>(s_tiles->out_row) + (r >> p.group_shift)
+                                    : static_cast<int64_t>(b) * p.S + token;
+    uint4* dst = reinterpret_cast<uint4*>(p.ctx + out_row * p.ld_ctx + head * HD);
 #pragma unroll
     for (int cc = 0; cc < HD / 32; ++cc) {
       float o[32];
       tmem_load_32cols(t_o + 32 * cc, o);
-      if (token < p.S) {
+      if (stored) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) o[k] = token < len ? o[k] * inv : 0.f;
+        for (int k = 0; k < 32; ++k) o[k] = some ? o[k] * inv : 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           dst[4 * cc + k] = make_uint4(pack_bf16x2(o[8 * k], o[8 * k + 1]), pack_bf16x2(o[8 * k + 2], o[8 * k + 3]),
@@ -572,6 +670,7 @@ struct WindowWideCfg {
   static constexpr int kPolyPairs = 0x1;  // as in AttnWideCfg
 };
 
+template <bool kPacked>
 __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
     window_wide_kernel(const __grid_constant__ WindowMaps maps, const WindowParams p) {
   using Cfg = WindowWideCfg;
@@ -624,10 +723,20 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
   }
   pdl_wait_previous_grid();
   pdl_allow_next_grid();
-  const int len = p.kv_len != nullptr ? min(max(p.kv_len[b], 0), p.S) : p.S;
-  const KeyList keys = window_keys(p, tile, len);
-  if (keys.i0 >= len) {  // uniform for the CTA; no tensor memory allocated yet
-    window_zero_rows<HD>(p, b, head0, keys.i0);
+  PackedTile seq;
+  if constexpr (kPacked) {
+    if (blockIdx.x == 0 && blockIdx.y == 0) packed_check(p);
+    if (!packed_tile(p, tile, seq)) return;
+  }
+  const int len = kPacked ? seq.n_kv : p.kv_len != nullptr ? min(max(p.kv_len[b], 0), p.S) : p.S;
+  const KeyList keys = kPacked ? window_keys(p, seq.tile, len, len - seq.n_q) : window_keys(p, tile, len);
+  const int q_row = kPacked ? seq.q0 + seq.tile * (128 >> p.group_shift) : keys.i0;  // of the tile's first query
+  const int kv_row = kPacked ? seq.k0 : 0;
+  if (kPacked ? keys.i1 <= 0 : keys.i0 >= len) {  // uniform for the CTA; no tensor memory allocated yet
+    if constexpr (kPacked)
+      window_zero_packed_rows<HD>(p, q_row, seq.rows, head0);
+    else
+      window_zero_rows<HD>(p, b, head0, keys.i0);
     return;
   }
   const int n = keys.tiles;
@@ -646,8 +755,8 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
     if (lane == 0) {
       const int kv_head = head0 / (p.heads / p.kv_heads);
       mbar_arrive_expect_tx(q_full, Cfg::kTileBytes);
-      tma_load_4d(s_q, &maps.q, q_full, 0, head0, keys.i0, b);
-      tma_load_4d(s_q + Cfg::kBoxBytes, &maps.q, q_full, 64, head0, keys.i0, b);
+      tma_load_4d(s_q, &maps.q, q_full, 0, head0, q_row, b);
+      tma_load_4d(s_q + Cfg::kBoxBytes, &maps.q, q_full, 64, head0, q_row, b);
       int k_next = 0, v_next = 0;
       bool ok = true;
       PollTimeout poll;
@@ -658,8 +767,8 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
           const int st = k_next % Cfg::kStages;
           uint8_t* dst = s_k + st * Cfg::kTileBytes;
           mbar_arrive_expect_tx(&k_full[st], Cfg::kTileBytes);
-          window_load_tile(dst, &maps.k, &maps.k16, &maps.k, &maps.k16, &k_full[st], keys, k_next, 0, kv_head, b);
-          window_load_tile(dst + Cfg::kBoxBytes, &maps.k, &maps.k16, &maps.k, &maps.k16, &k_full[st], keys, k_next, 64, kv_head, b);
+          window_load_tile(dst, &maps.k, &maps.k16, &maps.k, &maps.k16, &k_full[st], keys, k_next, 0, kv_head, kv_row, b);
+          window_load_tile(dst + Cfg::kBoxBytes, &maps.k, &maps.k16, &maps.k, &maps.k16, &k_full[st], keys, k_next, 64, kv_head, kv_row, b);
           ++k_next;
           progress = true;
         }
@@ -667,8 +776,8 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
           const int st = v_next % Cfg::kVStages;
           uint8_t* dst = s_v + st * Cfg::kTileBytes;
           mbar_arrive_expect_tx(&v_full[st], Cfg::kTileBytes);
-          window_load_tile(dst, &maps.v, &maps.v16, &maps.v_sinks, &maps.v16_sinks, &v_full[st], keys, v_next, 0, kv_head, b);
-          window_load_tile(dst + Cfg::kBoxBytes, &maps.v, &maps.v16, &maps.v_sinks, &maps.v16_sinks, &v_full[st], keys, v_next, 64, kv_head, b);
+          window_load_tile(dst, &maps.v, &maps.v16, &maps.v_sinks, &maps.v16_sinks, &v_full[st], keys, v_next, 0, kv_head, kv_row, b);
+          window_load_tile(dst + Cfg::kBoxBytes, &maps.v, &maps.v16, &maps.v_sinks, &maps.v16_sinks, &v_full[st], keys, v_next, 64, kv_head, kv_row, b);
           ++v_next;
           progress = true;
         }
@@ -840,13 +949,17 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
         }
       }
       if constexpr (decltype(hide)::value) {
-        if (j == n - 1 && (last_rows & 15) != 0) {
+        const bool at_sinks = kPacked && keys.sink_rows > p.sinks && j == p.sinks >> 7;  // as in window_solo_kernel
+        const bool at_end = j == n - 1 && (last_rows & 15) != 0;
+        if (at_end || at_sinks) {
           const int st = j % Cfg::kVStages;
           // First O += P(j-2) V, the stage's last reader: its barrier is then in this tile's phase.
           const int jv = j - Cfg::kVStages;
           if (jv >= 0) softmax_wait(&o_done[jv % Cfg::kBufs], (jv / Cfg::kBufs) & 1, 132, alive, abort_flag);
           softmax_wait(&v_full[st], (j / Cfg::kVStages) & 1, 131, alive, abort_flag);
-          window_clear_values<2>(s_v + st * Cfg::kTileBytes, last_rows, threadIdx.x - 64, 256);
+          if (at_end) window_clear_values<2>(s_v + st * Cfg::kTileBytes, last_rows, 128, threadIdx.x - 64, 256);
+          if (at_sinks)
+            window_clear_values<2>(s_v + st * Cfg::kTileBytes, p.sinks & 127, keys.sink_rows - 128 * j, threadIdx.x - 64, 256);
         }
       }
       tc_fence_before_sync();
@@ -867,16 +980,19 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
     softmax_wait(&o_done[(n - 1) % Cfg::kBufs], ((n - 1) / Cfg::kBufs) & 1, 128, alive, abort_flag);
     tc_fence_after_sync();
     const float inv = l_row != 0.f ? 1.0f / l_row : 0.f;
+    // (The polynomial's weight of a hidden key is 2^-126 or so, not 0, so the sum does not tell.)
+    const bool some = kPacked ? m_ref != -INFINITY : token < len;
+    const bool stored = kPacked ? (r >> p.group_shift) < seq.rows : token < p.S;
     const int head = head0 + (r & ((1 << p.group_shift) - 1));
-    uint4* dst =
-        reinterpret_cast<uint4*>(p.ctx + (static_cast<int64_t>(b) * p.S + token) * p.ld_ctx + head * HD + 64 * half);
+    const int64_t out_row = kPacked ? static_cast<int64_t>(q_row) + (r >> p.group_shift) : static_cast<int64_t>(b) * p.S + token;
+    uint4* dst = reinterpret_cast<uint4*>(p.ctx + out_row * p.ld_ctx + head * HD + 64 * half);
 #pragma unroll
     for (int cc = 0; cc < 2; ++cc) {
       float o[32];
       tmem_load_32cols(t_o + 32 * cc, o);
-      if (token < p.S) {
+      if (stored) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) o[k] = token < len ? o[k] * inv : 0.f;
+        for (int k = 0; k < 32; ++k) o[k] = some ? o[k] * inv : 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           dst[4 * cc + k] = make_uint4(pack_bf16x2(o[8 * k], o[8 * k + 1]), pack_bf16x2(o[8 * k + 2], o[8 * k + 3]),
@@ -912,6 +1028,8 @@ static cudaError_t launch_window(Kernel kernel, int threads, int smem, std::once
   return launch_pdl(kernel, p.head_major ? dim3(rows, bh) : dim3(bh, rows), dim3(threads), smem, stream, maps, p);
 }
 
+// Packed: rows of all sequences, q_rows of queries and kv_rows of keys; else p.B sequences of p.S rows.
+template <bool kPacked>
 static cudaError_t launch_window_attention(const __nv_bfloat16* q, int64_t ld_q, const __nv_bfloat16* k, int64_t ld_k,
                                            const __nv_bfloat16* v, int64_t ld_v, int64_t hd, WindowParams p,
                                            cudaStream_t stream) {
@@ -919,38 +1037,42 @@ static cudaError_t launch_window_attention(const __nv_bfloat16* q, int64_t ld_q,
   p.group_shift = 0;
   while (p.group_shift < 4 && group % (2 << p.group_shift) == 0) ++p.group_shift;
   const uint32_t tokens = 128u >> p.group_shift;
-  p.tiles = static_cast<int>((p.S + tokens - 1) / tokens);
+  if (kPacked) p.B = 1;
+  p.tiles = kPacked ? static_cast<int>(p.q_rows / tokens) + p.batch : static_cast<int>((p.S + tokens - 1) / tokens);
   const int64_t bh = static_cast<int64_t>(p.B) * (p.heads >> p.group_shift);
-  p.head_major = (p.S >= 16384 && bh <= 65535) || p.tiles > 65535;
+  const bool long_ones = kPacked ? p.kv_rows / p.batch >= 16384 : p.S >= 16384;
+  p.head_major = (long_ones && bh <= 65535) || p.tiles > 65535;
   if (p.head_major && bh > 65535) return cudaErrorInvalidConfiguration;
   WindowMaps maps;
-  const uint64_t h = static_cast<uint64_t>(hd), S = static_cast<uint64_t>(p.S), B = static_cast<uint64_t>(p.B);
+  const uint64_t h = static_cast<uint64_t>(hd), B = static_cast<uint64_t>(p.B);
+  const uint64_t q_rows = static_cast<uint64_t>(kPacked ? p.q_rows : p.S), kv_rows = static_cast<uint64_t>(kPacked ? std::max(p.kv_rows, 1) : p.S);
   auto make = [&](CUtensorMap* m, const __nv_bfloat16* base, int64_t ld, int heads, uint32_t box_heads, uint32_t box_rows,
-                  uint64_t rows) {
+                  uint64_t rows, uint64_t stride) {
     const uint64_t row = static_cast<uint64_t>(ld) * 2;
     const uint64_t dims[4] = {h, static_cast<uint64_t>(heads), rows, B};
-    const uint64_t strides[3] = {h * 2, row, row * S};
+    const uint64_t strides[3] = {h * 2, row, row * stride};
     const uint32_t box[4] = {64, box_heads, box_rows, 1};
     return make_tmap_bf16_4d(m, base, dims, strides, box);
   };
-  const uint64_t sinks = p.sinks > 0 ? static_cast<uint64_t>(p.sinks) : 1;
-  cudaError_t e = make(&maps.q, q, ld_q, p.heads, 1u << p.group_shift, tokens, S);
-  if (e == cudaSuccess) e = make(&maps.k, k, ld_k, p.kv_heads, 1, 128, S);
-  if (e == cudaSuccess) e = make(&maps.v, v, ld_v, p.kv_heads, 1, 128, S);
-  if (e == cudaSuccess) e = make(&maps.k16, k, ld_k, p.kv_heads, 1, 16, S);
-  if (e == cudaSuccess) e = make(&maps.v16, v, ld_v, p.kv_heads, 1, 16, S);
-  if (e == cudaSuccess) e = make(&maps.v_sinks, v, ld_v, p.kv_heads, 1, 128, sinks);
-  if (e == cudaSuccess) e = make(&maps.v16_sinks, v, ld_v, p.kv_heads, 1, 16, sinks);
+  const uint64_t sinks = kPacked ? kv_rows : p.sinks > 0 ? static_cast<uint64_t>(p.sinks) : 1;
+  cudaError_t e = make(&maps.q, q, ld_q, p.heads, 1u << p.group_shift, tokens, q_rows, q_rows);
+  if (e == cudaSuccess) e = make(&maps.k, k, ld_k, p.kv_heads, 1, 128, kv_rows, kv_rows);
+  if (e == cudaSuccess) e = make(&maps.v, v, ld_v, p.kv_heads, 1, 128, kv_rows, kv_rows);
+  if (e == cudaSuccess) e = make(&maps.k16, k, ld_k, p.kv_heads, 1, 16, kv_rows, kv_rows);
+  if (e == cudaSuccess) e = make(&maps.v16, v, ld_v, p.kv_heads, 1, 16, kv_rows, kv_rows);
+  if (e == cudaSuccess) e = make(&maps.v_sinks, v, ld_v, p.kv_heads, 1, 128, sinks, kv_rows);
+  if (e == cudaSuccess) e = make(&maps.v16_sinks, v, ld_v, p.kv_heads, 1, 16, sinks, kv_rows);
   if (e != cudaSuccess) return e;
   static std::once_flag once32[64], once64[64], once128[64];
-  constexpr int kSoloSmem = 5 * 128 * 128 + 256 + 1024;
+  constexpr int kSoloSmem = 5 * 128 * 128 + 512 + 1024;  // tiles, barriers and lists of keys, room to align
   switch (hd) {
     case 32:
-      return launch_window(window_solo_kernel<32>, 192, kSoloSmem, once32, maps, p, stream);
+      return launch_window(window_solo_kernel<32, kPacked>, 192, kSoloSmem, once32, maps, p, stream);
     case 64:
-      return launch_window(window_solo_kernel<64>, 192, kSoloSmem, once64, maps, p, stream);
+      return launch_window(window_solo_kernel<64, kPacked>, 192, kSoloSmem, once64, maps, p, stream);
     case 128:
-      return launch_window(window_wide_kernel, WindowWideCfg::kThreads, WindowWideCfg::kSmemBytes, once128, maps, p, stream);
+      return launch_window(window_wide_kernel<kPacked>, WindowWideCfg::kThreads, WindowWideCfg::kSmemBytes, once128, maps, p,
+                           stream);
     default:
       return cudaErrorInvalidValue;
   }

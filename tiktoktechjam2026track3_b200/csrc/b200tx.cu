@@ -30,6 +30,7 @@
 #include "rotary.cuh"
 #include "cache_append.cuh"
 #include "cache_attention.cuh"
+#include "cache_int4.cuh"
 #include "attention_window.cuh"
 
 #define B2_API extern "C" __attribute__((visibility("default")))
@@ -494,12 +495,17 @@ B2_API int b2_rotary_fwd(const b2_rotary_args* args, void* stream) {
 }
 
 // The pages of a cache as the kernels take them, or a status.
-static int cache_pages(const b2_kv_cache* c, const char* what, CachePages* out, bool* fp8) {
+static int cache_pages(const b2_kv_cache* c, const char* what, CachePages* out, int* type) {
   if (c == nullptr || c->k == nullptr || c->v == nullptr) return fail(1, "%s: null pointer argument", what);
-  if (c->dtype != B2_CACHE_E4M3 && c->dtype != B2_CACHE_BF16) return fail(1, "%s: unknown cache dtype %d", what, c->dtype);
-  *fp8 = c->dtype == B2_CACHE_E4M3;
-  if (*fp8 && (c->k_scale == nullptr || c->v_scale == nullptr))
+  static_assert(B2_CACHE_BF16 == kCacheBf16 && B2_CACHE_E4M3 == kCacheE4m3 && B2_CACHE_INT4 == kCacheInt4, "one numbering");
+  if (c->dtype != B2_CACHE_E4M3 && c->dtype != B2_CACHE_BF16 && c->dtype != B2_CACHE_INT4)
+    return fail(1, "%s: unknown cache dtype %d", what, c->dtype);
+  const bool int4 = c->dtype == B2_CACHE_INT4;
+  *type = c->dtype;
+  if (c->dtype == B2_CACHE_E4M3 && (c->k_scale == nullptr || c->v_scale == nullptr))
     return fail(1, "%s: an e4m3 cache needs k_scale and v_scale", what);
+  if (int4 && (c->k_group == nullptr || c->v_group == nullptr))
+    return fail(1, "%s: a 4-bit cache needs k_group and v_group", what);
   if (c->pages <= 0 || c->kv_heads <= 0) return fail(1, "%s: invalid cache shape", what);
   int shift = 0;
   while (shift < 8 && (int64_t{1} << shift) < c->page_size) ++shift;
@@ -507,6 +513,8 @@ static int cache_pages(const b2_kv_cache* c, const char* what, CachePages* out, 
     return fail(2, "%s: page_size=%lld must be 16, 32, 64, 128 or 256", what, (long long)c->page_size);
   if (c->head_dim % 16 != 0 || c->head_dim < 16 || c->head_dim > 256)
     return fail(2, "%s: head_dim=%lld must be a multiple of 16 up to 256", what, (long long)c->head_dim);
+  if (int4 && c->head_dim % 32 != 0)
+    return fail(2, "%s: head_dim=%lld of a 4-bit cache must be a multiple of 32", what, (long long)c->head_dim);
   if (c->kv_heads > 16384 || c->pages > 0x7fffffffLL || c->page_stride > (0x7fffffffLL >> 1))
     return fail(2, "%s: cache too large", what);
   const int64_t head = c->page_size * c->head_dim;
@@ -514,10 +522,14 @@ static int cache_pages(const b2_kv_cache* c, const char* what, CachePages* out, 
     return fail(1, "%s: page_stride or head_stride too small", what);
   if (c->head_stride % 16 != 0 || c->page_stride % 16 != 0 || !aligned16(c->k) || !aligned16(c->v))
     return fail(2, "%s: cache pointers must be 16-byte aligned, strides multiples of 16 elements", what);
+  if (int4 && (c->head_stride % 32 != 0 || c->page_stride % 32 != 0 || !aligned16(c->k_group) || !aligned16(c->v_group)))
+    return fail(2, "%s: strides of a 4-bit cache must be multiples of 32 elements, k_group and v_group 16-byte aligned", what);
   out->k = static_cast<uint8_t*>(c->k);
   out->v = static_cast<uint8_t*>(c->v);
   out->k_scale = c->k_scale;
   out->v_scale = c->v_scale;
+  out->k_group = int4 ? static_cast<uint16_t*>(c->k_group) : nullptr;  // (a cache of another type may be an older, shorter struct)
+  out->v_group = int4 ? static_cast<uint16_t*>(c->v_group) : nullptr;
   out->pages = c->pages;
   out->page_stride = c->page_stride;
   out->head_stride = c->head_stride;
@@ -532,8 +544,8 @@ B2_API int b2_cache_append_fwd(const b2_cache_append_args* args, void* stream) {
   const auto [cache, qkv, ld_qkv, q_col, k_col, v_col, tokens, num_heads, batch, new_start, new_len, past_len, page_table,
               table_pages, max_new, table, max_positions, rotary_dim, interleaved, q_out, ld_q_out, k_out, ld_k_out] = *args;
   AppendParams p{};
-  bool fp8 = false;
-  if (const int rc = cache_pages(cache, "b2_cache_append_fwd", &p.c, &fp8)) return rc;
+  int type = 0;
+  if (const int rc = cache_pages(cache, "b2_cache_append_fwd", &p.c, &type)) return rc;
   const int64_t hd = cache->head_dim, hk = cache->kv_heads;
   if (tokens < 0 || batch < 0 || max_new < 0 || num_heads <= 0 || table_pages <= 0)
     return fail(1, "b2_cache_append_fwd: invalid shape");
@@ -583,8 +595,51 @@ B2_API int b2_cache_append_fwd(const b2_cache_append_args* args, void* stream) {
   p.k_out = static_cast<__nv_bfloat16*>(k_out);
   p.ld_q_out = ld_q_out;
   p.ld_k_out = ld_k_out;
-  return check_launch(launch_cache_append(p, max_new, fp8, interleaved != 0, static_cast<cudaStream_t>(stream)),
+  if (type == kCacheInt4) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    return check_launch(launch_cache_append_int4(p, max_new, interleaved != 0, device_sm_count(dev), static_cast<cudaStream_t>(stream)),
+                        "b2_cache_append_fwd");
+  }
+  return check_launch(launch_cache_append(p, max_new, type == kCacheE4m3, interleaved != 0, static_cast<cudaStream_t>(stream)),
                       "b2_cache_append_fwd");
+}
+
+B2_API int b2_cache_read_fwd(const b2_cache_read_args* args, void* stream) {
+  if (args == nullptr) return fail(1, "b2_cache_read_fwd: null pointer argument");
+  const auto [cache, out_start, length, start, batch, page_table, table_pages, max_len, rows, k_out, ld_k_out, v_out,
+              ld_v_out] = *args;
+  ReadParams p{};
+  int type = 0;
+  if (const int rc = cache_pages(cache, "b2_cache_read_fwd", &p.c, &type)) return rc;
+  const int64_t width = cache->head_dim * cache->kv_heads;
+  if (batch < 0 || rows < 0 || max_len < 0 || table_pages <= 0) return fail(1, "b2_cache_read_fwd: invalid shape");
+  if (batch > 65535 || rows > 0x7fffffffLL || max_len > 0x7fffffffLL || table_pages > (0x7fffffffLL >> p.c.page_shift))
+    return fail(2, "b2_cache_read_fwd: problem too large");
+  if (k_out == nullptr && v_out == nullptr && rows > 0) return fail(1, "b2_cache_read_fwd: k_out and v_out are both null");
+  if ((k_out != nullptr && (ld_k_out < width || ld_k_out % 8 != 0)) || (v_out != nullptr && (ld_v_out < width || ld_v_out % 8 != 0)))
+    return fail(2, "b2_cache_read_fwd: row strides must be multiples of 8 and at least kv_heads * head_dim");
+  if (batch == 0 || rows == 0 || max_len == 0) return 0;
+  if (out_start == nullptr || length == nullptr || start == nullptr || page_table == nullptr)
+    return fail(1, "b2_cache_read_fwd: null pointer argument");
+  if (!aligned16(k_out) || !aligned16(v_out)) return fail(2, "b2_cache_read_fwd: pointers must be 16-byte aligned");
+  if (!is_sm100(nullptr)) return fail(2, "b2_cache_read_fwd: needs an sm_100 (B200) device");
+  p.batch = static_cast<int>(batch);
+  p.rows = rows;
+  p.max_len = max_len;
+  p.out_start = out_start;
+  p.length = length;
+  p.start = start;
+  p.page_table = page_table;
+  p.ld_table = table_pages;
+  p.table_pages = static_cast<int>(table_pages);
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.v_out = static_cast<__nv_bfloat16*>(v_out);
+  p.ld_k_out = ld_k_out;
+  p.ld_v_out = ld_v_out;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return check_launch(launch_cache_read(p, type, device_sm_count(dev), static_cast<cudaStream_t>(stream)), "b2_cache_read_fwd");
 }
 
 B2_API int b2_cache_attention_workspace(int64_t batch, int64_t q_len, int64_t num_heads, int64_t kv_heads,
@@ -612,8 +667,8 @@ B2_API int b2_cache_attention_fwd(const b2_cache_attention_args* args, void* str
               workspace, workspace_bytes] = *args;
   const float scale = static_cast<float>(scale64);
   CacheAttnParams p{};
-  bool fp8 = false;
-  if (const int rc = cache_pages(cache, "b2_cache_attention_fwd", &p.c, &fp8)) return rc;
+  int type = 0;
+  if (const int rc = cache_pages(cache, "b2_cache_attention_fwd", &p.c, &type)) return rc;
   const int64_t hd = cache->head_dim, hk = cache->kv_heads;
   if (hd != 32 && hd != 64 && hd != 128)
     return fail(2, "b2_cache_attention_fwd: head_dim=%lld not supported (32, 64, 128)", (long long)hd);
@@ -658,7 +713,7 @@ B2_API int b2_cache_attention_fwd(const b2_cache_attention_args* args, void* str
   p.window = static_cast<int>(window < (int64_t{1} << 30) ? window : 0);  // beyond every position: none
   p.sinks = static_cast<int>(sinks < (int64_t{1} << 30) ? sinks : (int64_t{1} << 30));
   p.scale_log2 = scale * 1.4426950408889634f;
-  return check_launch(launch_cache_attention(p, workspace, fp8, sms, static_cast<cudaStream_t>(stream)),
+  return check_launch(launch_cache_attention(p, workspace, type, sms, static_cast<cudaStream_t>(stream)),
                       "b2_cache_attention_fwd");
 }
 
@@ -704,9 +759,61 @@ B2_API int b2_window_attention_fwd(const b2_window_attention_args* args, void* s
   p.window = window < seq_len ? static_cast<int>(window) : 0;  // a window of the whole sequence hides nothing
   p.sinks = p.window > 0 ? static_cast<int>(sinks < seq_len ? sinks : seq_len) : 0;
   p.scale_log2 = scale * 1.4426950408889634f;
-  return check_launch(launch_window_attention(static_cast<const __nv_bfloat16*>(q), ld_q,
-                                              static_cast<const __nv_bfloat16*>(k), ld_k,
-                                              static_cast<const __nv_bfloat16*>(v), ld_v, head_dim, p,
-                                              static_cast<cudaStream_t>(stream)),
+  return check_launch(launch_window_attention<false>(static_cast<const __nv_bfloat16*>(q), ld_q,
+                                                     static_cast<const __nv_bfloat16*>(k), ld_k,
+                                                     static_cast<const __nv_bfloat16*>(v), ld_v, head_dim, p,
+                                                     static_cast<cudaStream_t>(stream)),
                       "b2_window_attention_fwd");
+}
+
+B2_API int b2_packed_attention_fwd(const b2_packed_attention_args* args, void* stream) {
+  if (args == nullptr) return fail(1, "b2_packed_attention_fwd: null pointer argument");
+  const auto [q, ld_q, q_rows, k, ld_k, v, ld_v, kv_rows, q_start, kv_start, batch, num_heads, kv_heads, head_dim, window,
+              sinks, scale64, out, ld_out] = *args;
+  const float scale = static_cast<float>(scale64);
+  if (batch < 0 || q_rows < 0 || kv_rows < 0 || num_heads <= 0 || kv_heads <= 0)
+    return fail(1, "b2_packed_attention_fwd: invalid shape");
+  if (num_heads > 65535) return fail(2, "b2_packed_attention_fwd: problem too large");
+  if (num_heads % kv_heads != 0)
+    return fail(1, "b2_packed_attention_fwd: num_heads=%lld must be a multiple of kv_heads=%lld", (long long)num_heads,
+                (long long)kv_heads);
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128)
+    return fail(2, "b2_packed_attention_fwd: head_dim=%lld not supported (32, 64, 128)", (long long)head_dim);
+  if (window < 0 || sinks < 0 || (window == 0 && sinks != 0))
+    return fail(1, "b2_packed_attention_fwd: window and sinks must not be negative, and sinks need a window");
+  if (!(scale > 0.f) || std::isinf(scale)) return fail(1, "b2_packed_attention_fwd: scale must be positive and finite");
+  const int64_t kv_width = kv_heads * head_dim;
+  if (ld_q < num_heads * head_dim || ld_out < num_heads * head_dim || ld_k < kv_width || ld_v < kv_width)
+    return fail(1, "b2_packed_attention_fwd: row strides must be at least heads * head_dim");
+  if (ld_q % 8 != 0 || ld_k % 8 != 0 || ld_v % 8 != 0 || ld_out % 8 != 0)
+    return fail(2, "b2_packed_attention_fwd: row strides must be multiples of 8");
+  // List places (sinks + window + tokens) stay below 2^31; the tensor maps' strides below 2^40 bytes.
+  const int64_t most = q_rows > kv_rows ? q_rows : kv_rows;
+  if (most > (int64_t{1} << 28) || batch > (int64_t{1} << 20) || (most > 0 && (ld_q | ld_k | ld_v) > ((int64_t{1} << 38) / most)))
+    return fail(2, "b2_packed_attention_fwd: problem too large");
+  if (batch == 0 || q_rows == 0) return 0;
+  if (q == nullptr || (kv_rows > 0 && (k == nullptr || v == nullptr)) || q_start == nullptr || kv_start == nullptr || out == nullptr)
+    return fail(1, "b2_packed_attention_fwd: null pointer argument");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+    return fail(2, "b2_packed_attention_fwd: pointers must be 16-byte aligned");
+  if (!is_sm100(nullptr)) return fail(2, "b2_packed_attention_fwd: needs an sm_100 (B200) device");
+  WindowParams p{};
+  p.ctx = static_cast<__nv_bfloat16*>(out);
+  p.ld_ctx = ld_out;
+  p.heads = static_cast<int>(num_heads);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.window = window < kv_rows ? static_cast<int>(window) : 0;  // a window of all keys hides nothing
+  p.sinks = p.window > 0 ? static_cast<int>(sinks < kv_rows ? sinks : kv_rows) : 0;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.q_start = q_start;
+  p.kv_start = kv_start;
+  p.batch = static_cast<int>(batch);
+  p.q_rows = static_cast<int>(q_rows);
+  p.kv_rows = static_cast<int>(kv_rows);
+  const bool keys = kv_rows > 0;  // without any, the queries' memory stands in for theirs: no row of it is read
+  return check_launch(launch_window_attention<true>(static_cast<const __nv_bfloat16*>(q), ld_q,
+                                                    static_cast<const __nv_bfloat16*>(keys ? k : q), keys ? ld_k : ld_q,
+                                                    static_cast<const __nv_bfloat16*>(keys ? v : q), keys ? ld_v : ld_q, head_dim,
+                                                    p, static_cast<cudaStream_t>(stream)),
+                      "b2_packed_attention_fwd");
 }

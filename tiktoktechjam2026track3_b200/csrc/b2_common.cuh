@@ -29,6 +29,8 @@ enum : uint32_t {
   kKernelRotary = 5,
   kKernelCacheAppend = 6,
   kKernelCacheAttention = 7,
+  kKernelCacheRead = 8,
+  kKernelPackedAttention = 9,
 };
 enum : uint32_t {
   kReasonTimeout = 1,

@@ -33,11 +33,18 @@ constexpr int kScaleExpMin = -40;
 constexpr int kScaleExpMax = 40;
 constexpr float kE4m3Max = 448.f;
 
+// Element types of a cache's pages (include/b200tx.h).
+constexpr int kCacheBf16 = 0;
+constexpr int kCacheE4m3 = 1;
+constexpr int kCacheInt4 = 2;  // cache_int4.cuh
+
 struct CachePages {
   uint8_t* k;
   uint8_t* v;
   float* k_scale;  // [pages][kv_heads]
   float* v_scale;
+  uint16_t* k_group;  // [pages][kv_heads][page_size][2][head_dim / 32], of 4-bit codes
+  uint16_t* v_group;
   int64_t pages, page_stride, head_stride;  // strides in elements
   int kv_heads, head_dim, page_shift;
 };
@@ -111,6 +118,50 @@ __device__ __forceinline__ uint32_t e4m3x4_scale(uint32_t w, float f) {
   return out;
 }
 
+// Whether a sequence's new tokens lie outside the rows, the pages or the table of positions.
+__device__ __forceinline__ bool append_bad_index(const AppendParams& p, int past, int count, int first) {
+  return past < 0 || first < 0 || count > p.max_new || static_cast<int64_t>(first) + count > p.tokens ||
+         static_cast<int64_t>(past) + count > (static_cast<int64_t>(p.table_pages) << p.c.page_shift) ||
+         (p.rotary_dim > 0 && static_cast<int64_t>(past) + count > p.max_positions);
+}
+
+// Rotated queries of one key head: `tokens` rows from row0 on, at positions pos0 ...; thread tt of `threads`.
+template <bool kInterleaved>
+__device__ __forceinline__ void append_queries(const AppendParams& p, int key_head, int64_t row0, int pos0, unsigned tokens,
+                                               unsigned tt, unsigned threads) {
+  const int hd = p.c.head_dim;
+  const unsigned chunks = static_cast<unsigned>(hd) >> 4;
+  const unsigned items = tokens * chunks;
+  const int ld = static_cast<int>(p.ld);
+  const int h0 = key_head * p.group;
+  const __nv_bfloat16* rows = p.qkv + row0 * p.ld + p.q_col + h0 * hd;
+  __nv_bfloat16* out = p.q_out + row0 * p.ld_q_out + h0 * hd;
+  for (unsigned i = tt; i < items; i += threads) {
+    const unsigned token = i / chunks;
+    const RotaryChunk ch = rotary_chunk<kInterleaved>(i - token * chunks, p.rotary_dim);
+    float c[8], s[8];
+    if (ch.pair0 >= 0)
+      rotary_load_table(p.table + static_cast<int64_t>(pos0 + static_cast<int>(token)) * (p.rotary_dim >> 1) + ch.pair0, c, s);
+    const __nv_bfloat16* x = rows + token * static_cast<int64_t>(ld);
+    __nv_bfloat16* y = out + token * p.ld_q_out;
+#pragma unroll 2
+    for (int g = 0; g < p.group; ++g, x += hd, y += hd) {
+      uint4 ua = *reinterpret_cast<const uint4*>(x + ch.off0);
+      uint4 ub = *reinterpret_cast<const uint4*>(x + ch.off1);
+      if (ch.pair0 >= 0) {
+        float a[8], bb[8];
+        unpack_bf16x8(ua, a);
+        unpack_bf16x8(ub, bb);
+        rotary_apply<kInterleaved>(a, bb, c, s);
+        ua = pack_bf16x8(a);
+        ub = pack_bf16x8(bb);
+      }
+      *reinterpret_cast<uint4*>(y + ch.off0) = ua;
+      *reinterpret_cast<uint4*>(y + ch.off1) = ub;
+    }
+  }
+}
+
 constexpr int kAppendMaxThreads = 512;
 constexpr int kAppendItems = 2;  // chunks that a thread holds
 
@@ -134,9 +185,7 @@ __global__ void __launch_bounds__(kAppendMaxThreads, 2)
   if (count <= 0) return;
   const int shift = p.c.page_shift;
   // Every index comes from device memory: one that does not fit is recorded and nothing is written.
-  if (past < 0 || first < 0 || count > p.max_new || static_cast<int64_t>(first) + count > p.tokens ||
-      static_cast<int64_t>(past) + count > (static_cast<int64_t>(p.table_pages) << shift) ||
-      (p.rotary_dim > 0 && static_cast<int64_t>(past) + count > p.max_positions)) {
+  if (append_bad_index(p, past, count, first)) {
     record_status(kKernelCacheAppend, 1, kReasonBadIndex);
     return;
   }
@@ -158,33 +207,7 @@ __global__ void __launch_bounds__(kAppendMaxThreads, 2)
   };
 
   if (role >= 2 * kv_heads) {
-    // The query heads of one key head.
-    const int h0 = (role - 2 * kv_heads) * p.group;
-    const __nv_bfloat16* rows = p.qkv + row0 * p.ld + p.q_col + h0 * hd;
-    __nv_bfloat16* out = p.q_out + row0 * p.ld_q_out + h0 * hd;
-    for (unsigned i = tt; i < items; i += team_threads) {
-      const unsigned token = i / chunks;
-      const RotaryChunk ch = rotary_chunk<kInterleaved>(i - token * chunks, rotary_dim);
-      float c[8], s[8];
-      if (ch.pair0 >= 0) angles_of(token, ch.pair0, c, s);
-      const __nv_bfloat16* x = rows + token * static_cast<int64_t>(ld);
-      __nv_bfloat16* y = out + token * p.ld_q_out;
-#pragma unroll 2
-      for (int g = 0; g < p.group; ++g, x += hd, y += hd) {
-        uint4 ua = *reinterpret_cast<const uint4*>(x + ch.off0);
-        uint4 ub = *reinterpret_cast<const uint4*>(x + ch.off1);
-        if (ch.pair0 >= 0) {
-          float a[8], bb[8];
-          unpack_bf16x8(ua, a);
-          unpack_bf16x8(ub, bb);
-          rotary_apply<kInterleaved>(a, bb, c, s);
-          ua = pack_bf16x8(a);
-          ub = pack_bf16x8(bb);
-        }
-        *reinterpret_cast<uint4*>(y + ch.off0) = ua;
-        *reinterpret_cast<uint4*>(y + ch.off1) = ub;
-      }
-    }
+    append_queries<kInterleaved>(p, role - 2 * kv_heads, row0, t0, static_cast<unsigned>(t1 - t0), tt, team_threads);
     return;
   }
 

@@ -146,6 +146,15 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
   return h;
 }
 
+__device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t bf16x2_less_136(uint32_t a) {
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), __float2bfloat162_rn(136.f));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -169,6 +178,12 @@ __device__ __forceinline__ uint2 load_once2(const void* p) {
 __device__ __forceinline__ uint32_t load_once(const void* p) {
   uint32_t u;
   asm("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(u) : "l"(p));
+  return u;
+}
+
+__device__ __forceinline__ uint16_t load_once_u16(const void* p) {
+  uint16_t u;
+  asm("ld.global.L1::no_allocate.u16 %0, [%1];" : "=h"(u) : "l"(p));
   return u;
 }
 
@@ -220,23 +235,26 @@ __device__ __forceinline__ float2 cluster_load2(uint32_t at) {
   return v;
 }
 
-template <int HD, bool kFp8, int NT, int kShare>
+template <int HD, int kType, int NT, int kShare>
 struct CacheAttnCfg {
   static constexpr int kRows = 8 * NT;
-  static constexpr int kBytes = kFp8 ? 1 : 2;
-  static constexpr int kKWords = HD * kBytes / 16;  // of one token, per thread: 4 threads share a row of K,
-  static constexpr int kVWords = HD * kBytes / 32;  // 8 a row of V
+  static constexpr int kBits = kType == kCacheBf16 ? 16 : kType == kCacheE4m3 ? 8 : 4;
+  static constexpr int kRowBytes = HD * kBits / 8;  // of a token and head
+  static constexpr int kKWords = kRowBytes / 16;  // of one token, per thread: 4 threads share a row of K,
+  static constexpr int kVWords = kRowBytes < 32 ? 1 : kRowBytes / 32;  // 8 a row of V (32 dims in 4 bits: half a word)
+  static constexpr int kGroups = HD / 32;  // of 4-bit codes
   static constexpr int kSteps = HD / 16;
   // A warp takes kSub tiles of 16 tokens at a time, interleaved: 4 KB of keys and values on their way per warp.
-  static constexpr int kSub = 128 / (HD * kBytes * NT) > 1 ? 128 / (HD * kBytes * NT) : 1;
+  static constexpr int kFill = 128 / (kRowBytes * NT);
+  static constexpr int kSub = kFill > 4 ? 4 : kFill > 1 ? kFill : 1;
   // Registers decide the warps: the loads' (32, or 64 for 256-byte rows), O's and Q's (6 per row block and 16 dims). 16
   // warps an SM at 128 registers, 12 at 168, 8 at 255; in CTAs of 4, so that one that joins does not idle many (64
   // sequences of up to 8192 tokens: 116 us, 122 in CTAs of 8), or of 6 where 12 is the number.
-  static constexpr bool kWide = HD == 128 && (!kFp8 || NT == 2);
-  static constexpr bool kSharedQ = NT == 2 || (HD == 128 && kFp8);
+  static constexpr bool kWide = HD == 128 && (kType == kCacheBf16 || NT == 2);
+  static constexpr bool kSharedQ = NT == 2 || (HD == 128 && kType != kCacheBf16);
   // kShare 1 or 4: a CTA takes a whole (sequence, head) with all the warps of an SM, or a quarter; kCacheCluster: a
   // cluster does, each CTA with those of an SM; 0: a stretch of the line.
-  static constexpr int kWarpsPerSm = !kWide ? 16 : kFp8 || NT == 1 ? 12 : 8;
+  static constexpr int kWarpsPerSm = !kWide ? 16 : kType != kCacheBf16 || NT == 1 ? 12 : 8;
   static constexpr int kWarps = kShare > 0 ? kWarpsPerSm / (kShare == 4 ? 4 : 1) : kWarpsPerSm == 12 ? 6 : 4;
   static constexpr int kCtasPerSm = kWarpsPerSm / kWarps;
   static constexpr int kThreads = 32 * kWarps;
@@ -244,8 +262,11 @@ struct CacheAttnCfg {
   static constexpr int kLeast = 16 / kWarps;
   static constexpr int kUnitTiles = kWarps * kSub;  // of 16 tokens: what a CTA takes at a time
   // Twelve warps with 8 KB on their way each need no prefetch (183 us with it, 168 without: 32 x 8192 tokens, 8 heads).
-  static constexpr bool kPrefetch = !(kWide && !kFp8 && NT == 1);
-  static constexpr int kLines = kSub * 2 * 16 * HD * kBytes / 128;  // 128-byte lines of a warp's part of a unit
+  static constexpr bool kPrefetch = !(kWide && kType == kCacheBf16 && NT == 1);
+  // 128-byte lines of a warp's part of a unit: keys (their codes, then their groups' parameters) and values alike.
+  static constexpr int kCodeLines = 16 * kRowBytes / 128;
+  static constexpr int kGroupLines = kType != kCacheInt4 ? 0 : kGroups > 1 ? kGroups / 2 : 1;
+  static constexpr int kLines = kSub * 2 * (kCodeLines + kGroupLines);
   static constexpr int kPartial = kRows * (HD + 2);  // floats of one partial result: outputs, then maxima, then sums
   // Shared memory: the join of the warps' results, or the factors of the join of CTAs; then (batch + 1) first units.
   static constexpr int kSmemBytes = kWarps * kPartial * 4 > 24576 ? kWarps * kPartial * 4 : 24576;
@@ -264,11 +285,14 @@ __device__ __forceinline__ int seq_units(const CacheAttnParams& p, int b) {
 
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
-template <int HD, bool kFp8, int NT, int kShare>
-__global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
-                                  CacheAttnCfg<HD, kFp8, NT, kShare>::kCtasPerSm)
+template <int HD, int kType, int NT, int kShare>
+__global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
+                                  CacheAttnCfg<HD, kType, NT, kShare>::kCtasPerSm)
     cache_attention_kernel(const CacheAttnParams p) {
-  using Cfg = CacheAttnCfg<HD, kFp8, NT, kShare>;
+  using Cfg = CacheAttnCfg<HD, kType, NT, kShare>;
+  constexpr bool kFp8 = kType == kCacheE4m3;
+  constexpr bool kInt4 = kType == kCacheInt4;
+  constexpr int G = Cfg::kGroups;
   constexpr bool kWhole = kShare > 0;
   constexpr bool kCluster = kShare == kCacheCluster;
   using KPieces = RowPieces<Cfg::kKWords, 4>;
@@ -280,6 +304,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
   float* s_merge = reinterpret_cast<float*>(s_dyn);
   int* s_first = reinterpret_cast<int*>(s_dyn + Cfg::kSmemBytes);  // [batch + 1] first unit of each sequence
   __shared__ uint2 s_q[Cfg::kSharedQ ? NT * Cfg::kSteps * 32 : 1];
+  __shared__ float2 s_qsum[kInt4 && Cfg::kSharedQ ? NT * G * 4 : 1];
   __shared__ int s_scan[kWarps];
   __shared__ Part s_part;  // what the join needs of `now`, out of the registers of the loop
   __shared__ int s_last;
@@ -336,7 +361,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
   constexpr int kNoTile = 1 << 30;         // a first token that no row sees
   constexpr int kIds = 32 / kSub;          // units whose page numbers the lanes hold
   constexpr int kAhead = kIds > 4 ? 3 : 2;  // units that the prefetch into L2 runs ahead
-  const int page_bytes = static_cast<int>(p.c.page_stride) * Cfg::kBytes;  // below 2^31 (checked by the host)
+  const int page_bytes = static_cast<int>(p.c.page_stride * Cfg::kBits / 8);  // below 2^31 (checked by the host)
   const int slot_mask = (1 << p.c.page_shift) - 1;
 
   auto part_from = [&](int w, int b) {
@@ -368,6 +393,10 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
       }
     }
   };
+  // Byte offset of the first parameter of token `tok` (of its sequence), in 4 bits.
+  auto group_row = [&](int page, int h, int tok) {
+    return (((static_cast<int64_t>(page) * kv_heads + h) << p.c.page_shift) + (tok & slot_mask)) * (4 * G);
+  };
   // The lines of the warp's part of unit u into L2, a lane each.
   auto prefetch = [&](const Part& x, int u) {
     constexpr int kTileLines = Cfg::kLines / kSub;  // K's, then V's
@@ -379,9 +408,15 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
       const int page = __shfl_sync(0xffffffffu, my_page, src);
       const int in = line % kTileLines;
       const bool keys = in < kTileLines / 2;
-      if (u < x.u1 && (Cfg::kLines % 32 == 0 || line < Cfg::kLines) && tok != kNoTile)
-        prefetch_l2((keys ? p.c.k : p.c.v) + static_cast<int64_t>(page) * page_bytes + x.h * p.c.head_stride * Cfg::kBytes +
-                    (tok & slot_mask) * (HD * Cfg::kBytes) + (keys ? in : in - kTileLines / 2) * 128);
+      const int at = keys ? in : in - kTileLines / 2;
+      if (u < x.u1 && (Cfg::kLines % 32 == 0 || line < Cfg::kLines) && tok != kNoTile) {
+        if (!kInt4 || at < Cfg::kCodeLines)
+          prefetch_l2((keys ? p.c.k : p.c.v) + static_cast<int64_t>(page) * page_bytes + x.h * p.c.head_stride * Cfg::kBits / 8 +
+                      (tok & slot_mask) * Cfg::kRowBytes + at * 128);
+        else
+          prefetch_l2(reinterpret_cast<const uint8_t*>(keys ? p.c.k_group : p.c.v_group) + group_row(page, x.h, tok) +
+                      (at - Cfg::kCodeLines) * 128);
+      }
     }
   };
   Part now;
@@ -409,11 +444,13 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
     read_ids(now, now.u0);
     if (tid == 0) s_part = now;
     const SeqTiles seq = now.seq;
-    const int64_t head_bytes = now.h * p.c.head_stride * Cfg::kBytes;
+    const int64_t head_bytes = now.h * p.c.head_stride * Cfg::kBits / 8;
 
     // Q: fragments of the 8-row operand(s), and the factor of its rows' scores.
     uint32_t qf[NT][Cfg::kSteps][2];  // (in shared memory where registers are short: it is alike for every warp)
     float row_scale[NT][2];
+    uint32_t qm[NT][2];    // 4 bits: the operand that the middles meet
+    float qsum[NT][G][2];  // 4 bits: -136 times the sum of Q over each group
     int limit[NT][2];  // position of the rows 2t, 2t + 1 of each operand, -1: no such row
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -448,6 +485,47 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
         const float down = exp2_int(e - 14) * p.scale_log2;
         row_scale[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);      // the thread that holds row 2t
         row_scale[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);  // row 2t + 1
+      } else if constexpr (kInt4) {
+        uint32_t part[3][G];  // the groups' sums as three bf16 terms each, 24 bits together
+#pragma unroll
+        for (int y = 0; y < G; ++y) {
+          const uint4 u = real ? *reinterpret_cast<const uint4*>(src + 32 * y + 8 * t) : make_uint4(0, 0, 0, 0);
+          // Elements i and i + 4 side by side, as the codes' halves hold them.
+          qf[nt][2 * y][0] = __byte_perm(u.x, u.z, 0x5410u);
+          qf[nt][2 * y][1] = __byte_perm(u.x, u.z, 0x7632u);
+          qf[nt][2 * y + 1][0] = __byte_perm(u.y, u.w, 0x5410u);
+          qf[nt][2 * y + 1][1] = __byte_perm(u.y, u.w, 0x7632u);
+          float f[8];
+          unpack_bf16x8(u, f);
+          float sum = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          qsum[nt][y][0] = -136.f * __shfl_sync(0xffffffffu, sum, 8 * t);  // the threads that hold rows 2t and 2t + 1
+          qsum[nt][y][1] = -136.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            const float term = bf16_round(sum);
+            part[i][y] = __float_as_uint(term) >> 16;
+            sum -= term;
+          }
+        }
+        // Which words of a token's parameters the threads of a row give to the product with the middles: see s below.
+        if constexpr (G == 4) {
+          const bool high = (t & 1) != 0;
+          uint32_t two[3];
+#pragma unroll
+          for (int i = 0; i < 3; ++i)
+            two[i] = (high ? part[i][G > 2 ? 2 : 0] : part[i][0]) | (high ? part[i][G > 3 ? 3 : 0] : part[i][G > 1 ? 1 : 0]) << 16;
+          qm[nt][0] = t < 2 ? two[0] : two[1];
+          qm[nt][1] = t < 2 ? two[2] : 0u;
+        } else {
+          uint32_t two[3];
+#pragma unroll
+          for (int i = 0; i < 3; ++i) two[i] = G == 2 ? part[i][0] | part[i][G - 1] << 16 : part[i][0] << 16;
+          qm[nt][0] = t == 0 ? two[0] : t == 1 ? two[1] : t == 2 ? two[2] : 0u;
+          qm[nt][1] = 0u;
+        }
+        row_scale[nt][0] = row_scale[nt][1] = p.scale_log2;
       } else {
 #pragma unroll
         for (int s = 0; s < Cfg::kSteps; ++s) {
@@ -470,14 +548,24 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
 #pragma unroll
           for (int st = 0; st < Cfg::kSteps; ++st)
             s_q[(nt * Cfg::kSteps + st) * 32 + lane] = make_uint2(qf[nt][st][0], qf[nt][st][1]);
+        if constexpr (kInt4) {
+          if (g == 0) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int y = 0; y < G; ++y) s_qsum[(nt * G + y) * 4 + t] = make_float2(qsum[nt][y][0], qsum[nt][y][1]);
+          }
+        }
       }
       __syncthreads();
     }
 
     float o[NT][Cfg::kSteps][4];
     float m[NT][2], l[NT][2];
+    float om[NT][4];  // 4 bits: weights' sums times the parameters, row g of which is the token's parameter number g
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      om[nt][0] = om[nt][1] = om[nt][2] = om[nt][3] = 0.f;
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
@@ -501,6 +589,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
       if ((u * kWarps + warp) * kSub >= seq.count) break;
       if (u + kAhead >= ids_from + kIds && ids_from + kIds < now.u1) read_ids(now, u);
       uint32_t kr[kSub][2][Cfg::kKWords], vr[kSub][4][Cfg::kVWords];
+      uint32_t kp[kSub][2][kInt4 ? G : 1], vp[kSub][2];  // 4 bits: parameters of tokens g and g + 8: all of K's, word t of V's
       float ks[kSub], vs[kSub];
       int tok[kSub];
 #pragma unroll
@@ -509,12 +598,23 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
         tok[c] = __shfl_sync(0xffffffffu, my_tok, src);
         const int page = __shfl_sync(0xffffffffu, my_page, src);
         // (a tile that is missing reads page 0, slot 0, whosever it is, and is masked)
-        const int64_t at = static_cast<int64_t>(page) * page_bytes + head_bytes + (tok[c] & slot_mask) * (HD * Cfg::kBytes);
+        const int64_t at = static_cast<int64_t>(page) * page_bytes + head_bytes + (tok[c] & slot_mask) * Cfg::kRowBytes;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) KPieces::load(p.c.k + at + (g + 8 * x) * (HD * Cfg::kBytes), t, kr[c][x]);
+        for (int x = 0; x < 2; ++x) KPieces::load(p.c.k + at + (g + 8 * x) * Cfg::kRowBytes, t, kr[c][x]);
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          VPieces::load(p.c.v + at + (2 * t + (x & 1) + 4 * (x & 2)) * (HD * Cfg::kBytes), g, vr[c][x]);
+          if constexpr (kInt4 && HD == 32)
+            vr[c][x][0] = load_once_u16(p.c.v + at + (2 * t + (x & 1) + 4 * (x & 2)) * Cfg::kRowBytes + 2 * g);
+          else
+            VPieces::load(p.c.v + at + (2 * t + (x & 1) + 4 * (x & 2)) * Cfg::kRowBytes, g, vr[c][x]);
+        if constexpr (kInt4) {
+          const int64_t prm = group_row(page, now.h, tok[c]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            RowPieces<G, 1>::load(reinterpret_cast<const uint8_t*>(p.c.k_group) + prm + (g + 8 * x) * (4 * G), 0, kp[c][x]);
+            vp[c][x] = t < G ? load_once(reinterpret_cast<const uint8_t*>(p.c.v_group) + prm + (g + 8 * x) * (4 * G) + 4 * t) : 0u;
+          }
+        }
         ks[c] = vs[c] = 1.f;
         if (kFp8) {
           ks[c] = p.c.k_scale[static_cast<int64_t>(page) * kv_heads + now.h];
@@ -528,6 +628,48 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
       for (int c = 0; c < kSub; ++c)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[c][nt][0] = s[c][nt][1] = s[c][nt][2] = s[c][nt][3] = 0.f;
+      if constexpr (kInt4) {
+        // Sum over the groups of middle * sum(q) + step * (sum(q (128 + code)) - 136 sum(q)). The middles are one product: its
+        // 16 columns hold each middle three times, against the three terms of sum(q) (the words of a row's threads t are its
+        // middles 2 (t & 1) and 2 (t & 1) + 1, or 0 and 1, or a step, against 0, and the only middle). 0x43004300 over two
+        // codes makes them 128 + code in bf16, and a group's product begins at -136 sum(q).
+#pragma unroll
+        for (int c = 0; c < kSub; ++c)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t a0 = G == 4 ? ((t & 1) != 0 ? kp[c][0][G - 1] : kp[c][0][G - (G > 1 ? 2 : 1)]) : kp[c][0][G - 1];
+            const uint32_t a1 = G == 4 ? ((t & 1) != 0 ? kp[c][1][G - 1] : kp[c][1][G - (G > 1 ? 2 : 1)]) : kp[c][1][G - 1];
+            mma_bf16(s[c][nt], a0, a1, G == 4 ? a0 : 0u, G == 4 ? a1 : 0u, qm[nt][0], qm[nt][1]);
+          }
+#pragma unroll
+        for (int y = 0; y < G; ++y)
+#pragma unroll
+          for (int c = 0; c < kSub; ++c) {
+            uint32_t w[2], code[2][4];
+            float step[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              w[x] = G == 1 ? kr[c][x][0] : __byte_perm(kr[c][x][y / 2], kr[c][x][G / 2 + y / 2], y % 2 ? 0x7632u : 0x5410u);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) code[x][i] = ((w[x] >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+              step[x] = __uint_as_float(y % 2 ? kp[c][x][y / 2] & 0xffff0000u : kp[c][x][y / 2] << 16);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float2 base = make_float2(qsum[nt][y][0], qsum[nt][y][1]);
+              if constexpr (Cfg::kSharedQ) base = s_qsum[(nt * G + y) * 4 + t];
+              float acc[4] = {base.x, base.y, base.x, base.y};
+#pragma unroll
+              for (int st = 0; st < 2; ++st) {
+                uint2 q2 = make_uint2(qf[nt][2 * y + st][0], qf[nt][2 * y + st][1]);
+                if constexpr (Cfg::kSharedQ) q2 = s_q[(nt * Cfg::kSteps + 2 * y + st) * 32 + lane];
+                mma_bf16(acc, code[0][2 * st], code[1][2 * st], code[0][2 * st + 1], code[1][2 * st + 1], q2.x, q2.y);
+              }
+#pragma unroll
+              for (int x = 0; x < 4; ++x) s[c][nt][x] = fmaf(step[x >> 1], acc[x], s[c][nt][x]);
+            }
+          }
+      } else {
 #pragma unroll
       for (int st = 0; st < Cfg::kSteps; ++st)
 #pragma unroll
@@ -551,6 +693,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
             cache_mma<kFp8>(s[c][nt], a0, a1, a2, a3, q2.x, q2.y);
           }
         }
+      }
 
       // Tokens g and g + 8 of rows 2t and 2t + 1, in exponents of 2 with V's scale in.
       float inv_v[kSub];
@@ -583,13 +726,21 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
               const int pos = limit[nt][x & 1];
               if (j > pos || (p.window > 0 && pos - j >= p.window && j >= p.sinks)) s[c][nt][x] = -INFINITY;
             }
-          // Values of tokens that no row sees may be anything (0 times a NaN is a NaN).
+          // Values of tokens that no row sees may be anything (0 times a NaN is a NaN); in 4 bits it is their parameters.
+          if constexpr (kInt4) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int j = tok[c] + 2 * t + (x & 1) + 4 * (x & 2);
-            if (j >= seq.len || (p.window > 0 && j < from && j >= p.sinks)) {
+            for (int x = 0; x < 2; ++x) {
+              const int j = tok[c] + g + 8 * x;
+              if (j >= seq.len || (p.window > 0 && j < from && j >= p.sinks)) vp[c][x] = 0u;
+            }
+          } else {
 #pragma unroll
-              for (int i2 = 0; i2 < Cfg::kVWords; ++i2) vr[c][x][i2] = 0u;
+            for (int x = 0; x < 4; ++x) {
+              const int j = tok[c] + 2 * t + (x & 1) + 4 * (x & 2);
+              if (j >= seq.len || (p.window > 0 && j < from && j >= p.sinks)) {
+#pragma unroll
+                for (int i2 = 0; i2 < Cfg::kVWords; ++i2) vr[c][x][i2] = 0u;
+              }
             }
           }
         }
@@ -619,6 +770,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
               const float alpha = fast_exp2(m[nt][x] - best);  // 0 the first time
               m[nt][x] = best;
               l[nt][x] *= alpha;
+              om[nt][x] *= alpha;
 #pragma unroll
               for (int j = 0; j < Cfg::kSteps; ++j) {
                 o[nt][j][x] *= alpha;
@@ -646,7 +798,36 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
 
 #pragma unroll
       for (int c = 0; c < kSub; ++c) {
-        if constexpr (kFp8) {
+        if constexpr (kInt4) {
+          // The parameters as rows, two tokens to a register; a group's steps go into the weights of its dims.
+          const uint32_t v0 = movmatrix_trans(vp[c][0]), v1 = movmatrix_trans(vp[c][1]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_bf16(om[nt], v0, 0u, v1, 0u, pf[c][nt][0], pf[c][nt][1]);
+#pragma unroll
+          for (int y = 0; y < G; ++y) {
+            const uint32_t step0 = __shfl_sync(0xffffffffu, v0, 4 * y + t), step1 = __shfl_sync(0xffffffffu, v1, 4 * y + t);
+            uint32_t w[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              w[nt][0] = bf16x2_mul(pf[c][nt][0], step0);
+              w[nt][1] = bf16x2_mul(pf[c][nt][1], step1);
+            }
+            const uint32_t sel = y % 2 ? 0x7632u : 0x5410u;
+            const uint32_t lo = __byte_perm(vr[c][0][y / 2], vr[c][1][y / 2], sel);  // tokens 2t, 2t+1 of four dims
+            const uint32_t hi = __byte_perm(vr[c][2][y / 2], vr[c][3][y / 2], sel);  // tokens 2t+8, 2t+9
+            uint32_t a[2][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              a[0][i] = bf16x2_less_136(((lo >> (4 * i)) & 0x000f000fu) | 0x43004300u);
+              a[1][i] = bf16x2_less_136(((hi >> (4 * i)) & 0x000f000fu) | 0x43004300u);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                mma_bf16(o[nt][2 * y + e], a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], w[nt][0], w[nt][1]);
+          }
+        } else if constexpr (kFp8) {
 #pragma unroll
           for (int i2 = 0; i2 < Cfg::kVWords; ++i2) {
 #pragma unroll
@@ -687,6 +868,12 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kFp8, NT, kShare>::kThreads,
         float* dst = s_merge + warp * Cfg::kPartial;
 #pragma unroll
         for (int j = 0; j < Cfg::kSteps; ++j) {
+          if constexpr (kInt4) {
+            const float mid = __shfl_sync(0xffffffffu, om[nt][x], 4 * (G + j / 2) + t);
+            *reinterpret_cast<float2*>(dst + r * HD + 32 * (j / 2) + 4 * g + 2 * (j & 1)) =
+                make_float2(o[nt][j][x] + mid, o[nt][j][x + 2] + mid);
+            continue;
+          }
           const int d = kFp8 ? VPieces::offset(j / 2, g) + 2 * (j & 1) : VPieces::offset(j, g) / 2;
           *reinterpret_cast<float2*>(dst + r * HD + d) = make_float2(o[nt][j][x], o[nt][j][x + 2]);
         }
@@ -958,10 +1145,10 @@ struct CacheClusterLaunch {
 
 // How many clusters of `cluster` CTAs run side by side on the current device. (It depends on which SMs a GPU has in each
 // of its parts: 16 SMs next to each other were found for 6 clusters, not for 8.)
-template <int HD, bool kFp8, int NT>
+template <int HD, int kType, int NT>
 static cudaError_t cache_attention_clusters(int cluster, int* side_by_side) {
-  using Cfg = CacheAttnCfg<HD, kFp8, NT, kCacheCluster>;
-  const auto kernel = cache_attention_kernel<HD, kFp8, NT, kCacheCluster>;
+  using Cfg = CacheAttnCfg<HD, kType, NT, kCacheCluster>;
+  const auto kernel = cache_attention_kernel<HD, kType, NT, kCacheCluster>;
   constexpr int kSmem = Cfg::kSmemBytes + Cfg::kPartial * 4;
   static std::once_flag once[64];
   static int fit[64][kCacheCluster + 1];
@@ -983,30 +1170,30 @@ static cudaError_t cache_attention_clusters(int cluster, int* side_by_side) {
   return result[dev];
 }
 
-template <int HD, bool kFp8, int NT>
+template <int HD, int kType, int NT>
 static cudaError_t launch_cache_attention_cluster(const CacheAttnParams& p, int64_t row_blocks, int cluster,
                                                   cudaStream_t stream) {
-  using Cfg = CacheAttnCfg<HD, kFp8, NT, kCacheCluster>;
+  using Cfg = CacheAttnCfg<HD, kType, NT, kCacheCluster>;
   const CacheClusterLaunch launch(dim3(p.batch * p.c.kv_heads * cluster, static_cast<unsigned>(row_blocks)), Cfg::kThreads,
                                   cluster, Cfg::kSmemBytes + Cfg::kPartial * 4, stream);
-  return cudaLaunchKernelEx(&launch.config, cache_attention_kernel<HD, kFp8, NT, kCacheCluster>, p);
+  return cudaLaunchKernelEx(&launch.config, cache_attention_kernel<HD, kType, NT, kCacheCluster>, p);
 }
 
-template <int HD, bool kFp8, int NT, int kShare>
+template <int HD, int kType, int NT, int kShare>
 static cudaError_t launch_cache_attention_t(const CacheAttnParams& p, int64_t row_blocks, int sm_count, cudaStream_t stream) {
-  using Cfg = CacheAttnCfg<HD, kFp8, NT, kShare>;
+  using Cfg = CacheAttnCfg<HD, kType, NT, kShare>;
   const size_t smem = Cfg::kSmemBytes + (kShare > 0 ? 0 : (static_cast<size_t>(p.batch) + 1) * 4);
   static std::once_flag once[64];
   int dev = 0;
   cudaGetDevice(&dev);
   cudaError_t e = cudaSuccess;
   std::call_once(once[dev & 63], [&] {
-    e = cudaFuncSetAttribute(cache_attention_kernel<HD, kFp8, NT, kShare>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(cache_attention_kernel<HD, kType, NT, kShare>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              Cfg::kSmemBytes + (kShare > 0 ? 0 : 4 * (kCacheMaxBatch + 1)));
   });
   if (e != cudaSuccess) return e;
   if constexpr (kShare > 0) {
-    return launch_pdl(cache_attention_kernel<HD, kFp8, NT, kShare>,
+    return launch_pdl(cache_attention_kernel<HD, kType, NT, kShare>,
                       dim3(p.batch * p.c.kv_heads, static_cast<unsigned>(row_blocks)), dim3(Cfg::kThreads), smem, stream, p);
   } else {
     static_assert(Cfg::kCtasPerSm <= (HD == 128 && NT == 2 ? 2 : 4), "as cache_attention_ctas says");
@@ -1014,14 +1201,14 @@ static cudaError_t launch_cache_attention_t(const CacheAttnParams& p, int64_t ro
     for (int64_t block = 0; block < row_blocks && e == cudaSuccess; block += kCacheBlocksAtOnce) {
       turn.block0 = static_cast<int>(block);
       const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(row_blocks - block, kCacheBlocksAtOnce));
-      e = launch_pdl(cache_attention_kernel<HD, kFp8, NT, kShare>, dim3(sm_count * Cfg::kCtasPerSm, blocks),
+      e = launch_pdl(cache_attention_kernel<HD, kType, NT, kShare>, dim3(sm_count * Cfg::kCtasPerSm, blocks),
                      dim3(Cfg::kThreads), smem, stream, turn);
     }
     return e;
   }
 }
 
-template <int HD, bool kFp8, int NT>
+template <int HD, int kType, int NT>
 static cudaError_t launch_cache_attention_nt(const CacheAttnParams& p, int64_t row_blocks, int sm_count, cudaStream_t stream) {
   // The most tokens that a sequence can see; the host does not know their lengths.
   const int64_t room = static_cast<int64_t>(p.table_pages) << p.c.page_shift;
@@ -1044,12 +1231,12 @@ static cudaError_t launch_cache_attention_nt(const CacheAttnParams& p, int64_t r
   //   else up to 8: 4 heads of 8000 10.4 / 18.0, of 32000 17.4 / 20.2; 1 of 8000 9.9 / 13.5, of 32000 16.7 / 17.1.
   const int64_t heads = static_cast<int64_t>(p.batch) * p.c.kv_heads * row_blocks;
   const bool sm_each = heads <= sm_count;
-  const int64_t round = 16 * (sm_each ? CacheAttnCfg<HD, kFp8, NT, 1>::kUnitTiles : CacheAttnCfg<HD, kFp8, NT, 4>::kUnitTiles);
+  const int64_t round = 16 * (sm_each ? CacheAttnCfg<HD, kType, NT, 1>::kUnitTiles : CacheAttnCfg<HD, kType, NT, 4>::kUnitTiles);
   int cluster = 1;
   if (sm_each && tokens > 2 * round) {
     while (cluster < kCacheCluster && tokens > cluster * round) {
       int side_by_side = 0;
-      const cudaError_t e = cache_attention_clusters<HD, kFp8, NT>(2 * cluster, &side_by_side);
+      const cudaError_t e = cache_attention_clusters<HD, kType, NT>(2 * cluster, &side_by_side);
       if (e != cudaSuccess) return e;
       if (heads > side_by_side) break;
       cluster *= 2;
@@ -1061,24 +1248,27 @@ static cudaError_t launch_cache_attention_nt(const CacheAttnParams& p, int64_t r
   const int64_t most = thirds >= 2 ? (windowed ? 72 : 32) : thirds == 1 || !sm_each ? 20 : 8;
   if (tokens <= most * cluster * round) {
     if (cluster > 1)
-      return launch_cache_attention_cluster<HD, kFp8, NT>(p, row_blocks, cluster, stream);
-    if (sm_each) return launch_cache_attention_t<HD, kFp8, NT, 1>(p, row_blocks, sm_count, stream);
-    return launch_cache_attention_t<HD, kFp8, NT, 4>(p, row_blocks, sm_count, stream);
+      return launch_cache_attention_cluster<HD, kType, NT>(p, row_blocks, cluster, stream);
+    if (sm_each) return launch_cache_attention_t<HD, kType, NT, 1>(p, row_blocks, sm_count, stream);
+    return launch_cache_attention_t<HD, kType, NT, 4>(p, row_blocks, sm_count, stream);
   }
-  return launch_cache_attention_t<HD, kFp8, NT, 0>(p, row_blocks, sm_count, stream);
+  return launch_cache_attention_t<HD, kType, NT, 0>(p, row_blocks, sm_count, stream);
 }
 
 template <int HD>
-static cudaError_t launch_cache_attention_hd(const CacheAttnParams& p, bool fp8, int nt, int64_t row_blocks, int sm_count,
+static cudaError_t launch_cache_attention_hd(const CacheAttnParams& p, int type, int nt, int64_t row_blocks, int sm_count,
                                              cudaStream_t stream) {
-  if (fp8)
-    return nt == 1 ? launch_cache_attention_nt<HD, true, 1>(p, row_blocks, sm_count, stream)
-                   : launch_cache_attention_nt<HD, true, 2>(p, row_blocks, sm_count, stream);
-  return nt == 1 ? launch_cache_attention_nt<HD, false, 1>(p, row_blocks, sm_count, stream)
-                 : launch_cache_attention_nt<HD, false, 2>(p, row_blocks, sm_count, stream);
+  if (type == kCacheE4m3)
+    return nt == 1 ? launch_cache_attention_nt<HD, kCacheE4m3, 1>(p, row_blocks, sm_count, stream)
+                   : launch_cache_attention_nt<HD, kCacheE4m3, 2>(p, row_blocks, sm_count, stream);
+  if (type == kCacheInt4)
+    return nt == 1 ? launch_cache_attention_nt<HD, kCacheInt4, 1>(p, row_blocks, sm_count, stream)
+                   : launch_cache_attention_nt<HD, kCacheInt4, 2>(p, row_blocks, sm_count, stream);
+  return nt == 1 ? launch_cache_attention_nt<HD, kCacheBf16, 1>(p, row_blocks, sm_count, stream)
+                 : launch_cache_attention_nt<HD, kCacheBf16, 2>(p, row_blocks, sm_count, stream);
 }
 
-static cudaError_t launch_cache_attention(CacheAttnParams p, void* workspace, bool fp8, int sm_count, cudaStream_t stream) {
+static cudaError_t launch_cache_attention(CacheAttnParams p, void* workspace, int type, int sm_count, cudaStream_t stream) {
   int nt = 1;
   const int64_t rows = static_cast<int64_t>(p.q_len) * p.group;
   const int64_t blocks = cache_attention_row_blocks(rows, &nt);
@@ -1087,11 +1277,11 @@ static cudaError_t launch_cache_attention(CacheAttnParams p, void* workspace, bo
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + cache_attention_counter_bytes(sm_count));
   switch (p.c.head_dim) {
     case 32:
-      return launch_cache_attention_hd<32>(p, fp8, nt, blocks, sm_count, stream);
+      return launch_cache_attention_hd<32>(p, type, nt, blocks, sm_count, stream);
     case 64:
-      return launch_cache_attention_hd<64>(p, fp8, nt, blocks, sm_count, stream);
+      return launch_cache_attention_hd<64>(p, type, nt, blocks, sm_count, stream);
     case 128:
-      return launch_cache_attention_hd<128>(p, fp8, nt, blocks, sm_count, stream);
+      return launch_cache_attention_hd<128>(p, type, nt, blocks, sm_count, stream);
     default:
       return cudaErrorInvalidValue;
   }
