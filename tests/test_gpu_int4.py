@@ -6,10 +6,11 @@ middle at a border may then be its neighbour. Any stored value is within 0.55 st
 value given: half a step, 8 * 2^-9 of one for the factor's rounding, 15 * 2^-9 of one for the step's at the ends, and
 the middle's own rounding.
 
-Attention: with steps s and middles m of a token's groups, a weight's part of a value, w (v - m), is rounded to bf16 twice
-(the weight, and its product with the step) and w m once, each by at most 2^-8 of itself; the output is bf16. A score's
-fp32 sums are over step * q * (128 + code), at most 143, after -136 step sum(q): 34 terms of at most 279 step |q|, off by
-2^-23 each in the worst case, and over middle * q.
+Attention: with steps s and middles m of a token's groups, a weight is rounded to fp16 (2^-11 of itself), its product with a
+step again, and a step or a middle loses at most 2^-25 of a power of two up to twice the largest parameter; the output is bf16. A
+score's fp32 sums begin at -1032 sum(q) (72 for half of the elements) and add q (1024 + code): 34 terms of at most 2071 |q|, off by
+2^-23 each in the worst case, and over middle * q. That worst case is far from what happens (the terms' errors are not alike),
+so the whole output is also held to 2^-8 of its norm, twice what its own rounding may take.
 """
 
 import math
@@ -335,9 +336,11 @@ def _check_attend(cache, seqs, lengths, heads, q_len, window, sinks, q, out, sca
             mid_ref, mid_sum, _ = oracle.attend(x, k[g], vm[g], seen, scale)
             part_sum = oracle.attend(x, k[g], v[g] - vm[g], seen, scale)[1]
             share = x.abs().view(q_len, d // 32, 32).sum(-1)
-            off = scale * 2**-23 * (34 * 279 * share @ ks[g].T + 20 * share @ km[g].T)
+            off = scale * 2**-23 * (34 * 2071 * share @ ks[g].T + 20 * share @ km[g].T)
             off = torch.where(used, off, 0.0).amax(-1, keepdim=True) if n else torch.zeros(q_len, 1, dtype=torch.float64)
-            _close(got[b, :, h], ref, 2**-8 * ref.abs() + 2**-7 * part_sum + 2**-8 * mid_sum + (2.1 * off + 2**-18) * absum)
+            _close(got[b, :, h], ref, 2**-8 * ref.abs() + 2**-10 * part_sum + 2**-11 * mid_sum + (2.1 * off + 2**-18) * absum
+                   + 2**-20 * params["v"][seqs.table[b, :-(-n // page)].long()].nan_to_num().abs().max() if n else 0 * ref)
+            assert float((got[b, :, h].double() - ref).norm()) <= 2**-8 * float(ref.norm()) + 2**-18
 
 
 ATTENDS = [
@@ -374,3 +377,31 @@ def test_attend(lengths, page, heads, kv_heads, head_dim, q_len, window, sinks, 
     _check_attend(cache, seqs, lengths, heads, q_len, window, sinks, q, out, head_dim**-0.5)
     again = cache.attend(q, seqs.table.cuda(), _i32(lengths), **args)
     assert torch.equal(out, again)  # the join's order does not depend on who comes last
+
+
+@pytest.mark.parametrize("d,heads,kv_heads", [(32, 2, 1), (64, 4, 4), (128, 8, 1)])
+@pytest.mark.parametrize("room", [0, 1 << 17])
+def test_attend_scores_far_apart(d, heads, kv_heads, room):
+    """Queries ten times as large, and of unlike sizes: the maximum moves far, and the weights rest on few tokens."""
+    lengths, page = [700, 90], 32
+    cache, seqs = _filled(lengths, page, kv_heads, d, INT4, 3)
+    seqs.table = torch.nn.functional.pad(seqs.table, (0, max(0, room // page - seqs.table.shape[1])), value=-1)
+    q = (torch.randn(2, heads * d, generator=_gen(d)) * 10.0 ** torch.tensor([[1.0], [-3.0]])).bfloat16().cuda()
+    out = cache.attend(q, seqs.table.cuda(), _i32(lengths))
+    _check_attend(cache, seqs, lengths, heads, 1, 0, 0, q, out, d**-0.5)
+
+
+@pytest.mark.parametrize("room", [0, 1 << 17])
+def test_attend_parameters_far_apart(room):
+    """Tokens whose values are 2^12 times those of others, at the start, in the middle and at the end."""
+    n, d, page = 600, 64, 16
+    seqs = _Sequences([n], page, 1)
+    cache = serving.KVCache.allocate(seqs.pages, 1, d, page, INT4)
+    _junk(cache)
+    qkv = torch.randn(n, 3 * d, generator=_gen(4))
+    qkv[:, 2 * d:] *= torch.where(torch.arange(n) % 250 < 3, 2.0**12, 1.0)[:, None]
+    cache.append(qkv.bfloat16().cuda(), 1, _i32([0]), _i32([n]), _i32([0]), seqs.table.cuda(), n)
+    seqs.table = torch.nn.functional.pad(seqs.table, (0, max(0, room // page - seqs.table.shape[1])), value=-1)
+    q = torch.randn(1, d, generator=_gen(5)).bfloat16().cuda()
+    out = cache.attend(q, seqs.table.cuda(), _i32([n]))
+    _check_attend(cache, seqs, [n], 1, 1, 0, 0, q, out, d**-0.5)

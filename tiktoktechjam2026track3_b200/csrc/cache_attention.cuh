@@ -146,20 +146,39 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
   return h;
 }
 
-__device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t bf16x2_less_136(uint32_t a) {
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), __float2bfloat162_rn(136.f));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
+__device__ __forceinline__ float2 f16x2_values(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+__device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t f16x2_add(uint32_t a, uint32_t b) {
+  const __half2 r = __hadd2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// d = a b
+__device__ __forceinline__ void mma_bf16_from_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                   uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// (w & mask) | bits is one instruction if one of the two constants is in a register.
+__device__ __forceinline__ uint32_t in_register(uint32_t x) {
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+  return r;
+}
 // Pages and scales may be written by the launch before this one, which is still running when this grid's first CTAs are
 // resident: they are not constant for the grid's time, as the read-only path asks, so they come by coherent loads. These
 // leave no line in L1, where nothing would read it again, and are not volatile, so that the compiler may place them
@@ -251,7 +270,7 @@ struct CacheAttnCfg {
   // warps an SM at 128 registers, 12 at 168, 8 at 255; in CTAs of 4, so that one that joins does not idle many (64
   // sequences of up to 8192 tokens: 116 us, 122 in CTAs of 8), or of 6 where 12 is the number.
   static constexpr bool kWide = HD == 128 && (kType == kCacheBf16 || NT == 2);
-  static constexpr bool kSharedQ = NT == 2 || (HD == 128 && kType != kCacheBf16);
+  static constexpr bool kSharedQ = kType != kCacheInt4 && (NT == 2 || (HD == 128 && kType == kCacheE4m3));
   // kShare 1 or 4: a CTA takes a whole (sequence, head) with all the warps of an SM, or a quarter; kCacheCluster: a
   // cluster does, each CTA with those of an SM; 0: a stretch of the line.
   static constexpr int kWarpsPerSm = !kWide ? 16 : kType != kCacheBf16 || NT == 1 ? 12 : 8;
@@ -262,11 +281,8 @@ struct CacheAttnCfg {
   static constexpr int kLeast = 16 / kWarps;
   static constexpr int kUnitTiles = kWarps * kSub;  // of 16 tokens: what a CTA takes at a time
   // Twelve warps with 8 KB on their way each need no prefetch (183 us with it, 168 without: 32 x 8192 tokens, 8 heads).
-  static constexpr bool kPrefetch = !(kWide && kType == kCacheBf16 && NT == 1);
-  // 128-byte lines of a warp's part of a unit: keys (their codes, then their groups' parameters) and values alike.
-  static constexpr int kCodeLines = 16 * kRowBytes / 128;
-  static constexpr int kGroupLines = kType != kCacheInt4 ? 0 : kGroups > 1 ? kGroups / 2 : 1;
-  static constexpr int kLines = kSub * 2 * (kCodeLines + kGroupLines);
+  static constexpr bool kPrefetch = kType != kCacheInt4 && !(kWide && kType == kCacheBf16 && NT == 1);
+  static constexpr int kLines = kSub * 2 * 16 * kRowBytes / 128;  // 128-byte lines of a warp's part of a unit
   static constexpr int kPartial = kRows * (HD + 2);  // floats of one partial result: outputs, then maxima, then sums
   // Shared memory: the join of the warps' results, or the factors of the join of CTAs; then (batch + 1) first units.
   static constexpr int kSmemBytes = kWarps * kPartial * 4 > 24576 ? kWarps * kPartial * 4 : 24576;
@@ -304,16 +320,20 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
   float* s_merge = reinterpret_cast<float*>(s_dyn);
   int* s_first = reinterpret_cast<int*>(s_dyn + Cfg::kSmemBytes);  // [batch + 1] first unit of each sequence
   __shared__ uint2 s_q[Cfg::kSharedQ ? NT * Cfg::kSteps * 32 : 1];
-  __shared__ float2 s_qsum[kInt4 && Cfg::kSharedQ ? NT * G * 4 : 1];
+  __shared__ uint4 s_q4[kInt4 ? NT * G * 32 : 1];    // 4 bits: Q as fragments,
+  __shared__ float4 s_qsum[kInt4 ? NT * G * 4 : 1];  // what its sums over the groups take from the products,
+  __shared__ int s_limit[kInt4 ? 8 * NT : 1];        // and the rows' positions
   __shared__ int s_scan[kWarps];
   __shared__ Part s_part;  // what the join needs of `now`, out of the registers of the loop
   __shared__ int s_last;
+  __shared__ int s_line[4];  // 4 bits: of the line, what its joins need: units, CTAs, this one's stretch
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
   const int g = lane >> 2;
   const int t = lane & 3;
+  const uint32_t low4 = kInt4 ? in_register(0x000f000fu) : 0u, high4 = kInt4 ? in_register(0x00f000f0u) : 0u;
   const int kv_heads = p.c.kv_heads;
   const int rows_total = p.q_len * p.group;
   const int row_block = (p.block0 + static_cast<int>(blockIdx.y)) * R;
@@ -356,6 +376,12 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
     if (cta >= ctas) return;
     w_begin = static_cast<int>(cta * total / ctas);
     w_end = static_cast<int>((cta + 1) * total / ctas);
+    if (kInt4 && tid == 0) {
+      s_line[0] = static_cast<int>(total);
+      s_line[1] = static_cast<int>(ctas);
+      s_line[2] = w_begin;
+      s_line[3] = w_end;
+    }
   }
 
   constexpr int kNoTile = 1 << 30;         // a first token that no row sees
@@ -393,10 +419,6 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
       }
     }
   };
-  // Byte offset of the first parameter of token `tok` (of its sequence), in 4 bits.
-  auto group_row = [&](int page, int h, int tok) {
-    return (((static_cast<int64_t>(page) * kv_heads + h) << p.c.page_shift) + (tok & slot_mask)) * (4 * G);
-  };
   // The lines of the warp's part of unit u into L2, a lane each.
   auto prefetch = [&](const Part& x, int u) {
     constexpr int kTileLines = Cfg::kLines / kSub;  // K's, then V's
@@ -408,15 +430,9 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
       const int page = __shfl_sync(0xffffffffu, my_page, src);
       const int in = line % kTileLines;
       const bool keys = in < kTileLines / 2;
-      const int at = keys ? in : in - kTileLines / 2;
-      if (u < x.u1 && (Cfg::kLines % 32 == 0 || line < Cfg::kLines) && tok != kNoTile) {
-        if (!kInt4 || at < Cfg::kCodeLines)
-          prefetch_l2((keys ? p.c.k : p.c.v) + static_cast<int64_t>(page) * page_bytes + x.h * p.c.head_stride * Cfg::kBits / 8 +
-                      (tok & slot_mask) * Cfg::kRowBytes + at * 128);
-        else
-          prefetch_l2(reinterpret_cast<const uint8_t*>(keys ? p.c.k_group : p.c.v_group) + group_row(page, x.h, tok) +
-                      (at - Cfg::kCodeLines) * 128);
-      }
+      if (u < x.u1 && (Cfg::kLines % 32 == 0 || line < Cfg::kLines) && tok != kNoTile)
+        prefetch_l2((keys ? p.c.k : p.c.v) + static_cast<int64_t>(page) * page_bytes + x.h * p.c.head_stride * Cfg::kBits / 8 +
+                    (tok & slot_mask) * Cfg::kRowBytes + (keys ? in : in - kTileLines / 2) * 128);
     }
   };
   Part now;
@@ -449,8 +465,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
     // Q: fragments of the 8-row operand(s), and the factor of its rows' scores.
     uint32_t qf[NT][Cfg::kSteps][2];  // (in shared memory where registers are short: it is alike for every warp)
     float row_scale[NT][2];
-    uint32_t qm[NT][2];    // 4 bits: the operand that the middles meet
-    float qsum[NT][G][2];  // 4 bits: -136 times the sum of Q over each group
+    uint32_t qm[NT][2];  // 4 bits: what the middles meet
     int limit[NT][2];  // position of the rows 2t, 2t + 1 of each operand, -1: no such row
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -486,46 +501,69 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
         row_scale[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);      // the thread that holds row 2t
         row_scale[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);  // row 2t + 1
       } else if constexpr (kInt4) {
-        uint32_t part[3][G];  // the groups' sums as three bf16 terms each, 24 bits together
+        // Q as fp16, after a power of two that brings the row's largest element to [2^14, 2^15).
+        float f[G][8];
+        float amax = 0.f;
 #pragma unroll
         for (int y = 0; y < G; ++y) {
           const uint4 u = real ? *reinterpret_cast<const uint4*>(src + 32 * y + 8 * t) : make_uint4(0, 0, 0, 0);
+          unpack_bf16x8(u, f[y]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[y][i]));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -100), 127);
+        const float up = exp2_int(14 - e);
+        uint32_t part[3][G];  // the groups' sums as three bf16 terms each, 24 bits together
+#pragma unroll
+        for (int y = 0; y < G; ++y) {
           // Elements i and i + 4 side by side, as the codes' halves hold them.
-          qf[nt][2 * y][0] = __byte_perm(u.x, u.z, 0x5410u);
-          qf[nt][2 * y][1] = __byte_perm(u.x, u.z, 0x7632u);
-          qf[nt][2 * y + 1][0] = __byte_perm(u.y, u.w, 0x5410u);
-          qf[nt][2 * y + 1][1] = __byte_perm(u.y, u.w, 0x7632u);
-          float f[8];
-          unpack_bf16x8(u, f);
-          float sum = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          qsum[nt][y][0] = -136.f * __shfl_sync(0xffffffffu, sum, 8 * t);  // the threads that hold rows 2t and 2t + 1
-          qsum[nt][y][1] = -136.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+          uint32_t pair[4];
+          float sum[2] = {0.f, 0.f};  // of the even elements, whose codes come as 1024 + code, and the odd ones: 64 + code
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            pair[i] = pack_f16x2(f[y][i] * up, f[y][i + 4] * up);
+            const float2 v = f16x2_values(pair[i]);
+            sum[i & 1] += v.x + v.y;
+          }
+          if (warp == 0) s_q4[(nt * G + y) * 32 + lane] = make_uint4(pair[0], pair[1], pair[2], pair[3]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+          }
+          const float base = -(1032.f * sum[0] + 72.f * sum[1]);
+          const float base0 = __shfl_sync(0xffffffffu, base, 8 * t);  // the threads that hold rows 2t and 2t + 1
+          const float base1 = __shfl_sync(0xffffffffu, base, 8 * t + 4);
+          if (warp == 0 && g == 0) s_qsum[(nt * G + y) * 4 + t] = make_float4(base0, base1, base0, base1);
+          float rest = sum[0] + sum[1];
 #pragma unroll
           for (int i = 0; i < 3; ++i) {
-            const float term = bf16_round(sum);
+            const float term = bf16_round(rest);
             part[i][y] = __float_as_uint(term) >> 16;
-            sum -= term;
+            rest -= term;
           }
         }
-        // Which words of a token's parameters the threads of a row give to the product with the middles: see s below.
-        if constexpr (G == 4) {
-          const bool high = (t & 1) != 0;
-          uint32_t two[3];
+        // What the threads of a row hold against the words of a token's parameters: see the middles below.
+        uint32_t two[3];
 #pragma unroll
-          for (int i = 0; i < 3; ++i)
-            two[i] = (high ? part[i][G > 2 ? 2 : 0] : part[i][0]) | (high ? part[i][G > 3 ? 3 : 0] : part[i][G > 1 ? 1 : 0]) << 16;
+        for (int i = 0; i < 3; ++i) {
+          if constexpr (G == 4)
+            two[i] = (t & 1) != 0 ? part[i][G / 2] | part[i][G - 1] << 16 : part[i][0] | part[i][G / 4] << 16;
+          else
+            two[i] = G == 2 ? part[i][0] | part[i][G - 1] << 16 : part[i][0] << 16;
+        }
+        if constexpr (G == 4) {
           qm[nt][0] = t < 2 ? two[0] : two[1];
           qm[nt][1] = t < 2 ? two[2] : 0u;
         } else {
-          uint32_t two[3];
-#pragma unroll
-          for (int i = 0; i < 3; ++i) two[i] = G == 2 ? part[i][0] | part[i][G - 1] << 16 : part[i][0] << 16;
           qm[nt][0] = t == 0 ? two[0] : t == 1 ? two[1] : t == 2 ? two[2] : 0u;
           qm[nt][1] = 0u;
         }
-        row_scale[nt][0] = row_scale[nt][1] = p.scale_log2;
+        const float down = exp2_int(e - 14) * p.scale_log2;
+        row_scale[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);
+        row_scale[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
       } else {
 #pragma unroll
         for (int s = 0; s < Cfg::kSteps; ++s) {
@@ -538,6 +576,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
       for (int i = 0; i < 2; ++i) {
         const int r = row_block + 8 * nt + 2 * t + i;
         limit[nt][i] = r < rows_total ? seq.len - p.q_len + r / p.group : -1;
+        if (kInt4 && warp == 0 && g == 0) s_limit[8 * nt + 2 * t + i] = limit[nt][i];
       }
     }
 
@@ -548,21 +587,16 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
 #pragma unroll
           for (int st = 0; st < Cfg::kSteps; ++st)
             s_q[(nt * Cfg::kSteps + st) * 32 + lane] = make_uint2(qf[nt][st][0], qf[nt][st][1]);
-        if constexpr (kInt4) {
-          if (g == 0) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int y = 0; y < G; ++y) s_qsum[(nt * G + y) * 4 + t] = make_float2(qsum[nt][y][0], qsum[nt][y][1]);
-          }
-        }
       }
       __syncthreads();
     }
 
+    if constexpr (kInt4) __syncthreads();
+
     float o[NT][Cfg::kSteps][4];
     float m[NT][2], l[NT][2];
-    float om[NT][4];  // 4 bits: weights' sums times the parameters, row g of which is the token's parameter number g
+    float om[NT][4];  // 4 bits: weights' sums times V's parameters, row g of which is the token's parameter number g;
+    float unit = 0x1p-100f;  // and what o and om count in, a power of two above every parameter so far
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       om[nt][0] = om[nt][1] = om[nt][2] = om[nt][3] = 0.f;
@@ -580,6 +614,19 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
       for (int d = 1; d < kAhead; ++d) prefetch(now, now.u0 + d);
     }
 
+    // 4 bits: where this thread's pieces of a page begin (of the token at slot 0).
+    const uint8_t* k_at = p.c.k + head_bytes + g * Cfg::kRowBytes + t * (Cfg::kRowBytes / 4);
+    const uint8_t* v_at = p.c.v + head_bytes + 2 * t * Cfg::kRowBytes + g * (Cfg::kRowBytes / 8);
+    const uint8_t* kp_at = nullptr;
+    const uint8_t* vp_at = nullptr;
+    int group_page = 0;  // bytes of a page's parameters, all heads
+    if constexpr (kInt4) {
+      const int64_t head = (static_cast<int64_t>(now.h) << p.c.page_shift) * (4 * G) + g * (4 * G);
+      kp_at = reinterpret_cast<const uint8_t*>(p.c.k_group) + head;
+      vp_at = reinterpret_cast<const uint8_t*>(p.c.v_group) + head + 4 * min(t, G - 1);
+      group_page = (kv_heads << p.c.page_shift) * (4 * G);
+    }
+
     // Tokens that every row sees lie below `all_see`, and (with a window) from `all_from` on or below the sinks.
     const int all_see = seq.len - p.q_len + 1;
     const int all_from = p.window > 0 ? max(0, seq.len - p.window) : 0;
@@ -587,9 +634,225 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
 #pragma unroll 1
     for (int u = now.u0; u < now.u1; ++u) {
       if ((u * kWarps + warp) * kSub >= seq.count) break;
-      if (u + kAhead >= ids_from + kIds && ids_from + kIds < now.u1) read_ids(now, u);
+      if (u + (kInt4 ? 0 : kAhead) >= ids_from + kIds && ids_from + kIds < now.u1) {
+        if constexpr (kInt4) {
+          const volatile Part& at = s_part;
+          Part x;
+          x.b = at.b;
+          x.seq.count = at.seq.count;
+          x.seq.sink_tiles = at.seq.sink_tiles;
+          x.seq.first_win = at.seq.first_win;
+          read_ids(x, u);
+        } else {
+          read_ids(now, u);
+        }
+      }
+      if constexpr (kInt4) {
+        const int mid_at = 8 + 4 * (t & 1);
+        uint32_t kr[kSub][2][Cfg::kKWords], vr[kSub][4][Cfg::kVWords];
+        uint32_t kp[kSub][2][G == 4 ? 2 : G], km[kSub][2], vp[kSub][2];  // parameters of tokens g and g + 8: K's steps, words of K's middles and V's
+        int tok[kSub];
+#pragma unroll
+        for (int c = 0; c < kSub; ++c) {
+          const int src = (u - ids_from) * kSub + c;
+          tok[c] = __shfl_sync(0xffffffffu, my_tok, src);
+          const int page = __shfl_sync(0xffffffffu, my_page, src);
+          // (a tile that is missing reads page 0, slot 0, whosever it is, and is masked)
+          const int slot = tok[c] & slot_mask;
+          const uint8_t* const k_row = k_at + static_cast<int64_t>(page) * page_bytes + slot * Cfg::kRowBytes;
+          const uint8_t* const v_row = v_at + static_cast<int64_t>(page) * page_bytes + slot * Cfg::kRowBytes;
+          const uint8_t* const kp_row = kp_at + static_cast<int64_t>(page) * group_page + slot * (4 * G);
+          const uint8_t* const vp_row = vp_at + static_cast<int64_t>(page) * group_page + slot * (4 * G);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            KPieces::load(k_row + 8 * x * Cfg::kRowBytes, 0, kr[c][x]);
+            RowPieces<G == 4 ? 2 : G, 1>::load(kp_row + 8 * x * (4 * G), 0, kp[c][x]);
+            km[c][x] = G == 4 ? load_once(kp_row + 8 * x * (4 * G) + mid_at) : kp[c][x][G == 4 ? 0 : G - 1];
+            vp[c][x] = load_once(vp_row + 8 * x * (4 * G));
+            if (G < 4) vp[c][x] = t < G ? vp[c][x] : 0u;
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint8_t* const row = v_row + ((x & 1) + 4 * (x & 2)) * Cfg::kRowBytes;
+            if constexpr (HD == 32)
+              vr[c][x][0] = load_once_u16(row);
+            else
+              VPieces::load(row, 0, vr[c][x]);
+          }
+        }
+
+        // Scores, in units of row_scale: the middles' product first, then the groups'.
+        float s[kSub][NT][4];
+#pragma unroll
+        for (int c = 0; c < kSub; ++c)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t a0 = km[c][0], a1 = km[c][1];
+            mma_bf16_from_zero(s[c][nt], a0, a1, G == 4 ? a0 : 0u, G == 4 ? a1 : 0u, qm[nt][0], qm[nt][1]);
+          }
+#pragma unroll
+        for (int y = 0; y < G; ++y)
+#pragma unroll
+          for (int c = 0; c < kSub; ++c) {
+            uint32_t code[2][4];  // [token][elements 8t + i, 8t + i + 4 of the group]
+            float step[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint32_t w =
+                  G == 1 ? kr[c][x][0] : __byte_perm(kr[c][x][y / 2], kr[c][x][G / 2 + y / 2], y % 2 ? 0x7632u : 0x5410u);
+              code[x][0] = and_or(w, low4, 0x64006400u);  // 1024 + code
+              code[x][1] = and_or(w, high4, 0x54005400u);  // 64 + code
+              code[x][2] = and_or(w >> 8, low4, 0x64006400u);
+              code[x][3] = and_or(w >> 8, high4, 0x54005400u);
+              step[x] = __uint_as_float(y % 2 ? kp[c][x][y / 2] & 0xffff0000u : kp[c][x][y / 2] << 16);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint4 q = s_q4[(nt * G + y) * 32 + lane];
+              const float4 base = s_qsum[(nt * G + y) * 4 + t];
+              float acc[4] = {base.x, base.y, base.z, base.w};
+              mma_f16(acc, code[0][0], code[1][0], code[0][1], code[1][1], q.x, q.y);
+              mma_f16(acc, code[0][2], code[1][2], code[0][3], code[1][3], q.z, q.w);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) s[c][nt][x] = fmaf(step[x >> 1], acc[x], s[c][nt][x]);
+            }
+          }
+
+        bool edge = false;
+#pragma unroll
+        for (int c = 0; c < kSub; ++c) edge |= tok[c] + 16 > all_see || (tok[c] < all_from && tok[c] + 16 > p.sinks);
+        if (__builtin_expect(__any_sync(0xffffffffu, edge), 0)) {
+          const int len = all_see + p.q_len - 1;
+          const int from = max(0, len - p.q_len - p.window + 1);
+#pragma unroll
+          for (int c = 0; c < kSub; ++c) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const int j = tok[c] + g + 8 * (x >> 1);
+                const int pos = s_limit[8 * nt + 2 * t + (x & 1)];
+                if (j > pos || (p.window > 0 && pos - j >= p.window && j >= p.sinks)) s[c][nt][x] = -INFINITY;
+              }
+            // Parameters of tokens that no row sees may be anything (0 times a NaN is a NaN).
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int j = tok[c] + g + 8 * x;
+              if (j >= len || (p.window > 0 && j < from && j >= p.sinks)) vp[c][x] = 0u;
+            }
+          }
+        }
+
+        float big = 0.f;  // of V's parameters
+        float top[NT][2];
+#pragma unroll
+        for (int c = 0; c < kSub; ++c)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            big = max3f(big, fabsf(__uint_as_float(vp[c][x] << 16)), fabsf(__uint_as_float(vp[c][x] & 0xffff0000u)));
+        bool grew = big > unit;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            top[nt][x] = fmaxf(s[0][nt][x], s[0][nt][x + 2]);
+#pragma unroll
+            for (int c = 1; c < kSub; ++c) top[nt][x] = max3f(top[nt][x], s[c][nt][x], s[c][nt][x + 2]);
+            top[nt][x] *= row_scale[nt][x];
+            grew |= top[nt][x] > m[nt][x] + kCacheRescale;
+          }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+          for (int i = 1; i < 32; i *= 2) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, i));
+          float other = 1.f;
+          if (big > unit) {  // a power of two above it, at most 2^100
+            const int e = min(static_cast<int>(__float_as_uint(big) >> 23) - 126, 100);
+            const float now_unit = exp2_int(e);
+            other = unit * exp2_int(-e);
+            unit = now_unit;
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              float best = top[nt][x];
+              best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
+              best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 8));
+              best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
+              float alpha = 1.f;
+              if (best > m[nt][x]) {
+                alpha = fast_exp2(m[nt][x] - best);  // 0 the first time
+                m[nt][x] = best;
+                l[nt][x] *= alpha;
+              }
+              alpha *= other;
+              om[nt][x] *= alpha;
+#pragma unroll
+              for (int j = 0; j < Cfg::kSteps; ++j) {
+                o[nt][j][x] *= alpha;
+                o[nt][j][x + 2] *= alpha;
+              }
+            }
+        }
+
+        uint32_t pf[kSub][NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float ref0 = m[nt][0] == -INFINITY ? -kCacheHeadroom : m[nt][0] - kCacheHeadroom;
+          const float ref1 = m[nt][1] == -INFINITY ? -kCacheHeadroom : m[nt][1] - kCacheHeadroom;
+#pragma unroll
+          for (int c = 0; c < kSub; ++c) {
+            const float w0 = fast_exp2(fmaf(s[c][nt][0], row_scale[nt][0], -ref0));
+            const float w1 = fast_exp2(fmaf(s[c][nt][1], row_scale[nt][1], -ref1));
+            const float w2 = fast_exp2(fmaf(s[c][nt][2], row_scale[nt][0], -ref0));
+            const float w3 = fast_exp2(fmaf(s[c][nt][3], row_scale[nt][1], -ref1));
+            l[nt][0] += w0 + w2;
+            l[nt][1] += w1 + w3;
+            pf[c][nt][0] = movmatrix_trans(pack_f16x2(w0, w1));
+            pf[c][nt][1] = movmatrix_trans(pack_f16x2(w2, w3));
+          }
+        }
+
+        const float per_unit = __uint_as_float(0x7f000000u - __float_as_uint(unit));  // 1 / unit, a power of two
+#pragma unroll
+        for (int c = 0; c < kSub; ++c) {
+          // The parameters as rows, two tokens to a register; a group's steps go into the weights of its dims.
+          uint32_t v[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            v[x] = movmatrix_trans(pack_f16x2(__uint_as_float(vp[c][x] << 16) * per_unit,
+                                              __uint_as_float(vp[c][x] & 0xffff0000u) * per_unit));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(om[nt], v[0], 0u, v[1], 0u, pf[c][nt][0], pf[c][nt][1]);
+#pragma unroll
+          for (int y = 0; y < G; ++y) {
+            uint32_t w[NT][2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint32_t step = __shfl_sync(0xffffffffu, v[x], 4 * y + t);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) w[nt][x] = f16x2_mul(pf[c][nt][x], step);
+            }
+            const uint32_t sel = y % 2 ? 0x7632u : 0x5410u;
+            uint32_t a[2][4];  // [tokens 2t, 2t+1; 2t+8, 2t+9][dims 4g ... 4g+3 of the group]: codes less 8
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint32_t pair = __byte_perm(vr[c][2 * x][y / 2], vr[c][2 * x + 1][y / 2], sel);
+              a[x][0] = f16x2_add(and_or(pair, low4, 0x64006400u), 0xe408e408u);       // 1024 + code, less 1032
+              a[x][1] = f16x2_add(and_or(pair, high4, 0x54005400u), 0xd480d480u);      // 64 + code, less 72
+              a[x][2] = f16x2_add(and_or(pair >> 8, low4, 0x64006400u), 0xe408e408u);
+              a[x][3] = f16x2_add(and_or(pair >> 8, high4, 0x54005400u), 0xd480d480u);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                mma_f16(o[nt][2 * y + e], a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], w[nt][0], w[nt][1]);
+          }
+        }
+        continue;
+      }
       uint32_t kr[kSub][2][Cfg::kKWords], vr[kSub][4][Cfg::kVWords];
-      uint32_t kp[kSub][2][kInt4 ? G : 1], vp[kSub][2];  // 4 bits: parameters of tokens g and g + 8: all of K's, word t of V's
       float ks[kSub], vs[kSub];
       int tok[kSub];
 #pragma unroll
@@ -603,18 +866,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
         for (int x = 0; x < 2; ++x) KPieces::load(p.c.k + at + (g + 8 * x) * Cfg::kRowBytes, t, kr[c][x]);
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          if constexpr (kInt4 && HD == 32)
-            vr[c][x][0] = load_once_u16(p.c.v + at + (2 * t + (x & 1) + 4 * (x & 2)) * Cfg::kRowBytes + 2 * g);
-          else
-            VPieces::load(p.c.v + at + (2 * t + (x & 1) + 4 * (x & 2)) * Cfg::kRowBytes, g, vr[c][x]);
-        if constexpr (kInt4) {
-          const int64_t prm = group_row(page, now.h, tok[c]);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            RowPieces<G, 1>::load(reinterpret_cast<const uint8_t*>(p.c.k_group) + prm + (g + 8 * x) * (4 * G), 0, kp[c][x]);
-            vp[c][x] = t < G ? load_once(reinterpret_cast<const uint8_t*>(p.c.v_group) + prm + (g + 8 * x) * (4 * G) + 4 * t) : 0u;
-          }
-        }
+          VPieces::load(p.c.v + at + (2 * t + (x & 1) + 4 * (x & 2)) * Cfg::kRowBytes, g, vr[c][x]);
         ks[c] = vs[c] = 1.f;
         if (kFp8) {
           ks[c] = p.c.k_scale[static_cast<int64_t>(page) * kv_heads + now.h];
@@ -628,48 +880,6 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
       for (int c = 0; c < kSub; ++c)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[c][nt][0] = s[c][nt][1] = s[c][nt][2] = s[c][nt][3] = 0.f;
-      if constexpr (kInt4) {
-        // Sum over the groups of middle * sum(q) + step * (sum(q (128 + code)) - 136 sum(q)). The middles are one product: its
-        // 16 columns hold each middle three times, against the three terms of sum(q) (the words of a row's threads t are its
-        // middles 2 (t & 1) and 2 (t & 1) + 1, or 0 and 1, or a step, against 0, and the only middle). 0x43004300 over two
-        // codes makes them 128 + code in bf16, and a group's product begins at -136 sum(q).
-#pragma unroll
-        for (int c = 0; c < kSub; ++c)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const uint32_t a0 = G == 4 ? ((t & 1) != 0 ? kp[c][0][G - 1] : kp[c][0][G - (G > 1 ? 2 : 1)]) : kp[c][0][G - 1];
-            const uint32_t a1 = G == 4 ? ((t & 1) != 0 ? kp[c][1][G - 1] : kp[c][1][G - (G > 1 ? 2 : 1)]) : kp[c][1][G - 1];
-            mma_bf16(s[c][nt], a0, a1, G == 4 ? a0 : 0u, G == 4 ? a1 : 0u, qm[nt][0], qm[nt][1]);
-          }
-#pragma unroll
-        for (int y = 0; y < G; ++y)
-#pragma unroll
-          for (int c = 0; c < kSub; ++c) {
-            uint32_t w[2], code[2][4];
-            float step[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              w[x] = G == 1 ? kr[c][x][0] : __byte_perm(kr[c][x][y / 2], kr[c][x][G / 2 + y / 2], y % 2 ? 0x7632u : 0x5410u);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) code[x][i] = ((w[x] >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-              step[x] = __uint_as_float(y % 2 ? kp[c][x][y / 2] & 0xffff0000u : kp[c][x][y / 2] << 16);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float2 base = make_float2(qsum[nt][y][0], qsum[nt][y][1]);
-              if constexpr (Cfg::kSharedQ) base = s_qsum[(nt * G + y) * 4 + t];
-              float acc[4] = {base.x, base.y, base.x, base.y};
-#pragma unroll
-              for (int st = 0; st < 2; ++st) {
-                uint2 q2 = make_uint2(qf[nt][2 * y + st][0], qf[nt][2 * y + st][1]);
-                if constexpr (Cfg::kSharedQ) q2 = s_q[(nt * Cfg::kSteps + 2 * y + st) * 32 + lane];
-                mma_bf16(acc, code[0][2 * st], code[1][2 * st], code[0][2 * st + 1], code[1][2 * st + 1], q2.x, q2.y);
-              }
-#pragma unroll
-              for (int x = 0; x < 4; ++x) s[c][nt][x] = fmaf(step[x >> 1], acc[x], s[c][nt][x]);
-            }
-          }
-      } else {
 #pragma unroll
       for (int st = 0; st < Cfg::kSteps; ++st)
 #pragma unroll
@@ -693,7 +903,6 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
             cache_mma<kFp8>(s[c][nt], a0, a1, a2, a3, q2.x, q2.y);
           }
         }
-      }
 
       // Tokens g and g + 8 of rows 2t and 2t + 1, in exponents of 2 with V's scale in.
       float inv_v[kSub];
@@ -726,21 +935,13 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
               const int pos = limit[nt][x & 1];
               if (j > pos || (p.window > 0 && pos - j >= p.window && j >= p.sinks)) s[c][nt][x] = -INFINITY;
             }
-          // Values of tokens that no row sees may be anything (0 times a NaN is a NaN); in 4 bits it is their parameters.
-          if constexpr (kInt4) {
+          // Values of tokens that no row sees may be anything (0 times a NaN is a NaN).
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int j = tok[c] + g + 8 * x;
-              if (j >= seq.len || (p.window > 0 && j < from && j >= p.sinks)) vp[c][x] = 0u;
-            }
-          } else {
+          for (int x = 0; x < 4; ++x) {
+            const int j = tok[c] + 2 * t + (x & 1) + 4 * (x & 2);
+            if (j >= seq.len || (p.window > 0 && j < from && j >= p.sinks)) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int j = tok[c] + 2 * t + (x & 1) + 4 * (x & 2);
-              if (j >= seq.len || (p.window > 0 && j < from && j >= p.sinks)) {
-#pragma unroll
-                for (int i2 = 0; i2 < Cfg::kVWords; ++i2) vr[c][x][i2] = 0u;
-              }
+              for (int i2 = 0; i2 < Cfg::kVWords; ++i2) vr[c][x][i2] = 0u;
             }
           }
         }
@@ -770,7 +971,6 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
               const float alpha = fast_exp2(m[nt][x] - best);  // 0 the first time
               m[nt][x] = best;
               l[nt][x] *= alpha;
-              om[nt][x] *= alpha;
 #pragma unroll
               for (int j = 0; j < Cfg::kSteps; ++j) {
                 o[nt][j][x] *= alpha;
@@ -798,36 +998,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
 
 #pragma unroll
       for (int c = 0; c < kSub; ++c) {
-        if constexpr (kInt4) {
-          // The parameters as rows, two tokens to a register; a group's steps go into the weights of its dims.
-          const uint32_t v0 = movmatrix_trans(vp[c][0]), v1 = movmatrix_trans(vp[c][1]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_bf16(om[nt], v0, 0u, v1, 0u, pf[c][nt][0], pf[c][nt][1]);
-#pragma unroll
-          for (int y = 0; y < G; ++y) {
-            const uint32_t step0 = __shfl_sync(0xffffffffu, v0, 4 * y + t), step1 = __shfl_sync(0xffffffffu, v1, 4 * y + t);
-            uint32_t w[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              w[nt][0] = bf16x2_mul(pf[c][nt][0], step0);
-              w[nt][1] = bf16x2_mul(pf[c][nt][1], step1);
-            }
-            const uint32_t sel = y % 2 ? 0x7632u : 0x5410u;
-            const uint32_t lo = __byte_perm(vr[c][0][y / 2], vr[c][1][y / 2], sel);  // tokens 2t, 2t+1 of four dims
-            const uint32_t hi = __byte_perm(vr[c][2][y / 2], vr[c][3][y / 2], sel);  // tokens 2t+8, 2t+9
-            uint32_t a[2][4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              a[0][i] = bf16x2_less_136(((lo >> (4 * i)) & 0x000f000fu) | 0x43004300u);
-              a[1][i] = bf16x2_less_136(((hi >> (4 * i)) & 0x000f000fu) | 0x43004300u);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                mma_bf16(o[nt][2 * y + e], a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], w[nt][0], w[nt][1]);
-          }
-        } else if constexpr (kFp8) {
+        if constexpr (kFp8) {
 #pragma unroll
           for (int i2 = 0; i2 < Cfg::kVWords; ++i2) {
 #pragma unroll
@@ -871,7 +1042,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
           if constexpr (kInt4) {
             const float mid = __shfl_sync(0xffffffffu, om[nt][x], 4 * (G + j / 2) + t);
             *reinterpret_cast<float2*>(dst + r * HD + 32 * (j / 2) + 4 * g + 2 * (j & 1)) =
-                make_float2(o[nt][j][x] + mid, o[nt][j][x + 2] + mid);
+                make_float2((o[nt][j][x] + mid) * unit, (o[nt][j][x + 2] + mid) * unit);
             continue;
           }
           const int d = kFp8 ? VPieces::offset(j / 2, g) + 2 * (j & 1) : VPieces::offset(j, g) / 2;
@@ -884,6 +1055,13 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
       }
     __syncthreads();
 
+    if constexpr (kInt4 && !kWhole) {
+      const volatile int* line = s_line;
+      total = line[0];
+      ctas = line[1];
+      w_begin = line[2];
+      w_end = line[3];
+    }
     const volatile Part& part_now = s_part;
     const int b = part_now.b, h = part_now.h, head_begin = part_now.head_begin, units = part_now.units;
     const int u0 = part_now.u0, u1 = part_now.u1;
