@@ -434,6 +434,13 @@ __global__ void __launch_bounds__(192, 2)
         const int vst = j % kStages;
         const uint32_t v_addr = smem_u32(s_v + vst * kTileBytes);
         const int steps = j == n - 1 ? (last_rows + 15) >> 4 : 8;
+        if constexpr (kPacked) {
+          // One sequence's sinks have no map of their own: what lies between the last one and the next multiple of 16 is
+          // cleared, by this thread (up to 15 rows; in the softmax threads' loop it costs registers on every tile: 148
+          // bytes of spills, packed prompts 282 us).
+          if (keys.sink_rows > p.sinks && j == p.sinks >> 7)
+            window_clear_values<1>(s_v + vst * kTileBytes, p.sinks & 127, keys.sink_rows - 128 * j, 0, 1);
+        }
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
           if (kk < steps)
@@ -603,14 +610,6 @@ __global__ void __launch_bounds__(192, 2)
       if (const int last_rows = s_tiles->rows - 128 * j; last_rows < 128 && (last_rows & 15) != 0) {
         softmax_wait(&v_full[j % kStages], (j / kStages) & 1, 111, alive, abort_flag);
         window_clear_values<1>(s_v + (j % kStages) * kTileBytes, last_rows, 128, threadIdx.x - 64, 128);
-      }
-      if constexpr (kPacked) {
-        // No map of one sequence's sinks: what lies between the last one and the next multiple of 16 is cleared, too.
-        if (s_tiles->sink_rows > p.sinks && j == p.sinks >> 7) {
-          softmax_wait(&v_full[j % kStages], (j / kStages) & 1, 112, alive, abort_flag);
-          window_clear_values<1>(s_v + (j % kStages) * kTileBytes, p.sinks & 127, s_tiles->sink_rows - 128 * j, threadIdx.x - 64,
-                                 128);
-        }
       }
       tc_fence_before_sync();
       __syncwarp();
@@ -949,7 +948,7 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
         }
       }
       if constexpr (decltype(hide)::value) {
-        const bool at_sinks = kPacked && keys.sink_rows > p.sinks && j == p.sinks >> 7;  // as in window_solo_kernel
+        const bool at_sinks = kPacked && keys.sink_rows > p.sinks && j == p.sinks >> 7;  // (as in window_solo_kernel)
         const bool at_end = j == n - 1 && (last_rows & 15) != 0;
         if (at_end || at_sinks) {
           const int st = j % Cfg::kVStages;

@@ -160,8 +160,9 @@ __device__ __forceinline__ uint32_t halves_together(const uint32_t (&w)[G], int 
   return __byte_perm(w[y / 2], w[(G + y) / 2], (y % 2 ? 0x32u : 0x10u) | ((G + y) % 2 ? 0x7600u : 0x5400u));
 }
 
+// (64 registers, four CTAs an SM, up to 4 groups: ragged prompts of 16 heads of 64 69 us, 78 with three.)
 template <int G, bool kInterleaved>
-__global__ void __launch_bounds__(kInt4Threads) cache_append_int4_kernel(const AppendParams p, const int tile_tokens,
+__global__ void __launch_bounds__(kInt4Threads, G <= 4 ? 4 : 2) cache_append_int4_kernel(const AppendParams p, const int tile_tokens,
                                                                          const unsigned role_blocks) {
   const unsigned tile = blockIdx.x / role_blocks;
   const unsigned lane = threadIdx.x & 31;
@@ -351,9 +352,9 @@ __device__ __forceinline__ uint4 int4_values(uint32_t w, uint32_t params) {
 // What is read comes by coherent loads: the launch before this one may be the append that wrote it. G: groups of 4-bit
 // codes; other types take 16 elements to a lane, 8 in each half of the head.
 template <int kType, int G>
-__global__ void __launch_bounds__(kInt4Threads) cache_read_kernel(const ReadParams p, const int tile_tokens,
+__global__ void __launch_bounds__(kInt4Threads, G <= 4 ? 4 : 2) cache_read_kernel(const ReadParams p, const int tile_tokens,
                                                                   const unsigned role_blocks) {
-  constexpr int kAtOnce = 2;  // turns in flight together
+  constexpr int kAtOnce = G <= 4 ? 4 : 2;  // turns in flight together
   const unsigned tile = blockIdx.x / role_blocks;
   const int lane = static_cast<int>(threadIdx.x & 31);
   const int kv_heads = p.c.kv_heads;
