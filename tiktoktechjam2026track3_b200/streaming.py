@@ -7,9 +7,11 @@ one token (or a few) of each sequence at a time:
     stream = StreamingTransformer(model, batch=8, max_tokens=4096, table=rotary_table(4096, 64), window=1024, sinks=4)
     y = stream.prompt(x, lengths)     # [8, S, D]; x's rows past lengths[b] are padding
     y = stream.step(x_next)           # [8, t, D], t new tokens of every sequence
+    y = stream.extend(x_more, counts) # [sum(counts), D], counts[b] more tokens of sequence b, packed without padding
 
 Per block: LayerNorm -> packed QKV GEMM -> KVCache.append (positions rotated, keys and values stored) -> window_attention
-(prompt) or KVCache.attend (step) -> out_proj + residual -> LayerNorm -> FFN + residual, all in libb200tx.so.
+(prompt), KVCache.attend (step) or KVCache.read and packed_attention (extend) -> out_proj + residual -> LayerNorm -> FFN +
+residual, all in libb200tx.so.
 Without a table, a window and 8 bits it computes what the model's own causal forward does.
 """
 
@@ -22,7 +24,7 @@ import torch
 
 from . import _capi
 from .models import UserOptimizedTransformer
-from .serving import CACHE_HEAD_DIMS, KVCache, window_attention
+from .serving import CACHE_HEAD_DIMS, KVCache, packed_attention, window_attention
 
 
 class _Rows:
@@ -50,8 +52,8 @@ class StreamingTransformer:
     """Prompt and step passes of a causal UserOptimizedTransformer over `batch` sequences of up to `max_tokens`.
 
     table, interleaved: rotary positions (`rotary_table`; None: none, as the model's own forward). window, sinks: each
-    token sees the `window` newest tokens and the first `sinks` ones (0: all). dtype: of the cache, float8_e4m3fn
-    or bfloat16. Every pass uses the model's weights as they are: a change since the last one is seen by the parameters'
+    token sees the `window` newest tokens and the first `sinks` ones (0: all). dtype: of the cache, float8_e4m3fn,
+    bfloat16 or uint8 (4-bit codes). Every pass uses the model's weights as they are: a change since the last one is seen by the parameters'
     storage and version, as in the model's own forward. What is in the cache stays as it was computed.
     """
 
@@ -173,6 +175,50 @@ class StreamingTransformer:
         self._status.after_forward(self.device)
         return out
 
+    @torch.no_grad()
+    def extend(self, x: torch.Tensor, lengths: Sequence[int]) -> torch.Tensor:
+        """lengths[b] further tokens of sequence b (0: none), all sequences' rows one after the other without padding: x
+        [sum(lengths), D] bf16 -> the same shape. Chunks of a long prompt, a turn of some conversations, or fresh sequences'
+        prompts. As in `step`, the tokens see keys and values as the cache holds them.
+        """
+        cfg = self.config
+        new = [int(n) for n in lengths]
+        if len(new) != self.batch or min(new) < 0:
+            raise ValueError(f"lengths must be {self.batch} numbers, none negative")
+        if x.dim() != 2 or x.shape[0] != sum(new) or x.shape[1] != cfg.d_model:
+            raise ValueError(f"x must be [{sum(new)}, {cfg.d_model}], got {tuple(x.shape)}")
+        self._check_place(x)
+        held = [p + n if n else 0 for p, n in zip(self.lengths, new)]  # keys of the sequences that go on
+        if max(held) > self.max_tokens:
+            raise ValueError(f"{max(held)} tokens do not fit max_tokens {self.max_tokens}")
+        if not x.shape[0]:
+            return torch.empty_like(x)
+        q_at, kv_at = [0], [0]
+        for n, m in zip(new, held):
+            q_at.append(q_at[-1] + n)
+            kv_at.append(kv_at[-1] + m)
+        sizes = [len(q_at), len(kv_at), self.batch, self.batch, self.batch]
+        q_start, kv_start, count, kv_len, zeros = torch.tensor(
+            q_at + kv_at + new + held + [0] * self.batch, dtype=torch.int32, device=self.device).split(sizes)
+        rows = _Rows(cfg, x.shape[0], self.device)
+        k_rows, v_rows = (torch.empty(kv_at[-1], cfg.d_model, dtype=torch.bfloat16, device=self.device) for _ in range(2))
+
+        def attend(cache: KVCache) -> None:
+            q = rows.qkv[:, :cfg.d_model]
+            cache.append(rows.qkv, cfg.num_heads, q_start[:-1], count, self.past, self.page_table, max(new), table=self.table,
+                         interleaved=self.interleaved, q_out=q if self.table is not None else None)
+            cache.read(kv_start[:-1], kv_len, zeros, self.page_table, max(held), k_out=k_rows, v_out=v_rows)
+            packed_attention(q, k_rows, v_rows, q_start, kv_start, cfg.head_dim, window=self.window, sinks=self.sinks,
+                             out=rows.ctx)
+
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        self._status.check()
+        self._with_weights(lambda: self._pass(x.contiguous(), rows, attend, None, out))
+        self.past.add_(count)
+        self.lengths = [p + n for p, n in zip(self.lengths, new)]
+        self._status.after_forward(self.device)
+        return out
+
     # ------------------------------------------------------------------ inside
     def _with_weights(self, launch: Callable[[], None], undo: Callable[[], object] = lambda: None) -> None:
         """launch() with the model's weights as they are (the packed projections are copies, and graphs hold addresses).
@@ -199,6 +245,9 @@ class StreamingTransformer:
     def _check(self, x: torch.Tensor) -> None:
         if x.dim() != 3 or x.shape[0] != self.batch or x.shape[2] != self.config.d_model or x.shape[1] == 0:
             raise ValueError(f"x must be [{self.batch}, tokens, {self.config.d_model}], got {tuple(x.shape)}")
+        self._check_place(x)
+
+    def _check_place(self, x: torch.Tensor) -> None:
         if x.device != self.device or x.dtype != torch.bfloat16:
             raise RuntimeError(f"StreamingTransformer computes in bfloat16 on the GPU of its weights, {self.device}")
         if torch.cuda.is_current_stream_capturing():
