@@ -89,6 +89,8 @@ struct SeqTiles {
   int len, sink_tiles, first_win, count;
 };
 
+// (In multiples of kAlign, a power of two, so that so many tiles in a row follow one another.)
+template <int kAlign>
 __device__ __forceinline__ SeqTiles seq_tiles(const CacheAttnParams& p, int len) {
   SeqTiles s;
   s.len = len;
@@ -96,8 +98,8 @@ __device__ __forceinline__ SeqTiles seq_tiles(const CacheAttnParams& p, int len)
   s.first_win = 0;
   if (p.window > 0) {
     const int lo = max(0, len - p.q_len - p.window + 1);
-    s.first_win = lo >> 4;
-    s.sink_tiles = min((p.sinks + 15) >> 4, s.first_win);
+    s.first_win = (lo >> 4) & -kAlign;
+    s.sink_tiles = min((((p.sinks + 15) >> 4) + kAlign - 1) & -kAlign, s.first_win);
   }
   s.count = s.sink_tiles + ((len + 15) >> 4) - s.first_win;
   return s;
@@ -160,20 +162,30 @@ __device__ __forceinline__ uint32_t f16x2_add(uint32_t a, uint32_t b) {
   const __half2 r = __hadd2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// d = a b
-__device__ __forceinline__ void mma_bf16_from_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                   uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+// d = a b, 8 columns of a
+__device__ __forceinline__ void mma_bf16_k8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(b), "f"(0.f));
 }
-// (w & mask) | bits is one instruction if one of the two constants is in a register.
-__device__ __forceinline__ uint32_t in_register(uint32_t x) {
+// Whatever a register holds.
+__device__ __forceinline__ uint32_t any_bits() {
   uint32_t r;
-  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(x));
+  asm volatile("" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ float4 load_shared4(const float4* p) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
+  return v;
+}
+__device__ __forceinline__ uint32_t bf16x2_max_abs(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), __habs2(*reinterpret_cast<__nv_bfloat162*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// (w & mask) | bits: one instruction if one of the two constants is in a register.
 __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
@@ -264,8 +276,11 @@ struct CacheAttnCfg {
   static constexpr int kGroups = HD / 32;  // of 4-bit codes
   static constexpr int kSteps = HD / 16;
   // A warp takes kSub tiles of 16 tokens at a time, interleaved: 4 KB of keys and values on their way per warp.
+  // In 4 bits 2, or 4 where the registers allow it (64 sequences of up to 8192 tokens, us with 1, 2, 4 tiles: 16 key heads of
+  // 64 172, 130, 127; 32 of 32 -, 198, 150; 16 rows of 128 199, 174, of 64 117, 96, 132, of 32 101, 71, 83).
   static constexpr int kFill = 128 / (kRowBytes * NT);
-  static constexpr int kSub = kFill > 4 ? 4 : kFill > 1 ? kFill : 1;
+  static constexpr int kSub = kType == kCacheInt4 ? (NT == 2 || HD == 128 ? 2 : 4) : kFill > 1 ? kFill : 1;
+  static constexpr int kAlign = kType == kCacheInt4 ? kSub : 1;  // 4 bits: a warp's tiles of a unit are neighbours
   // Registers decide the warps: the loads' (32, or 64 for 256-byte rows), O's and Q's (6 per row block and 16 dims). 16
   // warps an SM at 128 registers, 12 at 168, 8 at 255; in CTAs of 4, so that one that joins does not idle many (64
   // sequences of up to 8192 tokens: 116 us, 122 in CTAs of 8), or of 6 where 12 is the number.
@@ -296,7 +311,7 @@ struct Part {
 
 template <class Cfg>
 __device__ __forceinline__ int seq_units(const CacheAttnParams& p, int b) {
-  return max(1, (seq_tiles(p, seq_length(p, b)).count + Cfg::kUnitTiles - 1) / Cfg::kUnitTiles);
+  return max(1, (seq_tiles<Cfg::kAlign>(p, seq_length(p, b)).count + Cfg::kUnitTiles - 1) / Cfg::kUnitTiles);
 }
 
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
@@ -333,7 +348,8 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
   const int lane = tid & 31;
   const int g = lane >> 2;
   const int t = lane & 3;
-  const uint32_t low4 = kInt4 ? in_register(0x000f000fu) : 0u, high4 = kInt4 ? in_register(0x00f000f0u) : 0u;
+  __shared__ uint32_t s_mask[2];  // constants that shall stay in registers: one that is known is moved there anew for each use
+  if (kInt4 && tid < 2) s_mask[tid] = tid ? 0x00f000f0u : 0x000f000fu;
   const int kv_heads = p.c.kv_heads;
   const int rows_total = p.q_len * p.group;
   const int row_block = (p.block0 + static_cast<int>(blockIdx.y)) * R;
@@ -394,7 +410,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
     Part x;
     while (s_first[b + 1] <= w) ++b;
     x.b = b;
-    x.seq = seq_tiles(p, seq_length(p, b));
+    x.seq = seq_tiles<Cfg::kAlign>(p, seq_length(p, b));
     x.units = (s_first[b + 1] - s_first[b]) / kv_heads;
     x.h = (w - s_first[b]) / x.units;
     x.head_begin = s_first[b] + x.h * x.units;
@@ -443,7 +459,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
     const int head = static_cast<int>(blockIdx.x) >> ranks_shift;
     now.b = head / kv_heads;
     now.h = head - now.b * kv_heads;
-    now.seq = seq_tiles(p, seq_length(p, now.b));
+    now.seq = seq_tiles<Cfg::kAlign>(p, seq_length(p, now.b));
     now.units = max(1, (now.seq.count + Cfg::kUnitTiles - 1) / Cfg::kUnitTiles);
     now.head_begin = 0;
     now.u0 = static_cast<int>(static_cast<int64_t>(rank) * now.units >> ranks_shift);
@@ -465,7 +481,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
     // Q: fragments of the 8-row operand(s), and the factor of its rows' scores.
     uint32_t qf[NT][Cfg::kSteps][2];  // (in shared memory where registers are short: it is alike for every warp)
     float row_scale[NT][2];
-    uint32_t qm[NT][2];  // 4 bits: what the middles meet
+    uint32_t qm[NT];  // 4 bits: what the middles meet
     int limit[NT][2];  // position of the rows 2t, 2t + 1 of each operand, -1: no such row
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -515,7 +531,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -100), 127);
         const float up = exp2_int(14 - e);
-        uint32_t part[3][G];  // the groups' sums as three bf16 terms each, 24 bits together
+        uint32_t part[2][G];  // the groups' sums as two bf16 terms each, 2^-17 from the sum
 #pragma unroll
         for (int y = 0; y < G; ++y) {
           // Elements i and i + 4 side by side, as the codes' halves hold them.
@@ -539,28 +555,21 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
           if (warp == 0 && g == 0) s_qsum[(nt * G + y) * 4 + t] = make_float4(base0, base1, base0, base1);
           float rest = sum[0] + sum[1];
 #pragma unroll
-          for (int i = 0; i < 3; ++i) {
+          for (int i = 0; i < 2; ++i) {
             const float term = bf16_round(rest);
             part[i][y] = __float_as_uint(term) >> 16;
             rest -= term;
           }
         }
-        // What the threads of a row hold against the words of a token's parameters: see the middles below.
-        uint32_t two[3];
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          if constexpr (G == 4)
-            two[i] = (t & 1) != 0 ? part[i][G / 2] | part[i][G - 1] << 16 : part[i][0] | part[i][G / 4] << 16;
-          else
-            two[i] = G == 2 ? part[i][0] | part[i][G - 1] << 16 : part[i][0] << 16;
-        }
-        if constexpr (G == 4) {
-          qm[nt][0] = t < 2 ? two[0] : two[1];
-          qm[nt][1] = t < 2 ? two[2] : 0u;
-        } else {
-          qm[nt][0] = t == 0 ? two[0] : t == 1 ? two[1] : t == 2 ? two[2] : 0u;
-          qm[nt][1] = 0u;
-        }
+        // What thread t of a row holds against the word of a token's parameters that it has (mid_at): of 4 groups, middles
+        // 2 (t & 1) and 2 (t & 1) + 1; of 2, both; of one, the step, against 0, and the middle. Terms in turn.
+        if constexpr (G == 4)
+          qm[nt] = t < 2 ? (t == 0 ? part[0][0] | part[0][1 % G] << 16 : part[0][G / 2] | part[0][G - 1] << 16)
+                         : (t == 2 ? part[1][0] | part[1][1 % G] << 16 : part[1][G / 2] | part[1][G - 1] << 16);
+        else if constexpr (G == 2)
+          qm[nt] = t == 0 ? part[0][0] | part[0][G - 1] << 16 : t == 1 ? part[1][0] | part[1][G - 1] << 16 : 0u;
+        else
+          qm[nt] = t == 0 ? part[0][0] << 16 : t == 1 ? part[1][0] << 16 : 0u;
         const float down = exp2_int(e - 14) * p.scale_log2;
         row_scale[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);
         row_scale[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
@@ -592,6 +601,8 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
     }
 
     if constexpr (kInt4) __syncthreads();
+    const volatile uint32_t* masks = s_mask;
+    const uint32_t low4 = kInt4 ? masks[0] : 0u, high4 = kInt4 ? masks[1] : 0u;
 
     float o[NT][Cfg::kSteps][4];
     float m[NT][2], l[NT][2];
@@ -627,6 +638,8 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
       group_page = (kv_heads << p.c.page_shift) * (4 * G);
     }
 
+    const bool one_page = (kSub << 4) <= (1 << p.c.page_shift);  // a unit's tiles of a warp lie in one page
+
     // Tokens that every row sees lie below `all_see`, and (with a window) from `all_from` on or below the sinks.
     const int all_see = seq.len - p.q_len + 1;
     const int all_from = p.window > 0 ? max(0, seq.len - p.window) : 0;
@@ -652,17 +665,8 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
         uint32_t kr[kSub][2][Cfg::kKWords], vr[kSub][4][Cfg::kVWords];
         uint32_t kp[kSub][2][G == 4 ? 2 : G], km[kSub][2], vp[kSub][2];  // parameters of tokens g and g + 8: K's steps, words of K's middles and V's
         int tok[kSub];
-#pragma unroll
-        for (int c = 0; c < kSub; ++c) {
-          const int src = (u - ids_from) * kSub + c;
-          tok[c] = __shfl_sync(0xffffffffu, my_tok, src);
-          const int page = __shfl_sync(0xffffffffu, my_page, src);
-          // (a tile that is missing reads page 0, slot 0, whosever it is, and is masked)
-          const int slot = tok[c] & slot_mask;
-          const uint8_t* const k_row = k_at + static_cast<int64_t>(page) * page_bytes + slot * Cfg::kRowBytes;
-          const uint8_t* const v_row = v_at + static_cast<int64_t>(page) * page_bytes + slot * Cfg::kRowBytes;
-          const uint8_t* const kp_row = kp_at + static_cast<int64_t>(page) * group_page + slot * (4 * G);
-          const uint8_t* const vp_row = vp_at + static_cast<int64_t>(page) * group_page + slot * (4 * G);
+        bool edge = false;
+        auto load_tile = [&](int c, const uint8_t* k_row, const uint8_t* v_row, const uint8_t* kp_row, const uint8_t* vp_row) {
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             KPieces::load(k_row + 8 * x * Cfg::kRowBytes, 0, kr[c][x]);
@@ -679,6 +683,38 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
             else
               VPieces::load(row, 0, vr[c][x]);
           }
+        };
+        // (A tile that is missing reads page 0, slot 0, whosever it is, or what lies behind the last token in its page, and is
+        // masked.)
+        if (one_page) {
+          const int src = (u - ids_from) * kSub;
+          tok[0] = __shfl_sync(0xffffffffu, my_tok, src);
+          const int page = __shfl_sync(0xffffffffu, my_page, src);
+          const int slot = tok[0] & slot_mask;
+          const uint8_t* const k_row = k_at + static_cast<int64_t>(page) * page_bytes + slot * Cfg::kRowBytes;
+          const uint8_t* const v_row = v_at + static_cast<int64_t>(page) * page_bytes + slot * Cfg::kRowBytes;
+          const uint8_t* const kp_row = kp_at + static_cast<int64_t>(page) * group_page + slot * (4 * G);
+          const uint8_t* const vp_row = vp_at + static_cast<int64_t>(page) * group_page + slot * (4 * G);
+#pragma unroll
+          for (int c = 0; c < kSub; ++c) {
+            tok[c] = tok[0] + 16 * c;
+            load_tile(c, k_row + 16 * c * Cfg::kRowBytes, v_row + 16 * c * Cfg::kRowBytes, kp_row + 16 * c * (4 * G),
+                      vp_row + 16 * c * (4 * G));
+          }
+          edge = tok[0] + 16 * kSub > all_see || (tok[0] < all_from && tok[0] + 16 * kSub > p.sinks);
+        } else {
+#pragma unroll
+          for (int c = 0; c < kSub; ++c) {
+            const int src = (u - ids_from) * kSub + c;
+            tok[c] = __shfl_sync(0xffffffffu, my_tok, src);
+            const int page = __shfl_sync(0xffffffffu, my_page, src);
+            const int slot = tok[c] & slot_mask;
+            load_tile(c, k_at + static_cast<int64_t>(page) * page_bytes + slot * Cfg::kRowBytes,
+                      v_at + static_cast<int64_t>(page) * page_bytes + slot * Cfg::kRowBytes,
+                      kp_at + static_cast<int64_t>(page) * group_page + slot * (4 * G),
+                      vp_at + static_cast<int64_t>(page) * group_page + slot * (4 * G));
+            edge |= tok[c] + 16 > all_see || (tok[c] < all_from && tok[c] + 16 > p.sinks);
+          }
         }
 
         // Scores, in units of row_scale: the middles' product first, then the groups'.
@@ -687,8 +723,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
         for (int c = 0; c < kSub; ++c)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const uint32_t a0 = km[c][0], a1 = km[c][1];
-            mma_bf16_from_zero(s[c][nt], a0, a1, G == 4 ? a0 : 0u, G == 4 ? a1 : 0u, qm[nt][0], qm[nt][1]);
+            mma_bf16_k8(s[c][nt], km[c][0], km[c][1], qm[nt]);
           }
 #pragma unroll
         for (int y = 0; y < G; ++y)
@@ -709,7 +744,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               const uint4 q = s_q4[(nt * G + y) * 32 + lane];
-              const float4 base = s_qsum[(nt * G + y) * 4 + t];
+              const float4 base = load_shared4(&s_qsum[(nt * G + y) * 4 + t]);  // (each its own: a copy costs four moves)
               float acc[4] = {base.x, base.y, base.z, base.w};
               mma_f16(acc, code[0][0], code[1][0], code[0][1], code[1][1], q.x, q.y);
               mma_f16(acc, code[0][2], code[1][2], code[0][3], code[1][3], q.z, q.w);
@@ -718,9 +753,6 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
             }
           }
 
-        bool edge = false;
-#pragma unroll
-        for (int c = 0; c < kSub; ++c) edge |= tok[c] + 16 > all_see || (tok[c] < all_from && tok[c] + 16 > p.sinks);
         if (__builtin_expect(__any_sync(0xffffffffu, edge), 0)) {
           const int len = all_see + p.q_len - 1;
           const int from = max(0, len - p.q_len - p.window + 1);
@@ -743,13 +775,13 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
           }
         }
 
-        float big = 0.f;  // of V's parameters
+        uint32_t bigs = 0u;  // of V's parameters, two by two
         float top[NT][2];
 #pragma unroll
         for (int c = 0; c < kSub; ++c)
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            big = max3f(big, fabsf(__uint_as_float(vp[c][x] << 16)), fabsf(__uint_as_float(vp[c][x] & 0xffff0000u)));
+          for (int x = 0; x < 2; ++x) bigs = bf16x2_max_abs(bigs, vp[c][x]);
+        float big = fmaxf(__uint_as_float(bigs << 16), __uint_as_float(bigs & 0xffff0000u));
         bool grew = big > unit;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -823,7 +855,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
             v[x] = movmatrix_trans(pack_f16x2(__uint_as_float(vp[c][x] << 16) * per_unit,
                                               __uint_as_float(vp[c][x] & 0xffff0000u) * per_unit));
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16(om[nt], v[0], 0u, v[1], 0u, pf[c][nt][0], pf[c][nt][1]);
+          for (int nt = 0; nt < NT; ++nt) mma_f16(om[nt], v[0], any_bits(), v[1], any_bits(), pf[c][nt][0], pf[c][nt][1]);  // (8 rows)
 #pragma unroll
           for (int y = 0; y < G; ++y) {
             uint32_t w[NT][2];
