@@ -113,6 +113,41 @@ def test_a_group_that_is_not_finite_reaches_the_rows_that_see_it():
     assert not bool(torch.isfinite(cache.attend(q, seqs.table.cuda(), _i32(lengths))).any())
 
 
+@pytest.mark.parametrize("d,heads,kv_heads,page", [(32, 2, 1, 16), (64, 4, 2, 16), (64, 12, 1, 32), (64, 2, 2, 128), (128, 8, 1, 16),
+                                                   (128, 4, 4, 64), (32, 12, 1, 32)])
+@pytest.mark.parametrize("window,sinks,q_len", [(40, 4, 1), (100, 0, 2), (33, 70, 1), (1, 1, 1)])
+@pytest.mark.parametrize("room", [0, 1 << 17])
+def test_pages_that_no_row_sees_need_not_be_there(d, heads, kv_heads, page, window, sinks, q_len, room):
+    """Pages between the sinks and the window given back, as a streaming cache does: -1, or past the cache, in the table."""
+    lengths = [700, 333, 90]
+    cache, seqs = _filled(lengths, page, kv_heads, d, INT4, 9)
+    table = _wide(seqs, page, room) if room else seqs.table.cuda()
+    q = _randn(1, 3 * q_len, heads * d)
+    args = dict(window=window, sinks=sinks, q_len=q_len)
+    want = cache.attend(q, table, _i32(lengths), **args)
+    _check_attend(cache, seqs, lengths, heads, q_len, window, sinks, q, want, d**-0.5)
+    gone = 0
+    for b, n in enumerate(lengths):
+        for i in range(-(-n // page)):
+            if i * page >= sinks and (i + 1) * page <= n - q_len - window + 1:
+                table[b, i] = -1 if i % 2 else cache.pages + 5
+                gone += 1
+    assert gone
+    assert torch.equal(cache.attend(q, table, _i32(lengths), **args), want)
+
+
+def test_attend_with_a_scale_that_hides_nothing():
+    """Scales at the small end, where all weights are alike, and queries of zeros."""
+    lengths, d = [100, 17], 64
+    cache, seqs = _filled(lengths, 16, 1, d, INT4, 3)
+    mean = [_of(_decode(cache, "v"), seqs.table[b], 16, 0, n)[0].mean(0) for b, n in enumerate(lengths)]
+    for q, scale in ((_randn(1, 2, d), 1e-40), (torch.zeros(2, d, dtype=BF16, device="cuda"), 1e-40),
+                     (torch.zeros(2, d, dtype=BF16, device="cuda"), 1.0), (_randn(1, 2, d) * 2.0**-110, 1e-20)):
+        out = cache.attend(q, seqs.table.cuda(), _i32(lengths), scale=scale).cpu().double()
+        for b in range(2):
+            assert bool(((out[b] - mean[b]).abs() <= 2**-8 * mean[b].abs() + 2**-9 * 8).all())
+
+
 # ---------------------------------------------------------------------------------- calls
 @pytest.mark.parametrize("heads,kv_heads,d,q_len", [(16, 1, 64, 5), (40, 2, 128, 27), (12, 1, 32, 47)])
 def test_attend_with_many_row_blocks(heads, kv_heads, d, q_len):

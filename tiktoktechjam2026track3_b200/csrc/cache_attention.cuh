@@ -418,6 +418,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
     x.u1 = min(x.units, w_end - x.head_begin);
     return x;
   };
+  const bool one_page = (kSub << 4) <= (1 << p.c.page_shift);  // 4 bits: a unit's tiles of a warp lie in one page
   // Lane l: the first token (kNoTile: none) and the page of this warp's tile l % kSub in unit ids_from + l / kSub.
   int my_tok = kNoTile, my_page = 0, ids_from = 0;
   auto read_ids = [&](const Part& x, int u) {
@@ -427,6 +428,15 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
     my_page = 0;
     if (i < x.seq.count) {
       my_tok = 16 * (i < x.seq.sink_tiles ? i : i - x.seq.sink_tiles + x.seq.first_win);
+      if (Cfg::kAlign > 1 && p.window > 0) {
+        // Tiles (of one page) that are there only to fill a unit: no row sees them, and nobody need own their page.
+        const int span = one_page ? 16 * kSub : 16;
+        const int at = my_tok & -span;
+        if (at >= p.sinks && at + span <= x.seq.len - p.q_len - p.window + 1) {
+          my_tok = kNoTile;
+          return;
+        }
+      }
       my_page = p.page_table[x.b * p.ld_table + (my_tok >> p.c.page_shift)];
       if (my_page < 0 || my_page >= p.c.pages) {
         record_status(kKernelCacheAttention, 2, kReasonBadIndex);
@@ -570,7 +580,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
           qm[nt] = t == 0 ? part[0][0] | part[0][G - 1] << 16 : t == 1 ? part[1][0] | part[1][G - 1] << 16 : 0u;
         else
           qm[nt] = t == 0 ? part[0][0] << 16 : t == 1 ? part[1][0] << 16 : 0u;
-        const float down = exp2_int(e - 14) * p.scale_log2;
+        const float down = fmaxf(exp2_int(e - 14) * p.scale_log2, 0x1p-126f);  // (0 would make a NaN of a hidden score)
         row_scale[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);
         row_scale[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
       } else {
@@ -638,8 +648,6 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
       group_page = (kv_heads << p.c.page_shift) * (4 * G);
     }
 
-    const bool one_page = (kSub << 4) <= (1 << p.c.page_shift);  // a unit's tiles of a warp lie in one page
-
     // Tokens that every row sees lie below `all_see`, and (with a window) from `all_from` on or below the sinks.
     const int all_see = seq.len - p.q_len + 1;
     const int all_from = p.window > 0 ? max(0, seq.len - p.window) : 0;
@@ -652,6 +660,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
           const volatile Part& at = s_part;
           Part x;
           x.b = at.b;
+          x.seq.len = at.seq.len;
           x.seq.count = at.seq.count;
           x.seq.sink_tiles = at.seq.sink_tiles;
           x.seq.first_win = at.seq.first_win;
