@@ -572,6 +572,7 @@ def _launch(entry: str, layout: struct.Struct, device: int, *members) -> None:
         _check(status, entry)
 
 
+# (What follows asks a tensor for its shape once: size(i) parses arguments, which takes three times as long.)
 def _rows(t: torch.Tensor, name: str, device: int) -> int:
     """Row stride of a bf16 matrix on `device` whose rows are contiguous (a column slice of packed rows is one)."""
     stride = t.stride()
@@ -582,17 +583,19 @@ def _rows(t: torch.Tensor, name: str, device: int) -> int:
             raise ValueError(f"{name} must be {torch.bfloat16}, got {t.dtype}")
         raise ValueError(f"{name} must be 2-D with contiguous rows")
     # A single row's stride may be anything: its length takes the place.
-    return stride[0] if t.size(0) > 1 else (t.size(1) + 7) // 8 * 8
+    rows, width = t.shape
+    return stride[0] if rows > 1 else (width + 7) // 8 * 8
 
 
 def _table(t: torch.Tensor, device: int) -> Tuple[int, int]:
     """(positions, rotary_dim) of a rotary table [positions, rotary_dim / 2, 2]."""
-    if t.dim() != 3 or t.size(2) != 2:
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != 2:
         raise ValueError("table must be [positions, rotary_dim / 2, 2]")
     if t.get_device() != device:
         raise _elsewhere(t, "table", device)
     _require(t, torch.float32, "table")
-    return t.size(0), 2 * t.size(1)
+    return shape[0], 2 * shape[1]
 
 
 def _indices(t: torch.Tensor, n: int, name: str, device: int) -> int:
@@ -608,13 +611,14 @@ def _indices(t: torch.Tensor, n: int, name: str, device: int) -> int:
 
 def _page_table(t: torch.Tensor, batch: int, device: int) -> Tuple[int, int]:
     """(pointer, pages per sequence) of an int32 page table."""
-    if t.dim() != 2 or t.size(0) != batch:
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != batch:
         raise ValueError(f"page_table must be [{batch}, pages], got {tuple(t.shape)}")
     if t.get_device() != device:
         raise _elsewhere(t, "page_table", device)
     if t.dtype is not _INT32 or not t.is_contiguous():
         _require(t, _INT32, "page_table")
-    return t.data_ptr(), t.size(1)
+    return t.data_ptr(), shape[1]
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, head_dim: int, out: torch.Tensor,
@@ -622,8 +626,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, head_d
     """out = the rows of x with every head turned by its row's position (see b2_rotary_fwd)."""
     device = x.get_device()
     ld_x, ld_out = _rows(x, "x", device), _rows(out, "out", device)
-    tokens, width = x.size(0), x.size(1)
-    if head_dim < 1 or width % head_dim or out.size(0) != tokens or out.size(1) != width:
+    tokens, width = shape = x.shape
+    if head_dim < 1 or width % head_dim or out.shape != shape:
         raise ValueError(f"x and out must both be [tokens, heads * {head_dim}]")
     most, rotary_dim = _table(table, device)
     _launch(
@@ -639,7 +643,7 @@ def cache_append(cache: KVCacheDesc, qkv: torch.Tensor, num_heads: int, q_col: i
     """Stores (and with `table` rotates) the new tokens of packed rows qkv (see b2_cache_append_fwd)."""
     device = cache.device
     ld = _rows(qkv, "qkv", device)
-    batch, tokens = new_len.numel(), qkv.size(0)
+    batch, tokens = new_len.numel(), qkv.shape[0]
     pages, table_pages = _page_table(page_table, batch, device)
     positions = rotary_dim = ld_q = ld_k = 0
     if table is not None:
@@ -648,11 +652,11 @@ def cache_append(cache: KVCacheDesc, qkv: torch.Tensor, num_heads: int, q_col: i
             raise ValueError("a rotation needs q_out")
     if q_out is not None:
         ld_q = _rows(q_out, "q_out", device)
-        if table is None or q_out.size(0) != tokens or q_out.size(1) != num_heads * cache.head_dim:
+        if table is None or q_out.shape != (tokens, num_heads * cache.head_dim):
             raise ValueError("q_out needs a table and the shape [tokens, num_heads * head_dim]")
     if k_out is not None:
         ld_k = _rows(k_out, "k_out", device)
-        if k_out.size(0) != tokens or k_out.size(1) != cache.kv_heads * cache.head_dim:
+        if k_out.shape != (tokens, cache.kv_heads * cache.head_dim):
             raise ValueError("k_out must be [tokens, kv_heads * head_dim]")
     _launch(
         "b2_cache_append_fwd", CACHE_APPEND_ARGS, device, ctypes.addressof(cache), qkv.data_ptr(), ld, q_col, k_col,
@@ -674,9 +678,10 @@ def cache_read(cache: KVCacheDesc, out_start: torch.Tensor, length: torch.Tensor
     for i, (t, name) in enumerate(((k_out, "k_out"), (v_out, "v_out"))):
         if t is not None:
             strides[i] = _rows(t, name, device)
-            if t.size(1) != width or (rows >= 0 and t.size(0) != rows):
+            n, w = t.shape
+            if w != width or (rows >= 0 and n != rows):
                 raise ValueError(f"k_out and v_out must be [rows, {width}], alike")
-            rows = t.size(0)
+            rows = n
     _launch(
         "b2_cache_read_fwd", CACHE_READ_ARGS, device, ctypes.addressof(cache), _indices(out_start, batch, "out_start", device),
         _indices(length, batch, "length", device), _indices(start, batch, "start", device), batch, pages, table_pages, max_len,
@@ -699,13 +704,13 @@ def cache_attention(cache: KVCacheDesc, q: torch.Tensor, q_len: int, page_table:
     ld_q, ld_out = _rows(q, "q", device), _rows(out, "out", device)
     if workspace.get_device() != device:
         raise _elsewhere(workspace, "workspace", device)
-    rows, width = q.size(0), q.size(1)
+    rows, width = shape = q.shape
     batch = kv_len.numel()
     pages, table_pages = _page_table(page_table, batch, device)
     if rows != batch * q_len:
         raise ValueError("q needs q_len rows and kv_len an entry per sequence")
     head_dim = cache.head_dim
-    if width % head_dim or out.size(0) != rows or out.size(1) != width:
+    if width % head_dim or out.shape != shape:
         raise ValueError("q and out must both be [batch * q_len, heads * head_dim]")
     _launch(
         "b2_cache_attention_fwd", CACHE_ATTENTION_ARGS, device, ctypes.addressof(cache), q.data_ptr(), ld_q, batch, q_len,
@@ -719,9 +724,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: i
     device = q.get_device()
     ld_q, ld_k = _rows(q, "q", device), _rows(k, "k", device)
     ld_v, ld_out = _rows(v, "v", device), _rows(out, "out", device)
-    rows, width, k_width = q.size(0), q.size(1), k.size(1)
-    if (rows != batch * seq_len or k.size(0) != rows or v.size(0) != rows or out.size(0) != rows or v.size(1) != k_width
-            or out.size(1) != width):
+    rows, width = shape = q.shape
+    k_rows, k_width = k_shape = k.shape
+    if rows != batch * seq_len or k_rows != rows or v.shape != k_shape or out.shape != shape:
         raise ValueError("q, k, v and out must have batch * seq_len rows, k and v alike, out like q")
     if head_dim < 1 or width % head_dim or k_width % head_dim:
         raise ValueError(f"q and k must be whole heads of {head_dim}")
@@ -737,8 +742,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start:
     device = q.get_device()
     ld_q, ld_k = _rows(q, "q", device), _rows(k, "k", device)
     ld_v, ld_out = _rows(v, "v", device), _rows(out, "out", device)
-    rows, width, k_width = q.size(0), q.size(1), k.size(1)
-    if out.size(0) != rows or out.size(1) != width or v.size(0) != k.size(0) or v.size(1) != k_width:
+    rows, width = shape = q.shape
+    k_rows, k_width = k_shape = k.shape
+    if out.shape != shape or v.shape != k_shape:
         raise ValueError("out must be like q, and v like k")
     if head_dim < 1 or width % head_dim or k_width % head_dim:
         raise ValueError(f"q and k must be whole heads of {head_dim}")
@@ -747,5 +753,5 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start:
         raise ValueError("q_start must have an entry for every sequence and one behind the last")
     _launch(
         "b2_packed_attention_fwd", PACKED_ATTENTION_ARGS, device, q.data_ptr(), ld_q, rows, k.data_ptr(), ld_k, v.data_ptr(),
-        ld_v, k.size(0), _indices(q_start, batch + 1, "q_start", device), _indices(kv_start, batch + 1, "kv_start", device),
+        ld_v, k_rows, _indices(q_start, batch + 1, "q_start", device), _indices(kv_start, batch + 1, "kv_start", device),
         batch, width // head_dim, k_width // head_dim, head_dim, window, sinks, scale, out.data_ptr(), ld_out)

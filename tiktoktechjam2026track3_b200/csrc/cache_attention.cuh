@@ -29,6 +29,29 @@
 // page's scale of V loses bits from 2^21 below the largest on and is dropped from 2^32 on, even in dims where the page with the
 // large scale holds zeros.
 //
+// 4-bit pages (cache_int4.cuh): v = mid + (code - 8) step, a step and a middle for 32 dims of a token. What bounds them is
+// no longer HBM but the instructions that a code costs (343 for 16 tokens of 128 dims and up to 8 rows; ALU 50 % and issue 52
+// % busy, DRAM at 0.6 of the copy rate; with every load from L2 the time falls by a tenth only), so each is chosen for their
+// number:
+//   - a code becomes 1024 + code, or 64 + code, in fp16 by one instruction, (bits & mask) | constant, two at a time and without a
+//     shift for half of them. For K the excess leaves with the products' start, -1032 sum(q) (72 for the odd dims), Q in
+//     fp16 as over 8 bits (a sum of 1032 |q| in fp32 loses 2^-13 of |q|, which is nothing next to a code's half step). For V it
+//     is subtracted exactly.
+//   - K's steps multiply the products of their 32 dims; its middles meet the sums of Q over the groups, in two bf16 terms, in one
+//     product of 8 columns.
+//   - V's steps multiply the weights, per group: w step in fp16, 2^-11 of itself once more. Its middles are summed by a product
+//     whose rows are the parameters (a movmatrix brings them there), with the same fp16 weights, so that a weight's
+//     rounding does not part a value from its middle. (Weights times steps in bf16, and bf16 codes: 0.0034 of the norm from 64 bits,
+//     most of it because w (v - mid) and w mid were rounded apart; now 0.0017, the output's own rounding.) The parameters
+//     count in a power of two above all of them so far, which grows as the maximum of the scores does; what is 2^32 below the
+//     largest weight times parameter counts as zero.
+//   - the tiles that a warp takes at once are neighbours in one page (where a page has as many tokens): one address for all.
+// Measured, us (floor; 8-bit codes of the same tokens): 8 x 131072 tokens, 8 key heads of 128, 4 query heads each 296 (208;
+// 331); 64 sequences of up to 8192 106 (63; 115), 16 key heads of 64 127 (63; 180), 32 windows of 4096, 10 rows, 40 (13; 37).
+// Codes as e4m3, whose bits a code is in 2^-9ths, need no excess, but the product of that type is made of conversions and fp16
+// products here: 411 for the first. Prefetching into L2 costs what it saves: a bulk prefetch is a loop over the lanes
+// (380), lines by their lanes 342 where 347 without.
+//
 // Split: a (sequence, key head) is cut into units of 16 tokens per warp. Calls of moderate length give each to one CTA,
 // or to a cluster of CTAs that share its units and join their maxima, sums and outputs through shared memory. Else all
 // units of the call are laid on one line and the CTAs take equal stretches of it, so that one long sequence among short

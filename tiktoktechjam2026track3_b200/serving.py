@@ -210,7 +210,7 @@ class KVCache:
         qkv's own columns. max_new (host) is at least every new_len.
         """
         d, hk = self.head_dim, self.kv_heads
-        if qkv.size(-1) != (num_heads + 2 * hk) * d:
+        if qkv.shape[-1] != (num_heads + 2 * hk) * d:
             raise ValueError(f"qkv must be [tokens, {(num_heads + 2 * hk) * d}], got {tuple(qkv.shape)}")
         if table is not None and q_out is None:
             q_out = torch.empty(qkv.shape[0], num_heads * d, dtype=qkv.dtype, device=qkv.device)
@@ -258,17 +258,18 @@ class KVCache:
         """The current stream's workspace, kept between calls (those of one stream run one after the other) and made
         anew when a call is larger than all before it. A call that is being captured gets one of its own: its memory
         and its zeroing are part of the graph, which may run next to the stream's other calls and outlive the kept one."""
-        if q_len < 1 or q.dim() != 2:
+        shape = q.shape
+        if q_len < 1 or len(shape) != 2:
             raise ValueError("q must be [batch * q_len, heads * head_dim], q_len at least 1")
         device = self._desc.device
         if _capi._current_device() != device:  # the streams meant are those of the cache's GPU
             with torch.cuda.device(device):
                 return self._workspace(q, q_len)
         if torch.cuda.is_current_stream_capturing():
-            return self.workspace(q.size(0) // q_len, q.size(1) // self.head_dim, q_len)
-        stream, need = _capi._stream_of(device), q.size(1) * q_len
+            return self.workspace(shape[0] // q_len, shape[1] // self.head_dim, q_len)
+        stream, need = _capi._stream_of(device), shape[1] * q_len
         kept = self._workspaces.get(stream)
         if kept is None or need > kept[0]:
-            kept = need, self.workspace(q.size(0) // q_len, q.size(1) // self.head_dim, q_len)
+            kept = need, self.workspace(shape[0] // q_len, shape[1] // self.head_dim, q_len)
             self._workspaces[stream] = kept
         return kept[1]
