@@ -9,7 +9,9 @@ the middle's own rounding.
 Attention: with steps s and middles m of a token's groups, a weight is rounded to fp16 (2^-11 of itself), its product with a
 step again, and a step or a middle loses at most 2^-25 of a power of two up to twice the largest parameter; the output is bf16. A
 score's fp32 sums begin at -1032 sum(q) (72 for half of the elements) and add q (1024 + code): 34 terms of at most 2071 |q|, off by
-2^-23 each in the worst case, and over middle * q. That worst case is far from what happens (the terms' errors are not alike),
+2^-23 each in the worst case. A middle meets the sum of q over its group in two bf16 terms: the first is off by half a step, 2^-8
+of the sum's power of two, the second by 2^-8 of that one's, 2^-9 at most: 2^-17, or 64 * 2^-23, of sum |q| besides the 20
+fp32 sums. That worst case is far from what happens (the terms' errors are not alike),
 so the whole output is also held to 2^-8 of its norm, twice what its own rounding may take.
 """
 
@@ -336,7 +338,7 @@ def _check_attend(cache, seqs, lengths, heads, q_len, window, sinks, q, out, sca
             mid_ref, mid_sum, _ = oracle.attend(x, k[g], vm[g], seen, scale)
             part_sum = oracle.attend(x, k[g], v[g] - vm[g], seen, scale)[1]
             share = x.abs().view(q_len, d // 32, 32).sum(-1)
-            off = scale * 2**-23 * (34 * 2071 * share @ ks[g].T + 20 * share @ km[g].T)
+            off = scale * 2**-23 * (34 * 2071 * share @ ks[g].T + (20 + 64) * share @ km[g].T)
             off = torch.where(used, off, 0.0).amax(-1, keepdim=True) if n else torch.zeros(q_len, 1, dtype=torch.float64)
             _close(got[b, :, h], ref, 2**-8 * ref.abs() + 2**-10 * part_sum + 2**-11 * mid_sum + (2.1 * off + 2**-18) * absum
                    + 2**-20 * params["v"][seqs.table[b, :-(-n // page)].long()].nan_to_num().abs().max() if n else 0 * ref)

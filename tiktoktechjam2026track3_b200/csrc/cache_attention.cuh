@@ -1470,7 +1470,10 @@ static cudaError_t launch_cache_attention_nt(const CacheAttnParams& p, int64_t r
   //     heads 90.9 / 99.3 (of 8192 165.5 / 164.3), of 128 bf16 heads with 10 rows 51.6 / 64.0;
   //   a third, or in quarters, up to 20: 8 heads of 8000 12.5 / 19.5, of 32000 28.2 / 29.4, of 64000 47 / 39; 256 heads
   //     of 1000 20.8 / 28.0, of 4000 62.6 / 58.7;
-  //   else up to 8: 4 heads of 8000 10.4 / 18.0, of 32000 17.4 / 20.2; 1 of 8000 9.9 / 13.5, of 32000 16.7 / 17.1.
+  //   else up to 8: 4 heads of 8000 10.4 / 18.0, of 32000 17.4 / 20.2; 1 of 8000 9.9 / 13.5, of 32000 16.7 / 17.1;
+  //   4 bits, half as many rounds, each of twice the tokens: 32 heads of 16000 29.3 / 33.7, of 32000
+  //     51.7 / 50.8; 512 of 2000 46.1 / 52.4, of 4096 85.7 / 88.4 (of up to 4096 77.8 / 65.8), of 8192 162.9 / 157.3, windows of
+  //     8192 163.6 / 158.4; 256 of 1000 16.8 / 20.8, of 4000 61.0 / 51.4; 8 of 32000 27.1 / 26.9, of 64000 48.0 / 33.5.
   const int64_t heads = static_cast<int64_t>(p.batch) * p.c.kv_heads * row_blocks;
   const bool sm_each = heads <= sm_count;
   const int64_t round = 16 * (sm_each ? CacheAttnCfg<HD, kType, NT, 1>::kUnitTiles : CacheAttnCfg<HD, kType, NT, 4>::kUnitTiles);
@@ -1488,7 +1491,7 @@ static cudaError_t launch_cache_attention_nt(const CacheAttnParams& p, int64_t r
   const int64_t ctas = heads * cluster;
   const int64_t thirds = 3 * ctas / ((ctas + places - 1) / places * places);
   const int64_t most = thirds >= 2 ? (windowed ? 72 : 32) : thirds == 1 || !sm_each ? 20 : 8;
-  if (tokens <= most * cluster * round) {
+  if (tokens <= most * cluster * round / (kType == kCacheInt4 ? 2 : 1)) {
     if (cluster > 1)
       return launch_cache_attention_cluster<HD, kType, NT>(p, row_blocks, cluster, stream);
     if (sm_each) return launch_cache_attention_t<HD, kType, NT, 1>(p, row_blocks, sm_count, stream);
