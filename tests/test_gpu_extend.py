@@ -176,6 +176,23 @@ def test_packed_prompts_of_fresh_sequences_are_the_models_forward():
     _gate(y, ref.cpu(), 2**-7)
 
 
+@pytest.mark.parametrize("sinks,dtype", [(0, BF16), (5, E4M3), (40, INT4)])
+@torch.inference_mode()
+def test_a_chunk_behind_a_window_reads_what_it_sees(sinks, dtype):
+    """Pages between the sinks and the band of a chunk's first token need not be there: the outputs stay as they are."""
+    model, _ = _model(256, 4)
+    x, more = _randn(8, 430, 256).cuda(), _randn(9, 41, 256).cuda()
+    outs = []
+    for gone in (False, True):
+        stream = StreamingTransformer(model, 2, 480, window=33, sinks=sinks, page_size=16, dtype=dtype)
+        stream.extend(x, [400, 30])
+        if gone:  # the band of token 400 begins at 368; of the other sequence, at 30, everything is seen
+            stream.page_table[0, -(-sinks // 16):368 // 16] = -1
+        outs.append(stream.extend(more, [40, 1]))
+        stream.check_device_status()
+    assert torch.equal(outs[0], outs[1])
+
+
 @torch.no_grad()
 def test_extend_sees_changed_weights_and_any_autograd_mode():
     model, _ = _model(256, 4)

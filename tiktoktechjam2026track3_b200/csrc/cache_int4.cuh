@@ -73,7 +73,7 @@ __device__ __forceinline__ uint32_t bf16x2_fma(uint32_t a, uint32_t b, uint32_t 
 }
 
 // x / 15, rounded to nearest: the quotient by the rounded 1 / 15, and what it leaves, once more. Equal to the division for
-// every x whose remainder does not fall below fp32's normal range (checked over all mantissas; test_serving_host.py).
+// every x whose remainder does not fall below fp32's normal range (checked over all mantissas; test_more_serving_host.py).
 __device__ __forceinline__ float divide_by_15(float x) {
   constexpr float k = 1.f / 15.f;
   const float q = x * k;

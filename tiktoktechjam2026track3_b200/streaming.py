@@ -53,8 +53,8 @@ class StreamingTransformer:
 
     table, interleaved: rotary positions (`rotary_table`; None: none, as the model's own forward). window, sinks: each
     token sees the `window` newest tokens and the first `sinks` ones (0: all). dtype: of the cache, float8_e4m3fn,
-    bfloat16 or uint8 (4-bit codes). Every pass uses the model's weights as they are: a change since the last one is seen by the parameters'
-    storage and version, as in the model's own forward. What is in the cache stays as it was computed.
+    bfloat16 or uint8 (4-bit codes). Every pass uses the model's weights as they are: a change since the last one is seen by
+    the parameters' storage and version, as in the model's own forward. What is in the cache stays as it was computed.
     """
 
     @_plain_tensors
@@ -193,13 +193,23 @@ class StreamingTransformer:
             raise ValueError(f"{max(held)} tokens do not fit max_tokens {self.max_tokens}")
         if not x.shape[0]:
             return torch.empty_like(x)
+        # Behind a window the sinks and the band of the first new token on are read, one after the other: what lies between them
+        # no row sees, and distances within the band stay what they are.
+        cut = [max(0, p + 1 - self.window - self.sinks) if n and self.window else 0 for p, n in zip(self.lengths, new)]
         q_at, kv_at = [0], [0]
-        for n, m in zip(new, held):
+        for n, m, c in zip(new, held, cut):
             q_at.append(q_at[-1] + n)
-            kv_at.append(kv_at[-1] + m)
-        sizes = [len(q_at), len(kv_at), self.batch, self.batch, self.batch]
-        q_start, kv_start, count, kv_len, zeros = torch.tensor(
-            q_at + kv_at + new + held + [0] * self.batch, dtype=torch.int32, device=self.device).split(sizes)
+            kv_at.append(kv_at[-1] + m - c)
+        parts = [(r, m if c == 0 else self.sinks, 0) for r, m, c in zip(kv_at, held, cut)]  # first row, tokens, first token
+        page_table = self.page_table
+        if any(cut):
+            parts += [(r + self.sinks, m - c - self.sinks, c + self.sinks) if c else (0, 0, 0)
+                      for r, m, c in zip(kv_at, held, cut)]
+            page_table = page_table.repeat(2, 1)
+        lists = [q_at, kv_at, new, *map(list, zip(*parts))]
+        q_start, kv_start, count, read_row, read_len, read_from = torch.tensor(
+            sum(lists, []), dtype=torch.int32, device=self.device).split([len(n) for n in lists])
+        most = max(n for _, n, _ in parts)
         rows = _Rows(cfg, x.shape[0], self.device)
         k_rows, v_rows = (torch.empty(kv_at[-1], cfg.d_model, dtype=torch.bfloat16, device=self.device) for _ in range(2))
 
@@ -207,7 +217,7 @@ class StreamingTransformer:
             q = rows.qkv[:, :cfg.d_model]
             cache.append(rows.qkv, cfg.num_heads, q_start[:-1], count, self.past, self.page_table, max(new), table=self.table,
                          interleaved=self.interleaved, q_out=q if self.table is not None else None)
-            cache.read(kv_start[:-1], kv_len, zeros, self.page_table, max(held), k_out=k_rows, v_out=v_rows)
+            cache.read(read_row, read_len, read_from, page_table, most, k_out=k_rows, v_out=v_rows)
             packed_attention(q, k_rows, v_rows, q_start, kv_start, cfg.head_dim, window=self.window, sinks=self.sinks,
                              out=rows.ctx)
 
