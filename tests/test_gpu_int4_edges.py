@@ -10,6 +10,7 @@ import torch
 
 from test_gpu_int4 import BF16, E4M3, INT4, _check_attend, _decode, _filled, _gen, _i32, _of, _Sequences, _starts
 from test_gpu_packed import _check as _check_packed
+from oracle import serving_fp64 as oracle
 from tiktoktechjam2026track3_b200 import _capi, serving
 
 pytestmark = pytest.mark.gpu
@@ -30,6 +31,50 @@ def _wide(seqs, page, room=1 << 17):
 
 def _randn(seed, *shape):
     return torch.randn(*shape, generator=_gen(seed)).bfloat16().cuda()
+
+
+# ---------------------------------------------------------------------------------- codes at the ends of their range
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 256])
+def test_groups_far_from_zero_next_to_others(d):
+    """A middle that is rounded by steps takes codes beyond 0 ... 15 for some groups of a warp's tokens and not for others:
+    each ends where the range does. What is stored is compared bit for bit, as anywhere without a rotation."""
+    kv_heads, n = 3, 61
+    x = torch.randn(n, 2 * kv_heads, d // 32, 32, generator=_gen(d))
+    far = torch.randint(0, 3, (n, 2 * kv_heads, d // 32, 1), generator=_gen(1)) == 0
+    x = (x + far * torch.randn(far.shape, generator=_gen(2)) * 3000).bfloat16().view(n, 2 * kv_heads, d)
+    step, mid = oracle.int4_params(x)
+    by = ((x.double().view(n, 2 * kv_heads, -1, 32).amin(-1) - mid) / step).nan_to_num()
+    assert bool((by < -9).any()) and bool((by > -7).any())  # (codes that would lie below 0, and ranges that begin above it)
+    seqs = _Sequences([n], 16, 3)
+    cache = serving.KVCache.allocate(seqs.pages, kv_heads, d, 16, INT4)
+    qkv = torch.cat([torch.zeros(n, kv_heads * d, dtype=BF16), x.flatten(1)], 1).cuda()
+    cache.append(qkv, kv_heads, _i32([0]), _i32([n]), _i32([0]), seqs.table.cuda(), n)
+    for which, given in (("k", x[:, :kv_heads]), ("v", x[:, kv_heads:])):
+        got = _of(_decode(cache, which), seqs.table[0], 16, 0, n)
+        assert torch.equal(got.transpose(0, 1), oracle.int4(given))
+
+
+@pytest.mark.parametrize("dtype", [INT4, E4M3, BF16])
+@pytest.mark.parametrize("d,rotary_dim,interleaved,heads", [(64, 64, False, 2), (128, 32, True, 4), (96, 96, False, 3)])
+def test_a_table_that_begins_between_two_32_byte_blocks(dtype, d, rotary_dim, interleaved, heads):
+    """Tables need 16-byte alignment only; how they are loaded does not change a result."""
+    table = serving.rotary_table(128, rotary_dim)
+    room = torch.zeros(table.numel() + 4, device="cuda")
+    off = room[4:].view(table.shape)
+    off.copy_(table)
+    assert table.data_ptr() % 32 == 0 and off.data_ptr() % 32 == 16
+    qkv = _randn(4, 50, (heads + 2) * d)
+    seqs = _Sequences([50], 32, 1)
+    outs = []
+    for t in (table, off):
+        cache = serving.KVCache.allocate(seqs.pages, 1, d, 32, dtype)
+        q = cache.append(qkv, heads, _i32([0]), _i32([50]), _i32([0]), seqs.table.cuda(), 50, table=t, interleaved=interleaved)
+        turned = serving.rotary(qkv[:, :heads * d], torch.arange(50, dtype=torch.int32, device="cuda"), t, d,
+                                interleaved=interleaved)
+        assert torch.equal(q, turned)
+        outs.append((q, cache.k.view(torch.uint8), cache.v.view(torch.uint8)))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
 
 
 # ---------------------------------------------------------------------------------- memory

@@ -17,11 +17,12 @@
 // V (in 8 bits the page's maximum is then known before the first code is written, without reading twice; pages with
 // more than 1024 chunks are read twice), or the query heads of one key head, whose rows of the table stay in registers.
 // Measured on one B200 (us a call, floor in brackets): ragged prompts of 16 sequences of up to 2048 tokens, 16 heads of
-// 64, 8-bit pages of 32: 71 (43; 94 with a CTA of 128 threads per head that read its rows twice); 32768 tokens of 16
-// query and 4 key heads of 128: 82 (64; 92); bf16 chunks of three documents 30 (20); one token in each of 64 sequences
-// 3.9, a launch. Issue slots are 55 % busy and the L1 data pipe (the table, 64 bytes a thread) 54 %: more warps do not
-// fit their registers, and going through several heads with the table in registers cost more instructions than it saved.
+// 64, 8-bit pages of 32: 69 (43; 94 with a CTA of 128 threads per head that read its rows twice); 32768 tokens of 16
+// query and 4 key heads of 128: 70 (55; 77 a head at a time); bf16 chunks of three documents 28 (20); one token in each of 64
+// sequences 3.9, a launch. Issue slots are 55 % busy: more warps do not fit their registers, and going through several heads with the table in registers cost more instructions than it saved.
 #pragma once
+#include <type_traits>
+
 #include <cuda_fp16.h>
 
 #include "b2_common.cuh"
@@ -136,30 +137,48 @@ __device__ __forceinline__ void append_queries(const AppendParams& p, int key_he
   const int h0 = key_head * p.group;
   const __nv_bfloat16* rows = p.qkv + row0 * p.ld + p.q_col + h0 * hd;
   __nv_bfloat16* out = p.q_out + row0 * p.ld_q_out + h0 * hd;
-  for (unsigned i = tt; i < items; i += threads) {
-    const unsigned token = i / chunks;
-    const RotaryChunk ch = rotary_chunk<kInterleaved>(i - token * chunks, p.rotary_dim);
-    float c[8], s[8];
-    if (ch.pair0 >= 0)
-      rotary_load_table(p.table + static_cast<int64_t>(pos0 + static_cast<int>(token)) * (p.rotary_dim >> 1) + ch.pair0, c, s);
-    const __nv_bfloat16* x = rows + token * static_cast<int64_t>(ld);
-    __nv_bfloat16* y = out + token * p.ld_q_out;
-#pragma unroll 2
-    for (int g = 0; g < p.group; ++g, x += hd, y += hd) {
-      uint4 ua = *reinterpret_cast<const uint4*>(x + ch.off0);
-      uint4 ub = *reinterpret_cast<const uint4*>(x + ch.off1);
-      if (ch.pair0 >= 0) {
-        float a[8], bb[8];
-        unpack_bf16x8(ua, a);
-        unpack_bf16x8(ub, bb);
-        rotary_apply<kInterleaved>(a, bb, c, s);
-        ua = pack_bf16x8(a);
-        ub = pack_bf16x8(bb);
+  // Two heads' loads before their stores where the heads are even (q_out may be qkv, so the compiler cannot move them): 16 query
+  // heads of 128 on 4 key heads, ragged prompts, 57 -> 51 us, 67 -> 57 over 4 bits; four of them 53 and 54, but the registers
+  // cost 16 heads on 16 key heads more than a tenth.
+  auto turn = [&](auto at_once) {
+    constexpr int kAtOnce = decltype(at_once)::value;
+    for (unsigned i = tt; i < items; i += threads) {
+      const unsigned token = i / chunks;
+      const RotaryChunk ch = rotary_chunk<kInterleaved>(i - token * chunks, p.rotary_dim);
+      float c[8], s[8];
+      if (ch.pair0 >= 0)
+        rotary_load_table(p.table + static_cast<int64_t>(pos0 + static_cast<int>(token)) * (p.rotary_dim >> 1) + ch.pair0, c, s);
+      const __nv_bfloat16* x = rows + token * static_cast<int64_t>(ld);
+      __nv_bfloat16* y = out + token * p.ld_q_out;
+      for (int g = 0; g < p.group; g += kAtOnce) {
+        uint4 ua[kAtOnce], ub[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          ua[k] = *reinterpret_cast<const uint4*>(x + k * hd + ch.off0);
+          ub[k] = *reinterpret_cast<const uint4*>(x + k * hd + ch.off1);
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          if (ch.pair0 >= 0) {
+            float a[8], bb[8];
+            unpack_bf16x8(ua[k], a);
+            unpack_bf16x8(ub[k], bb);
+            rotary_apply<kInterleaved>(a, bb, c, s);
+            ua[k] = pack_bf16x8(a);
+            ub[k] = pack_bf16x8(bb);
+          }
+          *reinterpret_cast<uint4*>(y + k * hd + ch.off0) = ua[k];
+          *reinterpret_cast<uint4*>(y + k * hd + ch.off1) = ub[k];
+        }
+        x += kAtOnce * hd;
+        y += kAtOnce * hd;
       }
-      *reinterpret_cast<uint4*>(y + ch.off0) = ua;
-      *reinterpret_cast<uint4*>(y + ch.off1) = ub;
     }
-  }
+  };
+  if (p.group % 2 == 0)
+    turn(std::integral_constant<int, 2>{});
+  else
+    turn(std::integral_constant<int, 1>{});
 }
 
 constexpr int kAppendMaxThreads = 512;

@@ -23,11 +23,13 @@
 // to a token: a lane holds 8 elements of every group, so that two exchanges find a group's least and most value, the codes
 // and parameters are whole vectors of a lane's own, and where the whole head is turned in halves a pair's elements lie in one
 // lane. (A lane to 8 elements, with exchanges to put words together: prompts' append 138 us, 458 to read 4 x 65536 tokens.)
+// A token's parameters are worked out by one lane a group (for 2 and 4 groups) and handed round, the codes of two elements
+// come from one packed instruction each where there is one (69 -> 62 us with the next rows' loads ahead).
 // Measured on one B200 (us a call, floor at the measured copy rate in brackets): append of ragged prompts of 16 sequences of up to
-// 2048 tokens, 16 heads of 64, rotated queries and keys kept: 69 (40); chunks of three documents, 16 query and 4 key heads of
-// 128, a quarter turned: 18 (8); one token in each of 64 sequences 4, a launch. Reading 4 x 65536 tokens of 8 heads of 128 in 4
-// bits: 221 (218); 16 sequences of up to 4096 tokens of 16 heads of 64 in 8 bits: 50 (43). The append's issue slots are 57 %
-// busy (20 instructions an element for ranges and codes), its warps wait for their rows the rest of the time.
+// 2048 tokens, 16 heads of 64, rotated queries and keys kept: 60 (40); chunks of three documents, 16 query and 4 key heads of
+// 128, a quarter turned: 15 (8); one token in each of 64 sequences 4, a launch. Reading 4 x 65536 tokens of 8 heads of 128 in 4
+// bits: 221 (218); 16 sequences of up to 4096 tokens of 16 heads of 64 in 8 bits: 51 (43). The append's issue slots are 60 to 70
+// % busy and its ALU 60 to 75 (some 18 instructions an element for ranges and codes).
 #pragma once
 #include "b2_common.cuh"
 #include "cache_append.cuh"
@@ -80,35 +82,82 @@ __device__ __forceinline__ float divide_by_15(float x) {
   return fmaf(fmaf(-q, 15.f, x), k, q);
 }
 
-// 8 values of a group, whose other 24 are in the lanes that differ in bits 0 and 1, as codes in 4 bits each; `params`: the
-// group's step and middle as bf16 bits, the step in the lower half.
-__device__ __forceinline__ uint32_t int4_codes(const float (&x)[8], uint32_t& params) {
-  float lo = min3_nan(min3_nan(x[0], x[1], x[2]), x[3], x[4]);
-  float hi = max3_nan(max3_nan(x[0], x[1], x[2]), x[3], x[4]);
-  lo = min_nan(min3_nan(x[5], x[6], x[7]), lo);
-  hi = max_nan(max3_nan(x[5], x[6], x[7]), hi);
-  lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, 1));
-  hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
-  lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, 2));
-  hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, 2));
+// The least and the most value of each group, of 8 values in each of the four lanes that share a token: after it lane t (of
+// the four) holds those of group t (of t % 2 for two groups), or of all groups (`lo`, `hi` per group) otherwise.
+template <int G>
+__device__ __forceinline__ void int4_ranges(const float (&x)[G][8], int t, float (&lo)[G], float (&hi)[G]) {
+#pragma unroll
+  for (int y = 0; y < G; ++y) {
+    lo[y] = min_nan(min3_nan(x[y][5], x[y][6], x[y][7]), min3_nan(min3_nan(x[y][0], x[y][1], x[y][2]), x[y][3], x[y][4]));
+    hi[y] = max_nan(max3_nan(x[y][5], x[y][6], x[y][7]), max3_nan(max3_nan(x[y][0], x[y][1], x[y][2]), x[y][3], x[y][4]));
+  }
+  if constexpr (G == 2 || G == 4) {
+    // Each exchange leaves a lane half of the groups, those whose number agrees with its own in that bit.
+    const bool odd = t & 1;
+#pragma unroll
+    for (int y = 0; y < G; y += 2) {
+      const float lo_mine = odd ? lo[y + 1] : lo[y], hi_mine = odd ? hi[y + 1] : hi[y];
+      lo[y] = min_nan(lo_mine, __shfl_xor_sync(0xffffffffu, odd ? lo[y] : lo[y + 1], 1));
+      hi[y] = max_nan(hi_mine, __shfl_xor_sync(0xffffffffu, odd ? hi[y] : hi[y + 1], 1));
+    }
+    const bool high = G == 4 && (t & 2);
+    const float lo_mine = high ? lo[G - 2] : lo[0], hi_mine = high ? hi[G - 2] : hi[0];
+    lo[0] = min_nan(lo_mine, __shfl_xor_sync(0xffffffffu, high ? lo[0] : lo[G - 2], 2));
+    hi[0] = max_nan(hi_mine, __shfl_xor_sync(0xffffffffu, high ? hi[0] : hi[G - 2], 2));
+  } else {
+#pragma unroll
+    for (int i = 1; i < 4; i *= 2)
+#pragma unroll
+      for (int y = 0; y < G; ++y) {
+        lo[y] = min_nan(lo[y], __shfl_xor_sync(0xffffffffu, lo[y], i));
+        hi[y] = max_nan(hi[y], __shfl_xor_sync(0xffffffffu, hi[y], i));
+      }
+  }
+}
+
+// A group's step and middle as bf16 bits, the step in the lower half; `clamp`: whether a code may need it.
+struct Int4Group {
+  float mid, r;
+  uint32_t params;
+  bool clamp;
+};
+__device__ __forceinline__ Int4Group int4_group(float lo, float hi) {
   const float range = __fsub_rn(hi, lo);  // not finite where a value is not
   float step = bf16_round(divide_by_15(range));
   if (step < kInt4LeastStep) step = 0.f;
-  float mid = bf16_round(__fadd_rn(lo, 8.f * step));
-  if (!is_finite(range)) step = mid = __uint_as_float(0x7fc00000u);
+  Int4Group q;
+  q.mid = bf16_round(__fadd_rn(lo, 8.f * step));
+  if (!is_finite(range)) step = q.mid = __uint_as_float(0x7fc00000u);
   // (1 / step is never within 2^-17 of the middle between two bf16 values, so that an approximate one rounds alike)
-  const float r = step > 0.f ? bf16_round(fast_rcp(step)) : 0.f;
-  params = pack_bf16x2(step, mid);
+  q.r = step > 0.f ? bf16_round(fast_rcp(step)) : 0.f;
+  q.params = pack_bf16x2(step, q.mid);
+  // (Rounded to the nearest whole number they lie in [-8, 7] unless the middle's own rounding is half a step or more: the
+  // products grow with x, so the least and the most value tell.)
+  q.clamp = !(__fmul_rn(__fsub_rn(lo, q.mid), q.r) >= -8.5f && __fmul_rn(__fsub_rn(hi, q.mid), q.r) < 7.5f);
+  return q;
+}
+
+// 8 values of a group as codes in 4 bits each.
+__device__ __forceinline__ uint32_t int4_codes(const float (&x)[8], float mid, float r, bool clamp) {
+  float q[8];  // (each operation rounded by itself, two at a time)
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    asm("{.reg .b64 a, m, s;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 m, {%4, %4};\n\tmov.b64 s, {%5, %5};\n\t"
+        "add.rn.f32x2 a, a, m;\n\tmul.rn.f32x2 a, a, s;\n\tmov.b64 {%0, %1}, a;}"
+        : "=f"(q[i]), "=f"(q[i + 1]) : "f"(x[i]), "f"(x[i + 1]), "f"(-mid), "f"(r));
+  }
+  if (clamp) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = fmaxf(fminf(q[i], 7.f), -8.f);
+  }
   // Adding 1.5 * 2^23 rounds to a whole number (to the even one at a half), 8 more makes it the code in the lowest bits; the
   // words' sum in 16ths, less the constant's, has the codes side by side.
   constexpr float kMagic = 12582912.f + 8.f;
   constexpr uint32_t kOver = 0x4b400000u;
   uint32_t w = 0;
 #pragma unroll
-  for (int i = 7; i >= 0; --i) {
-    const float t = fmaxf(fminf(__fmul_rn(__fsub_rn(x[i], mid), r), 7.f), -8.f);
-    w = w * 16u + (__float_as_uint(__fadd_rn(t, kMagic)) - kOver);
-  }
+  for (int i = 7; i >= 0; --i) w = w * 16u + __float_as_uint(__fadd_rn(q[i], kMagic));
+  w -= kOver * 0x11111111u;
   return w;
 }
 
@@ -165,7 +214,7 @@ __device__ __forceinline__ uint32_t halves_together(const uint32_t (&w)[G], int 
   return __byte_perm(w[y / 2], w[(G + y) / 2], (y % 2 ? 0x32u : 0x10u) | ((G + y) % 2 ? 0x7600u : 0x5400u));
 }
 
-// (64 registers, four CTAs an SM, up to 4 groups: ragged prompts of 16 heads of 64 69 us, 78 with three.)
+// (64 registers, four CTAs an SM, up to 4 groups: ragged prompts of 16 heads of 64 63 us, 70 with three or with five.)
 template <int G, bool kInterleaved>
 __global__ void __launch_bounds__(kInt4Threads, G <= 4 ? 4 : 2) cache_append_int4_kernel(const AppendParams p, const int tile_tokens,
                                                                          const unsigned role_blocks) {
@@ -206,21 +255,29 @@ __global__ void __launch_bounds__(kInt4Threads, G <= 4 ? 4 : 2) cache_append_int
   uint8_t* const codes = (is_v ? p.c.v : p.c.k) + h * p.c.head_stride / 2 + 4 * G * t;
   uint16_t* const prms = is_v ? p.c.v_group : p.c.k_group;
 
-  for (int token0 = 0; token0 < tokens; token0 += 8) {
-    const int token = token0 + static_cast<int>(lane >> 2);
-    const bool real = token < tokens;
-    const __nv_bfloat16* src = x + token * p.ld;
-    const float2* row = p.table + static_cast<int64_t>(pos0 + token) * half;
-    int64_t page = -2;
-    uint4 u[G];
-    if (real) {
+  // Up to 2 groups the next tokens' rows are under way while these are coded (ragged prompts of 16 heads of 64 69 -> 64 us; of 4
+  // groups the registers do not hold both: 16 query and 4 key heads of 128 17.6 -> 18.7).
+  uint4 u[G];
+  int64_t page = -2;
+  auto fetch = [&](int token) {
+    page = -2;
+    if (token < tokens) {
       page = p.page_table[b * p.ld_table + ((pos0 + token) >> shift)];
 #pragma unroll
-      for (int y = 0; y < G; ++y) u[y] = *reinterpret_cast<const uint4*>(src + 32 * y);
+      for (int y = 0; y < G; ++y) u[y] = *reinterpret_cast<const uint4*>(x + token * p.ld + 32 * y);
     } else {
 #pragma unroll
       for (int y = 0; y < G; ++y) u[y] = make_uint4(0, 0, 0, 0);
     }
+  };
+  if constexpr (G <= 2) fetch(static_cast<int>(lane >> 2));
+  for (int token0 = 0; token0 < tokens; token0 += 8) {
+    const int token = token0 + static_cast<int>(lane >> 2);
+    if constexpr (G > 2) fetch(token);
+    const bool real = token < tokens;
+    const __nv_bfloat16* src = x + token * p.ld;
+    const float2* row = p.table + static_cast<int64_t>(pos0 + token) * half;
+    const int64_t my_page = page;
     float f[G][8];
 #pragma unroll
     for (int y = 0; y < G; ++y) unpack_bf16x8(u[y], f[y]);
@@ -258,12 +315,31 @@ __global__ void __launch_bounds__(kInt4Threads, G <= 4 ? 4 : 2) cache_append_int
         }
       }
     }
+    if constexpr (G <= 2) fetch(token + 8);
     __syncwarp();  // every lane has read its pieces: k_out may be the projection's own columns
     uint32_t w[G], params[G], out[G];
+    float lo[G], hi[G];
+    int4_ranges<G>(f, t, lo, hi);
+    if constexpr (G == 2 || G == 4) {
+      const Int4Group mine = int4_group(lo[0], hi[0]);
+      const bool clamp = __any_sync(0xffffffffu, mine.clamp);
 #pragma unroll
-    for (int y = 0; y < G; ++y) w[y] = int4_codes(f[y], params[y]);
+      for (int y = 0; y < G; ++y) {
+        const int from = (lane & 28) + y;
+        params[y] = __shfl_sync(0xffffffffu, mine.params, from);
+        const float r = __shfl_sync(0xffffffffu, mine.r, from);
+        w[y] = int4_codes(f[y], __uint_as_float(params[y] & 0xffff0000u), r, clamp);
+      }
+    } else {
+#pragma unroll
+      for (int y = 0; y < G; ++y) {
+        const Int4Group group = int4_group(lo[y], hi[y]);
+        params[y] = group.params;
+        w[y] = int4_codes(f[y], group.mid, group.r, __any_sync(0xffffffffu, group.clamp));
+      }
+    }
     if (!real) continue;
-    if (page < 0 || page >= p.c.pages) {
+    if (my_page < 0 || my_page >= p.c.pages) {
       record_status(kKernelCacheAppend, 2, kReasonBadIndex);
       continue;
     }
@@ -273,10 +349,10 @@ __global__ void __launch_bounds__(kInt4Threads, G <= 4 ? 4 : 2) cache_append_int
     }
     const int slot = (pos0 + token) & ((1 << shift) - 1);
     halves_apart(w, out);
-    store_words(codes + page * p.c.page_stride / 2 + slot * (hd / 2), out);
+    store_words(codes + my_page * p.c.page_stride / 2 + slot * (hd / 2), out);
     if (t == 0) {
       halves_apart(params, out);
-      store_words(prms + (((page * kv_heads + h) << shift) + slot) * (2 * G), out);
+      store_words(prms + (((my_page * kv_heads + h) << shift) + slot) * (2 * G), out);
     }
   }
 }
