@@ -322,6 +322,45 @@ def test_packed_attention_of_more_sequences_than_a_warp_looks_at_twice():
     _check_packed(q, k, v, out, q_at, kv_at, 2, 1, 32, 0, 0)
 
 
+@pytest.mark.parametrize("batch", [2, 31, 32, 33, 64])
+@pytest.mark.parametrize("heads,kv_heads,d,window,sinks", [(1, 1, 64, 0, 0), (4, 1, 128, 0, 0), (16, 1, 32, 40, 5), (6, 2, 64, 0, 0)])
+def test_packed_attention_of_many_unlike_sequences(batch, heads, kv_heads, d, window, sinks):
+    """Empty ones, chunks behind many keys, more queries than keys: every tile of every sequence has its CTA, whichever way a
+    CTA finds its own, and rows of no sequence stay as they are."""
+    new = [(0, 1, 37, 128, 129, 16, 3)[(5 * b) % 7] for b in range(batch)]
+    held = [max(0, n + (0, 300, -9, 0, 64, 1, -200)[(3 * b + b // 7) % 7]) for b, n in enumerate(new)]
+    q_at, kv_at = [3], [2]
+    for n, m in zip(new, held):
+        q_at.append(q_at[-1] + n)
+        kv_at.append(kv_at[-1] + m)
+    q, k, v = _randn(1, q_at[-1] + 4, heads * d), _randn(2, kv_at[-1] + 1, kv_heads * d), _randn(3, kv_at[-1] + 1, kv_heads * d)
+    out = torch.full_like(q, 9.0)
+    serving.packed_attention(q, k, v, _i32(q_at), _i32(kv_at), d, window=window, sinks=sinks, out=out)
+    _check_packed(q, k, v, out, q_at, kv_at, heads, kv_heads, d, window, sinks)
+    assert bool((out[:3] == 9).all()) and bool((out[q_at[-1]:] == 9).all())
+
+
+@pytest.mark.parametrize("batch", [6, 40])
+def test_sequences_next_to_one_outside_the_rows(batch):
+    """A start beyond the rows spoils the two sequences that it bounds; it is recorded, and the others are as they are alone."""
+    new = [(40, 0, 130, 7, 64)[b % 5] for b in range(batch)]
+    at = _starts(new) + [sum(new)]
+    q, k, v = (_randn(i, at[-1], 64) for i in range(3))
+    bad = list(at)
+    bad[3] = at[-1] + 5
+    want, got = (torch.full_like(q, 9.0) for _ in range(2))
+    serving.packed_attention(q, k, v, _i32(at), _i32(at), 64, out=want)
+    serving.packed_attention(q, k, v, _i32(bad), _i32(at), 64, out=got)
+    torch.cuda.synchronize()
+    assert _capi.device_status(clear=True) & 0xFF == _capi.REASON_BAD_INDEX
+    for b in range(batch):
+        rows = slice(at[b], at[b + 1])
+        if b not in (2, 3):
+            assert torch.equal(got[rows], want[rows])
+        else:
+            assert bool((got[rows] == 9).all())
+
+
 def test_the_largest_strides_and_narrow_slices():
     """Rows far apart: one head of many columns, for keys, values and outputs alike."""
     rows, d, wide = 50, 64, 20_000

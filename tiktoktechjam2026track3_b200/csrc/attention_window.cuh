@@ -35,11 +35,11 @@
 // its rows are found from q_start and kv_start by the CTA itself (the host does not know them), positions count from n_kv -
 // n_q on, and everything else is as above. The tensor maps cover all sequences' rows: what a box brings of a neighbour is hidden
 // like later keys, and cleared among the values.
-// Measured (us; floor): ragged prompts of 24 sequences of up to 2048 tokens, 16 heads of 64: 255 (64), 16 of 2048 tokens 273 where
+// Measured (us; floor): ragged prompts of 24 sequences of up to 2048 tokens, 16 heads of 64: 238 (64), 16 of 2048 tokens 260 where
 // the padded batch's kernel takes 249; four chunks of up to 2048 queries behind 14336 keys, 16 heads of 128 on 4 key heads:
-// 606 (386). The CTAs' order costs most of the difference to equal prompts: by the rows' order, a sequence's longest lists
-// first. Longest first over all sequences would save 7 %, but a CTA that works its place out (a sum over the sequences in a
-// search by halves) loses as much at its start.
+// 606 (386). What bounds the first is the softmax warps' chain: of 3200 to 3600 clocks a tile 1600 are its exponentials (1024 if a
+// warp had its quarter of the unit to itself), 170 the scores' load, 450 the maximum, 600 waits for products, which queue
+// behind the other CTA's.
 #pragma once
 #include <mutex>
 #include <type_traits>
@@ -228,11 +228,59 @@ struct PackedTile {
   int tile, rows;         // and of the tile
 };
 
+// Up to 32 sequences, a lane each: the query tiles of all in the order of their last keys' positions, the longest lists first,
+// and of equal ones by sequence. The position (in tiles) that has fewer than `place` tiles from itself on is found by halves, each a sum
+// over the lanes. A sequence that lies outside the rows has no tiles. False: no tile there.
+__device__ __forceinline__ bool packed_tile_of_few(const WindowParams& p, int place, PackedTile& t) {
+  const int lane = threadIdx.x & 31;
+  const int shift = 7 - p.group_shift;
+  int q0 = 0, k0 = 0, n_q = 0, n_kv = 0;
+  if (lane < p.batch) {
+    q0 = p.q_start[lane];
+    k0 = p.kv_start[lane];
+    const int q1 = p.q_start[lane + 1], k1 = p.kv_start[lane + 1];
+    if (q0 >= 0 && q1 >= q0 && q1 <= p.q_rows && k0 >= 0 && k1 >= k0 && k1 <= p.kv_rows) {
+      n_q = q1 - q0;
+      n_kv = k1 - k0;
+    }
+  }
+  const int tiles = (n_q + (1 << shift) - 1) >> shift;
+  const int begin = (n_kv - n_q) >> shift, end = begin + tiles;  // positions of its tiles
+  if (place >= __reduce_add_sync(0xffffffffu, tiles)) return false;
+  // More than `place` tiles lie from lo on, `before` <= place of them from hi on.
+  int lo = __reduce_min_sync(0xffffffffu, begin), hi = __reduce_max_sync(0xffffffffu, end), before = 0;
+  while (hi - lo > 1) {
+    const int mid = lo + ((hi - lo) >> 1);
+    const int from_mid = __reduce_add_sync(0xffffffffu, min(max(end - mid, 0), tiles));
+    if (from_mid > place) {
+      lo = mid;
+    } else {
+      hi = mid;
+      before = from_mid;
+    }
+  }
+  const bool has = begin <= lo && lo < end;
+  const uint32_t all = __ballot_sync(0xffffffffu, has);
+  const uint32_t mine = __ballot_sync(0xffffffffu, has && __popc(all & ((1u << lane) - 1u)) == place - before);
+  const int from = __ffs(mine) - 1;
+  t.q0 = __shfl_sync(0xffffffffu, q0, from);
+  t.k0 = __shfl_sync(0xffffffffu, k0, from);
+  t.n_q = __shfl_sync(0xffffffffu, n_q, from);
+  t.n_kv = __shfl_sync(0xffffffffu, n_kv, from);
+  t.tile = lo - __shfl_sync(0xffffffffu, begin, from);
+  t.rows = min(1 << shift, t.n_q - (t.tile << shift));
+  return true;
+}
+
 // Sequence b has places q_start[b] / tokens + b ... on the line of all query tiles: at least as many as it has tiles, since the
 // next one's first place lies a whole tile further than its rows do. A warp finds the sequence of a place in one turn for
 // every factor of 32 of the batch. False: no tile there (up to one place a sequence), or a sequence that lies outside
 // the rows.
 __device__ __forceinline__ bool packed_tile(const WindowParams& p, int place, PackedTile& t) {
+  // By the rows' order the last sequence's longest lists begin when little else is left to run beside them: ragged prompts of 24
+  // sequences 255 us, 238 longest first. Not where a head's tiles come before the next head's (four chunks behind 14336 keys 593,
+  // 601 longest first: a sequence's tiles share its keys in L2).
+  if (p.batch <= 32 && !p.head_major) return packed_tile_of_few(p, p.tiles - 1 - place, t);
   const int lane = threadIdx.x & 31;
   const int shift = 7 - p.group_shift;
   int lo = 0, n = p.batch, first = 0;
