@@ -35,7 +35,7 @@
 // its rows are found from q_start and kv_start by the CTA itself (the host does not know them), positions count from n_kv -
 // n_q on, and everything else is as above. The tensor maps cover all sequences' rows: what a box brings of a neighbour is hidden
 // like later keys, and cleared among the values.
-// Measured (us; floor): ragged prompts of 24 sequences of up to 2048 tokens, 16 heads of 64: 238 (64), 16 of 2048 tokens 260 where
+// Measured (us; floor): ragged prompts of 24 sequences of up to 2048 tokens, 16 heads of 64: 244 (64), 16 of 2048 tokens 265 where
 // the padded batch's kernel takes 249; four chunks of up to 2048 queries behind 14336 keys, 16 heads of 128 on 4 key heads:
 // 606 (386). What bounds the first is the softmax warps' chain: of 3200 to 3600 clocks a tile 1600 are its exponentials (1024 if a
 // warp had its quarter of the unit to itself), 170 the scores' load, 450 the maximum, 600 waits for products, which queue
@@ -64,6 +64,7 @@ struct WindowParams {
   const int32_t* q_start;
   const int32_t* kv_start;
   int batch, q_rows, kv_rows;
+  int side_by_side;  // sequences whose tiles are taken together, a power of two up to 32
 };
 
 // Keys and values [B][S][kv_heads][head_dim] in boxes of 64 columns and 128 or 16 rows; Q in boxes of a query tile.
@@ -228,89 +229,75 @@ struct PackedTile {
   int tile, rows;         // and of the tile
 };
 
-// Up to 32 sequences, a lane each: the query tiles of all in the order of their last keys' positions, the longest lists first,
-// and of equal ones by sequence. The position (in tiles) that has fewer than `place` tiles from itself on is found by halves, each a sum
-// over the lanes. A sequence that lies outside the rows has no tiles. False: no tile there.
-__device__ __forceinline__ bool packed_tile_of_few(const WindowParams& p, int place, PackedTile& t) {
+// Sequence b has places q_start[b] / tokens + b ... on the line of all query tiles: at least as many as it has tiles, since the
+// next one's first place lies a whole tile further than its rows do. A warp finds the sequence of a place in one turn for
+// every factor of 32 of the batch; in the last turn its lanes hold the rows of 32 neighbours. Of these, groups of side_by_side (a
+// power of two) share their places: the tiles of a group are taken in the order of their last keys' positions, the longest
+// lists first. The position (in tiles) at which a place's tile ends is found by halves, each a sum over the lanes. False: no tile
+// there (up to one place a sequence), or a sequence that lies outside the rows.
+__device__ __forceinline__ bool packed_tile(const WindowParams& p, int place, PackedTile& t) {
   const int lane = threadIdx.x & 31;
   const int shift = 7 - p.group_shift;
-  int q0 = 0, k0 = 0, n_q = 0, n_kv = 0;
-  if (lane < p.batch) {
-    q0 = p.q_start[lane];
-    k0 = p.kv_start[lane];
-    const int q1 = p.q_start[lane + 1], k1 = p.kv_start[lane + 1];
-    if (q0 >= 0 && q1 >= q0 && q1 <= p.q_rows && k0 >= 0 && k1 >= k0 && k1 <= p.kv_rows) {
+  int s0 = 0, step = 1;
+  while (step * 32 < p.batch) step *= 32;
+  for (; step > 1; step /= 32) {
+    const int b = s0 + lane * step;
+    const uint32_t seen = __ballot_sync(0xffffffffu, b < p.batch && (p.q_start[b] >> shift) + b <= place);
+    if (seen == 0) return false;
+    s0 += (31 - __clz(seen)) * step;
+  }
+  const int b = s0 + lane;
+  int q0 = 0, k0 = 0, n_q = 0, n_kv = 0, at = 0x7fffffff;
+  bool bad = false;
+  if (b < p.batch) {
+    q0 = p.q_start[b];
+    k0 = p.kv_start[b];
+    const int q1 = p.q_start[b + 1], k1 = p.kv_start[b + 1];
+    at = (q0 >> shift) + b;
+    bad = q0 < 0 || q1 < q0 || q1 > p.q_rows || k0 < 0 || k1 < k0 || k1 > p.kv_rows;
+    if (!bad) {
       n_q = q1 - q0;
       n_kv = k1 - k0;
     }
   }
+  const uint32_t seen = __ballot_sync(0xffffffffu, at <= place);
+  if (seen == 0) return false;
+  int from = 31 - __clz(seen);  // the place's sequence
   const int tiles = (n_q + (1 << shift) - 1) >> shift;
-  const int begin = (n_kv - n_q) >> shift, end = begin + tiles;  // positions of its tiles
-  if (place >= __reduce_add_sync(0xffffffffu, tiles)) return false;
-  // More than `place` tiles lie from lo on, `before` <= place of them from hi on.
-  int lo = __reduce_min_sync(0xffffffffu, begin), hi = __reduce_max_sync(0xffffffffu, end), before = 0;
-  while (hi - lo > 1) {
-    const int mid = lo + ((hi - lo) >> 1);
-    const int from_mid = __reduce_add_sync(0xffffffffu, min(max(end - mid, 0), tiles));
-    if (from_mid > place) {
-      lo = mid;
-    } else {
-      hi = mid;
-      before = from_mid;
+  const int head = from & -p.side_by_side;
+  const bool in_group = (lane & -p.side_by_side) == head;
+  if (p.side_by_side == 1 || __any_sync(0xffffffffu, in_group && bad)) {  // (a start that is bad moves no other sequence's places)
+    t.tile = __shfl_sync(0xffffffffu, tiles - 1 - (place - at), from);
+    if (t.tile < 0) return false;
+  } else {
+    const int rank = place - __shfl_sync(0xffffffffu, at, head);
+    const bool member = in_group && tiles > 0;
+    const int mine = member ? tiles : 0;
+    if (rank < 0 || rank >= __reduce_add_sync(0xffffffffu, mine)) return false;
+    const int begin = (n_kv - n_q) >> shift, end = begin + tiles;  // positions of its tiles
+    // More than `rank` tiles lie from lo on, `before` <= rank of them from hi on.
+    int lo = __reduce_min_sync(0xffffffffu, member ? begin : 0x7fffffff);
+    int hi = __reduce_max_sync(0xffffffffu, member ? end : -0x7fffffff), before = 0;
+    while (hi - lo > 1) {
+      const int mid = lo + ((hi - lo) >> 1);
+      const int from_mid = __reduce_add_sync(0xffffffffu, min(max(end - mid, 0), mine));
+      if (from_mid > rank) {
+        lo = mid;
+      } else {
+        hi = mid;
+        before = from_mid;
+      }
     }
+    const bool has = member && begin <= lo && lo < end;
+    const uint32_t all = __ballot_sync(0xffffffffu, has);
+    from = __ffs(__ballot_sync(0xffffffffu, has && __popc(all & ((1u << lane) - 1u)) == rank - before)) - 1;
+    t.tile = lo - __shfl_sync(0xffffffffu, begin, from);
   }
-  const bool has = begin <= lo && lo < end;
-  const uint32_t all = __ballot_sync(0xffffffffu, has);
-  const uint32_t mine = __ballot_sync(0xffffffffu, has && __popc(all & ((1u << lane) - 1u)) == place - before);
-  const int from = __ffs(mine) - 1;
   t.q0 = __shfl_sync(0xffffffffu, q0, from);
   t.k0 = __shfl_sync(0xffffffffu, k0, from);
   t.n_q = __shfl_sync(0xffffffffu, n_q, from);
   t.n_kv = __shfl_sync(0xffffffffu, n_kv, from);
-  t.tile = lo - __shfl_sync(0xffffffffu, begin, from);
   t.rows = min(1 << shift, t.n_q - (t.tile << shift));
-  return true;
-}
-
-// Sequence b has places q_start[b] / tokens + b ... on the line of all query tiles: at least as many as it has tiles, since the
-// next one's first place lies a whole tile further than its rows do. A warp finds the sequence of a place in one turn for
-// every factor of 32 of the batch. False: no tile there (up to one place a sequence), or a sequence that lies outside
-// the rows.
-__device__ __forceinline__ bool packed_tile(const WindowParams& p, int place, PackedTile& t) {
-  // By the rows' order the last sequence's longest lists begin when little else is left to run beside them: ragged prompts of 24
-  // sequences 255 us, 238 longest first. Not where a head's tiles come before the next head's (four chunks behind 14336 keys 593,
-  // 601 longest first: a sequence's tiles share its keys in L2).
-  if (p.batch <= 32 && !p.head_major) return packed_tile_of_few(p, p.tiles - 1 - place, t);
-  const int lane = threadIdx.x & 31;
-  const int shift = 7 - p.group_shift;
-  int lo = 0, n = p.batch, first = 0;
-  while (true) {
-    const int step = (n + 31) >> 5;
-    const int b = lo + lane * step;
-    int at = 0;
-    bool below = false;
-    if (lane * step < n) {
-      at = (p.q_start[b] >> shift) + b;
-      below = at <= place;
-    }
-    const uint32_t seen = __ballot_sync(0xffffffffu, below);
-    if (seen == 0) return false;
-    const int k = 31 - __clz(seen);
-    first = __shfl_sync(0xffffffffu, at, k);
-    lo += k * step;
-    n = min(step, n - k * step);
-    if (step == 1) break;
-  }
-  t.q0 = p.q_start[lo];
-  const int q1 = p.q_start[lo + 1];
-  t.k0 = p.kv_start[lo];
-  const int k1 = p.kv_start[lo + 1];
-  if (t.q0 < 0 || q1 < t.q0 || q1 > p.q_rows || t.k0 < 0 || k1 < t.k0 || k1 > p.kv_rows) return false;
-  t.n_q = q1 - t.q0;
-  t.n_kv = k1 - t.k0;
-  t.tile = place - first;
-  const int row = t.tile << shift;
-  t.rows = min(1 << shift, t.n_q - row);
   return t.rows > 0;
 }
 
@@ -384,7 +371,7 @@ __global__ void __launch_bounds__(192, 2)
   PackedTile seq;
   if constexpr (kPacked) {
     if (blockIdx.x == 0 && blockIdx.y == 0) packed_check(p);
-    if (!packed_tile(p, tile, seq)) return;
+    if (!packed_tile(p, p.tiles - 1 - tile, seq)) return;
   }
   const int len = kPacked ? seq.n_kv : p.kv_len != nullptr ? min(max(p.kv_len[b], 0), p.S) : p.S;
   const KeyList keys = kPacked ? window_keys(p, seq.tile, len, len - seq.n_q) : window_keys(p, tile, len);
@@ -784,7 +771,7 @@ __global__ void __launch_bounds__(WindowWideCfg::kThreads, 1)
   PackedTile seq;
   if constexpr (kPacked) {
     if (blockIdx.x == 0 && blockIdx.y == 0) packed_check(p);
-    if (!packed_tile(p, tile, seq)) return;
+    if (!packed_tile(p, p.tiles - 1 - tile, seq)) return;
   }
   const int len = kPacked ? seq.n_kv : p.kv_len != nullptr ? min(max(p.kv_len[b], 0), p.S) : p.S;
   const KeyList keys = kPacked ? window_keys(p, seq.tile, len, len - seq.n_q) : window_keys(p, tile, len);
@@ -1100,6 +1087,16 @@ static cudaError_t launch_window_attention(const __nv_bfloat16* q, int64_t ld_q,
   const int64_t bh = static_cast<int64_t>(p.B) * (p.heads >> p.group_shift);
   const bool long_ones = kPacked ? p.kv_rows / p.batch >= 16384 : p.S >= 16384;
   p.head_major = (long_ones && bh <= 65535) || p.tiles > 65535;
+  // By the rows' order a sequence's longest lists start when its neighbour's shortest run, and the last ones' with nothing left to
+  // run beside them; all sequences' longest first, their keys share L2 no longer, which costs time where DRAM does and power
+  // where the power limit sets the clock. So groups, of a size that leaves half of L2 to their keys. Cold and at the limit, us:
+  // prompts of 24 sequences of up to 2048, 16 heads of 64, by the rows' order 255 and 254, in groups of 8 244 and 246, all at once
+  // 237 and 264; 16 of 2048 273 and 278, in groups of 4 265 and 272, all at once 260 and 301; the first with a window of 512
+  // 147 and 140 at the limit. Four chunks behind 14336 keys of 4 heads of 128 stay one by one (601 for 593 all at once).
+  p.side_by_side = 1;
+  if (kPacked)
+    while (p.side_by_side < 8 && (p.kv_rows / p.batch + 1) * hd * p.kv_heads * 4 * 2 * p.side_by_side <= (int64_t{64} << 20))
+      p.side_by_side *= 2;
   if (p.head_major && bh > 65535) return cudaErrorInvalidConfiguration;
   WindowMaps maps{};
   const uint64_t h = static_cast<uint64_t>(hd), B = static_cast<uint64_t>(p.B);
