@@ -431,8 +431,9 @@ int b2_window_attention_fwd(const b2_window_attention_args* args, void* stream);
  * its query i stands at p = n_kv - n_q + i among its keys. It sees key j <= p iff window == 0, p - j < window or j < sinks;
  * a row that sees none (p < 0, no keys) gives zeros. Rows of out that belong to no sequence are left as they are.
  * What other sequences hold does not reach a sequence; what the previous entry point says of values that are not finite holds
- * within one. A sequence that lies outside the rows, or ends before it begins, is skipped and recorded; of more than 32
- * sequences, neighbours of it may be skipped as well.
+ * within one. A sequence that lies outside the rows, ends before it begins, or begins below an earlier start that lies inside
+ * the rows, is skipped, and the call is recorded; the others are computed. Of more than 32 sequences others may then be
+ * skipped as well, and a value that two sequences claim is either's.
  *   q_start, kv_start  [batch + 1] int32, ascending; the same pointer for whole prompts
  *   q, out  [q_rows, ld] bf16; k, v  [kv_rows, ld] bf16. head_dim 32, 64 or 128
  */

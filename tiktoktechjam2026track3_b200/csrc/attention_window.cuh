@@ -64,7 +64,7 @@ struct WindowParams {
   const int32_t* q_start;
   const int32_t* kv_start;
   int batch, q_rows, kv_rows;
-  int side_by_side;  // sequences whose tiles are taken together, a power of two up to 32
+  int side_by_side;  // sequences whose tiles are taken together, a power of two up to 8
 };
 
 // Keys and values [B][S][kv_heads][head_dim] in boxes of 64 columns and 128 or 16 rows; Q in boxes of a query tile.
@@ -234,7 +234,10 @@ struct PackedTile {
 // every factor of 32 of the batch; in the last turn its lanes hold the rows of 32 neighbours. Of these, groups of side_by_side (a
 // power of two) share their places: the tiles of a group are taken in the order of their last keys' positions, the longest
 // lists first. The position (in tiles) at which a place's tile ends is found by halves, each a sum over the lanes. False: no tile
-// there (up to one place a sequence), or a sequence that lies outside the rows.
+// there (up to one place a sequence), or a sequence that is skipped: one that lies outside the rows, ends before it begins, or begins
+// below an earlier start that lies inside them. Of 32 neighbours such starts are no places: the next start that is one lies at or
+// behind the end of every sequence that is computed, so that the others keep their tiles. (A further turn before does not look
+// for them: of more than 32 sequences others may be skipped too, and two that claim the same rows computed.)
 __device__ __forceinline__ bool packed_tile(const WindowParams& p, int place, PackedTile& t) {
   const int lane = threadIdx.x & 31;
   const int shift = 7 - p.group_shift;
@@ -260,13 +263,27 @@ __device__ __forceinline__ bool packed_tile(const WindowParams& p, int place, Pa
       n_kv = k1 - k0;
     }
   }
+  if (__any_sync(0xffffffffu, bad)) {  // (starts that descend are a sequence that ends before it begins)
+    const bool inside = b < p.batch && q0 >= 0 && q0 <= p.q_rows;
+    int most = inside ? q0 : -1;  // the largest start so far
+#pragma unroll
+    for (int i = 1; i < 32; i *= 2) {
+      const int before = __shfl_up_sync(0xffffffffu, most, i);
+      if (lane >= i) most = max(most, before);
+    }
+    if (!inside || q0 < most) {
+      at = 0x7fffffff;
+      bad = true;
+      n_q = n_kv = 0;
+    }
+  }
   const uint32_t seen = __ballot_sync(0xffffffffu, at <= place);
   if (seen == 0) return false;
   int from = 31 - __clz(seen);  // the place's sequence
   const int tiles = (n_q + (1 << shift) - 1) >> shift;
   const int head = from & -p.side_by_side;
   const bool in_group = (lane & -p.side_by_side) == head;
-  if (p.side_by_side == 1 || __any_sync(0xffffffffu, in_group && bad)) {  // (a start that is bad moves no other sequence's places)
+  if (p.side_by_side == 1 || __any_sync(0xffffffffu, in_group && bad)) {
     t.tile = __shfl_sync(0xffffffffu, tiles - 1 - (place - at), from);
     if (t.tile < 0) return false;
   } else {

@@ -115,7 +115,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start:
 
     Of n_q queries and n_kv keys, query i stands at p = n_kv - n_q + i and sees key j <= p iff window == 0, p - j < window or
     j < sinks; a row that sees none gives zeros. q [rows, heads * head_dim], k and v [rows, kv_heads * head_dim] (bf16, any row
-    strides), q_start and kv_start int32 [batch + 1]. Query head i reads key head i // (heads / kv_heads).
+    strides), q_start and kv_start int32 [batch + 1], ascending. Query head i reads key head i // (heads / kv_heads).
     scale is head_dim^-0.5 unless given. Rows of `out` that belong to no sequence are left as they are (made zero in one
     that is made here).
     """
