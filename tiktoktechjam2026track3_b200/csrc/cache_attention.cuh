@@ -42,9 +42,14 @@
 //   - V's steps multiply the weights, per group: w step in fp16, 2^-11 of itself once more. Its middles are summed by a product
 //     whose rows are the parameters (a movmatrix brings them there), with the same fp16 weights, so that a weight's
 //     rounding does not part a value from its middle. (Weights times steps in bf16, and bf16 codes: 0.0034 of the norm from 64 bits,
-//     most of it because w (v - mid) and w mid were rounded apart; now 0.0017, the output's own rounding.) The parameters
-//     count in a power of two above all of them so far, which grows as the maximum of the scores does; what is 2^32 below the
-//     largest weight times parameter counts as zero.
+//     most of it because w (v - mid) and w mid were rounded apart; now 0.0017, the output's own rounding.)
+//   - A token's parameters of V count in a power of two above them all, 2^e (e from -60 to 100), which goes into the exponent of its
+//     weight as a page's scale does in 8 bits: w = 2^(s + e - m), with m the running maximum of s + e, and the sum takes w 2^-e. So a
+//     token whose values are large and whose weight is not takes no bits from the others; what is 2^32 below the largest
+//     weight times parameter counts as zero. Within a token, fp16 holds middles of up to 2^15, whole down to 2^-29 of 2^e, and steps of up to 2^6:
+//     their products with the weights, at most 2^9 here (the maximum moves from 2^2 on), have to fit as well. So a step is whole down to 2^-20 of
+//     2^e, loses bits below and is zero from 2^-31 on: so much smaller may a group of a head be than another one. (One power of two
+//     for all that a warp met, as it was, lost what lay 2^14 and more below the largest parameter of any token, whatever its weight.)
 //   - the tiles that a warp takes at once are neighbours in one page (where a page has as many tokens): one address for all.
 // Measured, us (floor; 8-bit codes of the same tokens): 8 x 131072 tokens, 8 key heads of 128, 4 query heads each 296 (208;
 // 331); 64 sequences of up to 8192 106 (63; 115), 16 key heads of 64 127 (63; 180), 32 windows of 4096, 10 rows, 40 (13; 37).
@@ -106,6 +111,10 @@ constexpr int kCacheCluster = 16;  // CTAs of a cluster, at most (a power of two
 constexpr int kCacheBlocksAtOnce = 32;
 constexpr float kCacheRescale = 8.f;   // log2: the maximum moves when a score exceeds it by more
 constexpr float kCacheHeadroom = 7.f;  // log2: weights are at most 2^(8 + 7), below fp16's largest
+// In 4 bits weights and steps share fp16's range: weights are at most 2^(2 + 7), steps 2^6, their products 2^15.
+constexpr float kInt4Rescale = 2.f;
+constexpr int kInt4StepExp = 6;
+constexpr int kInt4MidExp = 15;  // middles meet the weights in a product: they have a range of their own
 
 // What a sequence's tokens come to in tiles of 16: those of the sinks that lie before the window, then the window's.
 struct SeqTiles {
@@ -204,8 +213,17 @@ __device__ __forceinline__ float4 load_shared4(const float4* p) {
                : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
   return v;
 }
-__device__ __forceinline__ uint32_t bf16x2_max_abs(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), __habs2(*reinterpret_cast<__nv_bfloat162*>(&b)));
+// Of a NaN and a number the number.
+__device__ __forceinline__ uint32_t bf16x2_max(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t bf16x2_min(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmin2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t bf16x2_abs(uint32_t a) {
+  const __nv_bfloat162 r = __habs2(*reinterpret_cast<__nv_bfloat162*>(&a));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 // (w & mask) | bits: one instruction if one of the two constants is in a register.
@@ -239,6 +257,12 @@ __device__ __forceinline__ uint16_t load_once_u16(const void* p) {
   uint16_t u;
   asm("ld.global.L1::no_allocate.u16 %0, [%1];" : "=h"(u) : "l"(p));
   return u;
+}
+
+// 4 bits: 2^(by - e) of the token in half x of a word of powers 2^(e - 1), bf16 (their mantissas are 0).
+__device__ __forceinline__ float int4_per_power(uint32_t power, int x, int by) {
+  const uint32_t bits = static_cast<uint32_t>(by + 253) << 23;
+  return __uint_as_float(x ? bits - (power & 0xffff0000u) : bits - power * 65536u);
 }
 
 // 32-bit words of a token that one thread holds, and where they lie: vectors of up to 4 words; a thread's vectors are
@@ -639,8 +663,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
 
     float o[NT][Cfg::kSteps][4];
     float m[NT][2], l[NT][2];
-    float om[NT][4];  // 4 bits: weights' sums times V's parameters, row g of which is the token's parameter number g;
-    float unit = 0x1p-100f;  // and what o and om count in, a power of two above every parameter so far
+    float om[NT][4];  // 4 bits: weights' sums times V's parameters, row g of which is the token's parameter number g
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       om[nt][0] = om[nt][1] = om[nt][2] = om[nt][3] = 0.f;
@@ -807,14 +830,30 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
           }
         }
 
-        uint32_t bigs = 0u;  // of V's parameters, two by two
+        // The power of two 2^e above each token's parameters of V, of tokens g and g + 8 in the halves of a word: 2^(e - 1) as bf16.
+        uint32_t power[kSub];
+#pragma unroll
+        for (int c = 0; c < kSub; ++c) {
+          uint32_t big = bf16x2_max(bf16x2_abs(__byte_perm(vp[c][0], vp[c][1], 0x5410u)),
+                                    bf16x2_abs(__byte_perm(vp[c][0], vp[c][1], 0x7632u)));
+          big = bf16x2_max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+          big = bf16x2_max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+          power[c] = bf16x2_min(bf16x2_max(big, 0x21002100u), 0x71007100u) & 0x7f807f80u;  // 2^-61 ... 2^99
+        }
+        bool grew = false;
         float top[NT][2];
 #pragma unroll
-        for (int c = 0; c < kSub; ++c)
+        for (int c = 0; c < kSub; ++c) {
+          // 2^23 + 128 (e + 126) by its bits
+          float e[2];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) bigs = bf16x2_max_abs(bigs, vp[c][x]);
-        float big = fmaxf(__uint_as_float(bigs << 16), __uint_as_float(bigs & 0xffff0000u));
-        bool grew = big > unit;
+          for (int x = 0; x < 2; ++x)
+            e[x] = fmaf(__uint_as_float(__byte_perm(power[c], 0x4b000000u, x ? 0x7432u : 0x7410u)), 0x1p-7f, -65662.f);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s[c][nt][x] = fmaf(s[c][nt][x], row_scale[nt][x & 1], e[x >> 1]);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -822,19 +861,9 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
             top[nt][x] = fmaxf(s[0][nt][x], s[0][nt][x + 2]);
 #pragma unroll
             for (int c = 1; c < kSub; ++c) top[nt][x] = max3f(top[nt][x], s[c][nt][x], s[c][nt][x + 2]);
-            top[nt][x] *= row_scale[nt][x];
-            grew |= top[nt][x] > m[nt][x] + kCacheRescale;
+            grew |= top[nt][x] > m[nt][x] + kInt4Rescale;
           }
         if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-          for (int i = 1; i < 32; i *= 2) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, i));
-          float other = 1.f;
-          if (big > unit) {  // a power of two above it, at most 2^100
-            const int e = min(static_cast<int>(__float_as_uint(big) >> 23) - 126, 100);
-            const float now_unit = exp2_int(e);
-            other = unit * exp2_int(-e);
-            unit = now_unit;
-          }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -843,18 +872,16 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
               best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
               best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 8));
               best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
-              float alpha = 1.f;
               if (best > m[nt][x]) {
-                alpha = fast_exp2(m[nt][x] - best);  // 0 the first time
+                const float alpha = fast_exp2(m[nt][x] - best);  // 0 the first time
                 m[nt][x] = best;
                 l[nt][x] *= alpha;
-              }
-              alpha *= other;
-              om[nt][x] *= alpha;
+                om[nt][x] *= alpha;
 #pragma unroll
-              for (int j = 0; j < Cfg::kSteps; ++j) {
-                o[nt][j][x] *= alpha;
-                o[nt][j][x + 2] *= alpha;
+                for (int j = 0; j < Cfg::kSteps; ++j) {
+                  o[nt][j][x] *= alpha;
+                  o[nt][j][x + 2] *= alpha;
+                }
               }
             }
         }
@@ -866,26 +893,26 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
           const float ref1 = m[nt][1] == -INFINITY ? -kCacheHeadroom : m[nt][1] - kCacheHeadroom;
 #pragma unroll
           for (int c = 0; c < kSub; ++c) {
-            const float w0 = fast_exp2(fmaf(s[c][nt][0], row_scale[nt][0], -ref0));
-            const float w1 = fast_exp2(fmaf(s[c][nt][1], row_scale[nt][1], -ref1));
-            const float w2 = fast_exp2(fmaf(s[c][nt][2], row_scale[nt][0], -ref0));
-            const float w3 = fast_exp2(fmaf(s[c][nt][3], row_scale[nt][1], -ref1));
-            l[nt][0] += w0 + w2;
-            l[nt][1] += w1 + w3;
+            const float w0 = fast_exp2(s[c][nt][0] - ref0), w1 = fast_exp2(s[c][nt][1] - ref1);
+            const float w2 = fast_exp2(s[c][nt][2] - ref0), w3 = fast_exp2(s[c][nt][3] - ref1);
+            const float inv0 = int4_per_power(power[c], 0, 0), inv1 = int4_per_power(power[c], 1, 0);
+            l[nt][0] = fmaf(w2, inv1, fmaf(w0, inv0, l[nt][0]));
+            l[nt][1] = fmaf(w3, inv1, fmaf(w1, inv0, l[nt][1]));
             pf[c][nt][0] = movmatrix_trans(pack_f16x2(w0, w1));
             pf[c][nt][1] = movmatrix_trans(pack_f16x2(w2, w3));
           }
         }
 
-        const float per_unit = __uint_as_float(0x7f000000u - __float_as_uint(unit));  // 1 / unit, a power of two
 #pragma unroll
         for (int c = 0; c < kSub; ++c) {
           // The parameters as rows, two tokens to a register; a group's steps go into the weights of its dims.
           uint32_t v[2];
 #pragma unroll
           for (int x = 0; x < 2; ++x)
-            v[x] = movmatrix_trans(pack_f16x2(__uint_as_float(vp[c][x] << 16) * per_unit,
-                                              __uint_as_float(vp[c][x] & 0xffff0000u) * per_unit));
+            v[x] = movmatrix_trans(
+                pack_f16x2(__uint_as_float(vp[c][x] << 16) * int4_per_power(power[c], x, G == 1 || t < G / 2 ? kInt4StepExp : kInt4MidExp),
+                           __uint_as_float(vp[c][x] & 0xffff0000u) *
+                               int4_per_power(power[c], x, G > 1 && t < G / 2 ? kInt4StepExp : kInt4MidExp)));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma_f16(om[nt], v[0], any_bits(), v[1], any_bits(), pf[c][nt][0], pf[c][nt][1]);  // (8 rows)
 #pragma unroll
@@ -1104,9 +1131,10 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
 #pragma unroll
         for (int j = 0; j < Cfg::kSteps; ++j) {
           if constexpr (kInt4) {
+            constexpr float kMid = 1.f / (1 << (kInt4MidExp - kInt4StepExp)), kUnit = 1.f / (1 << kInt4StepExp);
             const float mid = __shfl_sync(0xffffffffu, om[nt][x], 4 * (G + j / 2) + t);
             *reinterpret_cast<float2*>(dst + r * HD + 32 * (j / 2) + 4 * g + 2 * (j & 1)) =
-                make_float2((o[nt][j][x] + mid) * unit, (o[nt][j][x + 2] + mid) * unit);
+                make_float2(fmaf(mid, kMid, o[nt][j][x]) * kUnit, fmaf(mid, kMid, o[nt][j][x + 2]) * kUnit);
             continue;
           }
           const int d = kFp8 ? VPieces::offset(j / 2, g) + 2 * (j & 1) : VPieces::offset(j, g) / 2;
