@@ -690,7 +690,7 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
     if constexpr (kInt4) {
       const int64_t head = (static_cast<int64_t>(now.h) << p.c.page_shift) * (4 * G) + g * (4 * G);
       kp_at = reinterpret_cast<const uint8_t*>(p.c.k_group) + head;
-      vp_at = reinterpret_cast<const uint8_t*>(p.c.v_group) + head + 4 * min(t, G - 1);
+      vp_at = reinterpret_cast<const uint8_t*>(p.c.v_group) + head + 4 * (t & (G - 1));
       group_page = (kv_heads << p.c.page_shift) * (4 * G);
     }
 
@@ -728,7 +728,6 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
             RowPieces<G == 4 ? 2 : G, 1>::load(kp_row + 8 * x * (4 * G), 0, kp[c][x]);
             km[c][x] = G == 4 ? load_once(kp_row + 8 * x * (4 * G) + mid_at) : kp[c][x][G == 4 ? 0 : G - 1];
             vp[c][x] = load_once(vp_row + 8 * x * (4 * G));
-            if (G < 4) vp[c][x] = t < G ? vp[c][x] : 0u;
           }
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -836,8 +835,8 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
         for (int c = 0; c < kSub; ++c) {
           uint32_t big = bf16x2_max(bf16x2_abs(__byte_perm(vp[c][0], vp[c][1], 0x5410u)),
                                     bf16x2_abs(__byte_perm(vp[c][0], vp[c][1], 0x7632u)));
-          big = bf16x2_max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-          big = bf16x2_max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+          if (G > 1) big = bf16x2_max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+          if (G > 2) big = bf16x2_max(big, __shfl_xor_sync(0xffffffffu, big, 2));
           power[c] = bf16x2_min(bf16x2_max(big, 0x21002100u), 0x71007100u) & 0x7f807f80u;  // 2^-61 ... 2^99
         }
         bool grew = false;
@@ -905,14 +904,15 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
 
 #pragma unroll
         for (int c = 0; c < kSub; ++c) {
-          // The parameters as rows, two tokens to a register; a group's steps go into the weights of its dims.
+          // The parameters as rows (of 2 groups and of one there more than once), two tokens to a register; a group's steps go into
+          // the weights of its dims.
           uint32_t v[2];
 #pragma unroll
           for (int x = 0; x < 2; ++x)
             v[x] = movmatrix_trans(
-                pack_f16x2(__uint_as_float(vp[c][x] << 16) * int4_per_power(power[c], x, G == 1 || t < G / 2 ? kInt4StepExp : kInt4MidExp),
+                pack_f16x2(__uint_as_float(vp[c][x] << 16) * int4_per_power(power[c], x, G == 1 || (t & (G - 1)) < G / 2 ? kInt4StepExp : kInt4MidExp),
                            __uint_as_float(vp[c][x] & 0xffff0000u) *
-                               int4_per_power(power[c], x, G > 1 && t < G / 2 ? kInt4StepExp : kInt4MidExp)));
+                               int4_per_power(power[c], x, G > 1 && (t & (G - 1)) < G / 2 ? kInt4StepExp : kInt4MidExp)));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma_f16(om[nt], v[0], any_bits(), v[1], any_bits(), pf[c][nt][0], pf[c][nt][1]);  // (8 rows)
 #pragma unroll
