@@ -35,9 +35,10 @@
 // its rows are found from q_start and kv_start by the CTA itself (the host does not know them), positions count from n_kv -
 // n_q on, and everything else is as above. The tensor maps cover all sequences' rows: what a box brings of a neighbour is hidden
 // like later keys, and cleared among the values.
-// Measured (us; floor): ragged prompts of 24 sequences of up to 2048 tokens, 16 heads of 64: 244 (64), 16 of 2048 tokens 265 where
+// Measured (us; floor): ragged prompts of 24 sequences of up to 2048 tokens, 16 heads of 64: 245 (64), 16 of 2048 tokens 265 where
 // the padded batch's kernel takes 249; four chunks of up to 2048 queries behind 14336 keys, 16 heads of 128 on 4 key heads:
-// 606 (386). What bounds the first is the softmax warps' chain: of 3200 to 3600 clocks a tile 1600 are its exponentials (1024 if a
+// 602 before the clock drops at the 1000 W limit, 682 then (386). 24 sequences of 748 to 2048 tokens with a window of 512 and 4 sinks
+// 208 (42), of heads of 32 without a window 227 (30); one of 16000 among 40 of 100, 16 heads of 64: 721 (315). What bounds the first is the softmax warps' chain: of 3200 to 3600 clocks a tile 1600 are its exponentials (1024 if a
 // warp had its quarter of the unit to itself), 170 the scores' load, 450 the maximum, 600 waits for products, which queue
 // behind the other CTA's.
 #pragma once

@@ -139,7 +139,8 @@ __device__ __forceinline__ void append_queries(const AppendParams& p, int key_he
   __nv_bfloat16* out = p.q_out + row0 * p.ld_q_out + h0 * hd;
   // Two heads' loads before their stores where the heads are even (q_out may be qkv, so the compiler cannot move them): 16 query
   // heads of 128 on 4 key heads, ragged prompts, 57 -> 51 us, 67 -> 57 over 4 bits; four of them 53 and 54, but the registers
-  // cost 16 heads on 16 key heads more than a tenth.
+  // cost 16 heads on 16 key heads more than a tenth. (The bf16 and 8-bit kernels of half pairs spill 4 to 8 bytes for it; groups
+  // of 1, 3, 5, 7 and 71 heads take as long as without or up to 6 % less.)
   auto turn = [&](auto at_once) {
     constexpr int kAtOnce = decltype(at_once)::value;
     for (unsigned i = tt; i < items; i += threads) {

@@ -30,9 +30,9 @@
 // large scale holds zeros.
 //
 // 4-bit pages (cache_int4.cuh): v = mid + (code - 8) step, a step and a middle for 32 dims of a token. What bounds them is
-// no longer HBM but the instructions that a code costs (343 for 16 tokens of 128 dims and up to 8 rows; ALU 50 % and issue 52
+// no longer HBM but the instructions that a code costs (362 for 16 tokens of 128 dims and up to 8 rows; ALU 50 % and issue 53
 // % busy, DRAM at 0.6 of the copy rate; with every load from L2 the time falls by a tenth only), so each is chosen for their
-// number:
+// number. (The instances of 64 and 128 dims spill: 8 to 56 bytes for up to 8 rows, 28 to 136 for 16; fewer warps cost more.)
 //   - a code becomes 1024 + code, or 64 + code, in fp16 by one instruction, (bits & mask) | constant, two at a time and without a
 //     shift for half of them. For K the excess leaves with the products' start, -1032 sum(q) (72 for the odd dims), Q in
 //     fp16 as over 8 bits (a sum of 1032 |q| in fp32 loses 2^-13 of |q|, which is nothing next to a code's half step). For V it
@@ -51,8 +51,10 @@
 //     2^e, loses bits below and is zero from 2^-31 on: so much smaller may a group of a head be than another one. (One power of two
 //     for all that a warp met, as it was, lost what lay 2^14 and more below the largest parameter of any token, whatever its weight.)
 //   - the tiles that a warp takes at once are neighbours in one page (where a page has as many tokens): one address for all.
-// Measured, us (floor; 8-bit codes of the same tokens): 8 x 131072 tokens, 8 key heads of 128, 4 query heads each 296 (208;
-// 331); 64 sequences of up to 8192 106 (63; 115), 16 key heads of 64 127 (63; 180), 32 windows of 4096, 10 rows, 40 (13; 37).
+// Measured, us before the clock drops at the 1000 W limit (floor; 8-bit codes of the same tokens): 8 x 131072 tokens, 8 key heads
+// of 128, 4 query heads each 311 (208; 331; at the limit 332); 64 sequences of up to 8192 110 (63; 115), 16 key heads of 64
+// 124 (63; 180), 32 of 32 178, 32 windows of 4096, 10 rows, 41 (13; 37). A token's own power of two is 4 to 7 % of these (one for
+// all that a warp met 298, 106, 120, 166 and 40), 19 of the 362 instructions.
 // Codes as e4m3, whose bits a code is in 2^-9ths, need no excess, but the product of that type is made of conversions and fp16
 // products here: 411 for the first. Prefetching into L2 costs what it saves: a bulk prefetch is a loop over the lanes
 // (380), lines by their lanes 342 where 347 without.
@@ -323,8 +325,9 @@ struct CacheAttnCfg {
   static constexpr int kGroups = HD / 32;  // of 4-bit codes
   static constexpr int kSteps = HD / 16;
   // A warp takes kSub tiles of 16 tokens at a time, interleaved: 4 KB of keys and values on their way per warp.
-  // In 4 bits 2, or 4 where the registers allow it (64 sequences of up to 8192 tokens, us with 1, 2, 4 tiles: 16 key heads of
-  // 64 172, 130, 127; 32 of 32 -, 198, 150; 16 rows of 128 199, 174, of 64 117, 96, 132, of 32 101, 71, 83).
+  // In 4 bits 2, or 4 where the registers allow it (64 sequences of 2300 to 8192 tokens, us with 1, 2, 4 tiles: 8 key heads of 128
+  // 142, 121, 144; 16 of 64 189, 142, 124; 32 of 32 303, 222, 177; 16 rows to 8 key heads of 128 223, 190, 219, of 64 134, 112, 121, of 32
+  // 106, 84, 79, the last with 90 to 160 bytes of spills).
   static constexpr int kFill = 128 / (kRowBytes * NT);
   static constexpr int kSub = kType == kCacheInt4 ? (NT == 2 || HD == 128 ? 2 : 4) : kFill > 1 ? kFill : 1;
   static constexpr int kAlign = kType == kCacheInt4 ? kSub : 1;  // 4 bits: a warp's tiles of a unit are neighbours
@@ -1499,9 +1502,9 @@ static cudaError_t launch_cache_attention_nt(const CacheAttnParams& p, int64_t r
   //   a third, or in quarters, up to 20: 8 heads of 8000 12.5 / 19.5, of 32000 28.2 / 29.4, of 64000 47 / 39; 256 heads
   //     of 1000 20.8 / 28.0, of 4000 62.6 / 58.7;
   //   else up to 8: 4 heads of 8000 10.4 / 18.0, of 32000 17.4 / 20.2; 1 of 8000 9.9 / 13.5, of 32000 16.7 / 17.1;
-  //   4 bits, half as many rounds, each of twice the tokens: 32 heads of 16000 29.3 / 33.7, of 32000
-  //     51.7 / 50.8; 512 of 2000 46.1 / 52.4, of 4096 85.7 / 88.4 (of up to 4096 77.8 / 65.8), of 8192 162.9 / 157.3, windows of
-  //     8192 163.6 / 158.4; 256 of 1000 16.8 / 20.8, of 4000 61.0 / 51.4; 8 of 32000 27.1 / 26.9, of 64000 48.0 / 33.5.
+  //   4 bits, half as many rounds, each of twice the tokens: 32 heads of 16000 30.0 / 34.3, of 32000
+  //     53.5 / 52.0; 512 of 2000 47.2 / 53.6, of 4096 88.0 / 91.5 (of up to 4096 79.8 / 67.3), of 8192 167.5 / 163.8, windows of
+  //     8192 168.2 / 164.5; 256 of 1000 17.0 / 21.2, of 4000 62.6 / 52.9; 8 of 32000 27.8 / 27.1, of 64000 50.0 / 34.2.
   const int64_t heads = static_cast<int64_t>(p.batch) * p.c.kv_heads * row_blocks;
   const bool sm_each = heads <= sm_count;
   const int64_t round = 16 * (sm_each ? CacheAttnCfg<HD, kType, NT, 1>::kUnitTiles : CacheAttnCfg<HD, kType, NT, 4>::kUnitTiles);

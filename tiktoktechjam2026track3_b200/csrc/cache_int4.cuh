@@ -28,8 +28,9 @@
 // Measured on one B200 (us a call, floor at the measured copy rate in brackets): append of ragged prompts of 16 sequences of up to
 // 2048 tokens, 16 heads of 64, rotated queries and keys kept: 60 (40); chunks of three documents, 16 query and 4 key heads of
 // 128, a quarter turned: 15 (8); one token in each of 64 sequences 4, a launch. Reading 4 x 65536 tokens of 8 heads of 128 in 4
-// bits: 221 (218); 16 sequences of up to 4096 tokens of 16 heads of 64 in 8 bits: 51 (43). The append's issue slots are 60 to 70
-// % busy and its ALU 60 to 75 (some 18 instructions an element for ranges and codes).
+// bits: 221 (218); 16 sequences of up to 4096 tokens of 16 heads of 64 in 8 bits: 51 (43); in bf16 4 x 65536 tokens of 8 heads of
+// 128 328 (332), 16 x 4096 of 16 heads of 64 88 (83). The append's issue slots are 62 % busy and its ALU 56 (some 18
+// instructions an element for ranges and codes).
 #pragma once
 #include "b2_common.cuh"
 #include "cache_append.cuh"
@@ -214,7 +215,8 @@ __device__ __forceinline__ uint32_t halves_together(const uint32_t (&w)[G], int 
   return __byte_perm(w[y / 2], w[(G + y) / 2], (y % 2 ? 0x32u : 0x10u) | ((G + y) % 2 ? 0x7600u : 0x5400u));
 }
 
-// (64 registers, four CTAs an SM, up to 4 groups: ragged prompts of 16 heads of 64 63 us, 70 with three or with five.)
+// (64 registers, four CTAs an SM, up to 4 groups: ragged prompts of 16 heads of 64 63 us, 70 with three or with five. They are a few
+// too few: 4 to 12 bytes of spills for 2 groups, 24 for 3, 32 to 84 for 4; of 6 and 8 groups, with 128, 16 and 52 to 68.)
 template <int G, bool kInterleaved>
 __global__ void __launch_bounds__(kInt4Threads, G <= 4 ? 4 : 2) cache_append_int4_kernel(const AppendParams p, const int tile_tokens,
                                                                          const unsigned role_blocks) {

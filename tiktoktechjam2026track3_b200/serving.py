@@ -132,10 +132,11 @@ class KVCache:
     In 8 bits (torch.float8_e4m3fn) a page has one fp32 scale per head, a power of two, in k_scale / v_scale
     [pages, kv_heads]. In 4 bits (torch.uint8, two codes to a byte: [..., head_dim / 2]) k_scale and v_scale are bf16
     [pages, kv_heads, page_size, 2, head_dim / 32]: of every token, the steps of its groups of 32 elements, then their middles
-    (include/b200tx.h has the codes' meaning and order). Which pages a sequence owns is the caller's page table, int32 [batch, pages of the longest]:
-    token j of sequence b lies in slot j % page_size of page page_table[b, j // page_size].
+    (include/b200tx.h has the codes' meaning and order). Which pages a sequence owns is the caller's page table,
+    int32 [batch, pages of the longest]: token j of sequence b lies in slot j % page_size of page page_table[b, j // page_size].
     `allocate` makes the tensors; the constructor takes the caller's own (k and v may be slices of one
-    buffer: their first two strides are free, but alike).
+    buffer: their first two strides are free, but alike). `append` and `read` take any head_dim that is a multiple of 16 (4 bits:
+    32) up to 256, `attend` 32, 64 and 128.
     """
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
