@@ -372,8 +372,9 @@ int b2_cache_attention_workspace(int64_t batch, int64_t q_len, int64_t num_heads
  * out = softmax(scale * q k^T) v, zero where nothing is visible. What lies in pages and slots that no row
  * sees is not used, whatever it is. Of the tokens that some of the q_len rows see and others do not,
  * a value that is not finite reaches them all. In 8 bits, tokens whose weight times the scale of their page of V is
- * more than 2^32 below the largest count as if their values were zero; in 4 bits, tokens whose weight times 2^e is, where 2^e is a
- * power of two above their head's steps and middles of V, 2^-60 at least. Steps of V lose bits where they are more than 2^20
+ * more than 2^32 below the largest count as if their values were zero; in 4 bits, tokens whose weight times 2^e is, where 2^e is the
+ * least power of two above the token's steps and middles of V, 2^-60 at least and 2^100 at most (more than 2^120 below, their weights
+ * are missing from the sum as well: values of 0 beside others beyond 2^50). Steps of V lose bits where they are more than 2^20
  * below 2^e, and middles from 2^29 on: groups of one head whose values are further apart than that lose the smaller
  * ones' codes. Steps and middles beyond 2^100 may become infinite.
  *   q, out     [batch * q_len, ld] bf16, num_heads heads side by side, a multiple of the cache's kv_heads:
