@@ -4,8 +4,9 @@ A token's steps and middles count in a power of two 2^e above them all (e from -
 that what a token loses is measured by its own w 2^e. Steps are held as fp16 numbers of at most 2^6, middles of at most 2^15: a
 subnormal one is off by 2^-25 at most, which is 2^-31 and 2^-40 of 2^e; the weights' largest are 2^7 or more, so that a subnormal
 weight, or its product with a step, is off by at most 2^-32 of the largest w 2^e. A code is a whole number of up to 8 steps. Besides
-these, a weight is rounded to 2^-11 of itself and its product with a step again; a score's error is that of test_gpu_int4.py. The
-output is bf16.
+these, a weight is rounded to 2^-11 of itself and its product with a step again; a score's error is that of test_gpu_int4.py, and its
+sum with e, of up to 2^8 here, is off by 2^-17 at most, which moves a weight by 2^-17.5 and twice (weight and sum): 2^-16. The output
+is bf16.
 """
 
 import math

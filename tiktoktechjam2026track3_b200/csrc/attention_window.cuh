@@ -38,9 +38,9 @@
 // Measured (us; floor): ragged prompts of 24 sequences of up to 2048 tokens, 16 heads of 64: 245 (64), 16 of 2048 tokens 265 where
 // the padded batch's kernel takes 249; four chunks of up to 2048 queries behind 14336 keys, 16 heads of 128 on 4 key heads:
 // 602 before the clock drops at the 1000 W limit, 682 then (386). 24 sequences of 748 to 2048 tokens with a window of 512 and 4 sinks
-// 208 (42), of heads of 32 without a window 227 (30); one of 16000 among 40 of 100, 16 heads of 64: 721 (315). What bounds the first is the softmax warps' chain: of 3200 to 3600 clocks a tile 1600 are its exponentials (1024 if a
-// warp had its quarter of the unit to itself), 170 the scores' load, 450 the maximum, 600 waits for products, which queue
-// behind the other CTA's.
+// 208 (42), of heads of 32 without a window 227 (30); one of 16000 among 40 of 100, 16 heads of 64: 721 (315). What bounds the
+// first is the softmax warps' chain: of 3200 to 3600 clocks a tile 1600 are its exponentials (1024 if a warp had its quarter of the
+// unit to itself), 170 the scores' load, 450 the maximum, 600 waits for products, which queue behind the other CTA's.
 #pragma once
 #include <mutex>
 #include <type_traits>

@@ -46,10 +46,11 @@
 //   - A token's parameters of V count in a power of two above them all, 2^e (e from -60 to 100), which goes into the exponent of its
 //     weight as a page's scale does in 8 bits: w = 2^(s + e - m), with m the running maximum of s + e, and the sum takes w 2^-e. So a
 //     token whose values are large and whose weight is not takes no bits from the others; what is 2^32 below the largest
-//     weight times parameter counts as zero. Within a token, fp16 holds middles of up to 2^15, whole down to 2^-29 of 2^e, and steps of up to 2^6:
-//     their products with the weights, at most 2^9 here (the maximum moves from 2^2 on), have to fit as well. So a step is whole down to 2^-20 of
-//     2^e, loses bits below and is zero from 2^-31 on: so much smaller may a group of a head be than another one. (One power of two
-//     for all that a warp met, as it was, lost what lay 2^14 and more below the largest parameter of any token, whatever its weight.)
+//     weight times parameter counts as zero. Within a token, fp16 holds middles of up to 2^15, whole down to 2^-29 of 2^e, and
+//     steps of up to 2^6: their products with the weights, at most 2^9 here (the maximum moves from 2^2 on), have to fit as well.
+//     So a step is whole down to 2^-20 of 2^e, loses bits below and is zero from 2^-31 on: so much smaller may a group of a head
+//     be than another one. (One power of two for all that a warp met lost what lay 2^14 and more below the largest parameter of
+//     any token, whatever its weight.)
 //   - the tiles that a warp takes at once are neighbours in one page (where a page has as many tokens): one address for all.
 // Measured, us before the clock drops at the 1000 W limit (floor; 8-bit codes of the same tokens): 8 x 131072 tokens, 8 key heads
 // of 128, 4 query heads each 311 (208; 331; at the limit 332); 64 sequences of up to 8192 110 (63; 115), 16 key heads of 64
@@ -326,8 +327,8 @@ struct CacheAttnCfg {
   static constexpr int kSteps = HD / 16;
   // A warp takes kSub tiles of 16 tokens at a time, interleaved: 4 KB of keys and values on their way per warp.
   // In 4 bits 2, or 4 where the registers allow it (64 sequences of 2300 to 8192 tokens, us with 1, 2, 4 tiles: 8 key heads of 128
-  // 142, 121, 144; 16 of 64 189, 142, 124; 32 of 32 303, 222, 177; 16 rows to 8 key heads of 128 223, 190, 219, of 64 134, 112, 121, of 32
-  // 106, 84, 79, the last with 90 to 160 bytes of spills).
+  // 142, 121, 144; 16 of 64 189, 142, 124; 32 of 32 303, 222, 177; 16 rows to 8 key heads of 128 223, 190, 219, of 64 134, 112, 121,
+  // of 32 106, 84, 79, the last with 90 to 160 bytes of spills).
   static constexpr int kFill = 128 / (kRowBytes * NT);
   static constexpr int kSub = kType == kCacheInt4 ? (NT == 2 || HD == 128 ? 2 : 4) : kFill > 1 ? kFill : 1;
   static constexpr int kAlign = kType == kCacheInt4 ? kSub : 1;  // 4 bits: a warp's tiles of a unit are neighbours
@@ -913,7 +914,8 @@ __global__ void __launch_bounds__(CacheAttnCfg<HD, kType, NT, kShare>::kThreads,
 #pragma unroll
           for (int x = 0; x < 2; ++x)
             v[x] = movmatrix_trans(
-                pack_f16x2(__uint_as_float(vp[c][x] << 16) * int4_per_power(power[c], x, G == 1 || (t & (G - 1)) < G / 2 ? kInt4StepExp : kInt4MidExp),
+                pack_f16x2(__uint_as_float(vp[c][x] << 16) *
+                               int4_per_power(power[c], x, G == 1 || (t & (G - 1)) < G / 2 ? kInt4StepExp : kInt4MidExp),
                            __uint_as_float(vp[c][x] & 0xffff0000u) *
                                int4_per_power(power[c], x, G > 1 && (t & (G - 1)) < G / 2 ? kInt4StepExp : kInt4MidExp)));
 #pragma unroll
